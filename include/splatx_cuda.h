@@ -768,6 +768,140 @@ typedef struct SxSsimGradsIn {
 int32_t sxcuda_ssim_bwd(const SxSsimInputs* in, const SxSsimGradsIn* gin, float* v_img1,
                         sxcuda_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Network operators (no counterpart in the reference): what a network that predicts, refines or
+ * conditions splats is trained with beside the rasteriser. Device pointers and a caller stream as
+ * above; no call allocates device memory or synchronises. Sums, softmax statistics and moments
+ * are held in 32 bits whatever the element type; no result depends on the order of atomics.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Element types. */
+#define SXCUDA_F32 0
+#define SXCUDA_F16 1
+#define SXCUDA_BF16 2
+
+/* y = (x - mean) * rstd * weight + bias over the last axis; rstd = 1 / sqrt(var + eps), var the
+ * mean square about the mean. rows 0 is a no-op (the backward then writes zero weight
+ * gradients). */
+typedef struct SxLayerNormInputs {
+    const void* x;      /* [rows, cols], dtype, rows x_stride elements apart */
+    const void* weight; /* [cols], param_dtype; NULL = ones */
+    const void* bias;   /* [cols], param_dtype; NULL = zeros (the backward does not read it) */
+    int64_t rows, cols; /* cols >= 1 */
+    int64_t x_stride;   /* elements, >= cols unless rows <= 1 */
+    int32_t dtype, param_dtype;
+    float eps;
+} SxLayerNormInputs;
+
+/* y: [rows, cols] of dtype, rows y_stride elements apart. mean, rstd: [rows] (both or neither). */
+int32_t sxcuda_layer_norm_fwd(const SxLayerNormInputs* in, void* y, int64_t y_stride, float* mean,
+                              float* rstd, sxcuda_stream_t stream);
+
+typedef struct SxLayerNormGradsIn {
+    const float* mean; /* [rows], of the forward */
+    const float* rstd; /* [rows] */
+    const void* v_y;   /* [rows, cols], dtype */
+    int64_t v_y_stride;
+} SxLayerNormGradsIn;
+
+typedef struct SxLayerNormGrads {
+    void* v_x; /* [rows, cols], dtype */
+    int64_t v_x_stride;
+    void* v_weight; /* [cols], param_dtype, or NULL */
+    void* v_bias;   /* [cols], param_dtype, or NULL */
+} SxLayerNormGrads;
+
+/* Workspace query protocol. The rows' contributions to v_weight and v_bias are summed in a fixed
+ * order: the result is the same in every call. */
+int32_t sxcuda_layer_norm_bwd(const SxLayerNormInputs* in, const SxLayerNormGradsIn* gin,
+                              const SxLayerNormGrads* out, void* workspace,
+                              size_t* workspace_bytes, sxcuda_stream_t stream);
+
+/* One AdamW step (decoupled weight decay, bias correction) over many tensors in one launch per
+ * 400 of them:
+ *   g' = g * grad_scale            m' = b1 m + (1 - b1) g'        v' = b2 v + (1 - b2) g'^2
+ *   p' = p (1 - lr weight_decay) - lr / (1 - b1^step) * m' / (sqrt(v' / (1 - b2^step)) + eps)
+ * evaluated in 32 bits, every operation rounded by itself. (sxcuda_fused_adam is the reference's
+ * Adam without bias correction, over one tensor.)
+ * 8-bit moments: m and sqrt(v) are held as e4m3 codes, each run of 256 consecutive values with
+ * one 32-bit scale (largest magnitude / 448); a value above zero of sqrt(v) keeps at least the
+ * smallest code, so that a moment which is left of a gradient never stands over a zero. A run
+ * whose largest magnitude is below 1e-30 is held as zeros; one with a value that is not finite
+ * has no finite values afterwards, and its weights neither. */
+typedef struct SxAdamwTensor {
+    void* param;            /* [n], param_dtype; updated */
+    const void* grad;       /* [n], grad_dtype */
+    void* exp_avg;          /* [n] float, or uint8 codes; updated */
+    void* exp_avg_sq;       /* [n] float v, or uint8 codes of sqrt(v); updated */
+    float* exp_avg_scale;   /* [ceil(n / 256)] with 8-bit moments, else NULL; updated */
+    float* exp_avg_sq_scale;
+    int64_t n;              /* >= 0 */
+    double lr, weight_decay; /* of this tensor */
+    int32_t param_dtype, grad_dtype;
+} SxAdamwTensor;
+
+typedef struct SxAdamwConfig {
+    double b1, b2, eps; /* 0 <= b < 1, eps >= 0 */
+    double grad_scale;
+    int64_t step;       /* this step's number, from 1 */
+    int32_t state_bits; /* 32 or 8 */
+} SxAdamwConfig;
+
+/* tensors: HOST array of n_tensors, read before the call returns. */
+int32_t sxcuda_adamw_step(const SxAdamwTensor* tensors, int64_t n_tensors,
+                          const SxAdamwConfig* cfg, sxcuda_stream_t stream);
+
+/* softmax(scale q k^T + mask) v per head, with as many query heads to each key-value head as
+ * q_heads / kv_heads (head h reads key-value head h / (q_heads / kv_heads)).
+ * Query i of batch b sees key j where i < q_lens[b], j < kv_lens[b] and, when causal,
+ * j <= i + kv_lens[b] - q_lens[b] (without lengths: q_len and kv_len). A query that sees none has
+ * output 0, log-sum -inf and gradient 0; a key that none sees has gradient 0. Rows at or beyond
+ * the lengths may hold anything, NaN among it. */
+typedef struct SxAttentionView {
+    void* data;           /* [batch, tokens, heads, head_dim], head_dim contiguous */
+    int64_t batch_stride; /* elements */
+    int64_t token_stride;
+    int64_t head_stride;
+} SxAttentionView;
+
+typedef struct SxAttentionInputs {
+    SxAttentionView q;      /* [batch, q_len, q_heads, head_dim] */
+    SxAttentionView k, v;   /* [batch, kv_len, kv_heads, head_dim] */
+    const int32_t* q_lens;  /* [batch] or NULL; values are clamped to 0..q_len */
+    const int32_t* kv_lens; /* [batch] or NULL; values are clamped to 0..kv_len */
+    int64_t batch, q_len, kv_len;
+    int32_t q_heads, kv_heads;
+    int32_t head_dim;       /* 1..128 */
+    int32_t dtype;          /* of q, k, v, out and their gradients */
+    float scale;
+    int32_t causal;
+} SxAttentionInputs;
+
+/* out: like q. lse: [batch, q_heads, q_len] natural log of the sum of exponentials. Workspace
+ * query protocol (the size may be 0; a non-NULL workspace pointer is then not read). */
+int32_t sxcuda_attention_fwd(const SxAttentionInputs* in, const SxAttentionView* out, float* lse,
+                             void* workspace, size_t* workspace_bytes, sxcuda_stream_t stream);
+
+typedef struct SxAttentionGradsIn {
+    SxAttentionView out;   /* of the forward */
+    const float* lse;      /* of the forward */
+    SxAttentionView v_out; /* gradient of out */
+} SxAttentionGradsIn;
+
+typedef struct SxAttentionGrads {
+    SxAttentionView v_q, v_k, v_v; /* every row written; heads that share are summed */
+} SxAttentionGrads;
+
+/* The probabilities are recomputed from q, k and lse. Workspace query protocol. */
+int32_t sxcuda_attention_bwd(const SxAttentionInputs* in, const SxAttentionGradsIn* gin,
+                             const SxAttentionGrads* out, void* workspace,
+                             size_t* workspace_bytes, sxcuda_stream_t stream);
+
+/* Status bits of the attention kernels of the current device since the last call, then cleared:
+ * 1 = a bounded wait inside a kernel ran out and that call's outputs are invalid. Synchronises
+ * the device. */
+int32_t sxcuda_attention_status(uint32_t* status);
+
 #ifdef __cplusplus
 }
 #endif

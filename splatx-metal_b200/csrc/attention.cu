@@ -1,0 +1,402 @@
+// attention.cu — softmax attention, forward and backward, for any element type, head dimension up
+// to 128 and strides, on the CUDA cores in 32 bits. 16-bit inputs whose rows can be copied in
+// 16-byte pieces take the tensor-core kernels (attention_tc.cu).
+//
+// With s = scale q k^T, masked:  p = exp(s - lse), out = p v, lse = log sum exp(s), and for the
+// gradient g of out:  delta = sum(g out), v_v = p^T g, ds = p (g v^T - delta),
+// v_q = scale ds k, v_k = scale ds^T q. No matrix of scores is stored: the forward keeps a running
+// maximum and sum per query while it passes over the keys, the backward recomputes p from lse.
+// The backward is two kernels: one owns a tile of keys and passes over the queries (and over the
+// query heads that share the key-value head), one owns a tile of queries and passes over the keys.
+// That computes s and g v^T twice, and needs neither atomics nor partial sums in memory, so results
+// do not change between calls.
+#include "sx_attention.h"
+
+namespace sx {
+
+__device__ uint32_t g_attention_status;
+
+uint32_t attention_status() {
+    uint32_t st = 0;
+    const uint32_t zero = 0;
+    cuda_check(cudaDeviceSynchronize(), "attention_status");
+    cuda_check(cudaMemcpyFromSymbol(&st, g_attention_status, sizeof(st)), "attention_status");
+    if (st) cuda_check(cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(zero)), "attention_status");
+    return st;
+}
+uint32_t* attention_status_word() {
+    void* p = nullptr;
+    cuda_check(cudaGetSymbolAddress(&p, g_attention_status), "attention_status");
+    return static_cast<uint32_t*>(p);
+}
+
+namespace {
+
+constexpr int kT = 64;        // queries and keys of a tile
+constexpr int kThreads = 256;  // 16 x 16, four rows and four columns of a tile each
+constexpr int kLd = kT + 4;    // padded row of a score tile
+
+__device__ __forceinline__ int tx() { return threadIdx.x & 15; }
+__device__ __forceinline__ int ty() { return threadIdx.x >> 4; }
+__device__ __forceinline__ float sum16(float x) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) x += __shfl_xor_sync(kFullMask, x, o);
+    return x;
+}
+__device__ __forceinline__ float max16(float x) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(kFullMask, x, o));
+    return x;
+}
+
+// kT rows from row `r0` of a head into shared memory [kT][D + 4]; zeros beyond the length and the
+// head dimension.
+template <typename T, int D>
+__device__ __forceinline__ void load_tile(float* s, const SxAttentionView& a, int64_t b, int64_t h, int64_t r0,
+                                          int64_t len, int dim) {
+    const T* p = static_cast<const T*>(a.data) + b * a.batch_stride + h * a.head_stride;
+    for (int i = threadIdx.x; i < kT * D; i += kThreads) {
+        const int r = i / D, c = i % D;
+        s[r * (D + 4) + c] = r0 + r < len && c < dim ? to_f32(p[(r0 + r) * a.token_stride + c]) : 0.f;
+    }
+}
+
+// s[4 rows of ty][4 columns of tx] of A B^T, both [kT][D + 4].
+template <int D>
+__device__ __forceinline__ void dot_tile(float (&s)[4][4], const float* A, const float* B) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[i][j] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < D; c += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(A + (ty() * 4 + i) * (D + 4) + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(B + (tx() + 16 * j) * (D + 4) + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                s[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, s[i][j]))));
+    }
+}
+
+// acc[4 rows of ty][D / 16 columns: 4 tx + 64 k] += P V with P [kT][kLd] (row, key), V [kT][D + 4].
+template <int D>
+__device__ __forceinline__ void add_product(float (&acc)[4][D / 16], const float* P, const float* V) {
+#pragma unroll 4
+    for (int k = 0; k < kT; ++k) {
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = P[(ty() * 4 + i) * kLd + k];
+#pragma unroll
+        for (int n = 0; n < D / 64; ++n) {
+            const float4 v = *reinterpret_cast<const float4*>(V + k * (D + 4) + tx() * 4 + n * 64);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                acc[i][n * 4 + 0] = fmaf(p[i], v.x, acc[i][n * 4 + 0]);
+                acc[i][n * 4 + 1] = fmaf(p[i], v.y, acc[i][n * 4 + 1]);
+                acc[i][n * 4 + 2] = fmaf(p[i], v.z, acc[i][n * 4 + 2]);
+                acc[i][n * 4 + 3] = fmaf(p[i], v.w, acc[i][n * 4 + 3]);
+            }
+        }
+    }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void store_rows(const float (&acc)[4][D / 16], const float (&f)[4], const SxAttentionView& a,
+                                           int64_t b, int64_t h, int64_t r0, int64_t rows, int dim) {
+    T* p = static_cast<T*>(a.data) + b * a.batch_stride + h * a.head_stride;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + ty() * 4 + i;
+        if (r >= rows) continue;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) {
+            const int c = (n >> 2) * 64 + tx() * 4 + (n & 3);
+            if (c < dim) p[r * a.token_stride + c] = from_f32<T>(acc[i][n] * f[i]);
+        }
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attn_fwd_kernel(const AttnArgs a) {
+    extern __shared__ float smem[];
+    float* Q = smem;
+    float* K = Q + kT * (D + 4);
+    float* V = K + kT * (D + 4);
+    float* P = V + kT * (D + 4);
+    const AttnHead w = attn_head(a, blockIdx.y, blockIdx.z);
+    const int64_t q0 = static_cast<int64_t>(blockIdx.x) * kT;
+    const int64_t hk = w.h / a.group;
+    float acc[4][D / 16] = {}, m[4], l[4] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = -INFINITY;
+    load_tile<T, D>(Q, a.q, w.b, w.h, q0, w.q_len, a.dim);
+    const int64_t k_end = attn_keys_end(w, q0 + kT);
+    for (int64_t k0 = 0; k0 < k_end; k0 += kT) {
+        __syncthreads();
+        load_tile<T, D>(K, a.k, w.b, hk, k0, w.kv_len, a.dim);
+        load_tile<T, D>(V, a.v, w.b, hk, k0, w.kv_len, a.dim);
+        __syncthreads();
+        float s[4][4];
+        dot_tile<D>(s, Q, K);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t row = q0 + ty() * 4 + i;
+            float top = m[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[i][j] = attn_sees(w, row, k0 + tx() + 16 * j) ? s[i][j] * a.scale_log2 : -INFINITY;
+                top = fmaxf(top, s[i][j]);
+            }
+            top = max16(top);
+            const float base = top == -INFINITY ? 0.f : top;  // a row that has seen no key yet
+            const float old = exp2f(m[i] - base);
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float p = exp2f(s[i][j] - base);
+                sum += p;
+                P[(ty() * 4 + i) * kLd + tx() + 16 * j] = p;
+            }
+            l[i] = fmaf(l[i], old, sum16(sum));
+            m[i] = top;
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n) acc[i][n] *= old;
+        }
+        __syncthreads();
+        add_product<D>(acc, P, V);
+    }
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = q0 + ty() * 4 + i;
+        f[i] = l[i] > 0.f ? 1.f / l[i] : 0.f;
+        if (tx() == 0 && row < a.q_len)
+            a.lse[(w.b * a.heads + w.h) * a.q_len + row] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+    }
+    store_rows<T, D>(acc, f, a.out, w.b, w.h, q0, a.q_len, a.dim);
+}
+
+// delta = sum(g out) per query, and lse in base 2 with +inf for a query that sees no key (exp2 then
+// gives 0). A warp per query; both arrays have rows of a.q_pad (the tensor-core kernels read whole
+// tiles of them).
+template <typename T>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (i >= a.batch * a.heads * a.q_pad) return;
+    const int64_t row = i % a.q_pad, bh = i / a.q_pad;
+    const AttnHead w = attn_head(a, bh % a.heads, bh / a.heads);
+    const int lane = threadIdx.x & 31;
+    float s = 0.f, lse = INFINITY;
+    if (row < w.q_len) {
+        const T* o = static_cast<const T*>(a.out.data) + w.b * a.out.batch_stride + w.h * a.out.head_stride + row * a.out.token_stride;
+        const T* g = static_cast<const T*>(a.g.data) + w.b * a.g.batch_stride + w.h * a.g.head_stride + row * a.g.token_stride;
+        for (int c = lane; c < a.dim; c += 32) s = fmaf(to_f32(o[c]), to_f32(g[c]), s);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(kFullMask, s, off);
+        const float x = a.lse[bh * a.q_len + row];
+        if (x != -INFINITY) lse = x * kLog2e;
+    }
+    if (lane == 0) {
+        a.delta[i] = s;
+        a.lse2[i] = lse;
+    }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attn_bwd_kv_kernel(const AttnArgs a) {
+    extern __shared__ float smem[];
+    float* K = smem;
+    float* V = K + kT * (D + 4);
+    float* Q = V + kT * (D + 4);
+    float* G = Q + kT * (D + 4);
+    float* P = G + kT * (D + 4);
+    float* S = P + kT * kLd;
+    const int64_t k0 = static_cast<int64_t>(blockIdx.x) * kT, hk = blockIdx.y;
+    float dk[4][D / 16] = {}, dv[4][D / 16] = {};
+    {
+        const AttnHead w = attn_head(a, hk * a.group, blockIdx.z);
+        load_tile<T, D>(K, a.k, w.b, hk, k0, w.kv_len, a.dim);
+        load_tile<T, D>(V, a.v, w.b, hk, k0, w.kv_len, a.dim);
+    }
+    for (int64_t h = hk * a.group; h < (hk + 1) * a.group; ++h) {
+        const AttnHead w = attn_head(a, h, blockIdx.z);
+        const float* lse = a.lse2 + (w.b * a.heads + h) * a.q_pad;
+        const float* delta = a.delta + (w.b * a.heads + h) * a.q_pad;
+        if (k0 >= w.kv_len) break;
+        for (int64_t q0 = attn_queries_begin(w, k0) / kT * kT; q0 < w.q_len; q0 += kT) {
+            __syncthreads();
+            load_tile<T, D>(Q, a.q, w.b, h, q0, w.q_len, a.dim);
+            load_tile<T, D>(G, a.g, w.b, h, q0, w.q_len, a.dim);
+            __syncthreads();
+            float s[4][4], dp[4][4];
+            dot_tile<D>(s, K, Q);
+            dot_tile<D>(dp, V, G);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int64_t row = q0 + tx() + 16 * j;
+                const float x = row < w.q_len ? lse[row] : INFINITY, d = row < w.q_len ? delta[row] : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int64_t key = k0 + ty() * 4 + i;
+                    const bool seen = attn_sees(w, row, key);
+                    const float p = seen ? exp2f(fmaf(s[i][j], a.scale_log2, -x)) : 0.f;
+                    P[(ty() * 4 + i) * kLd + tx() + 16 * j] = p;
+                    S[(ty() * 4 + i) * kLd + tx() + 16 * j] = seen ? p * (dp[i][j] - d) : 0.f;
+                }
+            }
+            __syncthreads();
+            add_product<D>(dv, P, G);
+            add_product<D>(dk, S, Q);
+        }
+    }
+    const float one[4] = {1.f, 1.f, 1.f, 1.f}, sc[4] = {a.scale, a.scale, a.scale, a.scale};
+    store_rows<T, D>(dv, one, a.v_v, blockIdx.z, hk, k0, a.kv_len, a.dim);
+    store_rows<T, D>(dk, sc, a.v_k, blockIdx.z, hk, k0, a.kv_len, a.dim);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) attn_bwd_q_kernel(const AttnArgs a) {
+    extern __shared__ float smem[];
+    float* Q = smem;
+    float* G = Q + kT * (D + 4);
+    float* K = G + kT * (D + 4);
+    float* V = K + kT * (D + 4);
+    float* S = V + kT * (D + 4);
+    const AttnHead w = attn_head(a, blockIdx.y, blockIdx.z);
+    const int64_t q0 = static_cast<int64_t>(blockIdx.x) * kT, hk = w.h / a.group;
+    float dq[4][D / 16] = {}, x[4], d[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t row = q0 + ty() * 4 + i, at = (w.b * a.heads + w.h) * a.q_pad + row;
+        x[i] = row < w.q_len ? a.lse2[at] : INFINITY;
+        d[i] = row < w.q_len ? a.delta[at] : 0.f;
+    }
+    load_tile<T, D>(Q, a.q, w.b, w.h, q0, w.q_len, a.dim);
+    load_tile<T, D>(G, a.g, w.b, w.h, q0, w.q_len, a.dim);
+    const int64_t k_end = attn_keys_end(w, q0 + kT);
+    for (int64_t k0 = 0; k0 < k_end; k0 += kT) {
+        __syncthreads();
+        load_tile<T, D>(K, a.k, w.b, hk, k0, w.kv_len, a.dim);
+        load_tile<T, D>(V, a.v, w.b, hk, k0, w.kv_len, a.dim);
+        __syncthreads();
+        float s[4][4], dp[4][4];
+        dot_tile<D>(s, Q, K);
+        dot_tile<D>(dp, G, V);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool seen = attn_sees(w, q0 + ty() * 4 + i, k0 + tx() + 16 * j);
+                const float p = seen ? exp2f(fmaf(s[i][j], a.scale_log2, -x[i])) : 0.f;
+                S[(ty() * 4 + i) * kLd + tx() + 16 * j] = seen ? p * (dp[i][j] - d[i]) : 0.f;
+            }
+        __syncthreads();
+        add_product<D>(dq, S, K);
+    }
+    const float sc[4] = {a.scale, a.scale, a.scale, a.scale};
+    store_rows<T, D>(dq, sc, a.v_q, w.b, w.h, q0, a.q_len, a.dim);
+}
+
+int tile_bytes(int D, int tiles, int scores) {
+    return (tiles * kT * (D + 4) + scores * kT * kLd) * static_cast<int>(sizeof(float));
+}
+
+template <typename F>
+void by_dim(int dim, F&& f) {
+    if (dim <= 64) f(std::integral_constant<int, 64>{});
+    else f(std::integral_constant<int, 128>{});
+}
+
+dim3 tiles_of(const AttnArgs& a, int64_t len, int64_t heads) {
+    return dim3(static_cast<unsigned>((len + kT - 1) / kT), static_cast<unsigned>(heads), static_cast<unsigned>(a.batch));
+}
+
+}  // namespace
+
+AttnArgs attn_args(const SxAttentionInputs& in) {
+    AttnArgs a{};
+    a.q = in.q;
+    a.k = in.k;
+    a.v = in.v;
+    a.q_lens = in.q_lens;
+    a.kv_lens = in.kv_lens;
+    a.batch = in.batch;
+    a.q_len = in.q_len;
+    a.kv_len = in.kv_len;
+    a.q_pad = (in.q_len + 127) / 128 * 128;
+    a.heads = in.q_heads;
+    a.kv_heads = in.kv_heads;
+    a.group = in.kv_heads ? in.q_heads / in.kv_heads : 1;
+    a.dim = in.head_dim;
+    a.dtype = in.dtype;
+    a.causal = in.causal != 0;
+    a.scale = in.scale;
+    a.scale_log2 = static_cast<float>(static_cast<double>(in.scale) * 1.4426950408889634);
+    return a;
+}
+
+size_t attention_fwd_workspace(const SxAttentionInputs&) { return 0; }
+
+void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& out, float* lse, void*, cudaStream_t s) {
+    AttnArgs a = attn_args(in);
+    a.out = out;
+    a.lse = lse;
+    if (a.batch == 0 || a.q_len == 0 || a.heads == 0) return;
+    by_dtype(a.dtype, [&](auto t) {
+        by_dim(a.dim, [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            const auto kernel = attn_fwd_kernel<decltype(t), D>;
+            const int smem = tile_bytes(D, 3, 1);
+            smem_limit_once(reinterpret_cast<const void*>(kernel), smem, "attention_fwd");
+            SX_LAUNCH(kernel, tiles_of(a, a.q_len, a.heads), kThreads, smem, s, a);
+        });
+    });
+}
+
+size_t attention_bwd_workspace(const SxAttentionInputs& in) {
+    const AttnArgs a = attn_args(in);
+    return static_cast<size_t>(2 * a.batch * a.heads * a.q_pad) * sizeof(float);
+}
+
+void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn& g, const SxAttentionGrads& out,
+                          void* ws, cudaStream_t s) {
+    AttnArgs a = attn_args(in);
+    a.out = g.out;
+    a.g = g.v_out;
+    a.v_q = out.v_q;
+    a.v_k = out.v_k;
+    a.v_v = out.v_v;
+    a.lse = const_cast<float*>(g.lse);
+    a.lse2 = static_cast<float*>(ws);
+    a.delta = a.lse2 + a.batch * a.heads * a.q_pad;
+    if (a.batch == 0 || a.heads == 0) return;
+    by_dtype(a.dtype, [&](auto t) {
+        using T = decltype(t);
+        if (a.q_len) {
+            const auto delta = attn_delta_kernel<T>;
+            SX_LAUNCH(delta, blocks_for(a.batch * a.heads * a.q_pad, 8), 256, 0, s, a);
+        }
+        by_dim(a.dim, [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            if (a.kv_len) {
+                const auto kernel = attn_bwd_kv_kernel<T, D>;
+                const int smem = tile_bytes(D, 4, 2);
+                smem_limit_once(reinterpret_cast<const void*>(kernel), smem, "attention_bwd");
+                SX_LAUNCH(kernel, tiles_of(a, a.kv_len, a.kv_heads), kThreads, smem, s, a);
+            }
+            if (a.q_len) {
+                const auto kernel = attn_bwd_q_kernel<T, D>;
+                const int smem = tile_bytes(D, 4, 1);
+                smem_limit_once(reinterpret_cast<const void*>(kernel), smem, "attention_bwd");
+                SX_LAUNCH(kernel, tiles_of(a, a.q_len, a.heads), kThreads, smem, s, a);
+            }
+        });
+    });
+}
+
+}  // namespace sx

@@ -18,6 +18,7 @@
 #include "../../include/splatx_cuda.h"
 #include "sx_common.cuh"
 #include "sx_internal.h"
+#include "sx_network.h"
 
 namespace sx {
 
@@ -167,6 +168,88 @@ void validate_isect(const SxIsectTilesInputs* in, const char* w) {
     const uint32_t tb = bits_for_count(static_cast<int64_t>(in->tile_width) * in->tile_height);
     if (bits_for_count(in->I) + tb > 32) throw_invalid(w, "image_n_bits + tile_n_bits must be <= 32");
     if (in->N > 0 && in->I > INT32_MAX / in->N) throw_invalid(w, "I*N must fit in int32 (flatten_ids)");
+}
+
+// ---- network operators ----
+void validate_dtype(int32_t dtype, const char* w, const char* what) {
+    if (dtype != SXCUDA_F32 && dtype != SXCUDA_F16 && dtype != SXCUDA_BF16)
+        throw_invalid(w, std::string(what) + " must be SXCUDA_F32, SXCUDA_F16 or SXCUDA_BF16");
+}
+void validate_pointer(const void* p, int32_t dtype, const char* w, const char* what) {
+    if (!p) throw_invalid(w, std::string("null ") + what);
+    if (reinterpret_cast<uintptr_t>(p) % dtype_bytes(dtype) != 0)
+        throw_invalid(w, std::string(what) + " is not aligned to its element");
+}
+void validate_rows(const void* p, int64_t stride, const SxLayerNormInputs& in, const char* w, const char* what) {
+    if (in.rows == 0) return;
+    validate_pointer(p, in.dtype, w, what);
+    if (in.rows > 1 && stride < in.cols) throw_invalid(w, std::string(what) + ": rows overlap (stride < cols)");
+}
+void validate_layer_norm(const SxLayerNormInputs* in, const char* w) {
+    if (!in) throw_invalid(w, "null inputs");
+    validate_dtype(in->dtype, w, "dtype");
+    validate_dtype(in->param_dtype, w, "param_dtype");
+    if (in->rows < 0) throw_invalid(w, "negative rows");
+    if (in->cols < 1 || in->cols > INT32_MAX / 2) throw_invalid(w, "cols must be 1..2^30 - 1");
+    if (!(in->eps >= 0.0f) || !std::isfinite(in->eps)) throw_invalid(w, "eps must be finite and not negative");
+    validate_rows(in->x, in->x_stride, *in, w, "x");
+    if (in->weight) validate_pointer(in->weight, in->param_dtype, w, "weight");
+    if (in->bias) validate_pointer(in->bias, in->param_dtype, w, "bias");
+}
+
+void validate_adamw(const SxAdamwTensor* t, int64_t n, const SxAdamwConfig* c, const char* w) {
+    if (!c) throw_invalid(w, "null config");
+    if (n < 0) throw_invalid(w, "negative n_tensors");
+    if (n > 0 && !t) throw_invalid(w, "null tensors");
+    if (c->state_bits != 32 && c->state_bits != 8) throw_invalid(w, "state_bits must be 32 or 8");
+    if (c->step < 1) throw_invalid(w, "step counts from 1");
+    if (!(c->b1 >= 0.0 && c->b1 < 1.0) || !(c->b2 >= 0.0 && c->b2 < 1.0))
+        throw_invalid(w, "b1 and b2 must be in [0, 1)");
+    if (!(c->eps >= 0.0) || !std::isfinite(c->eps)) throw_invalid(w, "eps must be finite and not negative");
+    if (!std::isfinite(c->grad_scale)) throw_invalid(w, "grad_scale must be finite");
+    for (int64_t i = 0; i < n; ++i) {
+        if (t[i].n < 0) throw_invalid(w, "negative n");
+        validate_dtype(t[i].param_dtype, w, "param_dtype");
+        validate_dtype(t[i].grad_dtype, w, "grad_dtype");
+        if (!std::isfinite(t[i].lr) || !std::isfinite(t[i].weight_decay))
+            throw_invalid(w, "lr and weight_decay must be finite");
+        if (t[i].n == 0) continue;
+        validate_pointer(t[i].param, t[i].param_dtype, w, "param");
+        validate_pointer(t[i].grad, t[i].grad_dtype, w, "grad");
+        if (c->state_bits == 32) {
+            validate_pointer(t[i].exp_avg, SXCUDA_F32, w, "exp_avg");
+            validate_pointer(t[i].exp_avg_sq, SXCUDA_F32, w, "exp_avg_sq");
+        } else {
+            if (!t[i].exp_avg || !t[i].exp_avg_sq) throw_invalid(w, "null exp_avg/exp_avg_sq");
+            validate_pointer(t[i].exp_avg_scale, SXCUDA_F32, w, "exp_avg_scale");
+            validate_pointer(t[i].exp_avg_sq_scale, SXCUDA_F32, w, "exp_avg_sq_scale");
+        }
+    }
+}
+
+void validate_view(const SxAttentionView& v, const SxAttentionInputs& in, int64_t tokens, int64_t heads, bool written,
+                   const char* w, const char* what) {
+    if (in.batch == 0 || tokens == 0) return;
+    validate_pointer(v.data, in.dtype, w, what);
+    if (v.batch_stride < 0 || v.token_stride < 0 || v.head_stride < 0)
+        throw_invalid(w, std::string(what) + ": negative stride");
+    if (written && ((in.batch > 1 && v.batch_stride == 0) || (tokens > 1 && v.token_stride < in.head_dim) ||
+                    (heads > 1 && v.head_stride < in.head_dim)))
+        throw_invalid(w, std::string(what) + ": rows that are written overlap");
+}
+void validate_attention(const SxAttentionInputs* in, const char* w) {
+    if (!in) throw_invalid(w, "null inputs");
+    validate_dtype(in->dtype, w, "dtype");
+    if (in->batch < 0 || in->q_len < 0 || in->kv_len < 0) throw_invalid(w, "negative batch, q_len or kv_len");
+    if (in->batch > 65535 || in->q_heads > 65535) throw_invalid(w, "batch and q_heads must be at most 65535");
+    if (in->q_len > INT32_MAX / 2 || in->kv_len > INT32_MAX / 2) throw_invalid(w, "q_len and kv_len must be below 2^30");
+    if (in->kv_heads < 1 || in->q_heads < 1 || in->q_heads % in->kv_heads != 0)
+        throw_invalid(w, "q_heads must be a positive multiple of kv_heads");
+    if (in->head_dim < 1 || in->head_dim > 128) throw_invalid(w, "head_dim must be 1..128");
+    if (!std::isfinite(in->scale)) throw_invalid(w, "scale must be finite");
+    validate_view(in->q, *in, in->q_len, in->q_heads, false, w, "q");
+    validate_view(in->k, *in, in->kv_len, in->kv_heads, false, w, "k");
+    validate_view(in->v, *in, in->kv_len, in->kv_heads, false, w, "v");
 }
 
 void validate_raster(const SxRasterizeFwdInputs* in, const char* w) {
@@ -973,6 +1056,80 @@ int32_t sxcuda_ssim_bwd(const SxSsimInputs* in, const SxSsimGradsIn* g, float* v
     });
 }
 
+
+// ---- network operators ----
+int32_t sxcuda_layer_norm_fwd(const SxLayerNormInputs* in, void* y, int64_t y_stride, float* mean, float* rstd,
+                              sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "layer_norm_fwd";
+        validate_layer_norm(in, w);
+        validate_rows(y, y_stride, *in, w, "y");
+        if ((mean == nullptr) != (rstd == nullptr)) throw_invalid(w, "mean and rstd must be given together");
+        launch_layer_norm_fwd(*in, y, y_stride, mean, rstd, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_layer_norm_bwd(const SxLayerNormInputs* in, const SxLayerNormGradsIn* g, const SxLayerNormGrads* out,
+                              void* ws, size_t* ws_bytes, sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "layer_norm_bwd";
+        validate_layer_norm(in, w);
+        if (workspace_query(ws, ws_bytes, layer_norm_bwd_workspace(*in), w)) return;
+        if (!g || !out) throw_invalid(w, "null gradients");
+        if (in->rows && (!g->mean || !g->rstd)) throw_invalid(w, "null mean/rstd");
+        validate_rows(g->v_y, g->v_y_stride, *in, w, "v_y");
+        validate_rows(out->v_x, out->v_x_stride, *in, w, "v_x");
+        if (out->v_weight) validate_pointer(out->v_weight, in->param_dtype, w, "v_weight");
+        if (out->v_bias) validate_pointer(out->v_bias, in->param_dtype, w, "v_bias");
+        validate_pointer(ws, SXCUDA_F32, w, "workspace");
+        launch_layer_norm_bwd(*in, *g, *out, ws, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_adamw_step(const SxAdamwTensor* tensors, int64_t n, const SxAdamwConfig* cfg, sxcuda_stream_t stream) {
+    return guarded([&] {
+        validate_adamw(tensors, n, cfg, "adamw_step");
+        launch_adamw(tensors, n, *cfg, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_attention_fwd(const SxAttentionInputs* in, const SxAttentionView* out, float* lse, void* ws,
+                             size_t* ws_bytes, sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "attention_fwd";
+        validate_attention(in, w);
+        if (workspace_query(ws, ws_bytes, attention_fwd_workspace(*in), w)) return;
+        if (!out) throw_invalid(w, "null out");
+        validate_view(*out, *in, in->q_len, in->q_heads, true, w, "out");
+        if (in->batch && in->q_len) validate_pointer(lse, SXCUDA_F32, w, "lse");
+        launch_attention_fwd(*in, *out, lse, ws, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_attention_bwd(const SxAttentionInputs* in, const SxAttentionGradsIn* g, const SxAttentionGrads* out,
+                             void* ws, size_t* ws_bytes, sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "attention_bwd";
+        validate_attention(in, w);
+        if (workspace_query(ws, ws_bytes, attention_bwd_workspace(*in), w)) return;
+        if (!g || !out) throw_invalid(w, "null gradients");
+        validate_view(g->out, *in, in->q_len, in->q_heads, false, w, "out");
+        validate_view(g->v_out, *in, in->q_len, in->q_heads, false, w, "v_out");
+        if (in->batch && in->q_len) validate_pointer(g->lse, SXCUDA_F32, w, "lse");
+        validate_view(out->v_q, *in, in->q_len, in->q_heads, true, w, "v_q");
+        validate_view(out->v_k, *in, in->kv_len, in->kv_heads, true, w, "v_k");
+        validate_view(out->v_v, *in, in->kv_len, in->kv_heads, true, w, "v_v");
+        if (reinterpret_cast<uintptr_t>(ws) % 16 != 0) throw_invalid(w, "workspace must be 16-byte aligned");
+        launch_attention_bwd(*in, *g, *out, ws, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_attention_status(uint32_t* status) {
+    return guarded([&] {
+        if (!status) throw_invalid("attention_status", "null status");
+        *status = attention_status();
+    });
+}
 
 // ---- render session (sx_render_session_*, TrainC.cpp:1440-1584) ----------------------------
 struct SxRenderSession {

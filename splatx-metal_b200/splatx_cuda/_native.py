@@ -197,6 +197,53 @@ class SxSsimGradsIn(C.Structure):
     _fields_ = [("coeff_mu", vp), ("coeff_sigma", vp), ("coeff_cross", vp), ("v_loss", C.c_float)]
 
 
+class SxLayerNormInputs(C.Structure):
+    _fields_ = [("x", vp), ("weight", vp), ("bias", vp), ("rows", C.c_int64), ("cols", C.c_int64),
+                ("x_stride", C.c_int64), ("dtype", C.c_int32), ("param_dtype", C.c_int32),
+                ("eps", C.c_float)]
+
+
+class SxLayerNormGradsIn(C.Structure):
+    _fields_ = [("mean", vp), ("rstd", vp), ("v_y", vp), ("v_y_stride", C.c_int64)]
+
+
+class SxLayerNormGrads(C.Structure):
+    _fields_ = [("v_x", vp), ("v_x_stride", C.c_int64), ("v_weight", vp), ("v_bias", vp)]
+
+
+class SxAdamwTensor(C.Structure):
+    _fields_ = [("param", vp), ("grad", vp), ("exp_avg", vp), ("exp_avg_sq", vp),
+                ("exp_avg_scale", vp), ("exp_avg_sq_scale", vp), ("n", C.c_int64),
+                ("lr", C.c_double), ("weight_decay", C.c_double), ("param_dtype", C.c_int32),
+                ("grad_dtype", C.c_int32)]
+
+
+class SxAdamwConfig(C.Structure):
+    _fields_ = [("b1", C.c_double), ("b2", C.c_double), ("eps", C.c_double),
+                ("grad_scale", C.c_double), ("step", C.c_int64), ("state_bits", C.c_int32)]
+
+
+class SxAttentionView(C.Structure):
+    _fields_ = [("data", vp), ("batch_stride", C.c_int64), ("token_stride", C.c_int64),
+                ("head_stride", C.c_int64)]
+
+
+class SxAttentionInputs(C.Structure):
+    _fields_ = [("q", SxAttentionView), ("k", SxAttentionView), ("v", SxAttentionView),
+                ("q_lens", vp), ("kv_lens", vp), ("batch", C.c_int64), ("q_len", C.c_int64),
+                ("kv_len", C.c_int64), ("q_heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float),
+                ("causal", C.c_int32)]
+
+
+class SxAttentionGradsIn(C.Structure):
+    _fields_ = [("out", SxAttentionView), ("lse", vp), ("v_out", SxAttentionView)]
+
+
+class SxAttentionGrads(C.Structure):
+    _fields_ = [("v_q", SxAttentionView), ("v_k", SxAttentionView), ("v_v", SxAttentionView)]
+
+
 P = C.POINTER
 _SIGNATURES = {
     "sxcuda_last_error": (C.c_char_p, []),
@@ -292,6 +339,15 @@ _SIGNATURES = {
     "sxcuda_mcmc_perturb_positions": (C.c_int32, [P(SxPerturbInputs), vp]),
     "sxcuda_ssim_fwd": (C.c_int32, [P(SxSsimInputs), vp, vp, vp, vp, vp, vp, c_size_p, vp]),
     "sxcuda_ssim_bwd": (C.c_int32, [P(SxSsimInputs), P(SxSsimGradsIn), vp, vp]),
+    "sxcuda_layer_norm_fwd": (C.c_int32, [P(SxLayerNormInputs), vp, C.c_int64, vp, vp, vp]),
+    "sxcuda_layer_norm_bwd": (C.c_int32, [P(SxLayerNormInputs), P(SxLayerNormGradsIn),
+                                          P(SxLayerNormGrads), vp, c_size_p, vp]),
+    "sxcuda_adamw_step": (C.c_int32, [vp, C.c_int64, P(SxAdamwConfig), vp]),
+    "sxcuda_attention_fwd": (C.c_int32, [P(SxAttentionInputs), P(SxAttentionView), vp, vp,
+                                         c_size_p, vp]),
+    "sxcuda_attention_bwd": (C.c_int32, [P(SxAttentionInputs), P(SxAttentionGradsIn),
+                                         P(SxAttentionGrads), vp, c_size_p, vp]),
+    "sxcuda_attention_status": (C.c_int32, [c_uint32_p]),
 }
 
 _lib = None

@@ -1,0 +1,385 @@
+"""Operators for training a network beside the splats: attention, layer norm, AdamW.
+
+The reference has no counterpart: its trainer updates the Gaussians themselves. A network that
+predicts, refines or conditions them (tokens of splats or of image patches) trains with these.
+Inputs are CUDA tensors and stay where they are; every call enqueues on the current stream of the
+tensors' device, allocates its results (and a workspace, where it needs one) from torch and does
+not synchronise. Contract violations raise ``ValueError``, device failures ``RuntimeError``.
+
+    out, lse = attention_fwd(q, k, v, causal=True)           # [batch, tokens, heads, head_dim]
+    v_q, v_k, v_v = attention_bwd(v_out, q, k, v, out, lse, causal=True)
+    y, mean, rstd = layer_norm_fwd(x, weight, bias)
+    v_x, v_weight, v_bias = layer_norm_bwd(v_y, x, weight, mean, rstd)
+    AdamW(params, lr=1e-3, state_bits=8).step()              # params with .grad, or step(grads)
+
+``attention`` and ``layer_norm`` are the same with torch's autograd.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+import torch
+
+from . import _native as _nat
+from ._native import check
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+RUN = 256  # consecutive values of an 8-bit moment that share a scale
+
+
+def _dtype(t: torch.Tensor, what: str) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what}: float32, float16 or bfloat16 needed, got {t.dtype}")
+    return code
+
+
+def _on(first: torch.Tensor, what: str, **others) -> torch.device:
+    """The CUDA device that all of the call's tensors are on."""
+    if not first.is_cuda:
+        raise ValueError(f"{what}: CUDA tensors needed (there is no CPU path)")
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{what}: {name} is on {t.device}, not on {first.device}")
+    return first.device
+
+
+class _at:
+    """The device made current for one call (left alone where it is already) and its stream."""
+
+    def __init__(self, device):
+        self.index = device.index
+        self.other = torch.cuda.current_device() != self.index
+
+    def __enter__(self):
+        if self.other:
+            self.was = torch.cuda.current_device()
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self.other:
+            torch.cuda.set_device(self.was)
+        return False
+
+
+def attention_status() -> int:
+    """Status bits the attention kernels of the current device have set since the last call (0: all
+    is well; 1: a bounded wait inside a kernel ran out and its outputs are invalid). Synchronises."""
+    st = C.c_uint32(0)
+    check(_nat.lib().sxcuda_attention_status(C.byref(st)))
+    return int(st.value)
+
+
+# ---------------------------------------------------------------- attention
+
+def _view(t: torch.Tensor) -> _nat.SxAttentionView:
+    s = t.stride()
+    return _nat.SxAttentionView(t.data_ptr(), s[0], s[1], s[2])
+
+
+def _heads_last(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.dim() != 4:
+        raise ValueError(f"{what}: [batch, tokens, heads, head_dim] needed, got {tuple(t.shape)}")
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def _attention_inputs(what, q, k, v, scale, causal, q_lens, kv_lens):
+    q, k, v = _heads_last(q, what), _heads_last(k, what), _heads_last(v, what)
+    code = _dtype(q, what)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{what}: q, k and v must have one dtype")
+    b, n, h, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"{what}: k and v must both be [{b}, tokens, heads, {d}], got "
+                         f"{tuple(k.shape)} and {tuple(v.shape)}")
+    device = _on(q, what, k=k, v=v, q_lens=q_lens, kv_lens=kv_lens)
+    for name, lens in (("q_lens", q_lens), ("kv_lens", kv_lens)):
+        if lens is not None and (lens.dtype != torch.int32 or lens.shape != (b,) or
+                                 not lens.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of [{b}]")
+    ins = _nat.SxAttentionInputs(
+        _view(q), _view(k), _view(v), None if q_lens is None else q_lens.data_ptr(),
+        None if kv_lens is None else kv_lens.data_ptr(), b, n, k.shape[1], h, k.shape[2], d, code,
+        (1.0 / math.sqrt(d) if d else 1.0) if scale is None else float(scale), int(bool(causal)))
+    return q, k, v, ins, device
+
+
+def _workspace(nbytes: int, device) -> torch.Tensor | None:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def attention_fwd(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=None):
+    """softmax(scale q k^T) v per head: (out like q, lse [batch, heads, tokens] in float32).
+
+    q: [batch, q_len, heads, head_dim]; k, v: [batch, kv_len, kv_heads, head_dim] with heads a
+    multiple of kv_heads; float32, float16 or bfloat16, head_dim 1..128, any strides with the last
+    axis contiguous. scale defaults to 1 / sqrt(head_dim). q_lens, kv_lens: int32 [batch] token
+    counts of a padded batch; what lies beyond them is not used. causal: query i sees key j where
+    j <= i + kv_len - q_len (the lengths of its batch entry). A query that sees no key gets output 0
+    and log-sum -inf."""
+    q, k, v, ins, device = _attention_inputs("attention_fwd", q, k, v, scale, causal, q_lens, kv_lens)
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=device)
+    ov, nbytes, L = _view(out), C.c_size_t(0), _nat.lib()
+    with _at(device) as stream:
+        check(L.sxcuda_attention_fwd(C.byref(ins), C.byref(ov), lse.data_ptr(), None,
+                                     C.byref(nbytes), stream))
+        ws = _workspace(max(nbytes.value, 1), device)
+        check(L.sxcuda_attention_fwd(C.byref(ins), C.byref(ov), lse.data_ptr(), ws.data_ptr(),
+                                     C.byref(nbytes), stream))
+    return out, lse
+
+
+def attention_bwd(v_out, q, k, v, out, lse, *, scale=None, causal=False, q_lens=None, kv_lens=None):
+    """Gradients (v_q, v_k, v_v) of attention_fwd for the gradient v_out of its output; out and lse
+    are the forward's. Deterministic."""
+    what = "attention_bwd"
+    q, k, v, ins, device = _attention_inputs(what, q, k, v, scale, causal, q_lens, kv_lens)
+    for name, t in (("v_out", v_out), ("out", out)):
+        if t.shape != q.shape or t.dtype != q.dtype:
+            raise ValueError(f"{what}: {name} must be like q")
+    if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32 or \
+            not lse.is_contiguous():
+        raise ValueError(f"{what}: lse must be a contiguous float32 tensor of [batch, heads, tokens]")
+    _on(q, what, v_out=v_out, out=out, lse=lse)
+    v_out, out = _heads_last(v_out, what), _heads_last(out, what)
+    gin = _nat.SxAttentionGradsIn(_view(out), lse.data_ptr(), _view(v_out))
+    grads = [torch.empty(t.shape, dtype=q.dtype, device=device) for t in (q, k, v)]
+    gout = _nat.SxAttentionGrads(*(_view(t) for t in grads))
+    nbytes, L = C.c_size_t(0), _nat.lib()
+    with _at(device) as stream:
+        check(L.sxcuda_attention_bwd(C.byref(ins), None, None, None, C.byref(nbytes), stream))
+        ws = _workspace(max(nbytes.value, 1), device)
+        check(L.sxcuda_attention_bwd(C.byref(ins), C.byref(gin), C.byref(gout), ws.data_ptr(),
+                                     C.byref(nbytes), stream))
+    return tuple(grads)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, causal, q_lens, kv_lens):
+        out, lse = attention_fwd(q, k, v, scale=scale, causal=causal, q_lens=q_lens, kv_lens=kv_lens)
+        ctx.save_for_backward(q, k, v, out, lse, q_lens, kv_lens)
+        ctx.how = {"scale": scale, "causal": causal}
+        return out
+
+    @staticmethod
+    def backward(ctx, v_out):
+        q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
+        grads = attention_bwd(v_out, q, k, v, out, lse, q_lens=q_lens, kv_lens=kv_lens, **ctx.how)
+        return (*grads, None, None, None, None)
+
+
+def attention(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=None):
+    """attention_fwd's output, differentiable in q, k and v."""
+    return _Attention.apply(q, k, v, scale, causal, q_lens, kv_lens)
+
+
+# ---------------------------------------------------------------- layer norm
+
+def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
+    t = t.reshape(-1, cols) if cols else t
+    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= cols) else t.contiguous()
+
+
+def _norm_inputs(what, x, weight, bias, eps):
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError(f"{what}: x needs a last axis of at least 1, got {tuple(x.shape)}")
+    cols = x.shape[-1]
+    device = _on(x, what, weight=weight, bias=bias)
+    params = [p for p in (weight, bias) if p is not None]
+    for p in params:
+        if p.shape != (cols,) or not p.is_contiguous() or p.dtype != params[0].dtype:
+            raise ValueError(f"{what}: weight and bias must be contiguous tensors of [{cols}] with "
+                             "one dtype")
+    rows = _rows(x, cols)
+    ins = _nat.SxLayerNormInputs(
+        rows.data_ptr(), None if weight is None else weight.data_ptr(),
+        None if bias is None else bias.data_ptr(), rows.shape[0], cols, rows.stride(0),
+        _dtype(x, what), _dtype(params[0], what) if params else _DTYPES[torch.float32], float(eps))
+    return rows, ins, device
+
+
+def layer_norm_fwd(x, weight=None, bias=None, *, eps=1e-5):
+    """Layer norm over the last axis: (y like x, mean, rstd of x.shape[:-1] in float32). weight and
+    bias (each may be None: ones, zeros) have one dtype, which need not be x's."""
+    rows, ins, device = _norm_inputs("layer_norm_fwd", x, weight, bias, eps)
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+    rstd = torch.empty_like(mean)
+    with _at(device) as stream:
+        check(_nat.lib().sxcuda_layer_norm_fwd(C.byref(ins), y.data_ptr(), x.shape[-1],
+                                               mean.data_ptr(), rstd.data_ptr(), stream))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(v_y, x, weight, mean, rstd):
+    """Gradients (v_x, v_weight, v_bias) of layer_norm_fwd; the weights' have the weight's dtype
+    (float32 where weight is None). mean and rstd are the forward's. Deterministic."""
+    what = "layer_norm_bwd"
+    rows, ins, device = _norm_inputs(what, x, weight, None, 0.0)
+    cols = x.shape[-1]
+    if v_y.shape != x.shape or v_y.dtype != x.dtype:
+        raise ValueError(f"{what}: v_y must be like x")
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.shape != x.shape[:-1] or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{what}: {name} must be a contiguous float32 tensor of "
+                             f"{tuple(x.shape[:-1])}")
+    _on(x, what, v_y=v_y, mean=mean, rstd=rstd)
+    g = _rows(v_y, cols)
+    v_x = torch.empty(x.shape, dtype=x.dtype, device=device)
+    v_w = torch.empty(cols, dtype=torch.float32 if weight is None else weight.dtype, device=device)
+    v_b = torch.empty_like(v_w)
+    gin = _nat.SxLayerNormGradsIn(mean.data_ptr(), rstd.data_ptr(), g.data_ptr(), g.stride(0))
+    out = _nat.SxLayerNormGrads(v_x.data_ptr(), cols, v_w.data_ptr(), v_b.data_ptr())
+    nbytes, L = C.c_size_t(0), _nat.lib()
+    with _at(device) as stream:
+        check(L.sxcuda_layer_norm_bwd(C.byref(ins), None, None, None, C.byref(nbytes), stream))
+        ws = _workspace(nbytes.value, device)
+        check(L.sxcuda_layer_norm_bwd(C.byref(ins), C.byref(gin), C.byref(out), ws.data_ptr(),
+                                      C.byref(nbytes), stream))
+    return v_x, v_w, v_b
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = layer_norm_fwd(x, weight, bias, eps=eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias = bias is not None
+        return y
+
+    @staticmethod
+    def backward(ctx, v_y):
+        x, weight, mean, rstd = ctx.saved_tensors
+        v_x, v_w, v_b = layer_norm_bwd(v_y, x, weight, mean, rstd)
+        return v_x, None if weight is None else v_w, v_b if ctx.bias else None, None
+
+
+def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
+    """layer_norm_fwd's y, differentiable in x, weight and bias."""
+    return _LayerNorm.apply(x, weight, bias, float(eps))
+
+
+# ---------------------------------------------------------------- AdamW
+
+_TENSOR = np.dtype(_nat.SxAdamwTensor)
+
+
+class AdamW:
+    """AdamW (decoupled weight decay, bias correction) over all parameters in one launch.
+
+    params: tensors, or dicts {"params": [...], "lr": ..., "weight_decay": ...} for groups with a
+    rate or decay of their own. They must be contiguous CUDA tensors of one device. Moments are held
+    in 32 bits, or with state_bits=8 as e4m3 codes of m and of sqrt(v) with a float32 scale for
+    every 256 values (4.03 bytes less per value and moment pair than 8).
+
+    state: moments to go on from, {"exp_avg": [...], "exp_avg_sq": [...], "step": n} and, with 8
+    bits, "exp_avg_scale" and "exp_avg_sq_scale", one tensor per parameter in order; the tensors are
+    used and updated in place. ``state()`` returns them."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
+                 state_bits=32, state=None):
+        what = "AdamW"
+        if state_bits not in (8, 32):
+            raise ValueError(f"{what}: state_bits must be 8 or 32")
+        params = list(params)
+        groups = params if params and isinstance(params[0], dict) else [{"params": params}]
+        self.params, rates, decays = [], [], []
+        for g in groups:
+            mine = list(g["params"])
+            self.params += mine
+            rates += [float(g.get("lr", lr))] * len(mine)
+            decays += [float(g.get("weight_decay", weight_decay))] * len(mine)
+        if not self.params:
+            raise ValueError(f"{what}: no parameters")
+        self.device = _on(self.params[0], what)
+        for p in self.params:
+            _dtype(p, what)
+            _on(self.params[0], what, parameter=p)
+            if not p.is_contiguous():
+                raise ValueError(f"{what}: parameters must be contiguous")
+        self.bits = state_bits
+        self._cfg = _nat.SxAdamwConfig(float(betas[0]), float(betas[1]), float(eps), 1.0, 0,
+                                       state_bits)
+        self._state = self._bind(what, state)
+        n = len(self.params)
+        self._table = np.zeros(n, dtype=_TENSOR)
+        self._table["param"] = [p.data_ptr() for p in self.params]
+        self._table["n"] = [p.numel() for p in self.params]
+        self._table["param_dtype"] = [_DTYPES[p.dtype] for p in self.params]
+        self._table["lr"], self._table["weight_decay"] = rates, decays
+        for key, tensors in self._state.items():
+            self._table[key] = [t.data_ptr() for t in tensors]
+
+    def _bind(self, what, state):
+        eight = self.bits == 8
+        kinds = {"exp_avg": torch.float8_e4m3fn if eight else torch.float32}
+        kinds["exp_avg_sq"] = kinds["exp_avg"]
+        if eight:
+            kinds["exp_avg_scale"] = kinds["exp_avg_sq_scale"] = torch.float32
+        if state is not None and set(state) != {*kinds, "step"}:
+            raise ValueError(f"{what}: state needs {sorted({*kinds, 'step'})}")
+        self._cfg.step = 0 if state is None else int(state["step"])
+        if self._cfg.step < 0:
+            raise ValueError(f"{what}: negative step")
+        mine = {}
+        for key, dtype in kinds.items():
+            sizes = [-(-p.numel() // RUN) if key.endswith("scale") else p.numel()
+                     for p in self.params]
+            if state is None:
+                mine[key] = [torch.zeros(n, dtype=dtype, device=self.device) for n in sizes]
+                continue
+            mine[key] = list(state[key])
+            if len(mine[key]) != len(sizes):
+                raise ValueError(f"{what}: {key} needs {len(sizes)} tensors")
+            for t, n in zip(mine[key], sizes):
+                if t.dtype != dtype or t.numel() != n or not t.is_contiguous() or \
+                        t.device != self.device:
+                    raise ValueError(f"{what}: {key} needs contiguous {dtype} tensors of the "
+                                     "parameters' sizes and device")
+        return mine
+
+    def state(self) -> dict:
+        """The moments and the number of steps taken, as the constructor takes them."""
+        return {**self._state, "step": int(self._cfg.step)}
+
+    def set_lr(self, lr):
+        """The learning rate of the next steps: a number, or one per parameter."""
+        self._table["lr"] = lr
+
+    def step(self, grads=None, *, grad_scale=1.0):
+        """One step on `grads` (one per parameter) or on the parameters' .grad; parameters whose
+        gradient is None stay as they are. grad_scale multiplies every gradient."""
+        what = "AdamW.step"
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        if len(grads) != len(self.params):
+            raise ValueError(f"{what}: {len(self.params)} gradients needed, got {len(grads)}")
+        device, pointers, types = self.device, [], []
+        for p, g in zip(self.params, grads):
+            if g is None:
+                pointers.append(0)
+                types.append(0)
+                continue
+            if g.shape != p.shape or g.device != device or not g.is_contiguous() or \
+                    g.dtype not in _DTYPES:
+                raise ValueError(f"{what}: a gradient must be a contiguous tensor like its "
+                                 f"parameter, got {tuple(g.shape)} {g.dtype} on {g.device}")
+            pointers.append(g.data_ptr())
+            types.append(_DTYPES[g.dtype])
+        table = self._table
+        table["grad"], table["grad_dtype"] = pointers, types
+        if any(g is None for g in grads):
+            table = np.ascontiguousarray(table[table["grad"] != 0])
+        self._cfg.grad_scale = float(grad_scale)
+        self._cfg.step += 1
+        try:
+            with _at(device) as stream:
+                check(_nat.lib().sxcuda_adamw_step(table.ctypes.data, len(table),
+                                                   C.byref(self._cfg), stream))
+        except Exception:
+            self._cfg.step -= 1
+            raise
