@@ -14,22 +14,6 @@
 
 namespace sx {
 
-__device__ uint32_t g_attention_status;
-
-uint32_t attention_status() {
-    uint32_t st = 0;
-    const uint32_t zero = 0;
-    cuda_check(cudaDeviceSynchronize(), "attention_status");
-    cuda_check(cudaMemcpyFromSymbol(&st, g_attention_status, sizeof(st)), "attention_status");
-    if (st) cuda_check(cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(zero)), "attention_status");
-    return st;
-}
-uint32_t* attention_status_word() {
-    void* p = nullptr;
-    cuda_check(cudaGetSymbolAddress(&p, g_attention_status), "attention_status");
-    return static_cast<uint32_t*>(p);
-}
-
 namespace {
 
 constexpr int kT = 64;        // queries and keys of a tile
@@ -346,7 +330,11 @@ void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& ou
     AttnArgs a = attn_args(in);
     a.out = out;
     a.lse = lse;
-    if (a.batch == 0 || a.q_len == 0 || a.heads == 0) return;
+    if (a.batch == 0 || a.q_len == 0) return;
+    if (attention_tc_takes(a) && attention_tc_takes_view(a, a.out, a.q_len, a.heads)) {
+        launch_attention_fwd_tc(a, s);
+        return;
+    }
     by_dtype(a.dtype, [&](auto t) {
         by_dim(a.dim, [&](auto d) {
             constexpr int D = decltype(d)::value;
@@ -374,7 +362,7 @@ void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn&
     a.lse = const_cast<float*>(g.lse);
     a.lse2 = static_cast<float*>(ws);
     a.delta = a.lse2 + a.batch * a.heads * a.q_pad;
-    if (a.batch == 0 || a.heads == 0) return;
+    if (a.batch == 0) return;
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
         if (a.q_len) {

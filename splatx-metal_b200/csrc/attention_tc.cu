@@ -1,0 +1,374 @@
+// attention_tc.cu — attention on the tensor cores: 16-bit inputs, head dimensions that are multiples
+// of 8 up to 128 (padded by TMA's zero fill to 64 or 128), rows that TMA can copy.
+#include "sx_attention.h"
+#include "sx_tcgen05.cuh"
+
+namespace sx {
+
+__device__ uint32_t g_attention_status;
+
+uint32_t attention_status() {
+    uint32_t st = 0;
+    const uint32_t zero = 0;
+    cuda_check(cudaDeviceSynchronize(), "attention_status");
+    cuda_check(cudaMemcpyFromSymbol(&st, g_attention_status, sizeof(st)), "attention_status");
+    if (st) cuda_check(cudaMemcpyToSymbol(g_attention_status, &zero, sizeof(zero)), "attention_status");
+    return st;
+}
+
+namespace {
+
+constexpr int kRows = 128;            // rows of every tile: queries or keys
+constexpr int kPanel = kRows * 128;   // bytes of a tile's 64 columns
+constexpr int kSlots = 5;             // tiles of the key-value ring
+constexpr int kSmemMost = 232448;
+
+struct TcMaps {
+    CUtensorMap q, k, v, g;
+};
+
+// Rows from `first` of a tile in shared memory become zeros (the padding behind a batch entry's
+// length may hold NaN, which a probability of zero would not remove).
+template <int D>
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int lane) {
+    const int n = (kRows - first) * 8;  // 16-byte pieces of a panel's rows
+#pragma unroll
+    for (int p = 0; p < D / 64; ++p)
+        for (int i = lane; i < n; i += 32)
+            *reinterpret_cast<uint4*>(tile + p * kPanel + first * 128 + i * 16) = uint4{0, 0, 0, 0};
+    tc::fence_smem_to_async();
+    __syncwarp();
+}
+
+template <int D>
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, int batch, uint32_t bar) {
+    tc::bar_expect(bar, D / 64 * kPanel);
+#pragma unroll
+    for (int p = 0; p < D / 64; ++p) tc::tma_load(dst + p * kPanel, map, p * 64, row, head, batch, bar);
+}
+
+// Products over a whole tile. rows_rows: A and B both with rows along K = D (A B^T). tmem_rows: A in
+// tensor memory (128 lanes x 128 values of K, two a column), B's rows along N = D (A B).
+template <typename T, int D>
+__device__ __forceinline__ void rows_rows(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+        const uint32_t at = (k / 4) * kPanel + (k % 4) * 32;
+        tc::mma_ss(d, tc::operand(a + at, 16), tc::operand(b + at, 16), tc::shape<T>(kRows, false), k > 0);
+    }
+}
+template <typename T, int D, int HALF>  // HALF: columns between the two halves of K in tensor memory
+__device__ __forceinline__ void tmem_rows(uint32_t d, uint32_t a, uint32_t b, bool add) {
+#pragma unroll
+    for (int k = 0; k < kRows / 16; ++k)
+        tc::mma_ts(d, a + (k / 4) * HALF + (k % 4) * 8, tc::operand(b + k * 2048, kPanel), tc::shape<T>(D, true), add || k > 0);
+}
+
+// The forward. A CTA owns two tiles of 128 queries of one head; warps 0-3 and 4-7 are their softmax
+// warpgroups (a thread per query), warp 8 loads, warp 9 issues the products. While one warpgroup
+// works on its scores the tensor cores compute the other's: S = Q K^T into tensor memory, the
+// probabilities back over S's first half in 16 bits, O += P V from there.
+template <int D>
+struct FwdSmem {
+    static constexpr int kTileBytes = D / 64 * kPanel;
+    static constexpr int kQ = 0, kRing = 2 * kTileBytes, kBars = kRing + kSlots * kTileBytes;
+    static constexpr int kBytes = kBars + 256;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(320, 1) attn_fwd_tc_kernel(const AttnArgs a, const __grid_constant__ TcMaps maps) {
+    using S = FwdSmem<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t base = tc::smem_addr(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(bars + 24);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 25);
+    const uint32_t bar0 = base + S::kBars;
+    const auto kv_full = [&](int s) { return bar0 + 8 * s; };
+    const auto kv_free = [&](int s) { return bar0 + 8 * (kSlots + s); };
+    const auto q_full = [&](int t) { return bar0 + 8 * (2 * kSlots + t); };
+    const auto s_full = [&](int t) { return bar0 + 8 * (2 * kSlots + 2 + t); };
+    const auto p_full = [&](int t) { return bar0 + 8 * (2 * kSlots + 4 + t); };
+    const auto o_full = [&](int t) { return bar0 + 8 * (2 * kSlots + 6 + t); };
+    const uint32_t drained = bar0 + 8 * (2 * kSlots + 8);
+
+    // the last queries see the most keys when causal: they start first
+    const int64_t pairs = (a.q_len + 2 * kRows - 1) / (2 * kRows), heads = a.heads * a.batch;
+    const int64_t bh = blockIdx.x % heads;
+    const AttnHead w = attn_head(a, bh % a.heads, bh / a.heads);
+    const int q0 = static_cast<int>((pairs - 1 - blockIdx.x / heads) * 2 * kRows);
+    const int kv_len = static_cast<int>(w.kv_len), hk = static_cast<int>(w.h) / a.group;
+    int n[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int first = q0 + t * kRows;
+        n[t] = first >= w.q_len ? 0 : static_cast<int>((attn_keys_end(w, first + kRows) + kRows - 1) / kRows);
+    }
+    const int most = max(n[0], n[1]);
+
+    if (threadIdx.x == 0) {
+        *failed = 0;
+        for (int s = 0; s < kSlots; ++s) tc::bar_init(kv_full(s), 1), tc::bar_init(kv_free(s), 1);
+        for (int t = 0; t < 2; ++t) {
+            tc::bar_init(q_full(t), 1);
+            tc::bar_init(s_full(t), 1);
+            tc::bar_init(p_full(t), 4);
+            tc::bar_init(o_full(t), 1);
+        }
+        tc::bar_init(drained, 1);
+        tc::bar_init_fence();
+    }
+    if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *tmem_at;
+
+    if (warp == 8) {  // loads: Q tiles, then K0 V0 K1 V1 ... around the ring
+        if (lane == 0)
+            for (int t = 0; t < 2; ++t)
+                if (n[t]) load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t));
+        int it = 0;
+        for (; it < 2 * most; ++it) {
+            const int s = it % kSlots, round = it / kSlots;
+            if (round && !tc::bar_wait(kv_free(s), (round - 1) & 1, failed)) break;
+            if (lane == 0)
+                load_rows<D>(base + S::kRing + s * S::kTileBytes, it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, static_cast<int>(w.b), kv_full(s));
+            __syncwarp();
+        }
+        if (*failed) {  // nothing may land in this CTA's shared memory after it has gone
+            for (int t = 0; t < 2; ++t)
+                if (n[t]) tc::bar_drain(q_full(t), 0);
+            for (int i = max(0, it - kSlots); i < it; ++i) tc::bar_drain(kv_full(i % kSlots), (i / kSlots) & 1);
+        }
+    } else if (warp == 9) {  // products
+        const auto scores = [&](int t, int slot) {
+            if (lane == 0) {
+                rows_rows<T, D>(tmem + t * kRows, base + S::kQ + t * S::kTileBytes, base + S::kRing + slot * S::kTileBytes);
+                tc::commit(s_full(t));
+            }
+            __syncwarp();
+        };
+        bool ok = most == 0 || tc::bar_wait(kv_full(0), 0, failed);
+        for (int t = 0; ok && t < 2; ++t)
+            if (n[t]) {
+                ok = tc::bar_wait(q_full(t), 0, failed);
+                if (ok) scores(t, 0);
+            }
+        if (ok && most && lane == 0) tc::commit(kv_free(0));
+        for (int j = 0; ok && j < most; ++j) {
+            const int vi = 2 * j + 1, vs = vi % kSlots, ki = 2 * j + 2, ks = ki % kSlots;
+            ok = tc::bar_wait(kv_full(vs), (vi / kSlots) & 1, failed);
+            if (!ok) break;
+            if ((j + 1) * kRows > kv_len && kv_len < a.kv_len) zero_rows<D>(smem + S::kRing + vs * S::kTileBytes, kv_len - j * kRows, lane);
+            if (j + 1 < most) ok = tc::bar_wait(kv_full(ks), (ki / kSlots) & 1, failed);
+            for (int t = 0; ok && t < 2; ++t) {
+                if (j >= n[t]) continue;
+                ok = tc::bar_wait(p_full(t), j & 1, failed);
+                if (!ok) break;
+                tc::fence_after();
+                if (lane == 0) {
+                    tmem_rows<T, D, 32>(tmem + 2 * kRows + t * D, tmem + t * kRows, base + S::kRing + vs * S::kTileBytes, j > 0);
+                    if (j + 1 == n[t]) tc::commit(o_full(t));
+                }
+                __syncwarp();
+                if (j + 1 < n[t]) scores(t, ks);
+            }
+            if (ok && lane == 0) {
+                tc::commit(kv_free(vs));
+                if (j + 1 < most) tc::commit(kv_free(ks));
+            }
+            __syncwarp();
+        }
+        if (!ok) {
+            if (lane == 0) tc::commit(drained);
+            __syncwarp();
+            tc::bar_drain(drained, 0);
+        }
+    } else {  // softmax: a thread per query
+        const int t = warp >> 2, mine = n[t];
+        const int row = q0 + t * kRows + (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + 2 * kRows + t * D;
+        float m = -INFINITY, l = 0.f;  // m: the base-2 exponent the sums are relative to
+        bool ok = true;
+        for (int j = 0; j < mine; ++j) {
+            ok = tc::bar_wait(s_full(t), j & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            uint32_t r[4][32];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) tc::tmem_load32(r[c], s_at + c * 32);
+            tc::wait_ld(r[0], r[1], r[2], r[3]);
+            // keys of this tile that the query sees: those below `end`
+            const int64_t last = static_cast<int64_t>(row) + w.ahead + 1;
+            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j) * kRows);
+            if (__any_sync(kFullMask, end < kRows)) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c * 32 + i >= end) r[c][i] = 0xff800000u;
+            }
+            float top[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                top[c] = __uint_as_float(r[c][0]);
+#pragma unroll
+                for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(r[c][i]));
+            }
+            const float seen = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+            // The sums move to a new maximum only when it is 2^8 above the old one: 32 bits hold that,
+            // and the output's rows are then hardly ever read back and scaled.
+            if (j == 0) {
+                m = seen;
+            } else if (__any_sync(kFullMask, seen > m + 8.f)) {
+                const float to = fmaxf(m, seen);
+                const float f = to == -INFINITY ? 1.f : tc::exp2_approx(m - to);
+                l *= f;
+                m = to;
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tc::tmem_load32(o, o_at + c * 32);
+                    tc::wait_ld(o);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tc::tmem_store32(o_at + c * 32, o);
+                }
+            }
+            const float less = m == -INFINITY ? 0.f : m;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int e = c * 64 + i * 2;
+                    const float x = tc::exp2_approx(fmaf(__uint_as_float(r[e >> 5][e & 31]), a.scale_log2, -less));
+                    const float y = tc::exp2_approx(fmaf(__uint_as_float(r[e >> 5][(e & 31) + 1]), a.scale_log2, -less));
+                    sum[i & 1] += x;
+                    sum[2 + (i & 1)] += y;
+                    p[i] = tc::pack2<T>(x, y);
+                }
+                tc::tmem_store32(s_at + c * 32, p);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(p_full(t));
+        }
+        if (ok && mine) ok = tc::bar_wait(o_full(t), 0, failed);
+        if (ok) {
+            tc::fence_after();
+            const bool live = row < w.q_len && l > 0.f;
+            const float f = live ? 1.f / l : 0.f;
+            T* out = static_cast<T*>(a.out.data) + w.b * a.out.batch_stride + w.h * a.out.head_stride + row * a.out.token_stride;
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                if (mine) {
+                    tc::tmem_load32(o, o_at + c * 32);
+                    tc::wait_ld(o);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    uint4 x{0, 0, 0, 0};
+                    if (live) {
+                        uint32_t* px = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            px[e] = tc::pack2<T>(__uint_as_float(o[i + 2 * e]) * f, __uint_as_float(o[i + 2 * e + 1]) * f);
+                    }
+                    if (row < a.q_len && c * 32 + i < a.dim) *reinterpret_cast<uint4*>(out + c * 32 + i) = x;
+                }
+                __syncwarp();
+            }
+            if (row < a.q_len) a.lse[bh * a.q_len + row] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
+        }
+        tc::fence_before();
+    }
+    __syncthreads();
+    if (warp == 9) tc::tmem_free(tmem, 512);
+    if (threadIdx.x == 0 && *failed) atomicOr(&g_attention_status, 1u);
+}
+
+// ---- host ----
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+    static const EncodeFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        cuda_check(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found), "cuTensorMapEncodeTiled");
+        if (!p || found != cudaDriverEntryPointSuccess) throw RuntimeError("attention: the driver has no cuTensorMapEncodeTiled");
+        return reinterpret_cast<EncodeFn>(p);
+    }();
+    return fn;
+}
+
+// Boxes of 128 tokens x 64 values of one head; what lies beyond the tensor reads as zero.
+CUtensorMap make_map(const AttnArgs& a, const SxAttentionView& v, int64_t tokens, int64_t heads) {
+    CUtensorMap m;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(tokens),
+                                static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(a.batch)};
+    // an axis of one entry may have any stride: the row's own length stands for it
+    const auto bytes = [&](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(2 * (n > 1 ? stride : a.dim)); };
+    const cuuint64_t strides[3] = {bytes(tokens, v.token_stride), bytes(heads, v.head_stride), bytes(a.batch, v.batch_stride)};
+    const cuuint32_t box[4] = {64, kRows, 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encode_fn()(&m, a.dtype == SXCUDA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                   4, v.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw RuntimeError("attention: cuTensorMapEncodeTiled failed with " + std::to_string(static_cast<int>(r)));
+    return m;
+}
+
+// Rows that 16-byte copies reach, and strides a tensor map takes.
+bool copies(const AttnArgs& a, const SxAttentionView& v, int64_t tokens, int64_t heads) {
+    const auto fits = [](int64_t n, int64_t stride) { return n <= 1 || (stride > 0 && stride % 8 == 0 && stride < (1ll << 38)); };
+    return reinterpret_cast<uintptr_t>(v.data) % 16 == 0 && fits(tokens, v.token_stride) && fits(heads, v.head_stride) &&
+           fits(a.batch, v.batch_stride);
+}
+
+template <typename F>
+void by_type_dim(const AttnArgs& a, F&& f) {
+    const auto dim = [&](auto t) {
+        if (a.dim <= 64) f(t, std::integral_constant<int, 64>{});
+        else f(t, std::integral_constant<int, 128>{});
+    };
+    if (a.dtype == SXCUDA_F16) dim(__half{});
+    else dim(__nv_bfloat16{});
+}
+
+}  // namespace
+
+// A scale that is not above zero would turn the row maximum around; no key or query leaves nothing to map.
+bool attention_tc_takes(const AttnArgs& a) {
+    return a.dtype != SXCUDA_F32 && a.dim % 8 == 0 && a.scale > 0.f && a.q_len > 0 && a.kv_len > 0 &&
+           copies(a, a.q, a.q_len, a.heads) && copies(a, a.k, a.kv_len, a.kv_heads) && copies(a, a.v, a.kv_len, a.kv_heads);
+}
+bool attention_tc_takes_view(const AttnArgs& a, const SxAttentionView& v, int64_t tokens, int64_t heads) {
+    return copies(a, v, tokens, heads);
+}
+
+void launch_attention_fwd_tc(const AttnArgs& a, cudaStream_t s) {
+    by_type_dim(a, [&](auto t, auto d) {
+        constexpr int D = decltype(d)::value;
+        const auto kernel = attn_fwd_tc_kernel<decltype(t), D>;
+        constexpr int smem = FwdSmem<D>::kBytes;
+        static_assert(smem <= kSmemMost, "shared memory");
+        smem_limit_once(reinterpret_cast<const void*>(kernel), smem, "attention_fwd");
+        TcMaps maps;
+        maps.q = make_map(a, a.q, a.q_len, a.heads);
+        maps.k = make_map(a, a.k, a.kv_len, a.kv_heads);
+        maps.v = make_map(a, a.v, a.kv_len, a.kv_heads);
+        const int64_t grid = (a.q_len + 2 * kRows - 1) / (2 * kRows) * a.heads * a.batch;
+        if (grid > INT32_MAX) throw_invalid("attention_fwd", "too many query tiles");
+        SX_LAUNCH(kernel, static_cast<unsigned>(grid), 320, smem, s, a, maps);
+    });
+}
+
+}  // namespace sx

@@ -25,6 +25,12 @@ struct AttnArgs {
 };
 AttnArgs attn_args(const SxAttentionInputs& in);
 
+// The tensor-core kernels (attention_tc.cu): whether they take q, k and v, or another view of the
+// call, and their launch.
+bool attention_tc_takes(const AttnArgs& a);
+bool attention_tc_takes_view(const AttnArgs& a, const SxAttentionView& v, int64_t tokens, int64_t heads);
+void launch_attention_fwd_tc(const AttnArgs& a, cudaStream_t s);
+
 // One query head of one batch entry, with its lengths. Query i sees the keys j < kv_len with
 // j <= i + ahead.
 struct AttnHead {

@@ -56,9 +56,8 @@ void launch_layer_norm_bwd(const SxLayerNormInputs& in, const SxLayerNormGradsIn
 
 void launch_adamw(const SxAdamwTensor* t, int64_t n, const SxAdamwConfig& cfg, cudaStream_t s);
 
-// The status word of the current device: read and cleared (synchronises), and its address.
+// The attention kernels' status word of the current device, read and cleared (synchronises).
 uint32_t attention_status();
-uint32_t* attention_status_word();
 size_t attention_fwd_workspace(const SxAttentionInputs& in);
 void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& out, float* lse,
                           void* ws, cudaStream_t s);

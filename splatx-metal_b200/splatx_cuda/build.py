@@ -22,7 +22,7 @@ LIB_NAME = "libsplatx_cuda.so"
 
 SOURCES = ["forward.cu", "backward.cu", "sort.cu", "tile_bins.cu", "raster.cu", "ssim.cu", "executor.cu", "mcmc.cu",
            "io.cu", "eval.cu", "checkpoint.cu", "colmap.cu", "spz.cu",
-           "layer_norm.cu", "adamw.cu", "attention.cu",
+           "layer_norm.cu", "adamw.cu", "attention.cu", "attention_tc.cu",
            "capi.cu"]
 PER_FILE_FLAGS = {"forward.cu": ["-fmad=false"]}
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
