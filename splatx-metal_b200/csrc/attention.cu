@@ -166,29 +166,53 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_kernel(const AttnArgs a) {
 }
 
 // delta = sum(g out) per query, and lse in base 2 with +inf for a query that sees no key (exp2 then
-// gives 0). A warp per query; both arrays have rows of a.q_pad (the tensor-core kernels read whole
-// tiles of them).
-template <typename T>
+// gives 0). Both arrays have rows of a.q_pad: the tensor-core kernels read whole tiles of them. L
+// lanes share a query, each reading V values at a time. Bound by the reads of out and its gradient.
+template <typename T, int V, int L>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    if (i >= a.batch * a.heads * a.q_pad) return;
-    const int64_t row = i % a.q_pad, bh = i / a.q_pad;
+    constexpr int kQueries = 256 / L;
+    const int per_head = static_cast<int>(a.q_pad / kQueries);
+    const int64_t bh = blockIdx.x / per_head, row = static_cast<int64_t>(blockIdx.x % per_head) * kQueries + threadIdx.x / L;
     const AttnHead w = attn_head(a, bh % a.heads, bh / a.heads);
-    const int lane = threadIdx.x & 31;
     float s = 0.f, lse = INFINITY;
     if (row < w.q_len) {
         const T* o = static_cast<const T*>(a.out.data) + w.b * a.out.batch_stride + w.h * a.out.head_stride + row * a.out.token_stride;
         const T* g = static_cast<const T*>(a.g.data) + w.b * a.g.batch_stride + w.h * a.g.head_stride + row * a.g.token_stride;
-        for (int c = lane; c < a.dim; c += 32) s = fmaf(to_f32(o[c]), to_f32(g[c]), s);
+        for (int c = threadIdx.x % L * V; c < a.dim; c += L * V) {
+            const Pack<T, V> x = *reinterpret_cast<const Pack<T, V>*>(o + c), y = *reinterpret_cast<const Pack<T, V>*>(g + c);
 #pragma unroll
-        for (int off = 16; off; off >>= 1) s += __shfl_xor_sync(kFullMask, s, off);
+            for (int e = 0; e < V; ++e) s = fmaf(to_f32(x.v[e]), to_f32(y.v[e]), s);
+        }
         const float x = a.lse[bh * a.q_len + row];
-        if (x != -INFINITY) lse = x * kLog2e;
+        if (x != -INFINITY) lse = fmaf(x, kLog2e, -a.p_shift);
     }
-    if (lane == 0) {
-        a.delta[i] = s;
-        a.lse2[i] = lse;
+#pragma unroll
+    for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(kFullMask, s, off);
+    if (threadIdx.x % L == 0) {
+        a.delta[bh * a.q_pad + row] = s;
+        a.lse2[bh * a.q_pad + row] = lse;
     }
+}
+
+// The largest magnitude of a view's values below its lengths, as the bits of a float, which order
+// like unsigned numbers (so the atomic's order does not matter). A CTA per 64 rows of a head.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, const SxAttentionView v, const int32_t* lens,
+                                                           int64_t len, int32_t heads, uint32_t* most) {
+    const int per_head = static_cast<int>((len + 63) / 64);
+    const int64_t bh = blockIdx.x / per_head, b = bh / heads, r0 = static_cast<int64_t>(blockIdx.x % per_head) * 64;
+    const int64_t end = min(attn_length(lens, b, len), r0 + 64);
+    const T* p = static_cast<const T*>(v.data) + b * v.batch_stride + bh % heads * v.head_stride;
+    float top = 0.f;
+    for (int64_t r = r0 + threadIdx.x / 16; r < end; r += 16)
+        for (int c = threadIdx.x % 16 * 8; c < a.dim; c += 128) {
+            const Pack<T, 8> x = *reinterpret_cast<const Pack<T, 8>*>(p + r * v.token_stride + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f32(x.v[e])));
+        }
+#pragma unroll
+    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+    if (threadIdx.x % 32 == 0 && top > 0.f) atomicMax(most, __float_as_uint(top));
 }
 
 template <typename T, int D>
@@ -348,7 +372,7 @@ void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& ou
 
 size_t attention_bwd_workspace(const SxAttentionInputs& in) {
     const AttnArgs a = attn_args(in);
-    return static_cast<size_t>(2 * a.batch * a.heads * a.q_pad) * sizeof(float);
+    return static_cast<size_t>(2 * a.batch * a.heads * a.q_pad + 4) * sizeof(float);
 }
 
 void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn& g, const SxAttentionGrads& out,
@@ -363,12 +387,39 @@ void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn&
     a.lse2 = static_cast<float*>(ws);
     a.delta = a.lse2 + a.batch * a.heads * a.q_pad;
     if (a.batch == 0) return;
+    const bool tensor = attention_tc_takes(a) && attention_tc_takes_view(a, a.g, a.q_len, a.heads) &&
+                        attention_tc_takes_view(a, a.v_q, a.q_len, a.heads) &&
+                        attention_tc_takes_view(a, a.v_k, a.kv_len, a.kv_heads) &&
+                        attention_tc_takes_view(a, a.v_v, a.kv_len, a.kv_heads);
+    const bool half = tensor && a.dtype == SXCUDA_F16;
+    if (half) {
+        a.p_shift = kHalfShift;
+        a.largest = reinterpret_cast<uint32_t*>(a.delta + a.batch * a.heads * a.q_pad);
+        cuda_check(cudaMemsetAsync(a.largest, 0, 2 * sizeof(uint32_t), s), "attention_bwd");
+        const auto kernel = attn_largest_kernel<__half>;
+        SX_LAUNCH(kernel, blocks_for(a.q_len, 64) * a.heads * static_cast<unsigned>(a.batch), 256, 0, s, a, a.g, a.q_lens, a.q_len,
+                  a.heads, a.largest);
+        SX_LAUNCH(kernel, blocks_for(a.kv_len, 64) * a.kv_heads * static_cast<unsigned>(a.batch), 256, 0, s, a, a.v, a.kv_lens,
+                  a.kv_len, a.kv_heads, a.largest + 1);
+    }
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
         if (a.q_len) {
-            const auto delta = attn_delta_kernel<T>;
-            SX_LAUNCH(delta, blocks_for(a.batch * a.heads * a.q_pad, 8), 256, 0, s, a);
+            const auto run = [&](auto kernel, int lanes) {
+                SX_LAUNCH(kernel, static_cast<unsigned>(a.q_pad / (256 / lanes) * a.batch * a.heads), 256, 0, s, a);
+            };
+            if constexpr (sizeof(T) == 2) {
+                if (tensor && attention_tc_takes_view(a, a.out, a.q_len, a.heads)) {
+                    if (a.dim <= 64) run(attn_delta_kernel<T, 8, 8>, 8);
+                    else run(attn_delta_kernel<T, 8, 16>, 16);
+                } else {
+                    run(attn_delta_kernel<T, 1, 32>, 32);
+                }
+            } else {
+                run(attn_delta_kernel<T, 1, 32>, 32);
+            }
         }
+        if (tensor) return;
         by_dim(a.dim, [&](auto d) {
             constexpr int D = decltype(d)::value;
             if (a.kv_len) {
@@ -385,6 +436,7 @@ void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn&
             }
         });
     });
+    if (tensor) launch_attention_bwd_tc(a, s);
 }
 
 }  // namespace sx

@@ -295,6 +295,466 @@ __global__ void __launch_bounds__(320, 1) attn_fwd_tc_kernel(const AttnArgs a, c
     if (threadIdx.x == 0 && *failed) atomicOr(&g_attention_status, 1u);
 }
 
+// The backward. Both kinds of CTA run 256 threads over a 128 x 128 tile of scores, a thread per row,
+// each warpgroup on 64 of the columns; p and ds go back to tensor memory in 16 bits, over the scores
+// and over the products they came from, and are the A operands of the second products from there.
+//
+// A key-value CTA owns 128 keys (rows: keys, columns: queries) and passes over the queries of every
+// head that shares them: S = K Q^T, W = V G^T, v_v += P^T G, v_k += dS^T Q. While the warpgroups
+// turn S into P the tensor cores compute v_k of the tile before and W; while they turn W into dS,
+// v_v and the next S.
+//
+// A query CTA owns 128 queries (rows: queries, columns: keys): S = Q K^T, W = G V^T, v_q += dS K, with
+// the next S a tile ahead.
+template <int D>
+struct BwdSmem {
+    static constexpr int kTileBytes = D / 64 * kPanel;
+    static constexpr int kOwn = 0, kRing = 2 * kTileBytes, kStats = kRing + kSlots * kTileBytes;
+    static constexpr int kBars = kStats + 2 * 2 * kRows * 4;  // lse and delta of two query tiles
+    static constexpr int kBytes = kBars + 256;
+};
+
+struct BwdBars {
+    uint32_t at;
+    __device__ uint32_t full(int s) const { return at + 8 * s; }
+    __device__ uint32_t free(int s) const { return at + 8 * (kSlots + s); }
+    __device__ uint32_t own() const { return at + 8 * (2 * kSlots); }
+    __device__ uint32_t s_full(int k) const { return at + 8 * (2 * kSlots + 1 + k); }
+    __device__ uint32_t w_full() const { return at + 8 * (2 * kSlots + 3); }
+    __device__ uint32_t p_full() const { return at + 8 * (2 * kSlots + 4); }
+    __device__ uint32_t ds_full() const { return at + 8 * (2 * kSlots + 5); }
+    __device__ uint32_t out_full() const { return at + 8 * (2 * kSlots + 6); }
+    __device__ uint32_t stat_full(int k) const { return at + 8 * (2 * kSlots + 7 + k); }
+    __device__ uint32_t stat_free(int k) const { return at + 8 * (2 * kSlots + 9 + k); }
+    __device__ uint32_t drained() const { return at + 8 * (2 * kSlots + 11); }
+    static constexpr int kFailed = 2 * kSlots + 12, kTmem = kFailed + 1;  // words of 8 bytes behind the barriers
+};
+static_assert((BwdBars::kTmem + 1) * 8 <= 256, "barriers");
+
+__device__ __forceinline__ void bwd_init(const BwdBars& b, volatile uint32_t* failed) {
+    *failed = 0;
+    for (int s = 0; s < kSlots; ++s) tc::bar_init(b.full(s), 1), tc::bar_init(b.free(s), 1);
+    tc::bar_init(b.own(), 1);
+    tc::bar_init(b.w_full(), 1);
+    tc::bar_init(b.p_full(), 8);
+    tc::bar_init(b.ds_full(), 8);
+    tc::bar_init(b.out_full(), 1);
+    for (int k = 0; k < 2; ++k) tc::bar_init(b.s_full(k), 1), tc::bar_init(b.stat_full(k), 1), tc::bar_init(b.stat_free(k), 8);
+    tc::bar_init(b.drained(), 1);
+    tc::bar_init_fence();
+}
+
+// A thread's row of a finished D-column sum, times `f`, to memory; zeros where `live` is false.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(T* out, uint32_t at, float f, int dim, bool written, bool live, bool any) {
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (any) {
+            tc::tmem_load32(o, at + c * 32);
+            tc::wait_ld(o);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            uint4 x{0, 0, 0, 0};
+            if (live) {
+                uint32_t* px = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    px[e] = tc::pack2<T>(__uint_as_float(o[i + 2 * e]) * f, __uint_as_float(o[i + 2 * e + 1]) * f);
+            }
+            if (written && c * 32 + i < dim) *reinterpret_cast<uint4*>(out + c * 32 + i) = x;
+        }
+        __syncwarp();
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ T* row_of(const SxAttentionView& v, int64_t b, int64_t h, int64_t row) {
+    return static_cast<T*>(v.data) + b * v.batch_stride + h * v.head_stride + row * v.token_stride;
+}
+
+// float16 keeps 11 bits only above 2^-14: p and ds are held times powers of two, so that what a
+// gradient is summed from does not vanish before the sum. p is at most 1; for ds
+// |p (g v - delta)| <= 2 dim max|g| max|v|, which `ds` times takes to at most 2^15.
+struct HalfScale {
+    float p = 1.f, ds = 1.f;
+};
+template <typename T>
+__device__ __forceinline__ HalfScale half_scale(const AttnArgs& a) {
+    HalfScale h;
+    if constexpr (std::is_same_v<T, __half>) {
+        const float bound = 2.f * a.dim * __uint_as_float(a.largest[0]) * __uint_as_float(a.largest[1]);
+        h.p = 1.f / exp2f(kHalfShift);
+        if (bound > 0x1p-80f && bound < 0x1p80f) h.ds = exp2f(14.f - ceilf(log2f(bound)));
+    }
+    return h;
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void bwd_kv_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
+                                            const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
+    using S = BwdSmem<D>;
+    const uint32_t base = tc::smem_addr(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the first keys are seen by the most queries when causal: they start first
+    const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.batch;
+    const int hk = static_cast<int>(block % heads % a.kv_heads), batch = static_cast<int>(block % heads / a.kv_heads);
+    const int k0 = static_cast<int>(block / heads) * kRows;
+    const AttnHead w = attn_head(a, hk * a.group, batch);
+    const int q_len = static_cast<int>(w.q_len);
+    const int64_t begin = attn_queries_begin(w, k0);
+    const int first = static_cast<int>(begin / kRows);
+    const int tiles = k0 >= w.kv_len || begin >= q_len ? 0 : (q_len + kRows - 1) / kRows - first;
+    const int total = tiles * a.group;
+    const auto slot = [&](int item) { return base + S::kRing + item % kSlots * S::kTileBytes; };
+    constexpr uint32_t kW = kRows, kVV = 2 * kRows, kVK = 2 * kRows + D;
+
+    if (warp == 8) {  // loads: K and V, then Q0 G0 Q1 G1 ... around the ring, lse and delta beside each Q
+        if (lane == 0 && total) {
+            tc::bar_expect(bars.own(), 2 * S::kTileBytes);
+            for (int p = 0; p < D / 64; ++p) {
+                tc::tma_load(base + S::kOwn + p * kPanel, &maps.k, p * 64, k0, hk, batch, bars.own());
+                tc::tma_load(base + S::kOwn + S::kTileBytes + p * kPanel, &maps.v, p * 64, k0, hk, batch, bars.own());
+            }
+        }
+        int it = 0;
+        for (; it < 2 * total; ++it) {
+            const int s = it % kSlots, round = it / kSlots, i = it / 2;
+            if (round && !tc::bar_wait(bars.free(s), (round - 1) & 1, failed)) break;
+            if (!(it & 1) && i >= 2 && !tc::bar_wait(bars.stat_free(i & 1), (i / 2 - 1) & 1, failed)) break;
+            if (lane == 0) {
+                const int h = hk * a.group + i / tiles, row = (first + i % tiles) * kRows;
+                load_rows<D>(slot(it), it & 1 ? &maps.g : &maps.q, row, h, batch, bars.full(s));
+                if (!(it & 1)) {
+                    const int64_t at = (static_cast<int64_t>(batch) * a.heads + h) * a.q_pad + row;
+                    const uint32_t to = base + S::kStats + (i & 1) * 2 * kRows * 4;
+                    tc::bar_expect(bars.stat_full(i & 1), 2 * kRows * 4);
+                    tc::bulk_load(to, a.lse2 + at, kRows * 4, bars.stat_full(i & 1));
+                    tc::bulk_load(to + kRows * 4, a.delta + at, kRows * 4, bars.stat_full(i & 1));
+                }
+            }
+            __syncwarp();
+        }
+        if (*failed) {
+            if (total) tc::bar_drain(bars.own(), 0);
+            for (int i = max(0, it - kSlots); i < it; ++i) tc::bar_drain(bars.full(i % kSlots), (i / kSlots) & 1);
+            for (int i = max(0, (it + 1) / 2 - 2); i < (it + 1) / 2; ++i) tc::bar_drain(bars.stat_full(i & 1), (i / 2) & 1);
+        }
+    } else if (warp == 9) {  // products
+        const auto arrived = [&](int item) {  // the tile is there, padding behind the queries' end zeroed
+            if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
+            const int row = (first + item / 2 % tiles) * kRows;
+            if (row + kRows > q_len && q_len < a.q_len)
+                zero_rows<D>(smem + S::kRing + item % kSlots * S::kTileBytes, q_len - row, lane);
+            return true;
+        };
+        bool ok = total == 0 || (tc::bar_wait(bars.own(), 0, failed) && arrived(0));
+        if (ok && total) {
+            if (lane == 0) {
+                rows_rows<T, D>(tmem, base + S::kOwn, slot(0));
+                tc::commit(bars.s_full(0));
+            }
+            __syncwarp();
+            ok = arrived(1);
+            if (ok && lane == 0) {
+                rows_rows<T, D>(tmem + kW, base + S::kOwn + S::kTileBytes, slot(1));
+                tc::commit(bars.w_full());
+            }
+            __syncwarp();
+        }
+        for (int i = 0; ok && i < total; ++i) {
+            ok = tc::bar_wait(bars.p_full(), i & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            if (lane == 0) {
+                tmem_rows<T, D, 64>(tmem + kVV, tmem, slot(2 * i + 1), i > 0);
+                tc::commit(bars.free((2 * i + 1) % kSlots));
+            }
+            __syncwarp();
+            if (i + 1 < total) {
+                ok = arrived(2 * i + 2);
+                if (!ok) break;
+                if (lane == 0) {
+                    rows_rows<T, D>(tmem, base + S::kOwn, slot(2 * i + 2));
+                    tc::commit(bars.s_full(0));
+                }
+                __syncwarp();
+            }
+            ok = tc::bar_wait(bars.ds_full(), i & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            if (lane == 0) {
+                tmem_rows<T, D, 64>(tmem + kVK, tmem + kW, slot(2 * i), i > 0);
+                tc::commit(i + 1 < total ? bars.free(2 * i % kSlots) : bars.out_full());
+            }
+            __syncwarp();
+            if (i + 1 < total) {
+                ok = arrived(2 * i + 3);
+                if (!ok) break;
+                if (lane == 0) {
+                    rows_rows<T, D>(tmem + kW, base + S::kOwn + S::kTileBytes, slot(2 * i + 3));
+                    tc::commit(bars.w_full());
+                }
+                __syncwarp();
+            }
+        }
+        if (!ok) {
+            if (lane == 0) tc::commit(bars.drained());
+            __syncwarp();
+            tc::bar_drain(bars.drained(), 0);
+        }
+    } else {
+        const int half = warp >> 2;
+        const int64_t key = k0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + half * 64, w_at = s_at + kW;
+        const HalfScale scale = half_scale<T>(a);
+        bool ok = true;
+        for (int i = 0; i < total; ++i) {
+            const int64_t q0 = static_cast<int64_t>(first + i % tiles) * kRows + half * 64;
+            ok = tc::bar_wait(bars.s_full(0), i & 1, failed) && tc::bar_wait(bars.stat_full(i & 1), (i / 2) & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            const float4* lse = reinterpret_cast<const float4*>(smem + S::kStats + (i & 1) * 2 * kRows * 4) + half * 16;
+            const float4* delta = lse + kRows / 4;
+            uint32_t r[2][32];
+            tc::tmem_load32(r[0], s_at);
+            tc::tmem_load32(r[1], s_at + 32);
+            tc::wait_ld(r[0], r[1]);
+            // the queries of this half that see the key: columns lo..hi
+            const int lo = static_cast<int>(key < w.kv_len ? max(key - w.ahead - q0, static_cast<int64_t>(0)) : 64);
+            const int hi = static_cast<int>(min(w.q_len - q0, static_cast<int64_t>(64)));
+            const bool cut = __any_sync(kFullMask, lo > 0 || hi < 64);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 x = lse[c * 8 + e / 4];
+                    const float xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        float v = tc::exp2_approx(fmaf(__uint_as_float(r[c][e + k]), a.scale_log2, -xs[k]));
+                        if (cut && (c * 32 + e + k < lo || c * 32 + e + k >= hi)) v = 0.f;
+                        r[c][e + k] = __float_as_uint(v);
+                    }
+                    p[e / 2] = tc::pack2<T>(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
+                    p[e / 2 + 1] = tc::pack2<T>(__uint_as_float(r[c][e + 2]), __uint_as_float(r[c][e + 3]));
+                }
+                tc::tmem_store16(s_at + c * 16, p);
+            }
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(bars.p_full());
+            ok = tc::bar_wait(bars.w_full(), i & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            uint32_t g[2][32];
+            tc::tmem_load32(g[0], w_at);
+            tc::tmem_load32(g[1], w_at + 32);
+            tc::wait_ld(g[0], g[1]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 x = delta[c * 8 + e / 4];
+                    const float xs[4] = {x.x, x.y, x.z, x.w};
+                    float v[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        v[k] = __uint_as_float(r[c][e + k]) * (__uint_as_float(g[c][e + k]) - xs[k]);
+                        if constexpr (std::is_same_v<T, __half>) v[k] *= scale.p * scale.ds;
+                        if (cut && (c * 32 + e + k < lo || c * 32 + e + k >= hi)) v[k] = 0.f;
+                    }
+                    p[e / 2] = tc::pack2<T>(v[0], v[1]);
+                    p[e / 2 + 1] = tc::pack2<T>(v[2], v[3]);
+                }
+                tc::tmem_store16(w_at + c * 16, p);
+            }
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                tc::bar_arrive(bars.ds_full());
+                tc::bar_arrive(bars.stat_free(i & 1));
+            }
+        }
+        if (ok && total) ok = tc::bar_wait(bars.out_full(), 0, failed);
+        if (ok) {
+            tc::fence_after();
+            const bool written = key < a.kv_len, live = total && key < w.kv_len;
+            if (half == 0) store_row<T, D>(row_of<T>(a.v_v, batch, hk, key), tmem + lanes + kVV, scale.p, a.dim, written, live, total > 0);
+            else store_row<T, D>(row_of<T>(a.v_k, batch, hk, key), tmem + lanes + kVK, a.scale / scale.ds, a.dim, written, live, total > 0);
+        }
+    }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void bwd_q_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
+                                           const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
+    using S = BwdSmem<D>;
+    const uint32_t base = tc::smem_addr(smem);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int64_t heads = static_cast<int64_t>(a.heads) * a.batch, tiles = (a.q_len + kRows - 1) / kRows;
+    const int h = static_cast<int>(block % heads % a.heads), batch = static_cast<int>(block % heads / a.heads);
+    const int q0 = static_cast<int>(tiles - 1 - block / heads) * kRows, hk = h / a.group;
+    const AttnHead w = attn_head(a, h, batch);
+    const int kv_len = static_cast<int>(w.kv_len);
+    const int n = q0 >= w.q_len ? 0 : static_cast<int>((attn_keys_end(w, q0 + kRows) + kRows - 1) / kRows);
+    const auto slot = [&](int item) { return base + S::kRing + item % kSlots * S::kTileBytes; };
+    constexpr uint32_t kW = 2 * kRows, kVQ = 3 * kRows;
+
+    if (warp == 8) {  // loads: Q and G, then K0 V0 K1 V1 ... around the ring
+        if (lane == 0 && n) {
+            tc::bar_expect(bars.own(), 2 * S::kTileBytes);
+            for (int p = 0; p < D / 64; ++p) {
+                tc::tma_load(base + S::kOwn + p * kPanel, &maps.q, p * 64, q0, h, batch, bars.own());
+                tc::tma_load(base + S::kOwn + S::kTileBytes + p * kPanel, &maps.g, p * 64, q0, h, batch, bars.own());
+            }
+        }
+        int it = 0;
+        for (; it < 2 * n; ++it) {
+            const int s = it % kSlots, round = it / kSlots;
+            if (round && !tc::bar_wait(bars.free(s), (round - 1) & 1, failed)) break;
+            if (lane == 0) load_rows<D>(slot(it), it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, batch, bars.full(s));
+            __syncwarp();
+        }
+        if (*failed) {
+            if (n) tc::bar_drain(bars.own(), 0);
+            for (int i = max(0, it - kSlots); i < it; ++i) tc::bar_drain(bars.full(i % kSlots), (i / kSlots) & 1);
+        }
+    } else if (warp == 9) {  // products
+        const auto scores = [&](int j) {
+            const int item = 2 * j;
+            if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
+            if ((j + 1) * kRows > kv_len && kv_len < a.kv_len)
+                zero_rows<D>(smem + S::kRing + item % kSlots * S::kTileBytes, kv_len - j * kRows, lane);
+            if (lane == 0) {
+                rows_rows<T, D>(tmem + (j & 1) * kRows, base + S::kOwn, slot(item));
+                tc::commit(bars.s_full(j & 1));
+            }
+            __syncwarp();
+            return true;
+        };
+        const auto weights = [&](int j) {
+            const int item = 2 * j + 1;
+            if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
+            if (lane == 0) {
+                rows_rows<T, D>(tmem + kW, base + S::kOwn + S::kTileBytes, slot(item));
+                tc::commit(bars.w_full());
+                tc::commit(bars.free(item % kSlots));
+            }
+            __syncwarp();
+            return true;
+        };
+        bool ok = n == 0 || (tc::bar_wait(bars.own(), 0, failed) && scores(0) && weights(0));
+        for (int j = 0; ok && j < n; ++j) {
+            if (j + 1 < n) ok = scores(j + 1);
+            if (ok) ok = tc::bar_wait(bars.ds_full(), j & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            if (lane == 0) {
+                tmem_rows<T, D, 64>(tmem + kVQ, tmem + kW, slot(2 * j), j > 0);
+                tc::commit(j + 1 < n ? bars.free(2 * j % kSlots) : bars.out_full());
+            }
+            __syncwarp();
+            if (j + 1 < n) ok = weights(j + 1);
+        }
+        if (!ok) {
+            if (lane == 0) tc::commit(bars.drained());
+            __syncwarp();
+            tc::bar_drain(bars.drained(), 0);
+        }
+    } else {
+        const int half = warp >> 2;
+        const int64_t row = q0 + (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + half * 64, w_at = s_at + kW;
+        const int64_t at = (static_cast<int64_t>(batch) * a.heads + h) * a.q_pad + row;  // q_pad holds whole tiles
+        const float lse = a.lse2[at], delta = a.delta[at];
+        const HalfScale scale = half_scale<T>(a);
+        bool ok = true;
+        for (int j = 0; j < n; ++j) {
+            ok = tc::bar_wait(bars.s_full(j & 1), (j >> 1) & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            uint32_t r[2][32];
+            tc::tmem_load32(r[0], s_at + (j & 1) * kRows);
+            tc::tmem_load32(r[1], s_at + (j & 1) * kRows + 32);
+            tc::wait_ld(r[0], r[1]);
+            const int64_t last = row < w.q_len ? row + w.ahead + 1 : 0;
+            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j) * kRows - half * 64);
+            const bool cut = __any_sync(kFullMask, end < 64);
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                    r[c][e] = __float_as_uint(tc::exp2_approx(fmaf(__uint_as_float(r[c][e]), a.scale_log2, -lse)));
+            ok = tc::bar_wait(bars.w_full(), j & 1, failed);
+            if (!ok) break;
+            tc::fence_after();
+            uint32_t g[2][32];
+            tc::tmem_load32(g[0], w_at);
+            tc::tmem_load32(g[1], w_at + 32);
+            tc::wait_ld(g[0], g[1]);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    float x = __uint_as_float(r[c][e]) * (__uint_as_float(g[c][e]) - delta);
+                    float y = __uint_as_float(r[c][e + 1]) * (__uint_as_float(g[c][e + 1]) - delta);
+                    if constexpr (std::is_same_v<T, __half>) x *= scale.p * scale.ds, y *= scale.p * scale.ds;
+                    if (cut && c * 32 + e >= end) x = 0.f;
+                    if (cut && c * 32 + e + 1 >= end) y = 0.f;
+                    p[e / 2] = tc::pack2<T>(x, y);
+                }
+                tc::tmem_store16(w_at + c * 16, p);
+            }
+            tc::wait_st();
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(bars.ds_full());
+        }
+        if (ok && n) ok = tc::bar_wait(bars.out_full(), 0, failed);
+        if (ok) {
+            tc::fence_after();
+            // each warpgroup writes half of the row's columns
+            T* out = row_of<T>(a.v_q, batch, h, row) + half * (D / 2);
+            store_row<T, D / 2>(out, tmem + lanes + kVQ + half * (D / 2), a.scale / scale.ds, a.dim - half * (D / 2), row < a.q_len,
+                                n && row < w.q_len, n > 0);
+        }
+    }
+}
+
+// One launch holds both kinds of CTA: the query CTAs fill the SMs that the key-value CTAs' last wave
+// leaves idle.
+template <typename T, int D>
+__global__ void __launch_bounds__(320, 1) attn_bwd_tc_kernel(const AttnArgs a, const __grid_constant__ TcMaps maps, int64_t kv_blocks) {
+    using S = BwdSmem<D>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const BwdBars bars{tc::smem_addr(smem) + S::kBars};
+    uint64_t* words = reinterpret_cast<uint64_t*>(smem + S::kBars);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(words + BwdBars::kFailed);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(words + BwdBars::kTmem);
+    const int warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) bwd_init(bars, failed);
+    if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *tmem_at;
+    if (blockIdx.x < kv_blocks) bwd_kv_tile<T, D>(a, maps, blockIdx.x, smem, bars, tmem, failed);
+    else bwd_q_tile<T, D>(a, maps, blockIdx.x - kv_blocks, smem, bars, tmem, failed);
+    tc::fence_before();
+    __syncthreads();
+    if (warp == 9) tc::tmem_free(tmem, 512);
+    if (threadIdx.x == 0 && *failed) atomicOr(&g_attention_status, 1u);
+}
+
 // ---- host ----
 using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -368,6 +828,25 @@ void launch_attention_fwd_tc(const AttnArgs& a, cudaStream_t s) {
         const int64_t grid = (a.q_len + 2 * kRows - 1) / (2 * kRows) * a.heads * a.batch;
         if (grid > INT32_MAX) throw_invalid("attention_fwd", "too many query tiles");
         SX_LAUNCH(kernel, static_cast<unsigned>(grid), 320, smem, s, a, maps);
+    });
+}
+
+void launch_attention_bwd_tc(const AttnArgs& a, cudaStream_t s) {
+    by_type_dim(a, [&](auto t, auto d) {
+        constexpr int D = decltype(d)::value;
+        const auto kernel = attn_bwd_tc_kernel<decltype(t), D>;
+        constexpr int smem = BwdSmem<D>::kBytes;
+        static_assert(smem <= kSmemMost, "shared memory");
+        smem_limit_once(reinterpret_cast<const void*>(kernel), smem, "attention_bwd");
+        TcMaps maps;
+        maps.q = make_map(a, a.q, a.q_len, a.heads);
+        maps.k = make_map(a, a.k, a.kv_len, a.kv_heads);
+        maps.v = make_map(a, a.v, a.kv_len, a.kv_heads);
+        maps.g = make_map(a, a.g, a.q_len, a.heads);
+        const int64_t kv_blocks = (a.kv_len + kRows - 1) / kRows * a.kv_heads * a.batch;
+        const int64_t grid = kv_blocks + (a.q_len + kRows - 1) / kRows * a.heads * a.batch;
+        if (grid > INT32_MAX) throw_invalid("attention_bwd", "too many tiles");
+        SX_LAUNCH(kernel, static_cast<unsigned>(grid), 320, smem, s, a, maps, kv_blocks);
     });
 }
 

@@ -11,6 +11,9 @@ namespace sx {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// 2^14 times a probability is the most of them that float16 holds with room for rounding.
+constexpr float kHalfShift = 14.f;
+
 struct AttnArgs {
     SxAttentionView q, k, v, out, g, v_q, v_k, v_v;
     const int32_t* q_lens;
@@ -18,6 +21,10 @@ struct AttnArgs {
     float* lse;    // [batch, heads, q_len]
     float* lse2;   // [batch, heads, q_pad]: log-sums in base 2, +inf where nothing is seen
     float* delta;  // [batch, heads, q_pad]
+    // float16 on the tensor cores: probabilities are held times 2^p_shift, and ds times a power of two
+    // taken from the largest magnitudes of the output's gradient and of v (bits of a float each).
+    float p_shift;
+    uint32_t* largest;
     int64_t batch, q_len, kv_len, q_pad;
     int32_t heads, kv_heads, group, dim, dtype;
     bool causal;
@@ -30,6 +37,7 @@ AttnArgs attn_args(const SxAttentionInputs& in);
 bool attention_tc_takes(const AttnArgs& a);
 bool attention_tc_takes_view(const AttnArgs& a, const SxAttentionView& v, int64_t tokens, int64_t heads);
 void launch_attention_fwd_tc(const AttnArgs& a, cudaStream_t s);
+void launch_attention_bwd_tc(const AttnArgs& a, cudaStream_t s);
 
 // One query head of one batch entry, with its lengths. Query i sees the keys j < kv_len with
 // j <= i + ahead.
