@@ -57,26 +57,59 @@ __device__ __forceinline__ void rows_rows(uint32_t d, uint32_t a, uint32_t b) {
         tc::mma_ss(d, tc::operand(a + at, 16), tc::operand(b + at, 16), tc::shape<T>(kRows, false), k > 0);
     }
 }
-template <typename T, int D, int HALF>  // HALF: columns between the two halves of K in tensor memory
+template <typename T, int D>  // over 64 values of K
 __device__ __forceinline__ void tmem_rows(uint32_t d, uint32_t a, uint32_t b, bool add) {
 #pragma unroll
-    for (int k = 0; k < kRows / 16; ++k)
-        tc::mma_ts(d, a + (k / 4) * HALF + (k % 4) * 8, tc::operand(b + k * 2048, kPanel), tc::shape<T>(D, true), add || k > 0);
+    for (int k = 0; k < 4; ++k)
+        tc::mma_ts(d, a + k * 8, tc::operand(b + k * 2048, kPanel), tc::shape<T>(D, true), add || k > 0);
+}
+template <typename T, int D, int HALF>  // over 128, the second half HALF columns behind the first
+__device__ __forceinline__ void tmem_rows2(uint32_t d, uint32_t a, uint32_t b, bool add) {
+    tmem_rows<T, D>(d, a, b, add);
+    tmem_rows<T, D>(d, a + HALF, b + 64 * 128, true);
 }
 
-// The forward. A CTA owns two tiles of 128 queries of one head; warps 0-3 and 4-7 are their softmax
-// warpgroups (a thread per query), warp 8 loads, warp 9 issues the products. While one warpgroup
-// works on its scores the tensor cores compute the other's: S = Q K^T into tensor memory, the
-// probabilities back over S's first half in 16 bits, O += P V from there.
+// A thread's row of a finished D-column sum, times `f`, to memory; zeros where `live` is false.
+template <typename T, int D>
+__device__ __forceinline__ void store_row(T* out, uint32_t at, float f, int dim, bool written, bool live, bool any) {
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (any) {
+            tc::tmem_load32(o, at + c * 32);
+            tc::wait_ld(o);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) {
+            uint4 x{0, 0, 0, 0};
+            if (live) {
+                uint32_t* px = reinterpret_cast<uint32_t*>(&x);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    px[e] = tc::pack2<T>(__uint_as_float(o[i + 2 * e]) * f, __uint_as_float(o[i + 2 * e + 1]) * f);
+            }
+            if (written && c * 32 + i < dim) *reinterpret_cast<uint4*>(out + c * 32 + i) = x;
+        }
+        __syncwarp();
+    }
+}
+
+// The forward. A CTA owns two tiles of 128 queries of one head. Eight warps make a tile's
+// probabilities, two threads a query with 64 of a key tile's columns each (warps 0-7 the first tile,
+// 8-15 the second); warp 16 loads, warp 17 issues the products. While one tile's warps work on their
+// scores the tensor cores compute the other's: S = Q K^T into tensor memory, the probabilities back
+// over S in 16 bits, O += P V from there.
+constexpr int kFwdThreads = 640;  // warps 18 and 19 only give up their registers
 template <int D>
 struct FwdSmem {
     static constexpr int kTileBytes = D / 64 * kPanel;
-    static constexpr int kQ = 0, kRing = 2 * kTileBytes, kBars = kRing + kSlots * kTileBytes;
+    static constexpr int kQ = 0, kRing = 2 * kTileBytes, kTops = kRing + kSlots * kTileBytes;
+    static constexpr int kBars = kTops + 2 * 2 * kRows * 4;  // a value of each thread for its query's other one
     static constexpr int kBytes = kBars + 256;
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1) attn_fwd_tc_kernel(const AttnArgs a, const __grid_constant__ TcMaps maps) {
+__global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnArgs a, const __grid_constant__ TcMaps maps) {
     using S = FwdSmem<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = tc::smem_addr(smem);
@@ -113,100 +146,106 @@ __global__ void __launch_bounds__(320, 1) attn_fwd_tc_kernel(const AttnArgs a, c
         for (int t = 0; t < 2; ++t) {
             tc::bar_init(q_full(t), 1);
             tc::bar_init(s_full(t), 1);
-            tc::bar_init(p_full(t), 4);
+            tc::bar_init(p_full(t), 8);
             tc::bar_init(o_full(t), 1);
         }
         tc::bar_init(drained, 1);
         tc::bar_init_fence();
     }
-    if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
+    if (warp == 17) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *tmem_at;
 
-    if (warp == 8) {  // loads: Q tiles, then K0 V0 K1 V1 ... around the ring
-        if (lane == 0)
-            for (int t = 0; t < 2; ++t)
-                if (n[t]) load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t));
-        int it = 0;
-        for (; it < 2 * most; ++it) {
-            const int s = it % kSlots, round = it / kSlots;
-            if (round && !tc::bar_wait(kv_free(s), (round - 1) & 1, failed)) break;
+    int loaded = 0;  // tiles of the ring that warp 16 has asked for
+    // 640 x 96 registers at the launch = 512 x 104 + 128 x 64
+    if (warp >= 16) {
+        tc::fewer_registers<64>();
+        if (warp == 16) {  // loads: Q tiles, then K0 V0 K1 V1 ... around the ring
             if (lane == 0)
-                load_rows<D>(base + S::kRing + s * S::kTileBytes, it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, static_cast<int>(w.b), kv_full(s));
-            __syncwarp();
-        }
-        if (*failed) {  // nothing may land in this CTA's shared memory after it has gone
-            for (int t = 0; t < 2; ++t)
-                if (n[t]) tc::bar_drain(q_full(t), 0);
-            for (int i = max(0, it - kSlots); i < it; ++i) tc::bar_drain(kv_full(i % kSlots), (i / kSlots) & 1);
-        }
-    } else if (warp == 9) {  // products
-        const auto scores = [&](int t, int slot) {
-            if (lane == 0) {
-                rows_rows<T, D>(tmem + t * kRows, base + S::kQ + t * S::kTileBytes, base + S::kRing + slot * S::kTileBytes);
-                tc::commit(s_full(t));
+                for (int t = 0; t < 2; ++t)
+                    if (n[t]) load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t));
+            for (; loaded < 2 * most; ++loaded) {
+                const int s = loaded % kSlots, round = loaded / kSlots;
+                if (round && !tc::bar_wait(kv_free(s), (round - 1) & 1, failed)) break;
+                if (lane == 0)
+                    load_rows<D>(base + S::kRing + s * S::kTileBytes, loaded & 1 ? &maps.v : &maps.k, loaded / 2 * kRows, hk, static_cast<int>(w.b), kv_full(s));
+                __syncwarp();
             }
-            __syncwarp();
-        };
-        bool ok = most == 0 || tc::bar_wait(kv_full(0), 0, failed);
-        for (int t = 0; ok && t < 2; ++t)
-            if (n[t]) {
-                ok = tc::bar_wait(q_full(t), 0, failed);
-                if (ok) scores(t, 0);
-            }
-        if (ok && most && lane == 0) tc::commit(kv_free(0));
-        for (int j = 0; ok && j < most; ++j) {
-            const int vi = 2 * j + 1, vs = vi % kSlots, ki = 2 * j + 2, ks = ki % kSlots;
-            ok = tc::bar_wait(kv_full(vs), (vi / kSlots) & 1, failed);
-            if (!ok) break;
-            if ((j + 1) * kRows > kv_len && kv_len < a.kv_len) zero_rows<D>(smem + S::kRing + vs * S::kTileBytes, kv_len - j * kRows, lane);
-            if (j + 1 < most) ok = tc::bar_wait(kv_full(ks), (ki / kSlots) & 1, failed);
-            for (int t = 0; ok && t < 2; ++t) {
-                if (j >= n[t]) continue;
-                ok = tc::bar_wait(p_full(t), j & 1, failed);
-                if (!ok) break;
-                tc::fence_after();
+        } else if (warp == 17) {  // products
+            const auto scores = [&](int t, int slot) {
                 if (lane == 0) {
-                    tmem_rows<T, D, 32>(tmem + 2 * kRows + t * D, tmem + t * kRows, base + S::kRing + vs * S::kTileBytes, j > 0);
-                    if (j + 1 == n[t]) tc::commit(o_full(t));
+                    rows_rows<T, D>(tmem + t * kRows, base + S::kQ + t * S::kTileBytes, base + S::kRing + slot * S::kTileBytes);
+                    tc::commit(s_full(t));
                 }
                 __syncwarp();
-                if (j + 1 < n[t]) scores(t, ks);
+            };
+            bool ok = most == 0 || tc::bar_wait(kv_full(0), 0, failed);
+            for (int t = 0; ok && t < 2; ++t)
+                if (n[t]) {
+                    ok = tc::bar_wait(q_full(t), 0, failed);
+                    if (ok) scores(t, 0);
+                }
+            if (ok && most && lane == 0) tc::commit(kv_free(0));
+            for (int j = 0; ok && j < most; ++j) {
+                const int vi = 2 * j + 1, vs = vi % kSlots, ki = 2 * j + 2, ks = ki % kSlots;
+                ok = tc::bar_wait(kv_full(vs), (vi / kSlots) & 1, failed);
+                if (!ok) break;
+                if ((j + 1) * kRows > kv_len && kv_len < a.kv_len) zero_rows<D>(smem + S::kRing + vs * S::kTileBytes, kv_len - j * kRows, lane);
+                if (j + 1 < most) ok = tc::bar_wait(kv_full(ks), (ki / kSlots) & 1, failed);
+                for (int t = 0; ok && t < 2; ++t) {
+                    if (j >= n[t]) continue;
+                    ok = tc::bar_wait(p_full(t), j & 1, failed);
+                    if (!ok) break;
+                    tc::fence_after();
+                    if (lane == 0) {
+                        tmem_rows2<T, D, 64>(tmem + 2 * kRows + t * D, tmem + t * kRows, base + S::kRing + vs * S::kTileBytes, j > 0);
+                        if (j + 1 == n[t]) tc::commit(o_full(t));
+                    }
+                    __syncwarp();
+                    if (j + 1 < n[t]) scores(t, ks);
+                }
+                if (ok && lane == 0) {
+                    tc::commit(kv_free(vs));
+                    if (j + 1 < most) tc::commit(kv_free(ks));
+                }
+                __syncwarp();
             }
-            if (ok && lane == 0) {
-                tc::commit(kv_free(vs));
-                if (j + 1 < most) tc::commit(kv_free(ks));
-            }
-            __syncwarp();
         }
-        if (!ok) {
-            if (lane == 0) tc::commit(drained);
-            __syncwarp();
-            tc::bar_drain(drained, 0);
-        }
-    } else {  // softmax: a thread per query
-        const int t = warp >> 2, mine = n[t];
-        const int row = q0 + t * kRows + (warp & 3) * 32 + lane;
+    } else {  // probabilities
+        tc::more_registers<104>();
+        const int t = warp >> 3, half = warp >> 2 & 1, mine = n[t];
+        const int lane_row = (warp & 3) * 32 + lane, row = q0 + t * kRows + lane_row;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + 2 * kRows + t * D;
+        const uint32_t s_at = tmem + lanes + t * kRows + half * 64, o_at = tmem + lanes + 2 * kRows + t * D + half * (D / 2);
+        float* mine_to = reinterpret_cast<float*>(smem + S::kTops) + (t * 2 + half) * kRows + lane_row;
+        const float* other = reinterpret_cast<const float*>(smem + S::kTops) + (t * 2 + 1 - half) * kRows + lane_row;
+        // The value of the query's other thread. A warp that gives up still takes part in all of the
+        // exchanges, so that none of the others waits for it.
+        int exchanges = mine + 1;
+        const auto exchange = [&](float x) {
+            --exchanges;
+            *mine_to = x;
+            asm volatile("bar.sync %0, 256;" ::"r"(t + 1) : "memory");
+            return *other;
+        };
         float m = -INFINITY, l = 0.f;  // m: the base-2 exponent the sums are relative to
         bool ok = true;
         for (int j = 0; j < mine; ++j) {
             ok = tc::bar_wait(s_full(t), j & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            uint32_t r[4][32];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tc::tmem_load32(r[c], s_at + c * 32);
-            tc::wait_ld(r[0], r[1], r[2], r[3]);
-            // keys of this tile that the query sees: those below `end`
+            uint32_t r[2][32];
+            tc::tmem_load32(r[0], s_at);
+            tc::tmem_load32(r[1], s_at + 32);
+            tc::wait_ld(r[0], r[1]);
+            // keys of these columns that the query sees: those below `end`
             const int64_t last = static_cast<int64_t>(row) + w.ahead + 1;
-            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j) * kRows);
-            if (__any_sync(kFullMask, end < kRows)) {
+            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j) * kRows - half * 64);
+            if (__any_sync(kFullMask, end < 64)) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 2; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (c * 32 + i >= end) r[c][i] = 0xff800000u;
@@ -214,11 +253,13 @@ __global__ void __launch_bounds__(320, 1) attn_fwd_tc_kernel(const AttnArgs a, c
             float top[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                top[c] = __uint_as_float(r[c][0]);
+                const uint32_t* x = r[c >> 1] + (c & 1) * 16;
+                top[c] = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 #pragma unroll
-                for (int i = 1; i < 32; ++i) top[c] = fmaxf(top[c], __uint_as_float(r[c][i]));
+                for (int i = 2; i < 16; i += 2) top[c] = tc::max3(top[c], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
             }
-            const float seen = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+            float seen = fmaxf(tc::max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
+            seen = fmaxf(seen, exchange(seen));
             // The sums move to a new maximum only when it is 2^8 above the old one: 32 bits hold that,
             // and the output's rows are then hardly ever read back and scaled.
             if (j == 0) {
@@ -228,71 +269,70 @@ __global__ void __launch_bounds__(320, 1) attn_fwd_tc_kernel(const AttnArgs a, c
                 const float f = to == -INFINITY ? 1.f : tc::exp2_approx(m - to);
                 l *= f;
                 m = to;
-#pragma unroll
-                for (int c = 0; c < D / 32; ++c) {
-                    uint32_t o[32];
-                    tc::tmem_load32(o, o_at + c * 32);
+#pragma unroll 1
+                for (int c = 0; c < D / 2; c += 16) {
+                    uint32_t o[16];
+                    tc::tmem_load16(o, o_at + c);
                     tc::wait_ld(o);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                    tc::tmem_store32(o_at + c * 32, o);
+                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tc::tmem_store16(o_at + c, o);
                 }
             }
-            const float less = m == -INFINITY ? 0.f : m;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const float less = m == -INFINITY ? 0.f : -m;
+            const tc::Two times = tc::two(a.scale_log2, a.scale_log2), plus = tc::two(less, less);
+            tc::Two sum[2] = {tc::two(0.f, 0.f), tc::two(0.f, 0.f)};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t p[32];
+                uint32_t p[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int e = c * 64 + i * 2;
-                    const float x = tc::exp2_approx(fmaf(__uint_as_float(r[e >> 5][e & 31]), a.scale_log2, -less));
-                    const float y = tc::exp2_approx(fmaf(__uint_as_float(r[e >> 5][(e & 31) + 1]), a.scale_log2, -less));
-                    sum[i & 1] += x;
-                    sum[2 + (i & 1)] += y;
-                    p[i] = tc::pack2<T>(x, y);
+                for (int i = 0; i < 16; ++i) {
+                    const tc::Two x = tc::fma2(tc::two(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), times, plus);
+                    float lo, hi;
+                    tc::split(x, lo, hi);
+                    lo = tc::exp2_approx(lo);
+                    hi = tc::exp2_approx(hi);
+                    sum[i & 1] = tc::add2(sum[i & 1], tc::two(lo, hi));
+                    p[i] = tc::pack2<T>(lo, hi);
                 }
-                tc::tmem_store32(s_at + c * 32, p);
+                tc::tmem_store16(s_at + c * 16, p);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             tc::wait_st();
             tc::fence_before();
             __syncwarp();
             if (lane == 0) tc::bar_arrive(p_full(t));
+            float lo, hi;
+            tc::split(tc::add2(sum[0], sum[1]), lo, hi);
+            l += lo + hi;
         }
         if (ok && mine) ok = tc::bar_wait(o_full(t), 0, failed);
         if (ok) {
             tc::fence_after();
-            const bool live = row < w.q_len && l > 0.f;
-            const float f = live ? 1.f / l : 0.f;
+            l += exchange(l);
+            const bool live = row < w.q_len && m != -INFINITY;
+            // each of the two writes half of the query's columns
             T* out = static_cast<T*>(a.out.data) + w.b * a.out.batch_stride + w.h * a.out.head_stride + row * a.out.token_stride;
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-                uint32_t o[32];
-                if (mine) {
-                    tc::tmem_load32(o, o_at + c * 32);
-                    tc::wait_ld(o);
-                }
-#pragma unroll
-                for (int i = 0; i < 32; i += 8) {
-                    uint4 x{0, 0, 0, 0};
-                    if (live) {
-                        uint32_t* px = reinterpret_cast<uint32_t*>(&x);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            px[e] = tc::pack2<T>(__uint_as_float(o[i + 2 * e]) * f, __uint_as_float(o[i + 2 * e + 1]) * f);
-                    }
-                    if (row < a.q_len && c * 32 + i < a.dim) *reinterpret_cast<uint4*>(out + c * 32 + i) = x;
-                }
-                __syncwarp();
-            }
-            if (row < a.q_len) a.lse[bh * a.q_len + row] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
+            store_row<T, D / 2>(out + half * (D / 2), o_at, live ? 1.f / l : 0.f, a.dim - half * (D / 2), row < a.q_len, live, mine > 0);
+            if (row < a.q_len && half == 0) a.lse[bh * a.q_len + row] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
+        while (exchanges > 0) exchange(0.f);
         tc::fence_before();
     }
     __syncthreads();
-    if (warp == 9) tc::tmem_free(tmem, 512);
-    if (threadIdx.x == 0 && *failed) atomicOr(&g_attention_status, 1u);
+    if (*failed) {  // nothing may land in this CTA's memory after it has gone
+        if (warp == 16) {
+            for (int t = 0; t < 2; ++t)
+                if (n[t]) tc::bar_drain(q_full(t), 0);
+            for (int i = max(0, loaded - kSlots); i < loaded; ++i) tc::bar_drain(kv_full(i % kSlots), (i / kSlots) & 1);
+        } else if (warp == 17) {
+            if (lane == 0) tc::commit(drained);
+            __syncwarp();
+            tc::bar_drain(drained, 0);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) atomicOr(&g_attention_status, 1u);
+    }
+    if (warp == 17) tc::tmem_free(tmem, 512);
 }
 
 // The backward. Both kinds of CTA run 256 threads over a 128 x 128 tile of scores, a thread per row,
@@ -344,35 +384,17 @@ __device__ __forceinline__ void bwd_init(const BwdBars& b, volatile uint32_t* fa
     tc::bar_init_fence();
 }
 
-// A thread's row of a finished D-column sum, times `f`, to memory; zeros where `live` is false.
-template <typename T, int D>
-__device__ __forceinline__ void store_row(T* out, uint32_t at, float f, int dim, bool written, bool live, bool any) {
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        if (any) {
-            tc::tmem_load32(o, at + c * 32);
-            tc::wait_ld(o);
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            uint4 x{0, 0, 0, 0};
-            if (live) {
-                uint32_t* px = reinterpret_cast<uint32_t*>(&x);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    px[e] = tc::pack2<T>(__uint_as_float(o[i + 2 * e]) * f, __uint_as_float(o[i + 2 * e + 1]) * f);
-            }
-            if (written && c * 32 + i < dim) *reinterpret_cast<uint4*>(out + c * 32 + i) = x;
-        }
-        __syncwarp();
-    }
-}
-
 template <typename T>
 __device__ __forceinline__ T* row_of(const SxAttentionView& v, int64_t b, int64_t h, int64_t row) {
     return static_cast<T*>(v.data) + b * v.batch_stride + h * v.head_stride + row * v.token_stride;
 }
+
+// What the loading warp has asked for: tiles of the ring, the CTA's own tiles, lse and delta tiles.
+struct Loaded {
+    int ring = 0;
+    bool own = false;
+    int stats = 0;
+};
 
 // float16 keeps 11 bits only above 2^-14: p and ds are held times powers of two, so that what a
 // gradient is summed from does not vanish before the sum. p is at most 1; for ds
@@ -392,7 +414,7 @@ __device__ __forceinline__ HalfScale half_scale(const AttnArgs& a) {
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void bwd_kv_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
+__device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
                                             const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
     using S = BwdSmem<D>;
     const uint32_t base = tc::smem_addr(smem);
@@ -436,11 +458,7 @@ __device__ __forceinline__ void bwd_kv_tile(const AttnArgs& a, const TcMaps& map
             }
             __syncwarp();
         }
-        if (*failed) {
-            if (total) tc::bar_drain(bars.own(), 0);
-            for (int i = max(0, it - kSlots); i < it; ++i) tc::bar_drain(bars.full(i % kSlots), (i / kSlots) & 1);
-            for (int i = max(0, (it + 1) / 2 - 2); i < (it + 1) / 2; ++i) tc::bar_drain(bars.stat_full(i & 1), (i / 2) & 1);
-        }
+        return {it, total > 0, (it + 1) / 2};
     } else if (warp == 9) {  // products
         const auto arrived = [&](int item) {  // the tile is there, padding behind the queries' end zeroed
             if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
@@ -468,7 +486,7 @@ __device__ __forceinline__ void bwd_kv_tile(const AttnArgs& a, const TcMaps& map
             if (!ok) break;
             tc::fence_after();
             if (lane == 0) {
-                tmem_rows<T, D, 64>(tmem + kVV, tmem, slot(2 * i + 1), i > 0);
+                tmem_rows2<T, D, 64>(tmem + kVV, tmem, slot(2 * i + 1), i > 0);
                 tc::commit(bars.free((2 * i + 1) % kSlots));
             }
             __syncwarp();
@@ -485,7 +503,7 @@ __device__ __forceinline__ void bwd_kv_tile(const AttnArgs& a, const TcMaps& map
             if (!ok) break;
             tc::fence_after();
             if (lane == 0) {
-                tmem_rows<T, D, 64>(tmem + kVK, tmem + kW, slot(2 * i), i > 0);
+                tmem_rows2<T, D, 64>(tmem + kVK, tmem + kW, slot(2 * i), i > 0);
                 tc::commit(i + 1 < total ? bars.free(2 * i % kSlots) : bars.out_full());
             }
             __syncwarp();
@@ -498,11 +516,6 @@ __device__ __forceinline__ void bwd_kv_tile(const AttnArgs& a, const TcMaps& map
                 }
                 __syncwarp();
             }
-        }
-        if (!ok) {
-            if (lane == 0) tc::commit(bars.drained());
-            __syncwarp();
-            tc::bar_drain(bars.drained(), 0);
         }
     } else {
         const int half = warp >> 2;
@@ -590,10 +603,11 @@ __device__ __forceinline__ void bwd_kv_tile(const AttnArgs& a, const TcMaps& map
             else store_row<T, D>(row_of<T>(a.v_k, batch, hk, key), tmem + lanes + kVK, a.scale / scale.ds, a.dim, written, live, total > 0);
         }
     }
+    return {};
 }
 
 template <typename T, int D>
-__device__ __forceinline__ void bwd_q_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
+__device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
                                            const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
     using S = BwdSmem<D>;
     const uint32_t base = tc::smem_addr(smem);
@@ -622,10 +636,7 @@ __device__ __forceinline__ void bwd_q_tile(const AttnArgs& a, const TcMaps& maps
             if (lane == 0) load_rows<D>(slot(it), it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, batch, bars.full(s));
             __syncwarp();
         }
-        if (*failed) {
-            if (n) tc::bar_drain(bars.own(), 0);
-            for (int i = max(0, it - kSlots); i < it; ++i) tc::bar_drain(bars.full(i % kSlots), (i / kSlots) & 1);
-        }
+        return {it, n > 0, 0};
     } else if (warp == 9) {  // products
         const auto scores = [&](int j) {
             const int item = 2 * j;
@@ -657,16 +668,11 @@ __device__ __forceinline__ void bwd_q_tile(const AttnArgs& a, const TcMaps& maps
             if (!ok) break;
             tc::fence_after();
             if (lane == 0) {
-                tmem_rows<T, D, 64>(tmem + kVQ, tmem + kW, slot(2 * j), j > 0);
+                tmem_rows2<T, D, 64>(tmem + kVQ, tmem + kW, slot(2 * j), j > 0);
                 tc::commit(j + 1 < n ? bars.free(2 * j % kSlots) : bars.out_full());
             }
             __syncwarp();
             if (j + 1 < n) ok = weights(j + 1);
-        }
-        if (!ok) {
-            if (lane == 0) tc::commit(bars.drained());
-            __syncwarp();
-            tc::bar_drain(bars.drained(), 0);
         }
     } else {
         const int half = warp >> 2;
@@ -728,6 +734,7 @@ __device__ __forceinline__ void bwd_q_tile(const AttnArgs& a, const TcMaps& maps
                                 n && row < w.q_len, n > 0);
         }
     }
+    return {};
 }
 
 // One launch holds both kinds of CTA: the query CTAs fill the SMs that the key-value CTAs' last wave
@@ -747,12 +754,24 @@ __global__ void __launch_bounds__(320, 1) attn_bwd_tc_kernel(const AttnArgs a, c
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *tmem_at;
-    if (blockIdx.x < kv_blocks) bwd_kv_tile<T, D>(a, maps, blockIdx.x, smem, bars, tmem, failed);
-    else bwd_q_tile<T, D>(a, maps, blockIdx.x - kv_blocks, smem, bars, tmem, failed);
+    const Loaded asked = blockIdx.x < kv_blocks ? bwd_kv_tile<T, D>(a, maps, blockIdx.x, smem, bars, tmem, failed)
+                                                : bwd_q_tile<T, D>(a, maps, blockIdx.x - kv_blocks, smem, bars, tmem, failed);
     tc::fence_before();
     __syncthreads();
+    if (*failed) {  // nothing may land in this CTA's memory after it has gone
+        if (warp == 8) {
+            if (asked.own) tc::bar_drain(bars.own(), 0);
+            for (int i = max(0, asked.ring - kSlots); i < asked.ring; ++i) tc::bar_drain(bars.full(i % kSlots), (i / kSlots) & 1);
+            for (int i = max(0, asked.stats - 2); i < asked.stats; ++i) tc::bar_drain(bars.stat_full(i & 1), (i / 2) & 1);
+        } else if (warp == 9) {
+            if (threadIdx.x % 32 == 0) tc::commit(bars.drained());
+            __syncwarp();
+            tc::bar_drain(bars.drained(), 0);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) atomicOr(&g_attention_status, 1u);
+    }
     if (warp == 9) tc::tmem_free(tmem, 512);
-    if (threadIdx.x == 0 && *failed) atomicOr(&g_attention_status, 1u);
 }
 
 // ---- host ----
@@ -827,7 +846,7 @@ void launch_attention_fwd_tc(const AttnArgs& a, cudaStream_t s) {
         maps.v = make_map(a, a.v, a.kv_len, a.kv_heads);
         const int64_t grid = (a.q_len + 2 * kRows - 1) / (2 * kRows) * a.heads * a.batch;
         if (grid > INT32_MAX) throw_invalid("attention_fwd", "too many query tiles");
-        SX_LAUNCH(kernel, static_cast<unsigned>(grid), 320, smem, s, a, maps);
+        SX_LAUNCH(kernel, static_cast<unsigned>(grid), kFwdThreads, smem, s, a, maps);
     });
 }
 

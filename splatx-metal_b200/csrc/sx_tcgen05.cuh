@@ -104,6 +104,12 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
         : SX_R8(r, 0), SX_R8(r, 8), SX_R8(r, 16), SX_R8(r, 24)
         : "r"(at));
 }
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : SX_R8(r, 0), SX_R8(r, 8)
+        : "r"(at));
+}
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -121,6 +127,7 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16
 #define SX_T8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
 // Waits for the thread's loads. The registers are named as changed behind the wait, so that the
 // compiler moves no use of them before it.
+__device__ __forceinline__ void changed(uint32_t (&r)[16]) { asm volatile("" : SX_T8(r, 0), SX_T8(r, 8)); }
 __device__ __forceinline__ void changed(uint32_t (&r)[32]) {
     asm volatile("" : SX_T8(r, 0), SX_T8(r, 8));
     asm volatile("" : SX_T8(r, 16), SX_T8(r, 24));
@@ -176,6 +183,13 @@ __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
+// ---- registers ----
+// A warpgroup's threads take more or fewer registers; the sum over the CTA stays within its launch's.
+template <int N>
+__device__ __forceinline__ void more_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void fewer_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
 // ---- values ----
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -195,6 +209,38 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// Two 32-bit values that one instruction works on.
+struct Two {
+    uint64_t v;
+};
+__device__ __forceinline__ Two two(float lo, float hi) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void split(Two x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x.v)); }
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
 }
 
 }  // namespace tc
