@@ -50,23 +50,23 @@ __device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, 
 // Products over a whole tile. rows_rows: A and B both with rows along K = D (A B^T). tmem_rows: A in
 // tensor memory (128 lanes x 128 values of K, two a column), B's rows along N = D (A B).
 template <typename T, int D>
-__device__ __forceinline__ void rows_rows(uint32_t d, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void rows_rows(uint32_t one, uint32_t d, uint32_t a, uint32_t b) {
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
         const uint32_t at = (k / 4) * kPanel + (k % 4) * 32;
-        tc::mma_ss(d, tc::operand(a + at, 16), tc::operand(b + at, 16), tc::shape<T>(kRows, false), k > 0);
+        tc::mma_ss(one, d, tc::operand(a + at, 16), tc::operand(b + at, 16), tc::shape<T>(kRows, false), k > 0);
     }
 }
 template <typename T, int D>  // over 64 values of K
-__device__ __forceinline__ void tmem_rows(uint32_t d, uint32_t a, uint32_t b, bool add) {
+__device__ __forceinline__ void tmem_rows(uint32_t one, uint32_t d, uint32_t a, uint32_t b, bool add) {
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        tc::mma_ts(d, a + k * 8, tc::operand(b + k * 2048, kPanel), tc::shape<T>(D, true), add || k > 0);
+        tc::mma_ts(one, d, a + k * 8, tc::operand(b + k * 2048, kPanel), tc::shape<T>(D, true), add || k > 0);
 }
 template <typename T, int D, int HALF>  // over 128, the second half HALF columns behind the first
-__device__ __forceinline__ void tmem_rows2(uint32_t d, uint32_t a, uint32_t b, bool add) {
-    tmem_rows<T, D>(d, a, b, add);
-    tmem_rows<T, D>(d, a + HALF, b + 64 * 128, true);
+__device__ __forceinline__ void tmem_rows2(uint32_t one, uint32_t d, uint32_t a, uint32_t b, bool add) {
+    tmem_rows<T, D>(one, d, a, b, add);
+    tmem_rows<T, D>(one, d, a + HALF, b + 64 * 128, true);
 }
 
 // A thread's row of a finished D-column sum, times `f`, to memory; zeros where `live` is false.
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
     using S = FwdSmem<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = tc::smem_addr(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     volatile uint32_t* failed = reinterpret_cast<uint32_t*>(bars + 24);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 25);
@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = *tmem_at;
+    const uint32_t tmem = __shfl_sync(kFullMask, *tmem_at, 0);
 
     int loaded = 0;  // tiles of the ring that warp 16 has asked for
     // 640 x 96 registers at the launch = 512 x 104 + 128 x 64
@@ -174,12 +174,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 __syncwarp();
             }
         } else if (warp == 17) {  // products
+            const uint32_t one = tc::elect();
             const auto scores = [&](int t, int slot) {
-                if (lane == 0) {
-                    rows_rows<T, D>(tmem + t * kRows, base + S::kQ + t * S::kTileBytes, base + S::kRing + slot * S::kTileBytes);
-                    tc::commit(s_full(t));
-                }
-                __syncwarp();
+                rows_rows<T, D>(one, tmem + t * kRows, base + S::kQ + t * S::kTileBytes, base + S::kRing + slot * S::kTileBytes);
+                tc::commit(one, s_full(t));
             };
             bool ok = most == 0 || tc::bar_wait(kv_full(0), 0, failed);
             for (int t = 0; ok && t < 2; ++t)
@@ -187,7 +185,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                     ok = tc::bar_wait(q_full(t), 0, failed);
                     if (ok) scores(t, 0);
                 }
-            if (ok && most && lane == 0) tc::commit(kv_free(0));
+            if (ok && most) tc::commit(one, kv_free(0));
             for (int j = 0; ok && j < most; ++j) {
                 const int vi = 2 * j + 1, vs = vi % kSlots, ki = 2 * j + 2, ks = ki % kSlots;
                 ok = tc::bar_wait(kv_full(vs), (vi / kSlots) & 1, failed);
@@ -199,18 +197,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                     ok = tc::bar_wait(p_full(t), j & 1, failed);
                     if (!ok) break;
                     tc::fence_after();
-                    if (lane == 0) {
-                        tmem_rows2<T, D, 64>(tmem + 2 * kRows + t * D, tmem + t * kRows, base + S::kRing + vs * S::kTileBytes, j > 0);
-                        if (j + 1 == n[t]) tc::commit(o_full(t));
-                    }
-                    __syncwarp();
+                    tmem_rows2<T, D, 64>(one, tmem + 2 * kRows + t * D, tmem + t * kRows, base + S::kRing + vs * S::kTileBytes, j > 0);
+                    if (j + 1 == n[t]) tc::commit(one, o_full(t));
                     if (j + 1 < n[t]) scores(t, ks);
                 }
-                if (ok && lane == 0) {
-                    tc::commit(kv_free(vs));
-                    if (j + 1 < most) tc::commit(kv_free(ks));
+                if (ok) {
+                    tc::commit(one, kv_free(vs));
+                    if (j + 1 < most) tc::commit(one, kv_free(ks));
                 }
-                __syncwarp();
             }
         }
     } else {  // probabilities
@@ -325,8 +319,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 if (n[t]) tc::bar_drain(q_full(t), 0);
             for (int i = max(0, loaded - kSlots); i < loaded; ++i) tc::bar_drain(kv_full(i % kSlots), (i / kSlots) & 1);
         } else if (warp == 17) {
-            if (lane == 0) tc::commit(drained);
-            __syncwarp();
+            tc::commit(tc::elect(), drained);
             tc::bar_drain(drained, 0);
         }
         __syncthreads();
@@ -418,7 +411,7 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
                                             const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
     using S = BwdSmem<D>;
     const uint32_t base = tc::smem_addr(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     // the first keys are seen by the most queries when causal: they start first
     const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.batch;
     const int hk = static_cast<int>(block % heads % a.kv_heads), batch = static_cast<int>(block % heads / a.kv_heads);
@@ -460,6 +453,7 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
         }
         return {it, total > 0, (it + 1) / 2};
     } else if (warp == 9) {  // products
+        const uint32_t one = tc::elect();
         const auto arrived = [&](int item) {  // the tile is there, padding behind the queries' end zeroed
             if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
             const int row = (first + item / 2 % tiles) * kRows;
@@ -469,52 +463,36 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
         };
         bool ok = total == 0 || (tc::bar_wait(bars.own(), 0, failed) && arrived(0));
         if (ok && total) {
-            if (lane == 0) {
-                rows_rows<T, D>(tmem, base + S::kOwn, slot(0));
-                tc::commit(bars.s_full(0));
-            }
-            __syncwarp();
+            rows_rows<T, D>(one, tmem, base + S::kOwn, slot(0));
+            tc::commit(one, bars.s_full(0));
             ok = arrived(1);
-            if (ok && lane == 0) {
-                rows_rows<T, D>(tmem + kW, base + S::kOwn + S::kTileBytes, slot(1));
-                tc::commit(bars.w_full());
+            if (ok) {
+                rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(1));
+                tc::commit(one, bars.w_full());
             }
-            __syncwarp();
         }
         for (int i = 0; ok && i < total; ++i) {
             ok = tc::bar_wait(bars.p_full(), i & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            if (lane == 0) {
-                tmem_rows2<T, D, 64>(tmem + kVV, tmem, slot(2 * i + 1), i > 0);
-                tc::commit(bars.free((2 * i + 1) % kSlots));
-            }
-            __syncwarp();
+            tmem_rows2<T, D, 64>(one, tmem + kVV, tmem, slot(2 * i + 1), i > 0);
+            tc::commit(one, bars.free((2 * i + 1) % kSlots));
             if (i + 1 < total) {
                 ok = arrived(2 * i + 2);
                 if (!ok) break;
-                if (lane == 0) {
-                    rows_rows<T, D>(tmem, base + S::kOwn, slot(2 * i + 2));
-                    tc::commit(bars.s_full(0));
-                }
-                __syncwarp();
+                rows_rows<T, D>(one, tmem, base + S::kOwn, slot(2 * i + 2));
+                tc::commit(one, bars.s_full(0));
             }
             ok = tc::bar_wait(bars.ds_full(), i & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            if (lane == 0) {
-                tmem_rows2<T, D, 64>(tmem + kVK, tmem + kW, slot(2 * i), i > 0);
-                tc::commit(i + 1 < total ? bars.free(2 * i % kSlots) : bars.out_full());
-            }
-            __syncwarp();
+            tmem_rows2<T, D, 64>(one, tmem + kVK, tmem + kW, slot(2 * i), i > 0);
+            tc::commit(one, i + 1 < total ? bars.free(2 * i % kSlots) : bars.out_full());
             if (i + 1 < total) {
                 ok = arrived(2 * i + 3);
                 if (!ok) break;
-                if (lane == 0) {
-                    rows_rows<T, D>(tmem + kW, base + S::kOwn + S::kTileBytes, slot(2 * i + 3));
-                    tc::commit(bars.w_full());
-                }
-                __syncwarp();
+                rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(2 * i + 3));
+                tc::commit(one, bars.w_full());
             }
         }
     } else {
@@ -611,7 +589,7 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
                                            const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
     using S = BwdSmem<D>;
     const uint32_t base = tc::smem_addr(smem);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int64_t heads = static_cast<int64_t>(a.heads) * a.batch, tiles = (a.q_len + kRows - 1) / kRows;
     const int h = static_cast<int>(block % heads % a.heads), batch = static_cast<int>(block % heads / a.heads);
     const int q0 = static_cast<int>(tiles - 1 - block / heads) * kRows, hk = h / a.group;
@@ -638,27 +616,22 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
         }
         return {it, n > 0, 0};
     } else if (warp == 9) {  // products
+        const uint32_t one = tc::elect();
         const auto scores = [&](int j) {
             const int item = 2 * j;
             if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
             if ((j + 1) * kRows > kv_len && kv_len < a.kv_len)
                 zero_rows<D>(smem + S::kRing + item % kSlots * S::kTileBytes, kv_len - j * kRows, lane);
-            if (lane == 0) {
-                rows_rows<T, D>(tmem + (j & 1) * kRows, base + S::kOwn, slot(item));
-                tc::commit(bars.s_full(j & 1));
-            }
-            __syncwarp();
+            rows_rows<T, D>(one, tmem + (j & 1) * kRows, base + S::kOwn, slot(item));
+            tc::commit(one, bars.s_full(j & 1));
             return true;
         };
         const auto weights = [&](int j) {
             const int item = 2 * j + 1;
             if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
-            if (lane == 0) {
-                rows_rows<T, D>(tmem + kW, base + S::kOwn + S::kTileBytes, slot(item));
-                tc::commit(bars.w_full());
-                tc::commit(bars.free(item % kSlots));
-            }
-            __syncwarp();
+            rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(item));
+            tc::commit(one, bars.w_full());
+            tc::commit(one, bars.free(item % kSlots));
             return true;
         };
         bool ok = n == 0 || (tc::bar_wait(bars.own(), 0, failed) && scores(0) && weights(0));
@@ -667,11 +640,8 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
             if (ok) ok = tc::bar_wait(bars.ds_full(), j & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            if (lane == 0) {
-                tmem_rows2<T, D, 64>(tmem + kVQ, tmem + kW, slot(2 * j), j > 0);
-                tc::commit(j + 1 < n ? bars.free(2 * j % kSlots) : bars.out_full());
-            }
-            __syncwarp();
+            tmem_rows2<T, D, 64>(one, tmem + kVQ, tmem + kW, slot(2 * j), j > 0);
+            tc::commit(one, j + 1 < n ? bars.free(2 * j % kSlots) : bars.out_full());
             if (j + 1 < n) ok = weights(j + 1);
         }
     } else {
@@ -747,13 +717,13 @@ __global__ void __launch_bounds__(320, 1) attn_bwd_tc_kernel(const AttnArgs a, c
     uint64_t* words = reinterpret_cast<uint64_t*>(smem + S::kBars);
     volatile uint32_t* failed = reinterpret_cast<uint32_t*>(words + BwdBars::kFailed);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(words + BwdBars::kTmem);
-    const int warp = threadIdx.x >> 5;
+    const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0);
     if (threadIdx.x == 0) bwd_init(bars, failed);
     if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
-    const uint32_t tmem = *tmem_at;
+    const uint32_t tmem = __shfl_sync(kFullMask, *tmem_at, 0);
     const Loaded asked = blockIdx.x < kv_blocks ? bwd_kv_tile<T, D>(a, maps, blockIdx.x, smem, bars, tmem, failed)
                                                 : bwd_q_tile<T, D>(a, maps, blockIdx.x - kv_blocks, smem, bars, tmem, failed);
     tc::fence_before();
@@ -764,8 +734,7 @@ __global__ void __launch_bounds__(320, 1) attn_bwd_tc_kernel(const AttnArgs a, c
             for (int i = max(0, asked.ring - kSlots); i < asked.ring; ++i) tc::bar_drain(bars.full(i % kSlots), (i / kSlots) & 1);
             for (int i = max(0, asked.stats - 2); i < asked.stats; ++i) tc::bar_drain(bars.stat_full(i & 1), (i / 2) & 1);
         } else if (warp == 9) {
-            if (threadIdx.x % 32 == 0) tc::commit(bars.drained());
-            __syncwarp();
+            tc::commit(tc::elect(), bars.drained());
             tc::bar_drain(bars.drained(), 0);
         }
         __syncthreads();

@@ -26,43 +26,38 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// Whether the phase of `parity` is complete; the warp sleeps until it is, or for about 0.1 ms.
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(bar), "r"(parity)
+        : "r"(bar), "r"(parity), "r"(100000)
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
+constexpr long long kWaitCycles = 4000000000ll;  // two seconds at the highest clock
 
 // Waits, as a whole warp, for the barrier's phase of `parity`. Gives up after two seconds, or once
-// another warp of the CTA has: returns false then, the same for every lane, with *failed set.
+// another warp of the CTA has: returns false then, the same for every lane, with *failed set. The
+// waiting is left to the hardware: warps that poll take issue slots from those that compute.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
     if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
-    const uint64_t start = now_ns();
+    const long long start = clock64();
     for (;;) {
-#pragma unroll 1
-        for (int i = 0; i < 64; ++i)
-            if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
-        if (__any_sync(0xffffffffu, *failed != 0 || now_ns() - start > 2000000000ull)) {
+        if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, *failed != 0 || clock64() - start > kWaitCycles)) {
             *failed = 1;
             return false;
         }
     }
 }
-
 // The same wait whatever *failed says: for copies and products still in flight when a kernel gives up.
 __device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
-    const uint64_t start = now_ns();
-    while (!__all_sync(0xffffffffu, bar_try(bar, parity)) && !__any_sync(0xffffffffu, now_ns() - start > 2000000000ull)) {
+    const long long start = clock64();
+    while (!__all_sync(0xffffffffu, bar_try(bar, parity)) && !__any_sync(0xffffffffu, clock64() - start > kWaitCycles)) {
     }
 }
 
@@ -163,24 +158,35 @@ __host__ __device__ constexpr uint32_t shape(int n, bool b_along_n) {
     return 1u << 4 | Format<T>::code << 7 | Format<T>::code << 10 | (b_along_n ? 1u << 16 : 0u) |
            static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(128 >> 4) << 24;
 }
-// D (tensor memory) = A B + (add ? D : 0) over 16 values of K; one thread issues it.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+// One lane of a converged warp, always the same one. The products are issued by the whole warp under
+// this lane's predicate: their operands then stay in uniform registers. Behind a branch that one lane
+// takes, each product waited some 80 cycles for its operands to get there.
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+// D (tensor memory) = A B + (add ? D : 0) over 16 values of K, issued by the lane with `one`.
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add)), "r"(one)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add)), "r"(one)
         : "memory");
 }
-// Arrives on `bar` once every product this thread has issued is complete.
-__device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// Arrives on `bar` once every product that the lane with `one` has issued is complete.
+__device__ __forceinline__ void commit(uint32_t one, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one)
+        : "memory");
 }
 
 // ---- registers ----
@@ -241,6 +247,30 @@ __device__ __forceinline__ Two mul2(Two a, Two b) {
     Two r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
+}
+
+// 2^x on the multiply-add pipes, for x up to 127 (below -126: 2^-126): x = n + f with n the nearest
+// whole number (the low bits of x + 1.5 2^23), 2^f by a polynomial fitted for the least relative
+// error on [-1/2, 1/2] (2.2e-7 in 32 bits), and n added to the exponent. The special-function unit
+// gives 16 values a cycle and SM, half of what the products of 64-value rows leave time for.
+__device__ __forceinline__ void exp2_poly(Two x, float& lo, float& hi) {
+    float a, b;
+    split(x, a, b);
+    x = two(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const Two magic = two(12582912.f, 12582912.f), back = two(-12582912.f, -12582912.f), minus = two(-1.f, -1.f);
+    const Two t = add2(x, magic);
+    const Two f = fma2(add2(t, back), minus, x);
+    Two p = two(0x1.5c08e4p-10f, 0x1.5c08e4p-10f);
+    p = fma2(p, f, two(0x1.3d0c52p-7f, 0x1.3d0c52p-7f));
+    p = fma2(p, f, two(0x1.c6b6e4p-5f, 0x1.c6b6e4p-5f));
+    p = fma2(p, f, two(0x1.ebf918p-3f, 0x1.ebf918p-3f));
+    p = fma2(p, f, two(0x1.62e428p-1f, 0x1.62e428p-1f));
+    p = fma2(p, f, two(0x1.000002p+0f, 0x1.000002p+0f));
+    float n0, n1;
+    split(t, n0, n1);
+    split(p, lo, hi);
+    lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(n0) << 23));
+    hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(n1) << 23));
 }
 
 }  // namespace tc
