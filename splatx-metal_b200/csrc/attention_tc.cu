@@ -57,16 +57,16 @@ __device__ __forceinline__ void rows_rows(uint32_t one, uint32_t d, uint32_t a, 
         tc::mma_ss(one, d, tc::operand(a + at, 16), tc::operand(b + at, 16), tc::shape<T>(kRows, false), k > 0);
     }
 }
-template <typename T, int D>  // over 64 values of K
+template <typename T, int D, int STEPS>  // over 64 values of K
 __device__ __forceinline__ void tmem_rows(uint32_t one, uint32_t d, uint32_t a, uint32_t b, bool add) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < STEPS; ++k)
         tc::mma_ts(one, d, a + k * 8, tc::operand(b + k * 2048, kPanel), tc::shape<T>(D, true), add || k > 0);
 }
 template <typename T, int D, int HALF>  // over 128, the second half HALF columns behind the first
 __device__ __forceinline__ void tmem_rows2(uint32_t one, uint32_t d, uint32_t a, uint32_t b, bool add) {
-    tmem_rows<T, D>(one, d, a, b, add);
-    tmem_rows<T, D>(one, d, a + HALF, b + 64 * 128, true);
+    tmem_rows<T, D, 4>(one, d, a, b, add);
+    tmem_rows<T, D, 4>(one, d, a + HALF, b + 64 * 128, true);
 }
 
 // A thread's row of a finished D-column sum, times `f`, to memory; zeros where `live` is false.
@@ -94,17 +94,20 @@ __device__ __forceinline__ void store_row(T* out, uint32_t at, float f, int dim,
     }
 }
 
-// The forward. A CTA owns two tiles of 128 queries of one head. Eight warps make a tile's
-// probabilities, two threads a query with 64 of a key tile's columns each (warps 0-7 the first tile,
-// 8-15 the second); warp 16 loads, warp 17 issues the products. While one tile's warps work on their
-// scores the tensor cores compute the other's: S = Q K^T into tensor memory, the probabilities back
-// over S in 16 bits, O += P V from there.
-constexpr int kFwdThreads = 640;  // warps 18 and 19 only give up their registers
+// The forward. A CTA owns two tiles of 128 queries of one head; warps 0-3 and 4-7 make their
+// probabilities (a thread per query), warp 8 loads, warp 9 issues the products. While one tile's
+// warps work on its scores the tensor cores compute for the other: S = Q K^T into tensor memory, the
+// probabilities back there in 16 bits, O += P V from there. With 64 columns of O tensor memory has
+// room for P beside S, and the next S is computed while the probabilities of this one are made; with
+// 128 P lies over S.
+constexpr int kFwdThreads = 384;  // warps 10 and 11 only give up their registers
+// Of 16 pairs of exponentials, those on the multiply-add pipes.
+template <int D>
+constexpr int kPoly = D == 64 ? 1 : 3;
 template <int D>
 struct FwdSmem {
     static constexpr int kTileBytes = D / 64 * kPanel;
-    static constexpr int kQ = 0, kRing = 2 * kTileBytes, kTops = kRing + kSlots * kTileBytes;
-    static constexpr int kBars = kTops + 2 * 2 * kRows * 4;  // a value of each thread for its query's other one
+    static constexpr int kQ = 0, kRing = 2 * kTileBytes, kBars = kRing + kSlots * kTileBytes;
     static constexpr int kBytes = kBars + 256;
 };
 
@@ -115,16 +118,19 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
     const uint32_t base = tc::smem_addr(smem);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(bars + 24);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 25);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(bars + 28);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 29);
     const uint32_t bar0 = base + S::kBars;
     const auto kv_full = [&](int s) { return bar0 + 8 * s; };
     const auto kv_free = [&](int s) { return bar0 + 8 * (kSlots + s); };
     const auto q_full = [&](int t) { return bar0 + 8 * (2 * kSlots + t); };
     const auto s_full = [&](int t) { return bar0 + 8 * (2 * kSlots + 2 + t); };
-    const auto p_full = [&](int t) { return bar0 + 8 * (2 * kSlots + 4 + t); };
-    const auto o_full = [&](int t) { return bar0 + 8 * (2 * kSlots + 6 + t); };
-    const uint32_t drained = bar0 + 8 * (2 * kSlots + 8);
+    const auto p_full = [&](int t, int half) { return bar0 + 8 * (2 * kSlots + 4 + 2 * t + half); };
+    const auto o_full = [&](int t) { return bar0 + 8 * (2 * kSlots + 8 + t); };  // apart: of every tile, else of the last
+    const auto s_free = [&](int t) { return bar0 + 8 * (2 * kSlots + 10 + t); };
+    const uint32_t drained = bar0 + 8 * (2 * kSlots + 12);
+    constexpr bool kApart = D == 64;  // P beside S
+    constexpr uint32_t kO = 2 * kRows, kP = kApart ? kO + 2 * D : 0, kPStep = kApart ? 64 : kRows;
 
     // the last queries see the most keys when causal: they start first
     const int64_t pairs = (a.q_len + 2 * kRows - 1) / (2 * kRows), heads = a.heads * a.batch;
@@ -146,23 +152,25 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
         for (int t = 0; t < 2; ++t) {
             tc::bar_init(q_full(t), 1);
             tc::bar_init(s_full(t), 1);
-            tc::bar_init(p_full(t), 8);
+            tc::bar_init(p_full(t, 0), 4);
+            tc::bar_init(p_full(t, 1), 4);
             tc::bar_init(o_full(t), 1);
+            tc::bar_init(s_free(t), 4);
         }
         tc::bar_init(drained, 1);
         tc::bar_init_fence();
     }
-    if (warp == 17) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
+    if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = __shfl_sync(kFullMask, *tmem_at, 0);
 
-    int loaded = 0;  // tiles of the ring that warp 16 has asked for
-    // 640 x 96 registers at the launch = 512 x 104 + 128 x 64
-    if (warp >= 16) {
-        tc::fewer_registers<64>();
-        if (warp == 16) {  // loads: Q tiles, then K0 V0 K1 V1 ... around the ring
+    int loaded = 0;  // tiles of the ring that warp 8 has asked for
+    // 384 x 168 registers at the launch = 256 x 216 + 128 x 72
+    if (warp >= 8) {
+        tc::fewer_registers<72>();
+        if (warp == 8) {  // loads: Q tiles, then K0 V0 K1 V1 ... around the ring
             if (lane == 0)
                 for (int t = 0; t < 2; ++t)
                     if (n[t]) load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t));
@@ -173,7 +181,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                     load_rows<D>(base + S::kRing + s * S::kTileBytes, loaded & 1 ? &maps.v : &maps.k, loaded / 2 * kRows, hk, static_cast<int>(w.b), kv_full(s));
                 __syncwarp();
             }
-        } else if (warp == 17) {  // products
+        } else if (warp == 9) {  // products
             const uint32_t one = tc::elect();
             const auto scores = [&](int t, int slot) {
                 rows_rows<T, D>(one, tmem + t * kRows, base + S::kQ + t * S::kTileBytes, base + S::kRing + slot * S::kTileBytes);
@@ -194,12 +202,22 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 if (j + 1 < most) ok = tc::bar_wait(kv_full(ks), (ki / kSlots) & 1, failed);
                 for (int t = 0; ok && t < 2; ++t) {
                     if (j >= n[t]) continue;
-                    ok = tc::bar_wait(p_full(t), j & 1, failed);
+                    if (kApart && j + 1 < n[t]) {
+                        ok = tc::bar_wait(s_free(t), j & 1, failed);
+                        if (!ok) break;
+                        tc::fence_after();
+                        scores(t, ks);
+                    }
+                    for (int half = 0; ok && half < 2; ++half) {  // the first 64 keys while the others' p are made
+                        ok = tc::bar_wait(p_full(t, half), j & 1, failed);
+                        if (!ok) break;
+                        tc::fence_after();
+                        tmem_rows<T, D, 4>(one, tmem + kO + t * D, tmem + kP + t * kPStep + half * 32,
+                                           base + S::kRing + vs * S::kTileBytes + half * 64 * 128, j > 0 || half > 0);
+                    }
                     if (!ok) break;
-                    tc::fence_after();
-                    tmem_rows2<T, D, 64>(one, tmem + 2 * kRows + t * D, tmem + t * kRows, base + S::kRing + vs * S::kTileBytes, j > 0);
-                    if (j + 1 == n[t]) tc::commit(one, o_full(t));
-                    if (j + 1 < n[t]) scores(t, ks);
+                    if (kApart || j + 1 == n[t]) tc::commit(one, o_full(t));
+                    if (!kApart && j + 1 < n[t]) scores(t, ks);
                 }
                 if (ok) {
                     tc::commit(one, kv_free(vs));
@@ -207,39 +225,33 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 }
             }
         }
-    } else {  // probabilities
-        tc::more_registers<104>();
-        const int t = warp >> 3, half = warp >> 2 & 1, mine = n[t];
-        const int lane_row = (warp & 3) * 32 + lane, row = q0 + t * kRows + lane_row;
+    } else {  // softmax: a thread per query
+        tc::more_registers<216>();
+        const int t = warp >> 2, mine = n[t];
+        const int row = q0 + t * kRows + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + t * kRows + half * 64, o_at = tmem + lanes + 2 * kRows + t * D + half * (D / 2);
-        float* mine_to = reinterpret_cast<float*>(smem + S::kTops) + (t * 2 + half) * kRows + lane_row;
-        const float* other = reinterpret_cast<const float*>(smem + S::kTops) + (t * 2 + 1 - half) * kRows + lane_row;
-        // The value of the query's other thread. A warp that gives up still takes part in all of the
-        // exchanges, so that none of the others waits for it.
-        int exchanges = mine + 1;
-        const auto exchange = [&](float x) {
-            --exchanges;
-            *mine_to = x;
-            asm volatile("bar.sync %0, 256;" ::"r"(t + 1) : "memory");
-            return *other;
-        };
+        const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + kO + t * D, p_at = tmem + lanes + kP + t * kPStep;
         float m = -INFINITY, l = 0.f;  // m: the base-2 exponent the sums are relative to
         bool ok = true;
         for (int j = 0; j < mine; ++j) {
             ok = tc::bar_wait(s_full(t), j & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            uint32_t r[2][32];
-            tc::tmem_load32(r[0], s_at);
-            tc::tmem_load32(r[1], s_at + 32);
-            tc::wait_ld(r[0], r[1]);
-            // keys of these columns that the query sees: those below `end`
-            const int64_t last = static_cast<int64_t>(row) + w.ahead + 1;
-            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j) * kRows - half * 64);
-            if (__any_sync(kFullMask, end < 64)) {
+            uint32_t r[4][32];
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 4; ++c) tc::tmem_load32(r[c], s_at + c * 32);
+            tc::wait_ld(r[0], r[1], r[2], r[3]);
+            if (kApart) {
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(s_free(t));
+            }
+            // keys of this tile that the query sees: those below `end`
+            const int64_t last = static_cast<int64_t>(row) + w.ahead + 1;
+            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j) * kRows);
+            if (__any_sync(kFullMask, end < kRows)) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
 #pragma unroll
                     for (int i = 0; i < 32; ++i)
                         if (c * 32 + i >= end) r[c][i] = 0xff800000u;
@@ -247,30 +259,33 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
             float top[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                const uint32_t* x = r[c >> 1] + (c & 1) * 16;
-                top[c] = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+                top[c] = fmaxf(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]));
 #pragma unroll
-                for (int i = 2; i < 16; i += 2) top[c] = tc::max3(top[c], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                for (int i = 2; i < 32; i += 2) top[c] = tc::max3(top[c], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
             }
-            float seen = fmaxf(tc::max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
-            seen = fmaxf(seen, exchange(seen));
+            const float seen = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
             // The sums move to a new maximum only when it is 2^8 above the old one: 32 bits hold that,
             // and the output's rows are then hardly ever read back and scaled.
             if (j == 0) {
                 m = seen;
             } else if (__any_sync(kFullMask, seen > m + 8.f)) {
+                if (kApart) {  // the sums are at rest once the last tile's product is complete
+                    ok = tc::bar_wait(o_full(t), (j - 1) & 1, failed);
+                    if (!ok) break;
+                    tc::fence_after();
+                }
                 const float to = fmaxf(m, seen);
                 const float f = to == -INFINITY ? 1.f : tc::exp2_approx(m - to);
                 l *= f;
                 m = to;
-#pragma unroll 1
-                for (int c = 0; c < D / 2; c += 16) {
-                    uint32_t o[16];
-                    tc::tmem_load16(o, o_at + c);
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) {
+                    uint32_t o[32];
+                    tc::tmem_load32(o, o_at + c * 32);
                     tc::wait_ld(o);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                    tc::tmem_store16(o_at + c, o);
+                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                    tc::tmem_store32(o_at + c * 32, o);
                 }
             }
             const float less = m == -INFINITY ? 0.f : -m;
@@ -278,54 +293,62 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
             tc::Two sum[2] = {tc::two(0.f, 0.f), tc::two(0.f, 0.f)};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t p[16];
+                uint32_t p[32];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const tc::Two x = tc::fma2(tc::two(__uint_as_float(r[c][2 * i]), __uint_as_float(r[c][2 * i + 1])), times, plus);
+                for (int i = 0; i < 32; ++i) {
+                    const int e = c * 64 + i * 2;
+                    const tc::Two x = tc::fma2(tc::two(__uint_as_float(r[e >> 5][e & 31]), __uint_as_float(r[e >> 5][(e & 31) + 1])), times, plus);
                     float lo, hi;
-                    tc::split(x, lo, hi);
-                    lo = tc::exp2_approx(lo);
-                    hi = tc::exp2_approx(hi);
+                    if (i % 16 < kPoly<D>) {
+                        tc::exp2_poly(x, lo, hi);
+                    } else {
+                        tc::split(x, lo, hi);
+                        lo = tc::exp2_approx(lo);
+                        hi = tc::exp2_approx(hi);
+                    }
                     sum[i & 1] = tc::add2(sum[i & 1], tc::two(lo, hi));
                     p[i] = tc::pack2<T>(lo, hi);
                 }
-                tc::tmem_store16(s_at + c * 16, p);
+                if (kApart && c == 0 && j > 0) {  // the last tile's p have been read
+                    ok = tc::bar_wait(o_full(t), (j - 1) & 1, failed);
+                    if (!ok) break;
+                    tc::fence_after();
+                }
+                tc::tmem_store32(p_at + c * 32, p);
+                tc::wait_st();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(p_full(t, c));
             }
-            tc::wait_st();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::bar_arrive(p_full(t));
+            if (!ok) break;
             float lo, hi;
             tc::split(tc::add2(sum[0], sum[1]), lo, hi);
             l += lo + hi;
         }
-        if (ok && mine) ok = tc::bar_wait(o_full(t), 0, failed);
+        if (ok && mine) ok = tc::bar_wait(o_full(t), kApart ? (mine - 1) & 1 : 0, failed);
         if (ok) {
             tc::fence_after();
-            l += exchange(l);
             const bool live = row < w.q_len && m != -INFINITY;
-            // each of the two writes half of the query's columns
             T* out = static_cast<T*>(a.out.data) + w.b * a.out.batch_stride + w.h * a.out.head_stride + row * a.out.token_stride;
-            store_row<T, D / 2>(out + half * (D / 2), o_at, live ? 1.f / l : 0.f, a.dim - half * (D / 2), row < a.q_len, live, mine > 0);
-            if (row < a.q_len && half == 0) a.lse[bh * a.q_len + row] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
+            store_row<T, D>(out, o_at, live ? 1.f / l : 0.f, a.dim, row < a.q_len, live, mine > 0);
+            if (row < a.q_len) a.lse[bh * a.q_len + row] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
         }
-        while (exchanges > 0) exchange(0.f);
         tc::fence_before();
     }
     __syncthreads();
     if (*failed) {  // nothing may land in this CTA's memory after it has gone
-        if (warp == 16) {
+        if (warp == 8) {
             for (int t = 0; t < 2; ++t)
                 if (n[t]) tc::bar_drain(q_full(t), 0);
             for (int i = max(0, loaded - kSlots); i < loaded; ++i) tc::bar_drain(kv_full(i % kSlots), (i / kSlots) & 1);
-        } else if (warp == 17) {
+        } else if (warp == 9) {
             tc::commit(tc::elect(), drained);
             tc::bar_drain(drained, 0);
         }
         __syncthreads();
         if (threadIdx.x == 0) atomicOr(&g_attention_status, 1u);
     }
-    if (warp == 17) tc::tmem_free(tmem, 512);
+    if (warp == 9) tc::tmem_free(tmem, 512);
 }
 
 // The backward. Both kinds of CTA run 256 threads over a 128 x 128 tile of scores, a thread per row,
