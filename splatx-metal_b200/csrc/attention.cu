@@ -165,8 +165,8 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_kernel(const AttnArgs a) {
     store_rows<T, D>(acc, f, a.out, w.b, w.h, q0, a.q_len, a.dim);
 }
 
-// delta = sum(g out) per query, and lse in base 2 with +inf for a query that sees no key (exp2 then
-// gives 0). Both arrays have rows of a.q_pad: the tensor-core kernels read whole tiles of them. L
+// Minus delta = sum(g out) per query, and minus lse in base 2 with -inf for a query that sees no key
+// (exp2 then gives 0): what the scores' tiles add. Both arrays have rows of a.q_pad: the tensor-core kernels read whole tiles of them. L
 // lanes share a query, each reading V values at a time. Bound by the reads of out and its gradient.
 template <typename T, int V, int L>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     const int per_head = static_cast<int>(a.q_pad / kQueries);
     const int64_t bh = blockIdx.x / per_head, row = static_cast<int64_t>(blockIdx.x % per_head) * kQueries + threadIdx.x / L;
     const AttnHead w = attn_head(a, bh % a.heads, bh / a.heads);
-    float s = 0.f, lse = INFINITY;
+    float s = 0.f, lse = -INFINITY;
     if (row < w.q_len) {
         const T* o = static_cast<const T*>(a.out.data) + w.b * a.out.batch_stride + w.h * a.out.head_stride + row * a.out.token_stride;
         const T* g = static_cast<const T*>(a.g.data) + w.b * a.g.batch_stride + w.h * a.g.head_stride + row * a.g.token_stride;
@@ -184,13 +184,13 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
             for (int e = 0; e < V; ++e) s = fmaf(to_f32(x.v[e]), to_f32(y.v[e]), s);
         }
         const float x = a.lse[bh * a.q_len + row];
-        if (x != -INFINITY) lse = fmaf(x, kLog2e, -a.p_shift);
+        if (x != -INFINITY) lse = fmaf(x, -kLog2e, a.p_shift);
     }
 #pragma unroll
     for (int off = L / 2; off; off >>= 1) s += __shfl_xor_sync(kFullMask, s, off);
     if (threadIdx.x % L == 0) {
-        a.delta[bh * a.q_pad + row] = s;
-        a.lse2[bh * a.q_pad + row] = lse;
+        a.minus_delta[bh * a.q_pad + row] = -s;
+        a.minus_lse2[bh * a.q_pad + row] = lse;
     }
 }
 
@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_kv_kernel(const AttnArgs a)
     }
     for (int64_t h = hk * a.group; h < (hk + 1) * a.group; ++h) {
         const AttnHead w = attn_head(a, h, blockIdx.z);
-        const float* lse = a.lse2 + (w.b * a.heads + h) * a.q_pad;
-        const float* delta = a.delta + (w.b * a.heads + h) * a.q_pad;
+        const float* lse = a.minus_lse2 + (w.b * a.heads + h) * a.q_pad;
+        const float* delta = a.minus_delta + (w.b * a.heads + h) * a.q_pad;
         if (k0 >= w.kv_len) break;
         for (int64_t q0 = attn_queries_begin(w, k0) / kT * kT; q0 < w.q_len; q0 += kT) {
             __syncthreads();
@@ -247,14 +247,14 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_kv_kernel(const AttnArgs a)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int64_t row = q0 + tx() + 16 * j;
-                const float x = row < w.q_len ? lse[row] : INFINITY, d = row < w.q_len ? delta[row] : 0.f;
+                const float x = row < w.q_len ? lse[row] : -INFINITY, d = row < w.q_len ? delta[row] : 0.f;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int64_t key = k0 + ty() * 4 + i;
                     const bool seen = attn_sees(w, row, key);
-                    const float p = seen ? exp2f(fmaf(s[i][j], a.scale_log2, -x)) : 0.f;
+                    const float p = seen ? exp2f(fmaf(s[i][j], a.scale_log2, x)) : 0.f;
                     P[(ty() * 4 + i) * kLd + tx() + 16 * j] = p;
-                    S[(ty() * 4 + i) * kLd + tx() + 16 * j] = seen ? p * (dp[i][j] - d) : 0.f;
+                    S[(ty() * 4 + i) * kLd + tx() + 16 * j] = seen ? p * (dp[i][j] + d) : 0.f;
                 }
             }
             __syncthreads();
@@ -281,8 +281,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_q_kernel(const AttnArgs a) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = q0 + ty() * 4 + i, at = (w.b * a.heads + w.h) * a.q_pad + row;
-        x[i] = row < w.q_len ? a.lse2[at] : INFINITY;
-        d[i] = row < w.q_len ? a.delta[at] : 0.f;
+        x[i] = row < w.q_len ? a.minus_lse2[at] : -INFINITY;
+        d[i] = row < w.q_len ? a.minus_delta[at] : 0.f;
     }
     load_tile<T, D>(Q, a.q, w.b, w.h, q0, w.q_len, a.dim);
     load_tile<T, D>(G, a.g, w.b, w.h, q0, w.q_len, a.dim);
@@ -300,8 +300,8 @@ __global__ void __launch_bounds__(kThreads) attn_bwd_q_kernel(const AttnArgs a) 
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const bool seen = attn_sees(w, q0 + ty() * 4 + i, k0 + tx() + 16 * j);
-                const float p = seen ? exp2f(fmaf(s[i][j], a.scale_log2, -x[i])) : 0.f;
-                S[(ty() * 4 + i) * kLd + tx() + 16 * j] = seen ? p * (dp[i][j] - d[i]) : 0.f;
+                const float p = seen ? exp2f(fmaf(s[i][j], a.scale_log2, x[i])) : 0.f;
+                S[(ty() * 4 + i) * kLd + tx() + 16 * j] = seen ? p * (dp[i][j] + d[i]) : 0.f;
             }
         __syncthreads();
         add_product<D>(dq, S, K);
@@ -384,8 +384,8 @@ void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn&
     a.v_k = out.v_k;
     a.v_v = out.v_v;
     a.lse = const_cast<float*>(g.lse);
-    a.lse2 = static_cast<float*>(ws);
-    a.delta = a.lse2 + a.batch * a.heads * a.q_pad;
+    a.minus_lse2 = static_cast<float*>(ws);
+    a.minus_delta = a.minus_lse2 + a.batch * a.heads * a.q_pad;
     if (a.batch == 0) return;
     const bool tensor = attention_tc_takes(a) && attention_tc_takes_view(a, a.g, a.q_len, a.heads) &&
                         attention_tc_takes_view(a, a.v_q, a.q_len, a.heads) &&
@@ -394,7 +394,7 @@ void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn&
     const bool half = tensor && a.dtype == SXCUDA_F16;
     if (half) {
         a.p_shift = kHalfShift;
-        a.largest = reinterpret_cast<uint32_t*>(a.delta + a.batch * a.heads * a.q_pad);
+        a.largest = reinterpret_cast<uint32_t*>(a.minus_delta + a.batch * a.heads * a.q_pad);
         cuda_check(cudaMemsetAsync(a.largest, 0, 2 * sizeof(uint32_t), s), "attention_bwd");
         const auto kernel = attn_largest_kernel<__half>;
         SX_LAUNCH(kernel, blocks_for(a.q_len, 64) * a.heads * static_cast<unsigned>(a.batch), 256, 0, s, a, a.g, a.q_lens, a.q_len,

@@ -429,6 +429,25 @@ __device__ __forceinline__ HalfScale half_scale(const AttnArgs& a) {
     return h;
 }
 
+__device__ __forceinline__ tc::Two pair(const uint32_t (&r)[32], int i) { return tc::two(__uint_as_float(r[i]), __uint_as_float(r[i + 1])); }
+__device__ __forceinline__ void set_pair(uint32_t (&r)[32], int i, tc::Two x) {
+    float lo, hi;
+    tc::split(x, lo, hi);
+    r[i] = __float_as_uint(lo);
+    r[i + 1] = __float_as_uint(hi);
+}
+template <typename T>
+__device__ __forceinline__ tc::Two scaled(tc::Two x, tc::Two by) {
+    if constexpr (std::is_same_v<T, __half>) return tc::mul2(x, by);
+    return x;
+}
+// Columns outside lo..hi become zeros (a key or query that is not seen; what was there may be NaN).
+__device__ __forceinline__ void keep_columns(uint32_t (&r)[32], int lo, int hi) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (i < lo || i >= hi) r[i] = 0u;
+}
+
 template <typename T, int D>
 __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
                                             const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
@@ -468,8 +487,8 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
                     const int64_t at = (static_cast<int64_t>(batch) * a.heads + h) * a.q_pad + row;
                     const uint32_t to = base + S::kStats + (i & 1) * 2 * kRows * 4;
                     tc::bar_expect(bars.stat_full(i & 1), 2 * kRows * 4);
-                    tc::bulk_load(to, a.lse2 + at, kRows * 4, bars.stat_full(i & 1));
-                    tc::bulk_load(to + kRows * 4, a.delta + at, kRows * 4, bars.stat_full(i & 1));
+                    tc::bulk_load(to, a.minus_lse2 + at, kRows * 4, bars.stat_full(i & 1));
+                    tc::bulk_load(to + kRows * 4, a.minus_delta + at, kRows * 4, bars.stat_full(i & 1));
                 }
             }
             __syncwarp();
@@ -524,14 +543,15 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + half * 64, w_at = s_at + kW;
         const HalfScale scale = half_scale<T>(a);
+        const tc::Two times = tc::two(a.scale_log2, a.scale_log2), ds_scale = tc::two(scale.p * scale.ds, scale.p * scale.ds);
         bool ok = true;
         for (int i = 0; i < total; ++i) {
             const int64_t q0 = static_cast<int64_t>(first + i % tiles) * kRows + half * 64;
             ok = tc::bar_wait(bars.s_full(0), i & 1, failed) && tc::bar_wait(bars.stat_full(i & 1), (i / 2) & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            const float4* lse = reinterpret_cast<const float4*>(smem + S::kStats + (i & 1) * 2 * kRows * 4) + half * 16;
-            const float4* delta = lse + kRows / 4;
+            const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(smem + S::kStats + (i & 1) * 2 * kRows * 4) + half * 16;
+            const ulonglong2* delta = lse + kRows / 4;
             uint32_t r[2][32];
             tc::tmem_load32(r[0], s_at);
             tc::tmem_load32(r[1], s_at + 32);
@@ -542,20 +562,19 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
             const bool cut = __any_sync(kFullMask, lo > 0 || hi < 64);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
-                    const float4 x = lse[c * 8 + e / 4];
-                    const float xs[4] = {x.x, x.y, x.z, x.w};
+                    const ulonglong2 x = lse[c * 8 + e / 4];
+                    float v[4];
+                    tc::split(tc::fma2(pair(r[c], e), times, tc::Two{x.x}), v[0], v[1]);
+                    tc::split(tc::fma2(pair(r[c], e + 2), times, tc::Two{x.y}), v[2], v[3]);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        float v = tc::exp2_approx(fmaf(__uint_as_float(r[c][e + k]), a.scale_log2, -xs[k]));
-                        if (cut && (c * 32 + e + k < lo || c * 32 + e + k >= hi)) v = 0.f;
-                        r[c][e + k] = __float_as_uint(v);
-                    }
-                    p[e / 2] = tc::pack2<T>(__uint_as_float(r[c][e]), __uint_as_float(r[c][e + 1]));
-                    p[e / 2 + 1] = tc::pack2<T>(__uint_as_float(r[c][e + 2]), __uint_as_float(r[c][e + 3]));
+                    for (int k = 0; k < 4; ++k) r[c][e + k] = __float_as_uint(tc::exp2_approx(v[k]));
                 }
+                if (cut) keep_columns(r[c], lo - c * 32, hi - c * 32);
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p[e] = tc::pack2<T>(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1]));
                 tc::tmem_store16(s_at + c * 16, p);
             }
             tc::wait_st();
@@ -571,21 +590,16 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
             tc::wait_ld(g[0], g[1]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
-                    const float4 x = delta[c * 8 + e / 4];
-                    const float xs[4] = {x.x, x.y, x.z, x.w};
-                    float v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        v[k] = __uint_as_float(r[c][e + k]) * (__uint_as_float(g[c][e + k]) - xs[k]);
-                        if constexpr (std::is_same_v<T, __half>) v[k] *= scale.p * scale.ds;
-                        if (cut && (c * 32 + e + k < lo || c * 32 + e + k >= hi)) v[k] = 0.f;
-                    }
-                    p[e / 2] = tc::pack2<T>(v[0], v[1]);
-                    p[e / 2 + 1] = tc::pack2<T>(v[2], v[3]);
+                    const ulonglong2 x = delta[c * 8 + e / 4];
+                    set_pair(g[c], e, scaled<T>(tc::mul2(pair(r[c], e), tc::add2(pair(g[c], e), tc::Two{x.x})), ds_scale));
+                    set_pair(g[c], e + 2, scaled<T>(tc::mul2(pair(r[c], e + 2), tc::add2(pair(g[c], e + 2), tc::Two{x.y})), ds_scale));
                 }
+                if (cut) keep_columns(g[c], lo - c * 32, hi - c * 32);
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) p[e] = tc::pack2<T>(__uint_as_float(g[c][2 * e]), __uint_as_float(g[c][2 * e + 1]));
                 tc::tmem_store16(w_at + c * 16, p);
             }
             tc::wait_st();
@@ -673,8 +687,9 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + half * 64, w_at = s_at + kW;
         const int64_t at = (static_cast<int64_t>(batch) * a.heads + h) * a.q_pad + row;  // q_pad holds whole tiles
-        const float lse = a.lse2[at], delta = a.delta[at];
+        const tc::Two lse = tc::two(a.minus_lse2[at], a.minus_lse2[at]), delta = tc::two(a.minus_delta[at], a.minus_delta[at]);
         const HalfScale scale = half_scale<T>(a);
+        const tc::Two times = tc::two(a.scale_log2, a.scale_log2), ds_scale = tc::two(scale.p * scale.ds, scale.p * scale.ds);
         bool ok = true;
         for (int j = 0; j < n; ++j) {
             ok = tc::bar_wait(bars.s_full(j & 1), (j >> 1) & 1, failed);
@@ -690,8 +705,12 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    r[c][e] = __float_as_uint(tc::exp2_approx(fmaf(__uint_as_float(r[c][e]), a.scale_log2, -lse)));
+                for (int e = 0; e < 32; e += 2) {
+                    float x, y;
+                    tc::split(tc::fma2(pair(r[c], e), times, lse), x, y);
+                    r[c][e] = __float_as_uint(tc::exp2_approx(x));
+                    r[c][e + 1] = __float_as_uint(tc::exp2_approx(y));
+                }
             ok = tc::bar_wait(bars.w_full(), j & 1, failed);
             if (!ok) break;
             tc::fence_after();
@@ -701,16 +720,13 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
             tc::wait_ld(g[0], g[1]);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 2)
+                    set_pair(g[c], e, scaled<T>(tc::mul2(pair(r[c], e), tc::add2(pair(g[c], e), delta)), ds_scale));
+                if (cut) keep_columns(g[c], 0, end - c * 32);
                 uint32_t p[16];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float x = __uint_as_float(r[c][e]) * (__uint_as_float(g[c][e]) - delta);
-                    float y = __uint_as_float(r[c][e + 1]) * (__uint_as_float(g[c][e + 1]) - delta);
-                    if constexpr (std::is_same_v<T, __half>) x *= scale.p * scale.ds, y *= scale.p * scale.ds;
-                    if (cut && c * 32 + e >= end) x = 0.f;
-                    if (cut && c * 32 + e + 1 >= end) y = 0.f;
-                    p[e / 2] = tc::pack2<T>(x, y);
-                }
+                for (int e = 0; e < 16; ++e) p[e] = tc::pack2<T>(__uint_as_float(g[c][2 * e]), __uint_as_float(g[c][2 * e + 1]));
                 tc::tmem_store16(w_at + c * 16, p);
             }
             tc::wait_st();

@@ -19,8 +19,8 @@ struct AttnArgs {
     const int32_t* q_lens;
     const int32_t* kv_lens;
     float* lse;    // [batch, heads, q_len]
-    float* lse2;   // [batch, heads, q_pad]: log-sums in base 2, +inf where nothing is seen
-    float* delta;  // [batch, heads, q_pad]
+    float* minus_lse2;   // [batch, heads, q_pad]: minus the log-sums in base 2, -inf where nothing is seen
+    float* minus_delta;  // [batch, heads, q_pad]
     // float16 on the tensor cores: probabilities are held times 2^p_shift, and ds times a power of two
     // taken from the largest magnitudes of the output's gradient and of v (bits of a float each).
     float p_shift;
