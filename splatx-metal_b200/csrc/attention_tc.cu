@@ -377,13 +377,13 @@ struct BwdBars {
     __device__ uint32_t own() const { return at + 8 * (2 * kSlots); }
     __device__ uint32_t s_full(int k) const { return at + 8 * (2 * kSlots + 1 + k); }
     __device__ uint32_t w_full() const { return at + 8 * (2 * kSlots + 3); }
-    __device__ uint32_t p_full() const { return at + 8 * (2 * kSlots + 4); }
-    __device__ uint32_t ds_full() const { return at + 8 * (2 * kSlots + 5); }
-    __device__ uint32_t out_full() const { return at + 8 * (2 * kSlots + 6); }
-    __device__ uint32_t stat_full(int k) const { return at + 8 * (2 * kSlots + 7 + k); }
-    __device__ uint32_t stat_free(int k) const { return at + 8 * (2 * kSlots + 9 + k); }
-    __device__ uint32_t drained() const { return at + 8 * (2 * kSlots + 11); }
-    static constexpr int kFailed = 2 * kSlots + 12, kTmem = kFailed + 1;  // words of 8 bytes behind the barriers
+    __device__ uint32_t p_full(int c) const { return at + 8 * (2 * kSlots + 4 + c); }
+    __device__ uint32_t ds_full() const { return at + 8 * (2 * kSlots + 6); }
+    __device__ uint32_t out_full() const { return at + 8 * (2 * kSlots + 7); }
+    __device__ uint32_t stat_full(int k) const { return at + 8 * (2 * kSlots + 8 + k); }
+    __device__ uint32_t stat_free(int k) const { return at + 8 * (2 * kSlots + 10 + k); }
+    __device__ uint32_t drained() const { return at + 8 * (2 * kSlots + 12); }
+    static constexpr int kFailed = 2 * kSlots + 13, kTmem = kFailed + 1;  // words of 8 bytes behind the barriers
 };
 static_assert((BwdBars::kTmem + 1) * 8 <= 256, "barriers");
 
@@ -392,7 +392,7 @@ __device__ __forceinline__ void bwd_init(const BwdBars& b, volatile uint32_t* fa
     for (int s = 0; s < kSlots; ++s) tc::bar_init(b.full(s), 1), tc::bar_init(b.free(s), 1);
     tc::bar_init(b.own(), 1);
     tc::bar_init(b.w_full(), 1);
-    tc::bar_init(b.p_full(), 8);
+    for (int c = 0; c < 2; ++c) tc::bar_init(b.p_full(c), 8);
     tc::bar_init(b.ds_full(), 8);
     tc::bar_init(b.out_full(), 1);
     for (int k = 0; k < 2; ++k) tc::bar_init(b.s_full(k), 1), tc::bar_init(b.stat_full(k), 1), tc::bar_init(b.stat_free(k), 8);
@@ -436,6 +436,21 @@ __device__ __forceinline__ void set_pair(uint32_t (&r)[32], int i, tc::Two x) {
     r[i] = __float_as_uint(lo);
     r[i + 1] = __float_as_uint(hi);
 }
+// Of 16 pairs of exponentials of the backward, those on the multiply-add pipes.
+constexpr int kPolyBwd = 6;
+template <typename T>
+__device__ __forceinline__ void exp_pair(uint32_t (&r)[32], int i, tc::Two x) {
+    float lo, hi;
+    if (i / 2 % 16 * kPolyBwd % 16 < kPolyBwd) {
+        tc::exp2_poly(x, lo, hi);
+    } else {
+        tc::split(x, lo, hi);
+        lo = tc::exp2_approx(lo);
+        hi = tc::exp2_approx(hi);
+    }
+    r[i] = __float_as_uint(lo);
+    r[i + 1] = __float_as_uint(hi);
+}
 template <typename T>
 __device__ __forceinline__ tc::Two scaled(tc::Two x, tc::Two by) {
     if constexpr (std::is_same_v<T, __half>) return tc::mul2(x, by);
@@ -465,7 +480,12 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
     const int tiles = k0 >= w.kv_len || begin >= q_len ? 0 : (q_len + kRows - 1) / kRows - first;
     const int total = tiles * a.group;
     const auto slot = [&](int item) { return base + S::kRing + item % kSlots * S::kTileBytes; };
-    constexpr uint32_t kW = kRows, kVV = 2 * kRows, kVK = 2 * kRows + D;
+    // with 64 columns of the sums there is room for the next S beside this one
+    constexpr bool kAhead = D == 64;
+    constexpr uint32_t kW = kAhead ? 2 * kRows : kRows, kVV = kW + kRows, kVK = kVV + D;
+    const auto s_col = [](int i) { return kAhead ? static_cast<uint32_t>(i & 1) * kRows : 0u; };
+    const auto s_bar = [&](int i) { return bars.s_full(kAhead ? i & 1 : 0); };
+    const auto s_par = [](int i) { return static_cast<uint32_t>(kAhead ? i >> 1 : i) & 1; };
 
     if (warp == 8) {  // loads: K and V, then Q0 G0 Q1 G1 ... around the ring, lse and delta beside each Q
         if (lane == 0 && total) {
@@ -503,53 +523,54 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
                 zero_rows<D>(smem + S::kRing + item % kSlots * S::kTileBytes, q_len - row, lane);
             return true;
         };
-        bool ok = total == 0 || (tc::bar_wait(bars.own(), 0, failed) && arrived(0));
-        if (ok && total) {
-            rows_rows<T, D>(one, tmem, base + S::kOwn, slot(0));
-            tc::commit(one, bars.s_full(0));
-            ok = arrived(1);
-            if (ok) {
-                rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(1));
-                tc::commit(one, bars.w_full());
-            }
-        }
+        const auto scores = [&](int i) {
+            if (!arrived(2 * i)) return false;
+            rows_rows<T, D>(one, tmem + s_col(i), base + S::kOwn, slot(2 * i));
+            tc::commit(one, s_bar(i));
+            return true;
+        };
+        const auto weights = [&](int i) {
+            if (!arrived(2 * i + 1)) return false;
+            rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(2 * i + 1));
+            tc::commit(one, bars.w_full());
+            return true;
+        };
+        bool ok = total == 0 || (tc::bar_wait(bars.own(), 0, failed) && scores(0) && weights(0));
         for (int i = 0; ok && i < total; ++i) {
-            ok = tc::bar_wait(bars.p_full(), i & 1, failed);
-            if (!ok) break;
-            tc::fence_after();
-            tmem_rows2<T, D, 64>(one, tmem + kVV, tmem, slot(2 * i + 1), i > 0);
-            tc::commit(one, bars.free((2 * i + 1) % kSlots));
-            if (i + 1 < total) {
-                ok = arrived(2 * i + 2);
+            if (kAhead && i + 1 < total) ok = scores(i + 1);
+            for (int c = 0; ok && c < 2; ++c) {  // half of the queries while the others' p are made
+                ok = tc::bar_wait(bars.p_full(c), i & 1, failed);
                 if (!ok) break;
-                rows_rows<T, D>(one, tmem, base + S::kOwn, slot(2 * i + 2));
-                tc::commit(one, bars.s_full(0));
+                tc::fence_after();
+                const uint32_t p = tmem + s_col(i) + c * 16, g = slot(2 * i + 1) + c * 32 * 128;
+                tmem_rows<T, D, 2>(one, tmem + kVV, p, g, i > 0 || c > 0);
+                tmem_rows<T, D, 2>(one, tmem + kVV, p + 64, g + 64 * 128, true);
             }
+            if (!ok) break;
+            tc::commit(one, bars.free((2 * i + 1) % kSlots));
+            if (!kAhead && i + 1 < total) ok = scores(i + 1);
+            if (!ok) break;
             ok = tc::bar_wait(bars.ds_full(), i & 1, failed);
             if (!ok) break;
             tc::fence_after();
             tmem_rows2<T, D, 64>(one, tmem + kVK, tmem + kW, slot(2 * i), i > 0);
             tc::commit(one, i + 1 < total ? bars.free(2 * i % kSlots) : bars.out_full());
-            if (i + 1 < total) {
-                ok = arrived(2 * i + 3);
-                if (!ok) break;
-                rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(2 * i + 3));
-                tc::commit(one, bars.w_full());
-            }
+            if (i + 1 < total) ok = weights(i + 1);
         }
     } else {
         const int half = warp >> 2;
         const int64_t key = k0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + half * 64, w_at = s_at + kW;
+        const uint32_t w_at = tmem + lanes + half * 64 + kW;
         const HalfScale scale = half_scale<T>(a);
         const tc::Two times = tc::two(a.scale_log2, a.scale_log2), ds_scale = tc::two(scale.p * scale.ds, scale.p * scale.ds);
         bool ok = true;
         for (int i = 0; i < total; ++i) {
             const int64_t q0 = static_cast<int64_t>(first + i % tiles) * kRows + half * 64;
-            ok = tc::bar_wait(bars.s_full(0), i & 1, failed) && tc::bar_wait(bars.stat_full(i & 1), (i / 2) & 1, failed);
+            ok = tc::bar_wait(s_bar(i), s_par(i), failed) && tc::bar_wait(bars.stat_full(i & 1), (i / 2) & 1, failed);
             if (!ok) break;
             tc::fence_after();
+            const uint32_t s_at = tmem + lanes + half * 64 + s_col(i);
             const ulonglong2* lse = reinterpret_cast<const ulonglong2*>(smem + S::kStats + (i & 1) * 2 * kRows * 4) + half * 16;
             const ulonglong2* delta = lse + kRows / 4;
             uint32_t r[2][32];
@@ -565,22 +586,19 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
                     const ulonglong2 x = lse[c * 8 + e / 4];
-                    float v[4];
-                    tc::split(tc::fma2(pair(r[c], e), times, tc::Two{x.x}), v[0], v[1]);
-                    tc::split(tc::fma2(pair(r[c], e + 2), times, tc::Two{x.y}), v[2], v[3]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) r[c][e + k] = __float_as_uint(tc::exp2_approx(v[k]));
+                    exp_pair<T>(r[c], e, tc::fma2(pair(r[c], e), times, tc::Two{x.x}));
+                    exp_pair<T>(r[c], e + 2, tc::fma2(pair(r[c], e + 2), times, tc::Two{x.y}));
                 }
                 if (cut) keep_columns(r[c], lo - c * 32, hi - c * 32);
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) p[e] = tc::pack2<T>(__uint_as_float(r[c][2 * e]), __uint_as_float(r[c][2 * e + 1]));
                 tc::tmem_store16(s_at + c * 16, p);
+                tc::wait_st();
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(bars.p_full(c));
             }
-            tc::wait_st();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::bar_arrive(bars.p_full());
             ok = tc::bar_wait(bars.w_full(), i & 1, failed);
             if (!ok) break;
             tc::fence_after();
@@ -705,12 +723,7 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    float x, y;
-                    tc::split(tc::fma2(pair(r[c], e), times, lse), x, y);
-                    r[c][e] = __float_as_uint(tc::exp2_approx(x));
-                    r[c][e + 1] = __float_as_uint(tc::exp2_approx(y));
-                }
+                for (int e = 0; e < 32; e += 2) exp_pair<T>(r[c], e, tc::fma2(pair(r[c], e), times, lse));
             ok = tc::bar_wait(bars.w_full(), j & 1, failed);
             if (!ok) break;
             tc::fence_after();
