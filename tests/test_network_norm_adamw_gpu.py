@@ -275,6 +275,32 @@ def test_adamw_bit_for_bit(bits, ptype, gtype):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_bit_for_bit_over_all_magnitudes(bits):
+    """Four million gradients from 2^-70 to 2^60, and values beyond both ends of what the kernel's own
+    root and quotient are made for: every root and quotient is the rounded one (a quotient may be off
+    in its last bit where its residual is below 2^-126: the gradients here keep above that)."""
+    import torch
+    from splatx_cuda.network import AdamW
+    n = 1 << 22
+    rng = np.random.default_rng(bits)
+    g = (rng.standard_normal(n) * 2.0 ** rng.uniform(-40, 45, n)).astype(F)
+    g[: n // 8] = 0
+    g[n // 8: n // 4] = (rng.standard_normal(n // 8) * 2.0 ** np.repeat(rng.uniform(-62, 60, n // 8 // 256), 256)).astype(F)
+    p = torch.zeros(n, device="cuda")
+    opt = AdamW([p], state_bits=bits, **CFG)
+    opt.step([torch.from_numpy(g).cuda()])
+    new, m, v = _numpy_step(np.zeros(n, F), g, np.zeros(n, F), np.zeros(n, F), 1)
+    assert np.array_equal(_np(p), new)
+    st = opt.state()
+    if bits == 32:
+        assert np.array_equal(_np(st["exp_avg"][0]), m) and np.array_equal(_np(st["exp_avg_sq"][0]), v)
+    else:
+        codes, scale = _pack(np.sqrt(v), True)
+        assert np.array_equal(_np(st["exp_avg_sq"][0]), codes.float().numpy())
+        assert np.array_equal(_np(st["exp_avg_sq_scale"][0]), scale)
+
+
 def test_adamw_against_64_bits():
     """Twenty operations of relative error 2^-24 each, against the formula's value and its terms."""
     from splatx_cuda.network import AdamW
