@@ -36,31 +36,30 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _on(first: torch.Tensor, what: str, **others) -> torch.device:
-    """The CUDA device that all of the call's tensors are on."""
-    if not first.is_cuda:
+def _on(device: torch.device, what: str, *others) -> None:
+    """Refuses tensors (or None) that are not on the CUDA device of the call's first one."""
+    if device.type != "cuda":
         raise ValueError(f"{what}: CUDA tensors needed (there is no CPU path)")
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, not on {first.device}")
-    return first.device
+    for t in others:
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: a tensor is on {t.device}, not on {device}")
 
 
 class _at:
     """The device made current for one call (left alone where it is already) and its stream."""
 
+    __slots__ = ("index", "was")
+
     def __init__(self, device):
-        self.index = device.index
-        self.other = torch.cuda.current_device() != self.index
+        self.index, self.was = device.index, torch.cuda.current_device()
 
     def __enter__(self):
-        if self.other:
-            self.was = torch.cuda.current_device()
+        if self.was != self.index:
             torch.cuda.set_device(self.index)
         return torch.cuda.current_stream(self.index).cuda_stream
 
     def __exit__(self, *exc):
-        if self.other:
+        if self.was != self.index:
             torch.cuda.set_device(self.was)
         return False
 
@@ -75,9 +74,9 @@ def attention_status() -> int:
 
 # ---------------------------------------------------------------- attention
 
-def _view(t: torch.Tensor) -> _nat.SxAttentionView:
+def _view(t: torch.Tensor) -> tuple:
     s = t.stride()
-    return _nat.SxAttentionView(t.data_ptr(), s[0], s[1], s[2])
+    return t.data_ptr(), s[0], s[1], s[2]
 
 
 def _heads_last(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -92,23 +91,28 @@ def _attention_inputs(what, q, k, v, scale, causal, q_lens, kv_lens):
     if k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{what}: q, k and v must have one dtype")
     b, n, h, d = q.shape
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+    kb, kn, kh, kd = k.shape
+    if k.shape != v.shape or kb != b or kd != d:
         raise ValueError(f"{what}: k and v must both be [{b}, tokens, heads, {d}], got "
                          f"{tuple(k.shape)} and {tuple(v.shape)}")
-    device = _on(q, what, k=k, v=v, q_lens=q_lens, kv_lens=kv_lens)
+    device = q.device
+    _on(device, what, k, v, q_lens, kv_lens)
     for name, lens in (("q_lens", q_lens), ("kv_lens", kv_lens)):
         if lens is not None and (lens.dtype != torch.int32 or lens.shape != (b,) or
                                  not lens.is_contiguous()):
             raise ValueError(f"{what}: {name} must be a contiguous int32 tensor of [{b}]")
     ins = _nat.SxAttentionInputs(
         _view(q), _view(k), _view(v), None if q_lens is None else q_lens.data_ptr(),
-        None if kv_lens is None else kv_lens.data_ptr(), b, n, k.shape[1], h, k.shape[2], d, code,
-        (1.0 / math.sqrt(d) if d else 1.0) if scale is None else float(scale), int(bool(causal)))
+        None if kv_lens is None else kv_lens.data_ptr(), b, n, kn, h, kh, d, code,
+        (1.0 / math.sqrt(d) if d else 1.0) if scale is None else scale, causal)
     return q, k, v, ins, device
 
 
-def _workspace(nbytes: int, device) -> torch.Tensor | None:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _workspace(entry, device, ins, *rest) -> torch.Tensor:
+    """Device memory of the size that the entry point asks for (at least one byte: a pointer)."""
+    nbytes = C.c_size_t(0)
+    check(entry(C.byref(ins), *rest, None, C.byref(nbytes), None))
+    return torch.empty(max(nbytes.value, 1), dtype=torch.uint8, device=device)
 
 
 def attention_fwd(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=None):
@@ -121,15 +125,14 @@ def attention_fwd(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=Non
     j <= i + kv_len - q_len (the lengths of its batch entry). A query that sees no key gets output 0
     and log-sum -inf."""
     q, k, v, ins, device = _attention_inputs("attention_fwd", q, k, v, scale, causal, q_lens, kv_lens)
+    b, n, h, _ = q.shape
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=device)
-    ov, nbytes, L = _view(out), C.c_size_t(0), _nat.lib()
+    lse = torch.empty((b, h, n), dtype=torch.float32, device=device)
+    ov, entry = _nat.SxAttentionView(*_view(out)), _nat.lib().sxcuda_attention_fwd
     with _at(device) as stream:
-        check(L.sxcuda_attention_fwd(C.byref(ins), C.byref(ov), lse.data_ptr(), None,
-                                     C.byref(nbytes), stream))
-        ws = _workspace(max(nbytes.value, 1), device)
-        check(L.sxcuda_attention_fwd(C.byref(ins), C.byref(ov), lse.data_ptr(), ws.data_ptr(),
-                                     C.byref(nbytes), stream))
+        ws = _workspace(entry, device, ins, None, None)
+        check(entry(C.byref(ins), C.byref(ov), lse.data_ptr(), ws.data_ptr(),
+                    C.byref(C.c_size_t(ws.numel())), stream))
     return out, lse
 
 
@@ -144,18 +147,17 @@ def attention_bwd(v_out, q, k, v, out, lse, *, scale=None, causal=False, q_lens=
     if lse.shape != (q.shape[0], q.shape[2], q.shape[1]) or lse.dtype != torch.float32 or \
             not lse.is_contiguous():
         raise ValueError(f"{what}: lse must be a contiguous float32 tensor of [batch, heads, tokens]")
-    _on(q, what, v_out=v_out, out=out, lse=lse)
+    _on(device, what, v_out, out, lse)
     v_out, out = _heads_last(v_out, what), _heads_last(out, what)
     gin = _nat.SxAttentionGradsIn(_view(out), lse.data_ptr(), _view(v_out))
-    grads = [torch.empty(t.shape, dtype=q.dtype, device=device) for t in (q, k, v)]
+    grads = tuple(torch.empty(t.shape, dtype=q.dtype, device=device) for t in (q, k, v))
     gout = _nat.SxAttentionGrads(*(_view(t) for t in grads))
-    nbytes, L = C.c_size_t(0), _nat.lib()
+    entry = _nat.lib().sxcuda_attention_bwd
     with _at(device) as stream:
-        check(L.sxcuda_attention_bwd(C.byref(ins), None, None, None, C.byref(nbytes), stream))
-        ws = _workspace(max(nbytes.value, 1), device)
-        check(L.sxcuda_attention_bwd(C.byref(ins), C.byref(gin), C.byref(gout), ws.data_ptr(),
-                                     C.byref(nbytes), stream))
-    return tuple(grads)
+        ws = _workspace(entry, device, ins, None, None)
+        check(entry(C.byref(ins), C.byref(gin), C.byref(gout), ws.data_ptr(),
+                    C.byref(C.c_size_t(ws.numel())), stream))
+    return grads
 
 
 class _Attention(torch.autograd.Function):
@@ -180,39 +182,45 @@ def attention(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=None):
 
 # ---------------------------------------------------------------- layer norm
 
-def _rows(t: torch.Tensor, cols: int) -> torch.Tensor:
-    t = t.reshape(-1, cols) if cols else t
-    return t if t.stride(1) == 1 and (t.shape[0] <= 1 or t.stride(0) >= cols) else t.contiguous()
+def _rows(t: torch.Tensor, cols: int):
+    """t as (tensor, rows, distance of rows): as it is where its rows are, else a copy."""
+    if t.is_contiguous():
+        return t, t.numel() // cols, cols
+    if t.dim() != 2:
+        t = t.reshape(-1, cols)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t, t.shape[0], t.stride(0)
 
 
 def _norm_inputs(what, x, weight, bias, eps):
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{what}: x needs a last axis of at least 1, got {tuple(x.shape)}")
-    cols = x.shape[-1]
-    device = _on(x, what, weight=weight, bias=bias)
-    params = [p for p in (weight, bias) if p is not None]
-    for p in params:
-        if p.shape != (cols,) or not p.is_contiguous() or p.dtype != params[0].dtype:
+    cols, device, code = x.shape[-1], x.device, _dtype(x, what)
+    _on(device, what, weight, bias)
+    first = bias if weight is None else weight
+    for p in (weight, bias):
+        if p is not None and (p.shape != (cols,) or not p.is_contiguous() or p.dtype != first.dtype):
             raise ValueError(f"{what}: weight and bias must be contiguous tensors of [{cols}] with "
                              "one dtype")
-    rows = _rows(x, cols)
+    flat, rows, stride = _rows(x, cols)
     ins = _nat.SxLayerNormInputs(
-        rows.data_ptr(), None if weight is None else weight.data_ptr(),
-        None if bias is None else bias.data_ptr(), rows.shape[0], cols, rows.stride(0),
-        _dtype(x, what), _dtype(params[0], what) if params else _DTYPES[torch.float32], float(eps))
-    return rows, ins, device
+        flat.data_ptr(), None if weight is None else weight.data_ptr(),
+        None if bias is None else bias.data_ptr(), rows, cols, stride, code,
+        _DTYPES[torch.float32] if first is None else _dtype(first, what), eps)
+    return flat, ins, device, cols
 
 
 def layer_norm_fwd(x, weight=None, bias=None, *, eps=1e-5):
     """Layer norm over the last axis: (y like x, mean, rstd of x.shape[:-1] in float32). weight and
     bias (each may be None: ones, zeros) have one dtype, which need not be x's."""
-    rows, ins, device = _norm_inputs("layer_norm_fwd", x, weight, bias, eps)
+    flat, ins, device, cols = _norm_inputs("layer_norm_fwd", x, weight, bias, eps)
     y = torch.empty(x.shape, dtype=x.dtype, device=device)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
     rstd = torch.empty_like(mean)
     with _at(device) as stream:
-        check(_nat.lib().sxcuda_layer_norm_fwd(C.byref(ins), y.data_ptr(), x.shape[-1],
-                                               mean.data_ptr(), rstd.data_ptr(), stream))
+        check(_nat.lib().sxcuda_layer_norm_fwd(C.byref(ins), y.data_ptr(), cols, mean.data_ptr(),
+                                               rstd.data_ptr(), stream))
     return y, mean, rstd
 
 
@@ -220,27 +228,25 @@ def layer_norm_bwd(v_y, x, weight, mean, rstd):
     """Gradients (v_x, v_weight, v_bias) of layer_norm_fwd; the weights' have the weight's dtype
     (float32 where weight is None). mean and rstd are the forward's. Deterministic."""
     what = "layer_norm_bwd"
-    rows, ins, device = _norm_inputs(what, x, weight, None, 0.0)
-    cols = x.shape[-1]
+    flat, ins, device, cols = _norm_inputs(what, x, weight, None, 0.0)
     if v_y.shape != x.shape or v_y.dtype != x.dtype:
         raise ValueError(f"{what}: v_y must be like x")
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.shape != x.shape[:-1] or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{what}: {name} must be a contiguous float32 tensor of "
                              f"{tuple(x.shape[:-1])}")
-    _on(x, what, v_y=v_y, mean=mean, rstd=rstd)
-    g = _rows(v_y, cols)
+    _on(device, what, v_y, mean, rstd)
+    g, _, g_stride = _rows(v_y, cols)
     v_x = torch.empty(x.shape, dtype=x.dtype, device=device)
     v_w = torch.empty(cols, dtype=torch.float32 if weight is None else weight.dtype, device=device)
     v_b = torch.empty_like(v_w)
-    gin = _nat.SxLayerNormGradsIn(mean.data_ptr(), rstd.data_ptr(), g.data_ptr(), g.stride(0))
+    gin = _nat.SxLayerNormGradsIn(mean.data_ptr(), rstd.data_ptr(), g.data_ptr(), g_stride)
     out = _nat.SxLayerNormGrads(v_x.data_ptr(), cols, v_w.data_ptr(), v_b.data_ptr())
-    nbytes, L = C.c_size_t(0), _nat.lib()
+    entry = _nat.lib().sxcuda_layer_norm_bwd
     with _at(device) as stream:
-        check(L.sxcuda_layer_norm_bwd(C.byref(ins), None, None, None, C.byref(nbytes), stream))
-        ws = _workspace(nbytes.value, device)
-        check(L.sxcuda_layer_norm_bwd(C.byref(ins), C.byref(gin), C.byref(out), ws.data_ptr(),
-                                      C.byref(nbytes), stream))
+        ws = _workspace(entry, device, ins, None, None)
+        check(entry(C.byref(ins), C.byref(gin), C.byref(out), ws.data_ptr(),
+                    C.byref(C.c_size_t(ws.numel())), stream))
     return v_x, v_w, v_b
 
 
@@ -296,10 +302,10 @@ class AdamW:
             decays += [float(g.get("weight_decay", weight_decay))] * len(mine)
         if not self.params:
             raise ValueError(f"{what}: no parameters")
-        self.device = _on(self.params[0], what)
+        self.device = self.params[0].device
+        _on(self.device, what, *self.params)
         for p in self.params:
             _dtype(p, what)
-            _on(self.params[0], what, parameter=p)
             if not p.is_contiguous():
                 raise ValueError(f"{what}: parameters must be contiguous")
         self.bits = state_bits
