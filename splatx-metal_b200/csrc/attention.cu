@@ -348,12 +348,19 @@ AttnArgs attn_args(const SxAttentionInputs& in) {
     return a;
 }
 
-size_t attention_fwd_workspace(const SxAttentionInputs&) { return 0; }
+size_t attention_fwd_workspace(const SxAttentionInputs& in) {
+    const AttnArgs a = attn_args(in);
+    if (!attention_tc_takes(a)) return 0;
+    const AttnPlan p = attention_fwd_plan(a);
+    return p.splits > 1 ? static_cast<size_t>(p.splits * a.batch * a.heads * a.q_len) * (a.dim + 1) * sizeof(float) : 0;
+}
 
-void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& out, float* lse, void*, cudaStream_t s) {
+void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& out, float* lse, void* ws, cudaStream_t s) {
     AttnArgs a = attn_args(in);
     a.out = out;
     a.lse = lse;
+    a.part_out = static_cast<float*>(ws);
+    a.part_lse2 = a.part_out + attention_fwd_workspace(in) / (a.dim + 1) / sizeof(float) * a.dim;
     if (a.batch == 0 || a.q_len == 0) return;
     if (attention_tc_takes(a) && attention_tc_takes_view(a, a.out, a.q_len, a.heads)) {
         launch_attention_fwd_tc(a, s);

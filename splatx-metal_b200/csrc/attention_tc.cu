@@ -1,5 +1,7 @@
 // attention_tc.cu — attention on the tensor cores: 16-bit inputs, head dimensions that are multiples
 // of 8 up to 128 (padded by TMA's zero fill to 64 or 128), rows that TMA can copy.
+#include <algorithm>
+
 #include "sx_attention.h"
 #include "sx_tcgen05.cuh"
 
@@ -41,8 +43,9 @@ __device__ __forceinline__ void zero_rows(uint8_t* tile, int first, int lane) {
 }
 
 template <int D>
-__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, int batch, uint32_t bar) {
-    tc::bar_expect(bar, D / 64 * kPanel);
+__device__ __forceinline__ void load_rows(uint32_t dst, const CUtensorMap* map, int row, int head, int batch, uint32_t bar,
+                                          int rows = kRows) {
+    tc::bar_expect(bar, D / 64 * rows * 128);
 #pragma unroll
     for (int p = 0; p < D / 64; ++p) tc::tma_load(dst + p * kPanel, map, p * 64, row, head, batch, bar);
 }
@@ -94,6 +97,60 @@ __device__ __forceinline__ void store_row(T* out, uint32_t at, float f, int dim,
     }
 }
 
+// The same in 32 bits.
+template <int D>
+__device__ __forceinline__ void store_part(float* out, uint32_t at, float f, int dim, bool written, bool any) {
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        if (any) {
+            tc::tmem_load32(o, at + c * 32);
+            tc::wait_ld(o);
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 4)
+            if (written && c * 32 + i < dim)
+                *reinterpret_cast<float4*>(out + c * 32 + i) = float4{__uint_as_float(o[i]) * f, __uint_as_float(o[i + 1]) * f,
+                                                                       __uint_as_float(o[i + 2]) * f, __uint_as_float(o[i + 3]) * f};
+        __syncwarp();
+    }
+}
+
+// Joins the parts of a query that CTAs with different keys made: out = sum_s 2^(lse_s - lse) out_s. A
+// warp per query; parts that saw no key are not read.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+    const int64_t rows = a.batch * a.heads * a.q_len, at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    if (at >= rows) return;
+    const int lane = threadIdx.x & 31;
+    float top = -INFINITY;
+    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_lse2[s * rows + at]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
+    float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (top != -INFINITY)
+        for (int s = 0; s < a.splits; ++s) {
+            const float x = exp2f(a.part_lse2[s * rows + at] - top);
+            if (x == 0.f) continue;
+            total += x;
+            if (lane * 4 < a.dim) {
+                const float4 o = *reinterpret_cast<const float4*>(a.part_out + (s * rows + at) * a.dim + lane * 4);
+                acc[0] = fmaf(x, o.x, acc[0]);
+                acc[1] = fmaf(x, o.y, acc[1]);
+                acc[2] = fmaf(x, o.z, acc[2]);
+                acc[3] = fmaf(x, o.w, acc[3]);
+            }
+        }
+    const float f = total > 0.f ? 1.f / total : 0.f;
+    const int64_t i = at % a.q_len, bh = at / a.q_len;
+    T* out = static_cast<T*>(a.out.data) + bh / a.heads * a.out.batch_stride + bh % a.heads * a.out.head_stride + i * a.out.token_stride;
+    if (lane * 4 < a.dim) {
+        uint2 x{tc::pack2<T>(acc[0] * f, acc[1] * f), tc::pack2<T>(acc[2] * f, acc[3] * f)};
+        *reinterpret_cast<uint2*>(out + lane * 4) = x;
+    }
+    if (lane == 0) a.lse[at] = total > 0.f ? (top + log2f(total)) * kLn2 : -INFINITY;
+}
+
 // The forward. A CTA owns two tiles of 128 queries of one head; warps 0-3 and 4-7 make their
 // probabilities (a thread per query), warp 8 loads, warp 9 issues the products. While one tile's
 // warps work on its scores the tensor cores compute for the other: S = Q K^T into tensor memory, the
@@ -133,16 +190,23 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
     constexpr uint32_t kO = 2 * kRows, kP = kApart ? kO + 2 * D : 0, kPStep = kApart ? 64 : kRows;
 
     // the last queries see the most keys when causal: they start first
-    const int64_t pairs = (a.q_len + 2 * kRows - 1) / (2 * kRows), heads = a.heads * a.batch;
-    const int64_t bh = blockIdx.x % heads;
-    const AttnHead w = attn_head(a, bh % a.heads, bh / a.heads);
-    const int q0 = static_cast<int>((pairs - 1 - blockIdx.x / heads) * 2 * kRows);
+    const int split = static_cast<int>(blockIdx.x % a.splits);
+    const int64_t block = blockIdx.x / a.splits, heads = (a.packed ? a.kv_heads : a.heads) * a.batch;
+    const int64_t pairs = a.packed ? 1 : (a.q_len + 2 * kRows - 1) / (2 * kRows), bh = block % heads;
+    const AttnHead w = attn_head(a, a.packed ? bh % a.kv_heads * a.group : bh % a.heads, a.packed ? bh / a.kv_heads : bh / a.heads);
+    const int q0 = static_cast<int>((pairs - 1 - block / heads) * 2 * kRows);
     const int kv_len = static_cast<int>(w.kv_len), hk = static_cast<int>(w.h) / a.group;
-    int n[2];
+    // key tiles of each query tile: j0 and on, as many as n
+    int n[2], j0 = 0;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
         const int first = q0 + t * kRows;
-        n[t] = first >= w.q_len ? 0 : static_cast<int>((attn_keys_end(w, first + kRows) + kRows - 1) / kRows);
+        n[t] = first >= w.q_len || (a.packed && t) ? 0 : static_cast<int>((attn_keys_end(w, first + kRows) + kRows - 1) / kRows);
+    }
+    if (a.splits > 1) {
+        const int each = (max(n[0], n[1]) + a.splits - 1) / a.splits;
+        j0 = split * each;
+        for (int t = 0; t < 2; ++t) n[t] = max(min(n[t] - j0, each), 0);
     }
     const int most = max(n[0], n[1]);
 
@@ -173,12 +237,14 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
         if (warp == 8) {  // loads: Q tiles, then K0 V0 K1 V1 ... around the ring
             if (lane == 0)
                 for (int t = 0; t < 2; ++t)
-                    if (n[t]) load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t));
+                    if (n[t])
+                        load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t),
+                                     a.packed ? static_cast<int>(a.q_len) * a.group : kRows);
             for (; loaded < 2 * most; ++loaded) {
                 const int s = loaded % kSlots, round = loaded / kSlots;
                 if (round && !tc::bar_wait(kv_free(s), (round - 1) & 1, failed)) break;
                 if (lane == 0)
-                    load_rows<D>(base + S::kRing + s * S::kTileBytes, loaded & 1 ? &maps.v : &maps.k, loaded / 2 * kRows, hk, static_cast<int>(w.b), kv_full(s));
+                    load_rows<D>(base + S::kRing + s * S::kTileBytes, loaded & 1 ? &maps.v : &maps.k, (j0 + loaded / 2) * kRows, hk, static_cast<int>(w.b), kv_full(s));
                 __syncwarp();
             }
         } else if (warp == 9) {  // products
@@ -198,7 +264,8 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 const int vi = 2 * j + 1, vs = vi % kSlots, ki = 2 * j + 2, ks = ki % kSlots;
                 ok = tc::bar_wait(kv_full(vs), (vi / kSlots) & 1, failed);
                 if (!ok) break;
-                if ((j + 1) * kRows > kv_len && kv_len < a.kv_len) zero_rows<D>(smem + S::kRing + vs * S::kTileBytes, kv_len - j * kRows, lane);
+                if ((j0 + j + 1) * kRows > kv_len && kv_len < a.kv_len)
+                    zero_rows<D>(smem + S::kRing + vs * S::kTileBytes, kv_len - (j0 + j) * kRows, lane);
                 if (j + 1 < most) ok = tc::bar_wait(kv_full(ks), (ki / kSlots) & 1, failed);
                 for (int t = 0; ok && t < 2; ++t) {
                     if (j >= n[t]) continue;
@@ -228,7 +295,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
     } else {  // softmax: a thread per query
         tc::more_registers<216>();
         const int t = warp >> 2, mine = n[t];
-        const int row = q0 + t * kRows + (warp & 3) * 32 + lane;
+        // the row's query and head (packed: the heads of a group one after the other)
+        int row = q0 + t * kRows + (warp & 3) * 32 + lane, h = static_cast<int>(w.h);
+        bool mine_to_write = row < a.q_len;
+        if (a.packed) {
+            const int q_len = static_cast<int>(a.q_len);
+            mine_to_write = row < q_len * a.group;
+            h += mine_to_write ? row / q_len : 0;
+            row %= q_len;
+        }
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + kO + t * D, p_at = tmem + lanes + kP + t * kPStep;
         float m = -INFINITY, l = 0.f;  // m: the base-2 exponent the sums are relative to
@@ -248,7 +323,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
             }
             // keys of this tile that the query sees: those below `end`
             const int64_t last = static_cast<int64_t>(row) + w.ahead + 1;
-            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j) * kRows);
+            const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j0 + j) * kRows);
             if (__any_sync(kFullMask, end < kRows)) {
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
@@ -329,9 +404,17 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
         if (ok) {
             tc::fence_after();
             const bool live = row < w.q_len && m != -INFINITY;
-            T* out = static_cast<T*>(a.out.data) + w.b * a.out.batch_stride + w.h * a.out.head_stride + row * a.out.token_stride;
-            store_row<T, D>(out, o_at, live ? 1.f / l : 0.f, a.dim, row < a.q_len, live, mine > 0);
-            if (row < a.q_len) a.lse[bh * a.q_len + row] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
+            const int64_t at = (w.b * a.heads + h) * a.q_len + row;
+            const float f = live ? 1.f / l : 0.f;
+            if (a.splits > 1) {
+                const int64_t to = split * (a.batch * a.heads * a.q_len) + at;
+                store_part<D>(a.part_out + to * a.dim, o_at, f, a.dim, mine_to_write && live, mine > 0);
+                if (mine_to_write) a.part_lse2[to] = live ? m + log2f(l) : -INFINITY;
+            } else {
+                T* out = static_cast<T*>(a.out.data) + w.b * a.out.batch_stride + h * a.out.head_stride + row * a.out.token_stride;
+                store_row<T, D>(out, o_at, f, a.dim, mine_to_write, live, mine > 0);
+                if (mine_to_write) a.lse[at] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
+            }
         }
         tc::fence_before();
     }
@@ -811,14 +894,14 @@ EncodeFn encode_fn() {
 }
 
 // Boxes of 128 tokens x 64 values of one head; what lies beyond the tensor reads as zero.
-CUtensorMap make_map(const AttnArgs& a, const SxAttentionView& v, int64_t tokens, int64_t heads) {
+CUtensorMap make_map(const AttnArgs& a, const SxAttentionView& v, int64_t tokens, int64_t heads, int box_tokens = kRows, int box_heads = 1) {
     CUtensorMap m;
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.dim), static_cast<cuuint64_t>(tokens),
                                 static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(a.batch)};
     // an axis of one entry may have any stride: the row's own length stands for it
     const auto bytes = [&](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(2 * (n > 1 ? stride : a.dim)); };
     const cuuint64_t strides[3] = {bytes(tokens, v.token_stride), bytes(heads, v.head_stride), bytes(a.batch, v.batch_stride)};
-    const cuuint32_t box[4] = {64, kRows, 1, 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box_tokens), static_cast<cuuint32_t>(box_heads), 1}, step[4] = {1, 1, 1, 1};
     const CUresult r = encode_fn()(&m, a.dtype == SXCUDA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                                    4, v.data, dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -854,7 +937,23 @@ bool attention_tc_takes_view(const AttnArgs& a, const SxAttentionView& v, int64_
     return copies(a, v, tokens, heads);
 }
 
-void launch_attention_fwd_tc(const AttnArgs& a, cudaStream_t s) {
+// The queries of the heads that share a key-value head make one tile where they fit in it: the keys are
+// then read once for all of them. Where there are fewer CTAs than SMs the keys are split over several
+// (two tiles of them at least) and their parts joined.
+AttnPlan attention_fwd_plan(const AttnArgs& a) {
+    AttnPlan p;
+    p.packed = a.group > 1 && a.q_len * a.group <= kRows;
+    p.blocks = p.packed ? a.kv_heads * a.batch : (a.q_len + 2 * kRows - 1) / (2 * kRows) * a.heads * a.batch;
+    const int64_t tiles = (a.kv_len + kRows - 1) / kRows, sms = sm_count();
+    if (p.blocks > 0 && p.blocks * 2 <= sms) p.splits = static_cast<int32_t>(std::max<int64_t>(std::min(sms / p.blocks, tiles / 2), 1));
+    return p;
+}
+
+void launch_attention_fwd_tc(const AttnArgs& args, cudaStream_t s) {
+    AttnArgs a = args;
+    const AttnPlan plan = attention_fwd_plan(a);
+    a.packed = plan.packed;
+    a.splits = plan.splits;
     by_type_dim(a, [&](auto t, auto d) {
         constexpr int D = decltype(d)::value;
         const auto kernel = attn_fwd_tc_kernel<decltype(t), D>;
@@ -862,12 +961,16 @@ void launch_attention_fwd_tc(const AttnArgs& a, cudaStream_t s) {
         static_assert(smem <= kSmemMost, "shared memory");
         smem_limit_once(reinterpret_cast<const void*>(kernel), smem, "attention_fwd");
         TcMaps maps;
-        maps.q = make_map(a, a.q, a.q_len, a.heads);
+        maps.q = plan.packed ? make_map(a, a.q, a.q_len, a.heads, static_cast<int>(a.q_len), a.group) : make_map(a, a.q, a.q_len, a.heads);
         maps.k = make_map(a, a.k, a.kv_len, a.kv_heads);
         maps.v = make_map(a, a.v, a.kv_len, a.kv_heads);
-        const int64_t grid = (a.q_len + 2 * kRows - 1) / (2 * kRows) * a.heads * a.batch;
+        const int64_t grid = plan.blocks * plan.splits;
         if (grid > INT32_MAX) throw_invalid("attention_fwd", "too many query tiles");
         SX_LAUNCH(kernel, static_cast<unsigned>(grid), kFwdThreads, smem, s, a, maps);
+        if (plan.splits > 1) {
+            const auto join = attn_join_kernel<decltype(t)>;
+            SX_LAUNCH(join, blocks_for(a.batch * a.heads * a.q_len, 8), 256, 0, s, a);
+        }
     });
 }
 

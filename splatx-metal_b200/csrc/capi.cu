@@ -1102,6 +1102,7 @@ int32_t sxcuda_attention_fwd(const SxAttentionInputs* in, const SxAttentionView*
         if (!out) throw_invalid(w, "null out");
         validate_view(*out, *in, in->q_len, in->q_heads, true, w, "out");
         if (in->batch && in->q_len) validate_pointer(lse, SXCUDA_F32, w, "lse");
+        if (*ws_bytes && reinterpret_cast<uintptr_t>(ws) % 16 != 0) throw_invalid(w, "workspace must be 16-byte aligned");
         launch_attention_fwd(*in, *out, lse, ws, as_stream(stream));
     });
 }

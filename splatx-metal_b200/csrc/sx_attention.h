@@ -29,8 +29,20 @@ struct AttnArgs {
     int32_t heads, kv_heads, group, dim, dtype;
     bool causal;
     float scale, scale_log2;
+    // the tensor-core forward: heads of a group in one tile; parts of the keys per query, and what the
+    // CTAs of a part leave: [splits, batch, heads, q_len, dim] and the same without dim
+    bool packed;
+    int32_t splits;
+    float* part_out;
+    float* part_lse2;
 };
 AttnArgs attn_args(const SxAttentionInputs& in);
+struct AttnPlan {
+    bool packed = false;
+    int32_t splits = 1;
+    int64_t blocks = 0;
+};
+AttnPlan attention_fwd_plan(const AttnArgs& a);
 
 // The tensor-core kernels (attention_tc.cu): whether they take q, k and v, or another view of the
 // call, and their launch.
