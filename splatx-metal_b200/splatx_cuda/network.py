@@ -108,11 +108,15 @@ def _attention_inputs(what, q, k, v, scale, causal, q_lens, kv_lens):
     return q, k, v, ins, device
 
 
-def _workspace(entry, device, ins, *rest) -> torch.Tensor:
-    """Device memory of the size that the entry point asks for (at least one byte: a pointer)."""
+def _workspace(entry, device, ins):
+    """(tensor, its pointer, its size) of the workspace that the entry point asks for; where it needs
+    none, a pointer that it does not read."""
     nbytes = C.c_size_t(0)
-    check(entry(C.byref(ins), *rest, None, C.byref(nbytes), None))
-    return torch.empty(max(nbytes.value, 1), dtype=torch.uint8, device=device)
+    check(entry(C.byref(ins), None, None, None, C.byref(nbytes), None))
+    if not nbytes.value:
+        return None, 16, nbytes
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), nbytes
 
 
 def attention_fwd(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=None):
@@ -126,13 +130,12 @@ def attention_fwd(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=Non
     and log-sum -inf."""
     q, k, v, ins, device = _attention_inputs("attention_fwd", q, k, v, scale, causal, q_lens, kv_lens)
     b, n, h, _ = q.shape
-    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((b, h, n), dtype=torch.float32, device=device)
     ov, entry = _nat.SxAttentionView(*_view(out)), _nat.lib().sxcuda_attention_fwd
     with _at(device) as stream:
-        ws = _workspace(entry, device, ins, None, None)
-        check(entry(C.byref(ins), C.byref(ov), lse.data_ptr(), ws.data_ptr(),
-                    C.byref(C.c_size_t(ws.numel())), stream))
+        ws, at, nbytes = _workspace(entry, device, ins)
+        check(entry(C.byref(ins), C.byref(ov), lse.data_ptr(), at, C.byref(nbytes), stream))
     return out, lse
 
 
@@ -150,13 +153,12 @@ def attention_bwd(v_out, q, k, v, out, lse, *, scale=None, causal=False, q_lens=
     _on(device, what, v_out, out, lse)
     v_out, out = _heads_last(v_out, what), _heads_last(out, what)
     gin = _nat.SxAttentionGradsIn(_view(out), lse.data_ptr(), _view(v_out))
-    grads = tuple(torch.empty(t.shape, dtype=q.dtype, device=device) for t in (q, k, v))
+    grads = tuple(torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     gout = _nat.SxAttentionGrads(*(_view(t) for t in grads))
     entry = _nat.lib().sxcuda_attention_bwd
     with _at(device) as stream:
-        ws = _workspace(entry, device, ins, None, None)
-        check(entry(C.byref(ins), C.byref(gin), C.byref(gout), ws.data_ptr(),
-                    C.byref(C.c_size_t(ws.numel())), stream))
+        ws, at, nbytes = _workspace(entry, device, ins)
+        check(entry(C.byref(ins), C.byref(gin), C.byref(gout), at, C.byref(nbytes), stream))
     return grads
 
 
@@ -215,7 +217,7 @@ def layer_norm_fwd(x, weight=None, bias=None, *, eps=1e-5):
     """Layer norm over the last axis: (y like x, mean, rstd of x.shape[:-1] in float32). weight and
     bias (each may be None: ones, zeros) have one dtype, which need not be x's."""
     flat, ins, device, cols = _norm_inputs("layer_norm_fwd", x, weight, bias, eps)
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
     rstd = torch.empty_like(mean)
     with _at(device) as stream:
@@ -237,16 +239,15 @@ def layer_norm_bwd(v_y, x, weight, mean, rstd):
                              f"{tuple(x.shape[:-1])}")
     _on(device, what, v_y, mean, rstd)
     g, _, g_stride = _rows(v_y, cols)
-    v_x = torch.empty(x.shape, dtype=x.dtype, device=device)
-    v_w = torch.empty(cols, dtype=torch.float32 if weight is None else weight.dtype, device=device)
+    v_x = torch.empty_like(x, memory_format=torch.contiguous_format)
+    v_w = torch.empty(cols, dtype=torch.float32, device=device) if weight is None else torch.empty_like(weight)
     v_b = torch.empty_like(v_w)
     gin = _nat.SxLayerNormGradsIn(mean.data_ptr(), rstd.data_ptr(), g.data_ptr(), g_stride)
     out = _nat.SxLayerNormGrads(v_x.data_ptr(), cols, v_w.data_ptr(), v_b.data_ptr())
     entry = _nat.lib().sxcuda_layer_norm_bwd
     with _at(device) as stream:
-        ws = _workspace(entry, device, ins, None, None)
-        check(entry(C.byref(ins), C.byref(gin), C.byref(out), ws.data_ptr(),
-                    C.byref(C.c_size_t(ws.numel())), stream))
+        ws, at, nbytes = _workspace(entry, device, ins)
+        check(entry(C.byref(ins), C.byref(gin), C.byref(out), at, C.byref(nbytes), stream))
     return v_x, v_w, v_b
 
 
