@@ -22,7 +22,9 @@ namespace {
 
 constexpr int kRows = 128;            // rows of every tile: queries or keys
 constexpr int kPanel = kRows * 128;   // bytes of a tile's 64 columns
-constexpr int kSlots = 5;             // tiles of the key-value ring
+// Tiles of the ring: what shared memory holds beside a CTA's own two at 128 columns, enough at 64.
+template <int D>
+constexpr int kRing = D == 64 ? 8 : 5;
 constexpr int kSmemMost = 232448;
 
 struct TcMaps {
@@ -164,19 +166,20 @@ constexpr int kPoly = D == 64 ? 1 : 3;
 template <int D>
 struct FwdSmem {
     static constexpr int kTileBytes = D / 64 * kPanel;
-    static constexpr int kQ = 0, kRing = 2 * kTileBytes, kBars = kRing + kSlots * kTileBytes;
+    static constexpr int kQ = 0, kRing = 2 * kTileBytes, kSlots = sx::kRing<D>, kBars = kRing + kSlots * kTileBytes;
     static constexpr int kBytes = kBars + 256;
 };
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnArgs a, const __grid_constant__ TcMaps maps) {
     using S = FwdSmem<D>;
+    constexpr int kSlots = S::kSlots;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = tc::smem_addr(smem);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(bars + 28);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 29);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(bars + 30);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(bars + 31);
     const uint32_t bar0 = base + S::kBars;
     const auto kv_full = [&](int s) { return bar0 + 8 * s; };
     const auto kv_free = [&](int s) { return bar0 + 8 * (kSlots + s); };
@@ -445,14 +448,16 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
 //
 // A query CTA owns 128 queries (rows: queries, columns: keys): S = Q K^T, W = G V^T, v_q += dS K, with
 // the next S a tile ahead.
+constexpr int kBwdThreads = 352;
 template <int D>
 struct BwdSmem {
     static constexpr int kTileBytes = D / 64 * kPanel;
-    static constexpr int kOwn = 0, kRing = 2 * kTileBytes, kStats = kRing + kSlots * kTileBytes;
+    static constexpr int kOwn = 0, kRing = 2 * kTileBytes, kSlots = sx::kRing<D>, kStats = kRing + kSlots * kTileBytes;
     static constexpr int kBars = kStats + 2 * 2 * kRows * 4;  // lse and delta of two query tiles
     static constexpr int kBytes = kBars + 256;
 };
 
+template <int kSlots>
 struct BwdBars {
     uint32_t at;
     __device__ uint32_t full(int s) const { return at + 8 * s; }
@@ -468,9 +473,10 @@ struct BwdBars {
     __device__ uint32_t drained() const { return at + 8 * (2 * kSlots + 12); }
     static constexpr int kFailed = 2 * kSlots + 13, kTmem = kFailed + 1;  // words of 8 bytes behind the barriers
 };
-static_assert((BwdBars::kTmem + 1) * 8 <= 256, "barriers");
+static_assert((BwdBars<8>::kTmem + 1) * 8 <= 256, "barriers");
 
-__device__ __forceinline__ void bwd_init(const BwdBars& b, volatile uint32_t* failed) {
+template <int kSlots>
+__device__ __forceinline__ void bwd_init(const BwdBars<kSlots>& b, volatile uint32_t* failed) {
     *failed = 0;
     for (int s = 0; s < kSlots; ++s) tc::bar_init(b.full(s), 1), tc::bar_init(b.free(s), 1);
     tc::bar_init(b.own(), 1);
@@ -548,8 +554,9 @@ __device__ __forceinline__ void keep_columns(uint32_t (&r)[32], int lo, int hi) 
 
 template <typename T, int D>
 __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
-                                            const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
+                                            const BwdBars<kRing<D>>& bars, uint32_t tmem, volatile uint32_t* failed) {
     using S = BwdSmem<D>;
+    constexpr int kSlots = S::kSlots;
     const uint32_t base = tc::smem_addr(smem);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     // the first keys are seen by the most queries when causal: they start first
@@ -570,7 +577,7 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
     const auto s_bar = [&](int i) { return bars.s_full(kAhead ? i & 1 : 0); };
     const auto s_par = [](int i) { return static_cast<uint32_t>(kAhead ? i >> 1 : i) & 1; };
 
-    if (warp == 8) {  // loads: K and V, then Q0 G0 Q1 G1 ... around the ring, lse and delta beside each Q
+    if (warp == 8) {  // loads: K and V, then Q0 G0 Q1 G1 ... around the ring
         if (lane == 0 && total) {
             tc::bar_expect(bars.own(), 2 * S::kTileBytes);
             for (int p = 0; p < D / 64; ++p) {
@@ -582,21 +589,26 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
         for (; it < 2 * total; ++it) {
             const int s = it % kSlots, round = it / kSlots, i = it / 2;
             if (round && !tc::bar_wait(bars.free(s), (round - 1) & 1, failed)) break;
-            if (!(it & 1) && i >= 2 && !tc::bar_wait(bars.stat_free(i & 1), (i / 2 - 1) & 1, failed)) break;
+            if (lane == 0)
+                load_rows<D>(slot(it), it & 1 ? &maps.g : &maps.q, (first + i % tiles) * kRows, hk * a.group + i / tiles, batch, bars.full(s));
+            __syncwarp();
+        }
+        return {it, total > 0, 0};
+    } else if (warp == 10) {  // loads of lse and delta, two tiles ahead (a warp of their own: in line with
+                              // the others they held the next queries up until a tile's end)
+        int i = 0;
+        for (; i < total; ++i) {
+            if (i >= 2 && !tc::bar_wait(bars.stat_free(i & 1), (i / 2 - 1) & 1, failed)) break;
             if (lane == 0) {
-                const int h = hk * a.group + i / tiles, row = (first + i % tiles) * kRows;
-                load_rows<D>(slot(it), it & 1 ? &maps.g : &maps.q, row, h, batch, bars.full(s));
-                if (!(it & 1)) {
-                    const int64_t at = (static_cast<int64_t>(batch) * a.heads + h) * a.q_pad + row;
-                    const uint32_t to = base + S::kStats + (i & 1) * 2 * kRows * 4;
-                    tc::bar_expect(bars.stat_full(i & 1), 2 * kRows * 4);
-                    tc::bulk_load(to, a.minus_lse2 + at, kRows * 4, bars.stat_full(i & 1));
-                    tc::bulk_load(to + kRows * 4, a.minus_delta + at, kRows * 4, bars.stat_full(i & 1));
-                }
+                const int64_t at = (static_cast<int64_t>(batch) * a.heads + hk * a.group + i / tiles) * a.q_pad + (first + i % tiles) * kRows;
+                const uint32_t to = base + S::kStats + (i & 1) * 2 * kRows * 4;
+                tc::bar_expect(bars.stat_full(i & 1), 2 * kRows * 4);
+                tc::bulk_load(to, a.minus_lse2 + at, kRows * 4, bars.stat_full(i & 1));
+                tc::bulk_load(to + kRows * 4, a.minus_delta + at, kRows * 4, bars.stat_full(i & 1));
             }
             __syncwarp();
         }
-        return {it, total > 0, (it + 1) / 2};
+        return {0, false, i};
     } else if (warp == 9) {  // products
         const uint32_t one = tc::elect();
         const auto arrived = [&](int item) {  // the tile is there, padding behind the queries' end zeroed
@@ -724,8 +736,9 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
 
 template <typename T, int D>
 __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
-                                           const BwdBars& bars, uint32_t tmem, volatile uint32_t* failed) {
+                                           const BwdBars<kRing<D>>& bars, uint32_t tmem, volatile uint32_t* failed) {
     using S = BwdSmem<D>;
+    constexpr int kSlots = S::kSlots;
     const uint32_t base = tc::smem_addr(smem);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const int64_t heads = static_cast<int64_t>(a.heads) * a.batch, tiles = (a.q_len + kRows - 1) / kRows;
@@ -782,7 +795,7 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
             tc::commit(one, j + 1 < n ? bars.free(2 * j % kSlots) : bars.out_full());
             if (j + 1 < n) ok = weights(j + 1);
         }
-    } else {
+    } else if (warp < 8) {
         const int half = warp >> 2;
         const int64_t row = q0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -845,13 +858,14 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
 // One launch holds both kinds of CTA: the query CTAs fill the SMs that the key-value CTAs' last wave
 // leaves idle.
 template <typename T, int D>
-__global__ void __launch_bounds__(320, 1) attn_bwd_tc_kernel(const AttnArgs a, const __grid_constant__ TcMaps maps, int64_t kv_blocks) {
+__global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_tc_kernel(const AttnArgs a, const __grid_constant__ TcMaps maps, int64_t kv_blocks) {
     using S = BwdSmem<D>;
+    constexpr int kSlots = S::kSlots;
     extern __shared__ __align__(1024) uint8_t smem[];
-    const BwdBars bars{tc::smem_addr(smem) + S::kBars};
+    const BwdBars<S::kSlots> bars{tc::smem_addr(smem) + S::kBars};
     uint64_t* words = reinterpret_cast<uint64_t*>(smem + S::kBars);
-    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(words + BwdBars::kFailed);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(words + BwdBars::kTmem);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(words + bars.kFailed);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(words + bars.kTmem);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0);
     if (threadIdx.x == 0) bwd_init(bars, failed);
     if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
@@ -864,7 +878,7 @@ __global__ void __launch_bounds__(320, 1) attn_bwd_tc_kernel(const AttnArgs a, c
     tc::fence_before();
     __syncthreads();
     if (*failed) {  // nothing may land in this CTA's memory after it has gone
-        if (warp == 8) {
+        if (warp == 8 || warp == 10) {
             if (asked.own) tc::bar_drain(bars.own(), 0);
             for (int i = max(0, asked.ring - kSlots); i < asked.ring; ++i) tc::bar_drain(bars.full(i % kSlots), (i / kSlots) & 1);
             for (int i = max(0, asked.stats - 2); i < asked.stats; ++i) tc::bar_drain(bars.stat_full(i & 1), (i / 2) & 1);
@@ -989,7 +1003,7 @@ void launch_attention_bwd_tc(const AttnArgs& a, cudaStream_t s) {
         const int64_t kv_blocks = (a.kv_len + kRows - 1) / kRows * a.kv_heads * a.batch;
         const int64_t grid = kv_blocks + (a.q_len + kRows - 1) / kRows * a.heads * a.batch;
         if (grid > INT32_MAX) throw_invalid("attention_bwd", "too many tiles");
-        SX_LAUNCH(kernel, static_cast<unsigned>(grid), 320, smem, s, a, maps, kv_blocks);
+        SX_LAUNCH(kernel, static_cast<unsigned>(grid), kBwdThreads, smem, s, a, maps, kv_blocks);
     });
 }
 
