@@ -31,6 +31,18 @@ struct TcMaps {
     CUtensorMap q, k, v, g;
 };
 
+// A place in the ring that goes round with the tiles, in turn: the slot and the parity of its phase. The
+// warps that load and issue are one each, and what they compute between two instructions of theirs is
+// time that the tensor cores may wait: they count on instead of dividing.
+template <int N>
+struct Cursor {
+    int slot = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next() {
+        if (++slot == N) slot = 0, parity ^= 1;
+    }
+};
+
 // Rows from `first` of a tile in shared memory become zeros (the padding behind a batch entry's
 // length may hold NaN, which a probability of zero would not remove).
 template <int D>
@@ -243,9 +255,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                     if (n[t])
                         load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t),
                                      a.packed ? static_cast<int>(a.q_len) * a.group : kRows);
-            for (; loaded < 2 * most; ++loaded) {
-                const int s = loaded % kSlots, round = loaded / kSlots;
-                if (round && !tc::bar_wait(kv_free(s), (round - 1) & 1, failed)) break;
+            Cursor<kSlots> at;
+            for (; loaded < 2 * most; ++loaded, at.next()) {
+                const int s = at.slot;
+                if (loaded >= kSlots && !tc::bar_wait(kv_free(s), at.parity ^ 1, failed)) break;
                 if (lane == 0)
                     load_rows<D>(base + S::kRing + s * S::kTileBytes, loaded & 1 ? &maps.v : &maps.k, (j0 + loaded / 2) * kRows, hk, static_cast<int>(w.b), kv_full(s));
                 __syncwarp();
@@ -256,7 +269,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 rows_rows<T, D>(one, tmem + t * kRows, base + S::kQ + t * S::kTileBytes, base + S::kRing + slot * S::kTileBytes);
                 tc::commit(one, s_full(t));
             };
+            Cursor<kSlots> at;
+            const bool ragged = kv_len % kRows && kv_len < a.kv_len;
             bool ok = most == 0 || tc::bar_wait(kv_full(0), 0, failed);
+            at.next();
             for (int t = 0; ok && t < 2; ++t)
                 if (n[t]) {
                     ok = tc::bar_wait(q_full(t), 0, failed);
@@ -264,12 +280,15 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 }
             if (ok && most) tc::commit(one, kv_free(0));
             for (int j = 0; ok && j < most; ++j) {
-                const int vi = 2 * j + 1, vs = vi % kSlots, ki = 2 * j + 2, ks = ki % kSlots;
-                ok = tc::bar_wait(kv_full(vs), (vi / kSlots) & 1, failed);
+                const int vs = at.slot;
+                ok = tc::bar_wait(kv_full(vs), at.parity, failed);
                 if (!ok) break;
-                if ((j0 + j + 1) * kRows > kv_len && kv_len < a.kv_len)
+                at.next();
+                const int ks = at.slot;
+                if (ragged && (j0 + j + 1) * kRows > kv_len)
                     zero_rows<D>(smem + S::kRing + vs * S::kTileBytes, kv_len - (j0 + j) * kRows, lane);
-                if (j + 1 < most) ok = tc::bar_wait(kv_full(ks), (ki / kSlots) & 1, failed);
+                if (j + 1 < most) ok = tc::bar_wait(kv_full(ks), at.parity, failed);
+                at.next();
                 for (int t = 0; ok && t < 2; ++t) {
                     if (j >= n[t]) continue;
                     if (kApart && j + 1 < n[t]) {
@@ -569,7 +588,7 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
     const int first = static_cast<int>(begin / kRows);
     const int tiles = k0 >= w.kv_len || begin >= q_len ? 0 : (q_len + kRows - 1) / kRows - first;
     const int total = tiles * a.group;
-    const auto slot = [&](int item) { return base + S::kRing + item % kSlots * S::kTileBytes; };
+    const auto slot = [&](int s) { return base + S::kRing + s * S::kTileBytes; };
     // with 64 columns of the sums there is room for the next S beside this one
     constexpr bool kAhead = D == 64;
     constexpr uint32_t kW = kAhead ? 2 * kRows : kRows, kVV = kW + kRows, kVK = kVV + D;
@@ -585,72 +604,83 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
                 tc::tma_load(base + S::kOwn + S::kTileBytes + p * kPanel, &maps.v, p * 64, k0, hk, batch, bars.own());
             }
         }
-        int it = 0;
-        for (; it < 2 * total; ++it) {
-            const int s = it % kSlots, round = it / kSlots, i = it / 2;
-            if (round && !tc::bar_wait(bars.free(s), (round - 1) & 1, failed)) break;
-            if (lane == 0)
-                load_rows<D>(slot(it), it & 1 ? &maps.g : &maps.q, (first + i % tiles) * kRows, hk * a.group + i / tiles, batch, bars.full(s));
+        int it = 0, tile = 0, h = hk * a.group;
+        Cursor<kSlots> at;
+        for (; it < 2 * total; ++it, at.next()) {
+            if (it >= kSlots && !tc::bar_wait(bars.free(at.slot), at.parity ^ 1, failed)) break;
+            if (lane == 0) load_rows<D>(slot(at.slot), it & 1 ? &maps.g : &maps.q, (first + tile) * kRows, h, batch, bars.full(at.slot));
+            if (it & 1 && ++tile == tiles) tile = 0, ++h;
             __syncwarp();
         }
         return {it, total > 0, 0};
     } else if (warp == 10) {  // loads of lse and delta, two tiles ahead (a warp of their own: in line with
                               // the others they held the next queries up until a tile's end)
-        int i = 0;
+        int i = 0, tile = 0;
+        int64_t at = (static_cast<int64_t>(batch) * a.heads + hk * a.group) * a.q_pad + first * kRows;
         for (; i < total; ++i) {
             if (i >= 2 && !tc::bar_wait(bars.stat_free(i & 1), (i / 2 - 1) & 1, failed)) break;
             if (lane == 0) {
-                const int64_t at = (static_cast<int64_t>(batch) * a.heads + hk * a.group + i / tiles) * a.q_pad + (first + i % tiles) * kRows;
                 const uint32_t to = base + S::kStats + (i & 1) * 2 * kRows * 4;
                 tc::bar_expect(bars.stat_full(i & 1), 2 * kRows * 4);
                 tc::bulk_load(to, a.minus_lse2 + at, kRows * 4, bars.stat_full(i & 1));
                 tc::bulk_load(to + kRows * 4, a.minus_delta + at, kRows * 4, bars.stat_full(i & 1));
             }
+            at += kRows;
+            if (++tile == tiles) tile = 0, at += a.q_pad - tiles * kRows;
             __syncwarp();
         }
         return {0, false, i};
     } else if (warp == 9) {  // products
         const uint32_t one = tc::elect();
-        const auto arrived = [&](int item) {  // the tile is there, padding behind the queries' end zeroed
-            if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
-            const int row = (first + item / 2 % tiles) * kRows;
-            if (row + kRows > q_len && q_len < a.q_len)
-                zero_rows<D>(smem + S::kRing + item % kSlots * S::kTileBytes, q_len - row, lane);
+        Cursor<kSlots> at;
+        int to_end = tiles;  // tiles to the end of a head's queries, where padding is zeroed
+        const bool ragged = q_len % kRows && q_len < a.q_len;
+        uint32_t queries = 0, grads = 0;  // slots of the tile that is worked on
+        const auto arrived = [&] {
+            if (!tc::bar_wait(bars.full(at.slot), at.parity, failed)) return false;
+            if (ragged && to_end == 1) zero_rows<D>(smem + S::kRing + at.slot * S::kTileBytes, q_len % kRows, lane);
             return true;
         };
         const auto scores = [&](int i) {
-            if (!arrived(2 * i)) return false;
-            rows_rows<T, D>(one, tmem + s_col(i), base + S::kOwn, slot(2 * i));
+            if (!arrived()) return false;
+            rows_rows<T, D>(one, tmem + s_col(i), base + S::kOwn, slot(at.slot));
             tc::commit(one, s_bar(i));
+            at.next();
             return true;
         };
-        const auto weights = [&](int i) {
-            if (!arrived(2 * i + 1)) return false;
-            rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(2 * i + 1));
+        const auto weights = [&] {
+            if (!arrived()) return false;
+            rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(at.slot));
             tc::commit(one, bars.w_full());
+            at.next();
+            if (--to_end == 0) to_end = tiles;
             return true;
         };
-        bool ok = total == 0 || (tc::bar_wait(bars.own(), 0, failed) && scores(0) && weights(0));
+        bool ok = total == 0 || (tc::bar_wait(bars.own(), 0, failed) && scores(0) && weights());
+        grads = 1;
         for (int i = 0; ok && i < total; ++i) {
+            const uint32_t q_next = at.slot;
             if (kAhead && i + 1 < total) ok = scores(i + 1);
             for (int c = 0; ok && c < 2; ++c) {  // half of the queries while the others' p are made
                 ok = tc::bar_wait(bars.p_full(c), i & 1, failed);
                 if (!ok) break;
                 tc::fence_after();
-                const uint32_t p = tmem + s_col(i) + c * 16, g = slot(2 * i + 1) + c * 32 * 128;
+                const uint32_t p = tmem + s_col(i) + c * 16, g = slot(grads) + c * 32 * 128;
                 tmem_rows<T, D, 2>(one, tmem + kVV, p, g, i > 0 || c > 0);
                 tmem_rows<T, D, 2>(one, tmem + kVV, p + 64, g + 64 * 128, true);
             }
             if (!ok) break;
-            tc::commit(one, bars.free((2 * i + 1) % kSlots));
+            tc::commit(one, bars.free(grads));
             if (!kAhead && i + 1 < total) ok = scores(i + 1);
             if (!ok) break;
             ok = tc::bar_wait(bars.ds_full(), i & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            tmem_rows2<T, D, 64>(one, tmem + kVK, tmem + kW, slot(2 * i), i > 0);
-            tc::commit(one, i + 1 < total ? bars.free(2 * i % kSlots) : bars.out_full());
-            if (i + 1 < total) ok = weights(i + 1);
+            tmem_rows2<T, D, 64>(one, tmem + kVK, tmem + kW, slot(queries), i > 0);
+            tc::commit(one, i + 1 < total ? bars.free(queries) : bars.out_full());
+            queries = q_next;
+            grads = at.slot;
+            if (i + 1 < total) ok = weights();
         }
     } else {
         const int half = warp >> 2;
@@ -660,8 +690,10 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
         const HalfScale scale = half_scale<T>(a);
         const tc::Two times = tc::two(a.scale_log2, a.scale_log2), ds_scale = tc::two(scale.p * scale.ds, scale.p * scale.ds);
         bool ok = true;
+        int tile = 0;
         for (int i = 0; i < total; ++i) {
-            const int64_t q0 = static_cast<int64_t>(first + i % tiles) * kRows + half * 64;
+            const int64_t q0 = static_cast<int64_t>(first + tile) * kRows + half * 64;
+            if (++tile == tiles) tile = 0;
             ok = tc::bar_wait(s_bar(i), s_par(i), failed) && tc::bar_wait(bars.stat_full(i & 1), (i / 2) & 1, failed);
             if (!ok) break;
             tc::fence_after();
@@ -747,7 +779,7 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
     const AttnHead w = attn_head(a, h, batch);
     const int kv_len = static_cast<int>(w.kv_len);
     const int n = q0 >= w.q_len ? 0 : static_cast<int>((attn_keys_end(w, q0 + kRows) + kRows - 1) / kRows);
-    const auto slot = [&](int item) { return base + S::kRing + item % kSlots * S::kTileBytes; };
+    const auto slot = [&](int s) { return base + S::kRing + s * S::kTileBytes; };
     constexpr uint32_t kW = 2 * kRows, kVQ = 3 * kRows;
 
     if (warp == 8) {  // loads: Q and G, then K0 V0 K1 V1 ... around the ring
@@ -759,41 +791,45 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
             }
         }
         int it = 0;
-        for (; it < 2 * n; ++it) {
-            const int s = it % kSlots, round = it / kSlots;
-            if (round && !tc::bar_wait(bars.free(s), (round - 1) & 1, failed)) break;
-            if (lane == 0) load_rows<D>(slot(it), it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, batch, bars.full(s));
+        Cursor<kSlots> at;
+        for (; it < 2 * n; ++it, at.next()) {
+            if (it >= kSlots && !tc::bar_wait(bars.free(at.slot), at.parity ^ 1, failed)) break;
+            if (lane == 0) load_rows<D>(slot(at.slot), it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, batch, bars.full(at.slot));
             __syncwarp();
         }
         return {it, n > 0, 0};
     } else if (warp == 9) {  // products
         const uint32_t one = tc::elect();
+        Cursor<kSlots> at;  // the tiles are taken in the order K0 V0 K1 V1 ...
+        const bool ragged = kv_len % kRows && kv_len < a.kv_len;
+        uint32_t keys = 0, keys_next = 0;
         const auto scores = [&](int j) {
-            const int item = 2 * j;
-            if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
-            if ((j + 1) * kRows > kv_len && kv_len < a.kv_len)
-                zero_rows<D>(smem + S::kRing + item % kSlots * S::kTileBytes, kv_len - j * kRows, lane);
-            rows_rows<T, D>(one, tmem + (j & 1) * kRows, base + S::kOwn, slot(item));
+            if (!tc::bar_wait(bars.full(at.slot), at.parity, failed)) return false;
+            if (ragged && (j + 1) * kRows > kv_len) zero_rows<D>(smem + S::kRing + at.slot * S::kTileBytes, kv_len - j * kRows, lane);
+            rows_rows<T, D>(one, tmem + (j & 1) * kRows, base + S::kOwn, slot(at.slot));
             tc::commit(one, bars.s_full(j & 1));
+            keys_next = at.slot;
+            at.next();
             return true;
         };
-        const auto weights = [&](int j) {
-            const int item = 2 * j + 1;
-            if (!tc::bar_wait(bars.full(item % kSlots), (item / kSlots) & 1, failed)) return false;
-            rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(item));
+        const auto weights = [&] {
+            if (!tc::bar_wait(bars.full(at.slot), at.parity, failed)) return false;
+            rows_rows<T, D>(one, tmem + kW, base + S::kOwn + S::kTileBytes, slot(at.slot));
             tc::commit(one, bars.w_full());
-            tc::commit(one, bars.free(item % kSlots));
+            tc::commit(one, bars.free(at.slot));
+            at.next();
             return true;
         };
-        bool ok = n == 0 || (tc::bar_wait(bars.own(), 0, failed) && scores(0) && weights(0));
+        bool ok = n == 0 || (tc::bar_wait(bars.own(), 0, failed) && scores(0) && weights());
         for (int j = 0; ok && j < n; ++j) {
+            keys = keys_next;
             if (j + 1 < n) ok = scores(j + 1);
             if (ok) ok = tc::bar_wait(bars.ds_full(), j & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            tmem_rows2<T, D, 64>(one, tmem + kVQ, tmem + kW, slot(2 * j), j > 0);
-            tc::commit(one, j + 1 < n ? bars.free(2 * j % kSlots) : bars.out_full());
-            if (j + 1 < n) ok = weights(j + 1);
+            tmem_rows2<T, D, 64>(one, tmem + kVQ, tmem + kW, slot(keys), j > 0);
+            tc::commit(one, j + 1 < n ? bars.free(keys) : bars.out_full());
+            if (j + 1 < n) ok = weights();
         }
     } else if (warp < 8) {
         const int half = warp >> 2;

@@ -40,13 +40,24 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {  // without waiting
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 constexpr long long kWaitCycles = 4000000000ll;  // two seconds at the highest clock
 
 // Waits, as a whole warp, for the barrier's phase of `parity`. Gives up after two seconds, or once
 // another warp of the CTA has: returns false then, the same for every lane, with *failed set. The
 // waiting is left to the hardware: warps that poll take issue slots from those that compute.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* failed) {
-    if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
+    if (__all_sync(0xffffffffu, bar_test(bar, parity))) return true;
     const long long start = clock64();
     for (;;) {
         if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
