@@ -89,6 +89,7 @@ __device__ __forceinline__ void tmem_rows2(uint32_t one, uint32_t d, uint32_t a,
 // A thread's row of a finished D-column sum, times `f`, to memory; zeros where `live` is false.
 template <typename T, int D>
 __device__ __forceinline__ void store_row(T* out, uint32_t at, float f, int dim, bool written, bool live, bool any) {
+    const bool wide = reinterpret_cast<uintptr_t>(out) % 32 == 0;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -96,16 +97,20 @@ __device__ __forceinline__ void store_row(T* out, uint32_t at, float f, int dim,
             tc::tmem_load32(o, at + c * 32);
             tc::wait_ld(o);
         }
+        uint32_t x[16];
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) {
-            uint4 x{0, 0, 0, 0};
-            if (live) {
-                uint32_t* px = reinterpret_cast<uint32_t*>(&x);
+        for (int i = 0; i < 16; ++i)
+            x[i] = live ? tc::pack2<T>(__uint_as_float(o[2 * i]) * f, __uint_as_float(o[2 * i + 1]) * f) : 0u;
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    px[e] = tc::pack2<T>(__uint_as_float(o[i + 2 * e]) * f, __uint_as_float(o[i + 2 * e + 1]) * f);
+        for (int i = 0; i < 32; i += 16) {
+            uint32_t(&y)[8] = *reinterpret_cast<uint32_t(*)[8]>(x + i / 2);
+            if (!written) continue;
+            if (wide && c * 32 + i + 8 < dim) {
+                tc::store32(out + c * 32 + i, y);
+            } else {
+                if (c * 32 + i < dim) *reinterpret_cast<uint4*>(out + c * 32 + i) = uint4{y[0], y[1], y[2], y[3]};
+                if (c * 32 + i + 8 < dim) *reinterpret_cast<uint4*>(out + c * 32 + i + 8) = uint4{y[4], y[5], y[6], y[7]};
             }
-            if (written && c * 32 + i < dim) *reinterpret_cast<uint4*>(out + c * 32 + i) = x;
         }
         __syncwarp();
     }
@@ -225,7 +230,17 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
     }
     const int most = max(n[0], n[1]);
 
-    if (threadIdx.x == 0) {
+    // Warp 8 asks for the first tiles before anything else is ready.
+    int loaded = 0;  // tiles of the ring that warp 8 has asked for
+    Cursor<kSlots> load_at;
+    const auto load_kv = [&] {
+        load_rows<D>(base + S::kRing + load_at.slot * S::kTileBytes, loaded & 1 ? &maps.v : &maps.k, (j0 + loaded / 2) * kRows, hk,
+                     static_cast<int>(w.b), kv_full(load_at.slot));
+    };
+    if (warp == 8 && lane == 0) {
+        tc::prefetch_map(&maps.q);
+        tc::prefetch_map(&maps.k);
+        tc::prefetch_map(&maps.v);
         *failed = 0;
         for (int s = 0; s < kSlots; ++s) tc::bar_init(kv_full(s), 1), tc::bar_init(kv_free(s), 1);
         for (int t = 0; t < 2; ++t) {
@@ -238,29 +253,27 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
         }
         tc::bar_init(drained, 1);
         tc::bar_init_fence();
+        for (int t = 0; t < 2; ++t)
+            if (n[t])
+                load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t),
+                             a.packed ? static_cast<int>(a.q_len) * a.group : kRows);
     }
+    if (warp == 8)
+        for (; loaded < min(2 * most, kSlots); ++loaded, load_at.next())
+            if (lane == 0) load_kv();
     if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = __shfl_sync(kFullMask, *tmem_at, 0);
 
-    int loaded = 0;  // tiles of the ring that warp 8 has asked for
     // 384 x 168 registers at the launch = 256 x 216 + 128 x 72
     if (warp >= 8) {
         tc::fewer_registers<72>();
-        if (warp == 8) {  // loads: Q tiles, then K0 V0 K1 V1 ... around the ring
-            if (lane == 0)
-                for (int t = 0; t < 2; ++t)
-                    if (n[t])
-                        load_rows<D>(base + S::kQ + t * S::kTileBytes, &maps.q, q0 + t * kRows, static_cast<int>(w.h), static_cast<int>(w.b), q_full(t),
-                                     a.packed ? static_cast<int>(a.q_len) * a.group : kRows);
-            Cursor<kSlots> at;
-            for (; loaded < 2 * most; ++loaded, at.next()) {
-                const int s = at.slot;
-                if (loaded >= kSlots && !tc::bar_wait(kv_free(s), at.parity ^ 1, failed)) break;
-                if (lane == 0)
-                    load_rows<D>(base + S::kRing + s * S::kTileBytes, loaded & 1 ? &maps.v : &maps.k, (j0 + loaded / 2) * kRows, hk, static_cast<int>(w.b), kv_full(s));
+        if (warp == 8) {  // loads: K0 V0 K1 V1 ... around the ring
+            for (; loaded < 2 * most; ++loaded, load_at.next()) {
+                if (!tc::bar_wait(kv_free(load_at.slot), load_at.parity ^ 1, failed)) break;
+                if (lane == 0) load_kv();
                 __syncwarp();
             }
         } else if (warp == 9) {  // products
@@ -513,6 +526,15 @@ __device__ __forceinline__ T* row_of(const SxAttentionView& v, int64_t b, int64_
     return static_cast<T*>(v.data) + b * v.batch_stride + h * v.head_stride + row * v.token_stride;
 }
 
+// Tensor memory for the CTA, and everything set up seen by everyone: its address.
+__device__ __forceinline__ uint32_t bwd_start(uint32_t* tmem_at, int warp) {
+    if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    return __shfl_sync(kFullMask, *tmem_at, 0);
+}
+
 // What the loading warp has asked for: tiles of the ring, the CTA's own tiles, lse and delta tiles.
 struct Loaded {
     int ring = 0;
@@ -573,7 +595,7 @@ __device__ __forceinline__ void keep_columns(uint32_t (&r)[32], int lo, int hi) 
 
 template <typename T, int D>
 __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
-                                            const BwdBars<kRing<D>>& bars, uint32_t tmem, volatile uint32_t* failed) {
+                                            const BwdBars<kRing<D>>& bars, volatile uint32_t* failed, uint32_t* tmem_at) {
     using S = BwdSmem<D>;
     constexpr int kSlots = S::kSlots;
     const uint32_t base = tc::smem_addr(smem);
@@ -596,21 +618,37 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
     const auto s_bar = [&](int i) { return bars.s_full(kAhead ? i & 1 : 0); };
     const auto s_par = [](int i) { return static_cast<uint32_t>(kAhead ? i >> 1 : i) & 1; };
 
-    if (warp == 8) {  // loads: K and V, then Q0 G0 Q1 G1 ... around the ring
-        if (lane == 0 && total) {
-            tc::bar_expect(bars.own(), 2 * S::kTileBytes);
-            for (int p = 0; p < D / 64; ++p) {
-                tc::tma_load(base + S::kOwn + p * kPanel, &maps.k, p * 64, k0, hk, batch, bars.own());
-                tc::tma_load(base + S::kOwn + S::kTileBytes + p * kPanel, &maps.v, p * 64, k0, hk, batch, bars.own());
+    int it = 0, load_tile = 0, load_h = hk * a.group;
+    Cursor<kSlots> load_at;
+    const auto load_next = [&] {
+        if (lane == 0)
+            load_rows<D>(slot(load_at.slot), it & 1 ? &maps.g : &maps.q, (first + load_tile) * kRows, load_h, batch, bars.full(load_at.slot));
+        if (it & 1 && ++load_tile == tiles) load_tile = 0, ++load_h;
+        ++it;
+        load_at.next();
+        __syncwarp();
+    };
+    if (warp == 8) {  // the first tiles are asked for before anything else is ready
+        if (lane == 0) {
+            tc::prefetch_map(&maps.q);
+            tc::prefetch_map(&maps.g);
+            bwd_init(bars, failed);
+            if (total) {
+                tc::bar_expect(bars.own(), 2 * S::kTileBytes);
+                for (int p = 0; p < D / 64; ++p) {
+                    tc::tma_load(base + S::kOwn + p * kPanel, &maps.k, p * 64, k0, hk, batch, bars.own());
+                    tc::tma_load(base + S::kOwn + S::kTileBytes + p * kPanel, &maps.v, p * 64, k0, hk, batch, bars.own());
+                }
             }
         }
-        int it = 0, tile = 0, h = hk * a.group;
-        Cursor<kSlots> at;
-        for (; it < 2 * total; ++it, at.next()) {
-            if (it >= kSlots && !tc::bar_wait(bars.free(at.slot), at.parity ^ 1, failed)) break;
-            if (lane == 0) load_rows<D>(slot(at.slot), it & 1 ? &maps.g : &maps.q, (first + tile) * kRows, h, batch, bars.full(at.slot));
-            if (it & 1 && ++tile == tiles) tile = 0, ++h;
-            __syncwarp();
+        while (it < min(2 * total, kSlots)) load_next();
+    }
+    const uint32_t tmem = bwd_start(tmem_at, warp);
+
+    if (warp == 8) {  // loads: Q0 G0 Q1 G1 ... around the ring
+        while (it < 2 * total) {
+            if (!tc::bar_wait(bars.free(load_at.slot), load_at.parity ^ 1, failed)) break;
+            load_next();
         }
         return {it, total > 0, 0};
     } else if (warp == 10) {  // loads of lse and delta, two tiles ahead (a warp of their own: in line with
@@ -768,7 +806,7 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
 
 template <typename T, int D>
 __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& maps, int64_t block, uint8_t* smem,
-                                           const BwdBars<kRing<D>>& bars, uint32_t tmem, volatile uint32_t* failed) {
+                                           const BwdBars<kRing<D>>& bars, volatile uint32_t* failed, uint32_t* tmem_at) {
     using S = BwdSmem<D>;
     constexpr int kSlots = S::kSlots;
     const uint32_t base = tc::smem_addr(smem);
@@ -782,20 +820,35 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
     const auto slot = [&](int s) { return base + S::kRing + s * S::kTileBytes; };
     constexpr uint32_t kW = 2 * kRows, kVQ = 3 * kRows;
 
-    if (warp == 8) {  // loads: Q and G, then K0 V0 K1 V1 ... around the ring
-        if (lane == 0 && n) {
-            tc::bar_expect(bars.own(), 2 * S::kTileBytes);
-            for (int p = 0; p < D / 64; ++p) {
-                tc::tma_load(base + S::kOwn + p * kPanel, &maps.q, p * 64, q0, h, batch, bars.own());
-                tc::tma_load(base + S::kOwn + S::kTileBytes + p * kPanel, &maps.g, p * 64, q0, h, batch, bars.own());
+    int it = 0;
+    Cursor<kSlots> load_at;
+    const auto load_next = [&] {
+        if (lane == 0) load_rows<D>(slot(load_at.slot), it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, batch, bars.full(load_at.slot));
+        ++it;
+        load_at.next();
+        __syncwarp();
+    };
+    if (warp == 8) {  // the first tiles are asked for before anything else is ready
+        if (lane == 0) {
+            tc::prefetch_map(&maps.k);
+            tc::prefetch_map(&maps.v);
+            bwd_init(bars, failed);
+            if (n) {
+                tc::bar_expect(bars.own(), 2 * S::kTileBytes);
+                for (int p = 0; p < D / 64; ++p) {
+                    tc::tma_load(base + S::kOwn + p * kPanel, &maps.q, p * 64, q0, h, batch, bars.own());
+                    tc::tma_load(base + S::kOwn + S::kTileBytes + p * kPanel, &maps.g, p * 64, q0, h, batch, bars.own());
+                }
             }
         }
-        int it = 0;
-        Cursor<kSlots> at;
-        for (; it < 2 * n; ++it, at.next()) {
-            if (it >= kSlots && !tc::bar_wait(bars.free(at.slot), at.parity ^ 1, failed)) break;
-            if (lane == 0) load_rows<D>(slot(at.slot), it & 1 ? &maps.v : &maps.k, it / 2 * kRows, hk, batch, bars.full(at.slot));
-            __syncwarp();
+        while (it < min(2 * n, kSlots)) load_next();
+    }
+    const uint32_t tmem = bwd_start(tmem_at, warp);
+
+    if (warp == 8) {  // loads: K0 V0 K1 V1 ... around the ring
+        while (it < 2 * n) {
+            if (!tc::bar_wait(bars.free(load_at.slot), load_at.parity ^ 1, failed)) break;
+            load_next();
         }
         return {it, n > 0, 0};
     } else if (warp == 9) {  // products
@@ -903,14 +956,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_tc_kernel(const AttnA
     volatile uint32_t* failed = reinterpret_cast<uint32_t*>(words + bars.kFailed);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(words + bars.kTmem);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0);
-    if (threadIdx.x == 0) bwd_init(bars, failed);
-    if (warp == 9) tc::tmem_alloc(tc::smem_addr(tmem_at), 512);
-    tc::fence_before();
-    __syncthreads();
-    tc::fence_after();
-    const uint32_t tmem = __shfl_sync(kFullMask, *tmem_at, 0);
-    const Loaded asked = blockIdx.x < kv_blocks ? bwd_kv_tile<T, D>(a, maps, blockIdx.x, smem, bars, tmem, failed)
-                                                : bwd_q_tile<T, D>(a, maps, blockIdx.x - kv_blocks, smem, bars, tmem, failed);
+    const Loaded asked = blockIdx.x < kv_blocks ? bwd_kv_tile<T, D>(a, maps, blockIdx.x, smem, bars, failed, tmem_at)
+                                                : bwd_q_tile<T, D>(a, maps, blockIdx.x - kv_blocks, smem, bars, failed, tmem_at);
     tc::fence_before();
     __syncthreads();
     if (*failed) {  // nothing may land in this CTA's memory after it has gone
@@ -925,7 +972,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1) attn_bwd_tc_kernel(const AttnA
         __syncthreads();
         if (threadIdx.x == 0) atomicOr(&g_attention_status, 1u);
     }
-    if (warp == 9) tc::tmem_free(tmem, 512);
+    if (warp == 9) tc::tmem_free(__shfl_sync(kFullMask, *tmem_at, 0), 512);
 }
 
 // ---- host ----
