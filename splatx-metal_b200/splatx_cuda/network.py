@@ -80,9 +80,18 @@ def _view(t: torch.Tensor) -> tuple:
 
 
 def _heads_last(t: torch.Tensor, what: str) -> torch.Tensor:
+    """t with a contiguous last axis. A 16-bit t whose rows the tensor-core kernels' copies do not
+    reach (an odd offset or stride, a broadcast axis such as the gradient of a sum) is copied: that
+    costs a pass over it, the kernel without tensor cores many times the whole call."""
     if t.dim() != 4:
         raise ValueError(f"{what}: [batch, tokens, heads, head_dim] needed, got {tuple(t.shape)}")
-    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+    n, s = t.shape, t.stride()
+    if s[3] != 1 and n[3] != 1:
+        return t.contiguous()
+    if n[3] % 8 == 0 and t.dtype in (torch.float16, torch.bfloat16) and (
+            t.data_ptr() % 16 or any(n[i] > 1 and (s[i] % 8 or s[i] <= 0) for i in range(3))):
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def _attention_inputs(what, q, k, v, scale, causal, q_lens, kv_lens):
@@ -309,13 +318,13 @@ class AdamW:
             _dtype(p, what)
             if not p.is_contiguous():
                 raise ValueError(f"{what}: parameters must be contiguous")
+        self._kept = self._facts()
         self.bits = state_bits
         self._cfg = _nat.SxAdamwConfig(float(betas[0]), float(betas[1]), float(eps), 1.0, 0,
                                        state_bits)
         self._state = self._bind(what, state)
         n = len(self.params)
         self._table = np.zeros(n, dtype=_TENSOR)
-        self._table["param"] = [p.data_ptr() for p in self.params]
         self._table["n"] = [p.numel() for p in self.params]
         self._table["param_dtype"] = [_DTYPES[p.dtype] for p in self.params]
         self._table["lr"], self._table["weight_decay"] = rates, decays
@@ -350,6 +359,10 @@ class AdamW:
                                      "parameters' sizes and device")
         return mine
 
+    def _facts(self) -> list:
+        """What a step relies on of the parameters, which may have been given other memory since."""
+        return [(p.numel(), p.dtype, p.get_device()) for p in self.params]
+
     def state(self) -> dict:
         """The moments and the number of steps taken, as the constructor takes them."""
         return {**self._state, "step": int(self._cfg.step)}
@@ -365,6 +378,8 @@ class AdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"{what}: {len(self.params)} gradients needed, got {len(grads)}")
+        if self._facts() != self._kept or not all(p.is_contiguous() for p in self.params):
+            raise ValueError(f"{what}: a parameter's size, dtype, device or layout has changed")
         device, pointers, types = self.device, [], []
         for p, g in zip(self.params, grads):
             if g is None:
@@ -378,6 +393,7 @@ class AdamW:
             pointers.append(g.data_ptr())
             types.append(_DTYPES[g.dtype])
         table = self._table
+        table["param"] = [p.data_ptr() for p in self.params]
         table["grad"], table["grad_dtype"] = pointers, types
         if any(g is None for g in grads):
             table = np.ascontiguousarray(table[table["grad"] != 0])

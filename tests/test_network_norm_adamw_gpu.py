@@ -401,6 +401,26 @@ def test_adamw_follows_the_32_bit_moments():
     assert last[32] < 1e-2 and last[8] < 2e-2, last
 
 
+def test_adamw_parameters_given_other_memory():
+    """A parameter whose data moves between steps is updated where it is then; one that changes its
+    size or type is refused."""
+    import torch
+    from splatx_cuda.network import AdamW
+    p = torch.nn.Parameter(torch.randn(500, device="cuda"))
+    g = torch.randn(500, device="cuda")
+    opt = AdamW([p], **CFG)
+    opt.step([g])
+    was, old = _np(p), p.data
+    kept = old.clone()
+    p.data = old.clone()
+    opt.step([g])
+    assert torch.equal(old, kept) and not np.array_equal(_np(p), was)
+    for bad in (torch.randn(499, device="cuda"), torch.randn(500, device="cuda").half(), torch.randn(500, 2, device="cuda")[:, 0]):
+        p.data = bad
+        with pytest.raises(ValueError):
+            opt.step([torch.randn_like(bad).contiguous()])
+
+
 def test_adamw_refusals():
     import ctypes as C
     import torch
