@@ -88,10 +88,12 @@ def _heads_last(t: torch.Tensor, what: str) -> torch.Tensor:
     n, s = t.shape, t.stride()
     if s[3] != 1 and n[3] != 1:
         return t.contiguous()
-    if n[3] % 8 == 0 and t.dtype in (torch.float16, torch.bfloat16) and (
-            t.data_ptr() % 16 or any(n[i] > 1 and (s[i] % 8 or s[i] <= 0) for i in range(3))):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    if n[3] % 8 or t.dtype == torch.float32:
+        return t
+    reached = not ((s[0] | s[1] | s[2] | t.data_ptr() >> 1) & 7) and s[0] and s[1] and s[2]
+    if reached or not (t.data_ptr() % 16 or any(n[i] > 1 and (s[i] % 8 or not s[i]) for i in range(3))):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _attention_inputs(what, q, k, v, scale, causal, q_lens, kv_lens):
@@ -361,7 +363,8 @@ class AdamW:
 
     def _facts(self) -> list:
         """What a step relies on of the parameters, which may have been given other memory since."""
-        return [(p.numel(), p.dtype, p.get_device()) for p in self.params]
+        ps = self.params
+        return [[p.numel() for p in ps], [p.dtype for p in ps], [p.get_device() for p in ps]]
 
     def state(self) -> dict:
         """The moments and the number of steps taken, as the constructor takes them."""
@@ -378,29 +381,25 @@ class AdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError(f"{what}: {len(self.params)} gradients needed, got {len(grads)}")
-        if self._facts() != self._kept or not all(p.is_contiguous() for p in self.params):
+        params = self.params
+        if self._facts() != self._kept or not all([p.is_contiguous() for p in params]):
             raise ValueError(f"{what}: a parameter's size, dtype, device or layout has changed")
-        device, pointers, types = self.device, [], []
-        for p, g in zip(self.params, grads):
-            if g is None:
-                pointers.append(0)
-                types.append(0)
-                continue
-            if g.shape != p.shape or g.device != device or not g.is_contiguous() or \
-                    g.dtype not in _DTYPES:
-                raise ValueError(f"{what}: a gradient must be a contiguous tensor like its "
-                                 f"parameter, got {tuple(g.shape)} {g.dtype} on {g.device}")
-            pointers.append(g.data_ptr())
-            types.append(_DTYPES[g.dtype])
         table = self._table
-        table["param"] = [p.data_ptr() for p in self.params]
-        table["grad"], table["grad_dtype"] = pointers, types
-        if any(g is None for g in grads):
-            table = np.ascontiguousarray(table[table["grad"] != 0])
+        table["param"] = [p.data_ptr() for p in params]
+        there = [i for i, g in enumerate(grads) if g is not None]
+        if len(there) < len(grads):
+            params, grads = [params[i] for i in there], [grads[i] for i in there]
+            table = np.ascontiguousarray(table[there])
+        kinds, index = [_DTYPES.get(g.dtype) for g in grads], self.device.index
+        if None in kinds or [g.shape for g in grads] != [p.shape for p in params] or \
+                not all([g.is_contiguous() and g.get_device() == index for g in grads]):
+            raise ValueError(f"{what}: a gradient must be a contiguous float32, float16 or bfloat16 "
+                             "tensor of its parameter's shape and device")
+        table["grad"], table["grad_dtype"] = [g.data_ptr() for g in grads], kinds
         self._cfg.grad_scale = float(grad_scale)
         self._cfg.step += 1
         try:
-            with _at(device) as stream:
+            with _at(self.device) as stream:
                 check(_nat.lib().sxcuda_adamw_step(table.ctypes.data, len(table),
                                                    C.byref(self._cfg), stream))
         except Exception:
