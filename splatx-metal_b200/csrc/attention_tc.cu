@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
 constexpr int kFwdThreads = 384;  // warps 10 and 11 only give up their registers
 // Of 16 pairs of exponentials, those on the multiply-add pipes.
 template <int D>
-constexpr int kPoly = D == 64 ? 1 : 3;
+constexpr int kPoly = D == 64 ? 2 : 4;
 template <int D>
 struct FwdSmem {
     static constexpr int kTileBytes = D / 64 * kPanel;
@@ -567,7 +567,7 @@ __device__ __forceinline__ void set_pair(uint32_t (&r)[32], int i, tc::Two x) {
     r[i + 1] = __float_as_uint(hi);
 }
 // Of 16 pairs of exponentials of the backward, those on the multiply-add pipes.
-constexpr int kPolyBwd = 6;
+constexpr int kPolyBwd = 5;
 template <typename T>
 __device__ __forceinline__ void exp_pair(uint32_t (&r)[32], int i, tc::Two x) {
     float lo, hi;
