@@ -2,6 +2,7 @@
 
 ``CudaBackend`` mirrors ``KernelBackend`` (per-kernel verification surface), ``TrainStepExecutor``
 mirrors the resident step executor; both call libsplatx_cuda.so through include/splatx_cuda.h.
+``network`` has the operators of a network beside the splats (attention, layer norm, AdamW).
 """
 from .build import build, lib_path  # noqa: F401
 
@@ -13,6 +14,9 @@ def __getattr__(name):
     if name == "TrainStepExecutor":
         from .executor import TrainStepExecutor
         return TrainStepExecutor
+    if name == "network":
+        import importlib
+        return importlib.import_module(".network", __name__)
     if name == "make_binoms_lut":
         from .backend import make_binoms_lut
         return make_binoms_lut
