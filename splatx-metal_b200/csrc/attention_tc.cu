@@ -355,6 +355,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
             h += mine_to_write ? row / q_len : 0;
             row %= q_len;
         }
+        // rows of no query see nothing: what lies in them (the tile's rest may be anything) must not
+        // make the warp move its sums to another maximum
+        const bool asked = mine_to_write && row < w.q_len;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + kO + t * D, p_at = tmem + lanes + kP + t * kPStep;
         float m = -INFINITY, l = 0.f;  // m: the base-2 exponent the sums are relative to
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                 if (lane == 0) tc::bar_arrive(s_free(t));
             }
             // keys of this tile that the query sees: those below `end`
-            const int64_t last = static_cast<int64_t>(row) + w.ahead + 1;
+            const int64_t last = asked ? static_cast<int64_t>(row) + w.ahead + 1 : 0;
             const int end = static_cast<int>((last < kv_len ? last : kv_len) - static_cast<int64_t>(j0 + j) * kRows);
             if (__any_sync(kFullMask, end < kRows)) {
 #pragma unroll
@@ -454,7 +457,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
         if (ok && mine) ok = tc::bar_wait(o_full(t), kApart ? (mine - 1) & 1 : 0, failed);
         if (ok) {
             tc::fence_after();
-            const bool live = row < w.q_len && m != -INFINITY;
+            const bool live = asked && m != -INFINITY;
             const int64_t at = (w.b * a.heads + h) * a.q_len + row;
             const float f = live ? 1.f / l : 0.f;
             if (a.splits > 1) {

@@ -207,6 +207,24 @@ def test_same_result_in_every_call_and_on_another_stream():
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("lq,lk,h,hk,q_len", [(37, 769, 8, 4, 37), (1, 900, 16, 2, 1), (200, 300, 2, 2, 77), (18, 345, 4, 1, 5)])
+def test_rows_of_no_query_change_nothing(lq, lk, h, hk, q_len):
+    """The rest of a tile of queries (padding, or what another call left in shared memory where the
+    heads of a group share a tile) changes no bit: the same in every call, and with NaN and large
+    values behind the length."""
+    import torch
+    from splatx_cuda import network
+    q, k, v, _ = _inputs(lq, 1, lq, lk, h, hk, 128, "bfloat16")
+    lens = torch.tensor([q_len], dtype=torch.int32, device="cuda")
+    first = network.attention_fwd(q, k, v, q_lens=lens)
+    other = [t * 30 for t in _inputs(3, 2, 512, 512, 8, 8, 128, "bfloat16")]
+    for fill in (math.nan, 1e4, -1e4):
+        network.attention_fwd(*other[:3])
+        q[:, q_len:] = fill
+        again = network.attention_fwd(q, k, v, q_lens=lens)
+        assert all(torch.equal(x, y) for x, y in zip(first, again))
+
+
 def test_captured_in_a_graph():
     import torch
     from splatx_cuda import network
