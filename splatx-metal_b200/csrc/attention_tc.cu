@@ -360,7 +360,10 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
         const bool asked = mine_to_write && row < w.q_len;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_at = tmem + lanes + t * kRows, o_at = tmem + lanes + kO + t * D, p_at = tmem + lanes + kP + t * kPStep;
-        float m = -INFINITY, l = 0.f;  // m: the base-2 exponent the sums are relative to
+        // m: the base-2 exponent the sums are relative to. In float16, which keeps 11 bits only above
+        // 2^-14, probabilities are held times 2^6 (at most 2^14 then); the division by their sum undoes it.
+        constexpr float kUp = std::is_same_v<T, __half> ? 6.f : 0.f;
+        float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int j = 0; j < mine; ++j) {
             ok = tc::bar_wait(s_full(t), j & 1, failed);
@@ -417,7 +420,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                     tc::tmem_store32(o_at + c * 32, o);
                 }
             }
-            const float less = m == -INFINITY ? 0.f : -m;
+            const float less = m == -INFINITY ? 0.f : kUp - m;
             const tc::Two times = tc::two(a.scale_log2, a.scale_log2), plus = tc::two(less, less);
             tc::Two sum[2] = {tc::two(0.f, 0.f), tc::two(0.f, 0.f)};
 #pragma unroll
@@ -463,11 +466,11 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
             if (a.splits > 1) {
                 const int64_t to = split * (a.batch * a.heads * a.q_len) + at;
                 store_part<D>(a.part_out + to * a.dim, o_at, f, a.dim, mine_to_write && live, mine > 0);
-                if (mine_to_write) a.part_lse2[to] = live ? m + log2f(l) : -INFINITY;
+                if (mine_to_write) a.part_lse2[to] = live ? m - kUp + log2f(l) : -INFINITY;
             } else {
                 T* out = static_cast<T*>(a.out.data) + w.b * a.out.batch_stride + h * a.out.head_stride + row * a.out.token_stride;
                 store_row<T, D>(out, o_at, f, a.dim, mine_to_write, live, mine > 0);
-                if (mine_to_write) a.lse[at] = live ? (m + log2f(l)) * kLn2 : -INFINITY;
+                if (mine_to_write) a.lse[at] = live ? (m - kUp + log2f(l)) * kLn2 : -INFINITY;
             }
         }
         tc::fence_before();
