@@ -196,14 +196,18 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     }
 }
 
-// The largest magnitude of a view's values below its lengths, as the bits of a float, which order
-// like unsigned numbers (so the atomic's order does not matter). A CTA per 64 rows of a head.
+// The largest magnitudes of the output's gradient and of v below the lengths, as the bits of a float,
+// which order like unsigned numbers (so the atomics' order does not matter). A CTA per 64 rows of a
+// head: the first `g_blocks` for the gradient, the others for v.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, const SxAttentionView v, const int32_t* lens,
-                                                           int64_t len, int32_t heads, uint32_t* most) {
-    const int per_head = static_cast<int>((len + 63) / 64);
-    const int64_t bh = blockIdx.x / per_head, b = bh / heads, r0 = static_cast<int64_t>(blockIdx.x % per_head) * 64;
-    const int64_t end = min(attn_length(lens, b, len), r0 + 64);
+__global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, uint32_t g_blocks) {
+    const bool is_g = blockIdx.x < g_blocks;
+    const SxAttentionView& v = is_g ? a.g : a.v;
+    const uint32_t block = is_g ? blockIdx.x : blockIdx.x - g_blocks;
+    const int64_t len = is_g ? a.q_len : a.kv_len;
+    const int heads = is_g ? a.heads : a.kv_heads, per_head = static_cast<int>((len + 63) / 64);
+    const int64_t bh = block / per_head, b = bh / heads, r0 = static_cast<int64_t>(block % per_head) * 64;
+    const int64_t end = min(attn_length(is_g ? a.q_lens : a.kv_lens, b, len), r0 + 64);
     const T* p = static_cast<const T*>(v.data) + b * v.batch_stride + bh % heads * v.head_stride;
     float top = 0.f;
     for (int64_t r = r0 + threadIdx.x / 16; r < end; r += 16)
@@ -214,7 +218,7 @@ __global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, con
         }
 #pragma unroll
     for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
-    if (threadIdx.x % 32 == 0 && top > 0.f) atomicMax(most, __float_as_uint(top));
+    if (threadIdx.x % 32 == 0 && top > 0.f) atomicMax(a.largest + !is_g, __float_as_uint(top));
 }
 
 template <typename T, int D>
@@ -405,11 +409,10 @@ void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn&
         a.p_shift = kHalfShift;
         a.largest = reinterpret_cast<uint32_t*>(a.minus_delta + a.batch * a.heads * a.q_pad);
         cuda_check(cudaMemsetAsync(a.largest, 0, 2 * sizeof(uint32_t), s), "attention_bwd");
+        const unsigned g_blocks = blocks_for(a.q_len, 64) * a.heads * static_cast<unsigned>(a.batch);
+        const unsigned v_blocks = blocks_for(a.kv_len, 64) * a.kv_heads * static_cast<unsigned>(a.batch);
         const auto kernel = attn_largest_kernel<__half>;
-        SX_LAUNCH(kernel, blocks_for(a.q_len, 64) * a.heads * static_cast<unsigned>(a.batch), 256, 0, s, a, a.g, a.q_lens, a.q_len,
-                  a.heads, a.largest);
-        SX_LAUNCH(kernel, blocks_for(a.kv_len, 64) * a.kv_heads * static_cast<unsigned>(a.batch), 256, 0, s, a, a.v, a.kv_lens,
-                  a.kv_len, a.kv_heads, a.largest + 1);
+        SX_LAUNCH(kernel, g_blocks + v_blocks, 256, 0, s, a, g_blocks);
     }
     by_dtype(a.dtype, [&](auto t) {
         using T = decltype(t);
