@@ -12,7 +12,8 @@ not synchronise. Contract violations raise ``ValueError``, device failures ``Run
     v_x, v_weight, v_bias = layer_norm_bwd(v_y, x, weight, mean, rstd)
     AdamW(params, lr=1e-3, state_bits=8).step()              # params with .grad, or step(grads)
 
-``attention`` and ``layer_norm`` are the same with torch's autograd.
+``attention`` and ``layer_norm`` are the same with torch's autograd (first derivatives; a second one
+raises ``RuntimeError``).
 """
 from __future__ import annotations
 
@@ -21,6 +22,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as _nat
 from ._native import check
@@ -142,7 +144,7 @@ def attention_fwd(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=Non
     q, k, v, ins, device = _attention_inputs("attention_fwd", q, k, v, scale, causal, q_lens, kv_lens)
     b, n, h, _ = q.shape
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((b, h, n), dtype=torch.float32, device=device)
+    lse = q.new_empty((b, h, n), dtype=torch.float32)
     ov, entry = _nat.SxAttentionView(*_view(out)), _nat.lib().sxcuda_attention_fwd
     with _at(device) as stream:
         ws, at, nbytes = _workspace(entry, device, ins)
@@ -182,6 +184,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, v_out):
         q, k, v, out, lse, q_lens, kv_lens = ctx.saved_tensors
         grads = attention_bwd(v_out, q, k, v, out, lse, q_lens=q_lens, kv_lens=kv_lens, **ctx.how)
@@ -229,7 +232,7 @@ def layer_norm_fwd(x, weight=None, bias=None, *, eps=1e-5):
     bias (each may be None: ones, zeros) have one dtype, which need not be x's."""
     flat, ins, device, cols = _norm_inputs("layer_norm_fwd", x, weight, bias, eps)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=device)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     with _at(device) as stream:
         check(_nat.lib().sxcuda_layer_norm_fwd(C.byref(ins), y.data_ptr(), cols, mean.data_ptr(),
@@ -271,6 +274,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, v_y):
         x, weight, mean, rstd = ctx.saved_tensors
         v_x, v_w, v_b = layer_norm_bwd(v_y, x, weight, mean, rstd)
@@ -293,7 +297,7 @@ class AdamW:
     params: tensors, or dicts {"params": [...], "lr": ..., "weight_decay": ...} for groups with a
     rate or decay of their own. They must be contiguous CUDA tensors of one device. Moments are held
     in 32 bits, or with state_bits=8 as e4m3 codes of m and of sqrt(v) with a float32 scale for
-    every 256 values (4.03 bytes less per value and moment pair than 8).
+    every 256 values (2.03 bytes for a value's two moments in place of 8).
 
     state: moments to go on from, {"exp_avg": [...], "exp_avg_sq": [...], "step": n} and, with 8
     bits, "exp_avg_scale" and "exp_avg_sq_scale", one tensor per parameter in order; the tensors are
@@ -320,6 +324,10 @@ class AdamW:
             _dtype(p, what)
             if not p.is_contiguous():
                 raise ValueError(f"{what}: parameters must be contiguous")
+        # two updates of one tensor in a launch would race
+        at = [p.data_ptr() for p in self.params if p.numel()]
+        if len(set(at)) != len(at):
+            raise ValueError(f"{what}: a parameter is given more than once")
         self._kept = self._facts()
         self.bits = state_bits
         self._cfg = _nat.SxAdamwConfig(float(betas[0]), float(betas[1]), float(eps), 1.0, 0,
@@ -405,3 +413,5 @@ class AdamW:
         except Exception:
             self._cfg.step -= 1
             raise
+        # autograd's check of saved tensors sees that the parameters are no longer what they were
+        torch.autograd.graph.increment_version(params)

@@ -454,3 +454,40 @@ def test_adamw_refusals():
     assert L.sxcuda_adamw_step(None, 0, C.byref(cfg), None) == n.SXCUDA_OK
     torch.cuda.synchronize()
     assert not p.any()
+
+
+def test_adamw_refuses_a_parameter_given_twice():
+    import torch
+    from splatx_cuda.network import AdamW
+    p, empty = torch.zeros(8, device="cuda"), torch.zeros(0, device="cuda")
+    with pytest.raises(ValueError):
+        AdamW([p, p])
+    with pytest.raises(ValueError):
+        AdamW([{"params": [p]}, {"params": [p.view(2, 4)]}])
+    AdamW([p, empty, empty])
+
+
+def test_adamw_step_shows_to_autograd():
+    """A graph that saved a parameter's value must not run backward on the updated one."""
+    import torch
+    from splatx_cuda.network import AdamW
+    p, kept = (torch.ones(8, device="cuda", requires_grad=True) for _ in range(2))
+    lost, fine = (p * p).sum(), (kept * kept).sum()
+    AdamW([p, kept], **CFG).step([torch.ones_like(p), None])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        lost.backward()
+    fine.backward()
+    assert kept.grad.eq(2).all()
+
+
+def test_second_derivatives_are_refused():
+    import torch
+    from splatx_cuda import network
+    x = torch.randn(4, 16, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(network.layer_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+    q = torch.randn(1, 4, 2, 16, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(network.attention(q, q, q).square().sum(), q, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
