@@ -196,9 +196,9 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     }
 }
 
-// The largest magnitudes of the output's gradient and of v below the lengths, as the bits of a float,
-// which order like unsigned numbers (so the atomics' order does not matter). A CTA per 64 rows of a
-// head: the first `g_blocks` for the gradient, the others for v.
+// The largest magnitudes of the output's gradient and of v below the lengths, per batch entry and key
+// head, as the bits of a float, which order like unsigned numbers (so the atomics' order does not
+// matter). A CTA per 64 rows of a head: the first `g_blocks` for the gradient, the others for v.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, uint32_t g_blocks) {
     const bool is_g = blockIdx.x < g_blocks;
@@ -218,7 +218,10 @@ __global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, uin
         }
 #pragma unroll
     for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
-    if (threadIdx.x % 32 == 0 && top > 0.f) atomicMax(a.largest + !is_g, __float_as_uint(top));
+    if (threadIdx.x % 32 == 0 && top > 0.f) {
+        const int64_t hk = is_g ? bh % heads / a.group : bh % heads;
+        atomicMax(a.largest + 2 * (b * a.kv_heads + hk) + !is_g, __float_as_uint(top));
+    }
 }
 
 template <typename T, int D>
@@ -385,7 +388,7 @@ void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& ou
 
 size_t attention_bwd_workspace(const SxAttentionInputs& in) {
     const AttnArgs a = attn_args(in);
-    return static_cast<size_t>(2 * a.batch * a.heads * a.q_pad + 4) * sizeof(float);
+    return static_cast<size_t>(2 * a.batch * (a.heads * a.q_pad + a.kv_heads) + 4) * sizeof(float);
 }
 
 void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn& g, const SxAttentionGrads& out,
@@ -408,7 +411,7 @@ void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn&
     if (half) {
         a.p_shift = kHalfShift;
         a.largest = reinterpret_cast<uint32_t*>(a.minus_delta + a.batch * a.heads * a.q_pad);
-        cuda_check(cudaMemsetAsync(a.largest, 0, 2 * sizeof(uint32_t), s), "attention_bwd");
+        cuda_check(cudaMemsetAsync(a.largest, 0, 2 * a.batch * a.kv_heads * sizeof(uint32_t), s), "attention_bwd");
         const unsigned g_blocks = blocks_for(a.q_len, 64) * a.heads * static_cast<unsigned>(a.batch);
         const unsigned v_blocks = blocks_for(a.kv_len, 64) * a.kv_heads * static_cast<unsigned>(a.batch);
         const auto kernel = attn_largest_kernel<__half>;

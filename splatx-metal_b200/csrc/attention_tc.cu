@@ -566,15 +566,18 @@ struct Loaded {
 
 // float16 keeps 11 bits only above 2^-14: p and ds are held times powers of two, so that what a
 // gradient is summed from does not vanish before the sum. p is at most 1; for ds
-// |p (g v - delta)| <= 2 dim max|g| max|v|, which `ds` times takes to at most 2^15.
+// |p (g v - delta)| <= 2 dim max|g| max|v|, which `ds` times takes to at most 2^15. The maxima are those
+// of the heads that share a key head (whose gradient is one sum), so that no other head's or batch
+// entry's magnitudes take bits away.
 struct HalfScale {
     float p = 1.f, ds = 1.f;
 };
 template <typename T>
-__device__ __forceinline__ HalfScale half_scale(const AttnArgs& a) {
+__device__ __forceinline__ HalfScale half_scale(const AttnArgs& a, int64_t b, int64_t hk) {
     HalfScale h;
     if constexpr (std::is_same_v<T, __half>) {
-        const float bound = 2.f * a.dim * __uint_as_float(a.largest[0]) * __uint_as_float(a.largest[1]);
+        const uint32_t* largest = a.largest + 2 * (b * a.kv_heads + hk);
+        const float bound = 2.f * a.dim * __uint_as_float(largest[0]) * __uint_as_float(largest[1]);
         h.p = 1.f / exp2f(kHalfShift);
         if (bound > 0x1p-80f && bound < 0x1p80f) h.ds = exp2f(14.f - ceilf(log2f(bound)));
     }
@@ -747,7 +750,7 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
         const int64_t key = k0 + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t w_at = tmem + lanes + half * 64 + kW;
-        const HalfScale scale = half_scale<T>(a);
+        const HalfScale scale = half_scale<T>(a, batch, hk);
         const tc::Two times = tc::two(a.scale_log2, a.scale_log2), ds_scale = tc::two(scale.p * scale.ds, scale.p * scale.ds);
         bool ok = true;
         int tile = 0;
@@ -913,7 +916,7 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
         const uint32_t s_at = tmem + lanes + half * 64, w_at = s_at + kW;
         const int64_t at = (static_cast<int64_t>(batch) * a.heads + h) * a.q_pad + row;  // q_pad holds whole tiles
         const tc::Two lse = tc::two(a.minus_lse2[at], a.minus_lse2[at]), delta = tc::two(a.minus_delta[at], a.minus_delta[at]);
-        const HalfScale scale = half_scale<T>(a);
+        const HalfScale scale = half_scale<T>(a, batch, hk);
         const tc::Two times = tc::two(a.scale_log2, a.scale_log2), ds_scale = tc::two(scale.p * scale.ds, scale.p * scale.ds);
         bool ok = true;
         for (int j = 0; j < n; ++j) {

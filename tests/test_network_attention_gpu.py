@@ -367,3 +367,30 @@ def test_c_entry_refusals():
              L.sxcuda_attention_status(None)]
     assert cases == [n.SXCUDA_EINVAL] * len(cases), cases
     assert np.all(t.cpu().float().numpy() == 0)
+
+
+def _of_two_magnitudes():
+    """float16 inputs with key heads that are 2^18 apart in g v."""
+    import torch
+    q, k, v, g = _inputs(31, 2, 300, 260, 4, 2, 64, "float16")
+    g[0, :, :2] *= 2.0 ** 9  # key head 0's two query heads
+    v[0, :, 0] *= 2.0 ** 3
+    g[0, :, 2:] *= 2.0 ** -6
+    return q, k, v, g
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_half_gradients_beside_larger_ones(causal):
+    _run(*_of_two_magnitudes(), causal=causal)
+
+
+def test_half_gradients_do_not_depend_on_other_heads_or_entries():
+    import torch
+    q, k, v, g = _of_two_magnitudes()
+    _, _, first = _run(q, k, v, g)
+    g[0, :, :2] *= 2.0 ** -12
+    v[0, :, 0] = 0
+    _, _, again = _run(q, k, v, g)
+    for x, y in zip(first, again):
+        per = x.shape[2] // 2
+        assert torch.equal(x[1], y[1]) and torch.equal(x[0, :, per:], y[0, :, per:])
