@@ -1,0 +1,87 @@
+"""Attention where what a query sees is not finite.
+
+softmax of scores among which one is NaN or +inf, or of which all are -inf, is NaN, and so is its
+log-sum and every gradient that such a row takes part in. Only a query that sees no key has output 0
+and log-sum -inf. A key that a query does not see has weight 0, whatever its value. Rows that see
+only finite scores keep the definition's values, within the bounds of test_network_attention_gpu.
+"""
+import math
+
+import pytest
+
+from test_network_attention_gpu import ROUND, _check, _definition, _inputs, _seen
+
+pytestmark = pytest.mark.gpu
+
+NAN, INF = math.nan, math.inf
+# columns of every kind that a tile of scores has: one batch entry for each
+AT = [*range(0, 32), *range(64, 96)]
+_name = lambda s: "x".join(map(str, s))  # noqa: E731
+
+
+def _fwd_bwd(q, k, v, g, **how):
+    from splatx_cuda import network
+    out, lse = network.attention_fwd(q, k, v, **how)
+    return out, lse, network.attention_bwd(g, q, k, v, out, lse, **how)
+
+
+def _all_nan(**results):
+    """Of each result every value, in every batch entry."""
+    for name, t in results.items():
+        assert bool(t.isnan().all()), (name, [b for b in range(len(t)) if not t[b].isnan().all()])
+
+
+def _nan_queries(shape, causal, dtype):
+    """Some queries are NaN: their rows are NaN and the others as they were."""
+    from splatx_cuda import network
+    q, k, v, g = _inputs(sum(shape), *shape, dtype)
+    lq = shape[1]
+    rows = sorted({0, lq // 3, lq - 1})
+    clean = q.clone()
+    q[:, rows] = NAN
+    out, lse = network.attention_fwd(q, k, v, causal=causal)
+    _all_nan(out=out[:, rows], lse=lse[:, :, rows])
+    seen = _seen(shape[0], lq, shape[2], causal, None, None)
+    want = _definition(clean, k, v, g, None, seen, shape[5] ** -0.5, ROUND[dtype])
+    fine = [i for i in range(lq) if i not in rows]
+    _check("out", out.transpose(1, 2)[:, :, fine], *(t[:, :, fine] for t in want["out"]))
+    _check("lse", lse[:, :, fine], *(t[:, :, fine] for t in want["lse"]))
+
+
+def _key_at_every_place(value, d, lk, dtype):
+    """Batch entry i has `value` at key AT[i]: every row and every gradient is NaN. (The first value of
+    each query is 1, so that with +inf the score is +inf.)"""
+    q, k, v, g = _inputs(d + lk, len(AT), 40, lk, 2, 1, d, dtype)
+    q[..., 0] = 1
+    for b, at in enumerate(AT):
+        k[b, at, :, 0] = value
+    out, lse, (v_q, v_k, v_v) = _fwd_bwd(q, k, v, g)
+    _all_nan(out=out, lse=lse, v_q=v_q, v_k=v_k, v_v=v_v)
+
+
+def _query_in_the_keys_gradients(d, dtype):
+    """Batch entry i has NaN at query AT[i]; the other queries' own gradients stay finite."""
+    q, k, v, g = _inputs(d, len(AT), 96, 140, 2, 1, d, dtype)
+    for b, at in enumerate(AT):
+        q[b, at] = NAN
+    _, _, (v_q, v_k, v_v) = _fwd_bwd(q, k, v, g)
+    _all_nan(v_k=v_k, v_v=v_v)
+    bad = v_q.isnan().flatten(2)
+    for b, at in enumerate(AT):
+        assert bool(bad[b, at].all()) and int(bad[b].any(1).sum()) == 1, at
+
+
+# the kernels without tensor cores: 32 bits, and rows that are not in pieces of 16 bytes
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape,dtype", [((2, 96, 96, 2, 2, 64), "float32"), ((1, 300, 300, 2, 1, 128), "float32"),
+                                         ((2, 1, 900, 4, 4, 128), "float32"), ((1, 90, 90, 2, 2, 36), "bfloat16"),
+                                         ((1, 90, 90, 2, 2, 33), "float16")])
+def test_cuda_core_kernels_keep_a_nan_query(shape, dtype, causal):
+    _nan_queries(shape, causal, dtype)
+
+
+@pytest.mark.parametrize("d,dtype", [(64, "float32"), (128, "float32"), (36, "bfloat16")])
+def test_cuda_core_kernels_keep_what_is_not_finite_at_every_place(d, dtype):
+    _key_at_every_place(NAN, d, 96, dtype)
+    _key_at_every_place(INF, d, 300, dtype)
+    _query_in_the_keys_gradients(d, dtype)
