@@ -388,25 +388,27 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
                     for (int i = 0; i < 32; ++i)
                         if (c * 32 + i >= end) r[c][i] = 0xff800000u;
             }
+            // A score that is NaN makes the maximum NaN, and by it the whole row: beside masked scores it
+            // would else leave -inf, which stands for a row that has seen no key.
             float top[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                top[c] = fmaxf(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]));
+                top[c] = tc::max_nan(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]));
 #pragma unroll
-                for (int i = 2; i < 32; i += 2) top[c] = tc::max3(top[c], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+                for (int i = 2; i < 32; i += 2) top[c] = tc::max_nan(top[c], __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
             }
-            const float seen = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+            const float seen = tc::max_nan(tc::max_nan(top[0], top[1]), tc::max_nan(top[2], top[3])) * a.scale_log2;
             // The sums move to a new maximum only when it is 2^8 above the old one: 32 bits hold that,
             // and the output's rows are then hardly ever read back and scaled.
             if (j == 0) {
                 m = seen;
-            } else if (__any_sync(kFullMask, seen > m + 8.f)) {
+            } else if (__any_sync(kFullMask, !(seen <= m + 8.f))) {
                 if (kApart) {  // the sums are at rest once the last tile's product is complete
                     ok = tc::bar_wait(o_full(t), (j - 1) & 1, failed);
                     if (!ok) break;
                     tc::fence_after();
                 }
-                const float to = fmaxf(m, seen);
+                const float to = tc::max_nan(m, seen);
                 const float f = to == -INFINITY ? 1.f : tc::exp2_approx(m - to);
                 l *= f;
                 m = to;

@@ -238,9 +238,15 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+// The largest; NaN where one of them is (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float a, float b) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 

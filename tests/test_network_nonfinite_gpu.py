@@ -85,3 +85,12 @@ def test_cuda_core_kernels_keep_what_is_not_finite_at_every_place(d, dtype):
     _key_at_every_place(NAN, d, 96, dtype)
     _key_at_every_place(INF, d, 300, dtype)
     _query_in_the_keys_gradients(d, dtype)
+
+
+# tensor cores: the first key tile whole, partly behind the mask or the length; several tiles
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", [(2, 96, 96, 2, 2, 64), (2, 96, 96, 2, 2, 128), (40, 300, 300, 4, 2, 128),
+                                   (40, 300, 300, 4, 2, 64), (1, 128, 128, 1, 1, 80)], ids=_name)
+def test_a_nan_query_is_nan_and_alone(shape, causal, dtype):
+    _nan_queries(shape, causal, dtype)
