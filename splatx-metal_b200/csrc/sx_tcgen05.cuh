@@ -250,15 +250,17 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
     return r;
 }
 
-// 2^x on the multiply-add pipes, for x up to 127 (below -126: 2^-126): x = n + f with n the nearest
-// whole number (the low bits of x + 1.5 2^23), 2^f by a polynomial fitted for the least relative
-// error on [-1/2, 1/2] (2.2e-7 in 32 bits), and n added to the exponent. The special-function unit
-// gives 16 values a cycle and SM, half of what the products of 64-value rows leave time for.
+// 2^x on the multiply-add pipes, for x up to 127 (0 below -126.5, -inf among it: a masked key has no
+// weight at all): x = n + f with n the nearest whole number, 2^f by a polynomial fitted for the least
+// relative error on [-1/2, 1/2] (2.2e-7 in 32 bits), times 2^n. The low bits of x + 1.5 2^23 + 127 are
+// n + 127, which is 2^n once they stand in the exponent's place, and zero for n = -127. The
+// special-function unit gives 16 values a cycle and SM, half of what the products of 64-value rows leave
+// time for.
 __device__ __forceinline__ void exp2_poly(Two x, float& lo, float& hi) {
     float a, b;
     split(x, a, b);
-    x = two(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const Two magic = two(12582912.f, 12582912.f), back = two(-12582912.f, -12582912.f), minus = two(-1.f, -1.f);
+    x = two(fmaxf(a, -127.f), fmaxf(b, -127.f));
+    const Two magic = two(12583039.f, 12583039.f), back = two(-12583039.f, -12583039.f), minus = two(-1.f, -1.f);
     const Two t = add2(x, magic);
     const Two f = fma2(add2(t, back), minus, x);
     Two p = two(0x1.5c08e4p-10f, 0x1.5c08e4p-10f);
@@ -269,9 +271,7 @@ __device__ __forceinline__ void exp2_poly(Two x, float& lo, float& hi) {
     p = fma2(p, f, two(0x1.000002p+0f, 0x1.000002p+0f));
     float n0, n1;
     split(t, n0, n1);
-    split(p, lo, hi);
-    lo = __uint_as_float(__float_as_uint(lo) + (__float_as_uint(n0) << 23));
-    hi = __uint_as_float(__float_as_uint(hi) + (__float_as_uint(n1) << 23));
+    split(mul2(p, two(__uint_as_float(__float_as_uint(n0) << 23), __uint_as_float(__float_as_uint(n1) << 23))), lo, hi);
 }
 
 }  // namespace tc

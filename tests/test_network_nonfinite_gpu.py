@@ -94,3 +94,20 @@ def test_cuda_core_kernels_keep_what_is_not_finite_at_every_place(d, dtype):
                                    (40, 300, 300, 4, 2, 64), (1, 128, 128, 1, 1, 80)], ids=_name)
 def test_a_nan_query_is_nan_and_alone(shape, causal, dtype):
     _nan_queries(shape, causal, dtype)
+
+
+@pytest.mark.parametrize("dtype,large", [("bfloat16", 3e38), ("float16", 6e4), ("float32", 3e38)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_an_unseen_key_has_weight_zero_at_every_place(d, dtype, large):
+    """Batch entry i has large values at key AT[i]: the rows before it, which do not see it in the
+    causal square, do not change by a bit."""
+    import torch
+    from splatx_cuda import network
+    q, k, v, _ = _inputs(d, len(AT), 128, 128, 2, 1, d, dtype)
+    out, lse = network.attention_fwd(q, k, v, causal=True)
+    for b, at in enumerate(AT):
+        v[b, at] = large
+    again, lse2 = network.attention_fwd(q, k, v, causal=True)
+    assert torch.equal(lse, lse2)
+    for b, at in enumerate(AT):
+        assert torch.equal(out[b, :at], again[b, :at]), at
