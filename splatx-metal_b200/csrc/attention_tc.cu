@@ -152,18 +152,18 @@ __device__ __forceinline__ void store_part(float* out, uint32_t at, float f, int
 }
 
 // Joins the parts of a query that CTAs with different keys made: out = sum_s 2^(lse_s - lse) out_s. A
-// warp per query; parts that saw no key are not read.
+// warp per query; parts that saw no key are not read. A part that is NaN makes the query NaN.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     const int64_t rows = a.batch * a.heads * a.q_len, at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
     if (at >= rows) return;
     const int lane = threadIdx.x & 31;
     float top = -INFINITY;
-    for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_lse2[s * rows + at]);
+    for (int s = lane; s < a.splits; s += 32) top = tc::max_nan(top, a.part_lse2[s * rows + at]);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, o));
-    float total = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    if (top != -INFINITY)
+    for (int o = 16; o; o >>= 1) top = tc::max_nan(top, __shfl_xor_sync(kFullMask, top, o));
+    float total = isnan(top) ? top : 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (top > -INFINITY)
         for (int s = 0; s < a.splits; ++s) {
             const float x = exp2f(a.part_lse2[s * rows + at] - top);
             if (x == 0.f) continue;
@@ -176,14 +176,14 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
                 acc[3] = fmaf(x, o.w, acc[3]);
             }
         }
-    const float f = total > 0.f ? 1.f / total : 0.f;
+    const float f = total == 0.f ? 0.f : 1.f / total;
     const int64_t i = at % a.q_len, bh = at / a.q_len;
     T* out = static_cast<T*>(a.out.data) + bh / a.heads * a.out.batch_stride + bh % a.heads * a.out.head_stride + i * a.out.token_stride;
     if (lane * 4 < a.dim) {
         uint2 x{tc::pack2<T>(acc[0] * f, acc[1] * f), tc::pack2<T>(acc[2] * f, acc[3] * f)};
         *reinterpret_cast<uint2*>(out + lane * 4) = x;
     }
-    if (lane == 0) a.lse[at] = total > 0.f ? (top + log2f(total)) * kLn2 : -INFINITY;
+    if (lane == 0) a.lse[at] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
 }
 
 // The forward. A CTA owns two tiles of 128 queries of one head; warps 0-3 and 4-7 make their

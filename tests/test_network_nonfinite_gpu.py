@@ -111,3 +111,24 @@ def test_an_unseen_key_has_weight_zero_at_every_place(d, dtype, large):
     assert torch.equal(lse, lse2)
     for b, at in enumerate(AT):
         assert torch.equal(out[b, :at], again[b, :at]), at
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("shape", [(2, 1, 8000, 4, 4, 128), (1, 1, 8000, 4, 4, 64), (2, 5, 3000, 8, 2, 128),
+                                   (1, 300, 2000, 2, 2, 64)], ids=_name)
+def test_a_nan_query_over_split_keys(shape, dtype):
+    """Few queries: the keys are split over CTAs and the parts joined."""
+    _nan_queries(shape, False, dtype)
+    _nan_queries(shape, True, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lq,h,hk", [(1, 4, 4), (3, 8, 2)])
+def test_a_key_that_is_not_finite_among_split_keys(lq, h, hk, d, dtype):
+    """One part of the keys is NaN, the others are not."""
+    from splatx_cuda import network
+    q, k, v, _ = _inputs(3, 1, lq, 8000, h, hk, d, dtype)
+    k[:, 5000] = NAN
+    out, lse = network.attention_fwd(q, k, v)
+    _all_nan(out=out, lse=lse)
