@@ -259,7 +259,7 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 __device__ __forceinline__ void exp2_poly(Two x, float& lo, float& hi) {
     float a, b;
     split(x, a, b);
-    x = two(fmaxf(a, -127.f), fmaxf(b, -127.f));
+    x = two(max_nan(a, -127.f), max_nan(b, -127.f));  // NaN stays, as it does in exp2_approx
     const Two magic = two(12583039.f, 12583039.f), back = two(-12583039.f, -12583039.f), minus = two(-1.f, -1.f);
     const Two t = add2(x, magic);
     const Two f = fma2(add2(t, back), minus, x);

@@ -132,3 +132,17 @@ def test_a_key_that_is_not_finite_among_split_keys(lq, h, hk, d, dtype):
     k[:, 5000] = NAN
     out, lse = network.attention_fwd(q, k, v)
     _all_nan(out=out, lse=lse)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("lk", [96, 500])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_a_key_that_is_not_finite_shows_at_every_place(value, d, lk, dtype):
+    _key_at_every_place(value, d, lk, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_nan_query_shows_in_the_keys_gradients_at_every_place(d, dtype):
+    _query_in_the_keys_gradients(d, dtype)
