@@ -160,9 +160,12 @@ __global__ void __launch_bounds__(kThreads) attn_fwd_kernel(const AttnArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int64_t row = q0 + ty() * 4 + i;
-        f[i] = l[i] == 0.f ? 0.f : 1.f / l[i];  // a sum that is NaN is no row without keys
+        // a row without keys is one by its mask: a sum that is NaN or zero (every score -inf) is none
+        const bool any = attn_sees_any(w, row);
+        if (l[i] == 0.f) l[i] = NAN;
+        f[i] = any ? 1.f / l[i] : 0.f;
         if (tx() == 0 && row < a.q_len)
-            a.lse[(w.b * a.heads + w.h) * a.q_len + row] = l[i] == 0.f ? -INFINITY : (m[i] + log2f(l[i])) * kLn2;
+            a.lse[(w.b * a.heads + w.h) * a.q_len + row] = any ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
     }
     store_rows<T, D>(acc, f, a.out, w.b, w.h, q0, a.q_len, a.dim);
 }

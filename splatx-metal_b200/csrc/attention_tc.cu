@@ -152,7 +152,8 @@ __device__ __forceinline__ void store_part(float* out, uint32_t at, float f, int
 }
 
 // Joins the parts of a query that CTAs with different keys made: out = sum_s 2^(lse_s - lse) out_s. A
-// warp per query; parts that saw no key are not read. A part that is NaN makes the query NaN.
+// warp per query; parts that saw no key, or none with a score above -inf, are not read. A part that is
+// NaN makes the query NaN, and so do scores that are all -inf.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
     const int64_t rows = a.batch * a.heads * a.q_len, at = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -176,14 +177,16 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
                 acc[3] = fmaf(x, o.w, acc[3]);
             }
         }
-    const float f = total == 0.f ? 0.f : 1.f / total;
     const int64_t i = at % a.q_len, bh = at / a.q_len;
+    const bool any = attn_sees_any(attn_head(a, bh % a.heads, bh / a.heads), i);
+    if (total == 0.f) total = NAN;
+    const float f = any ? 1.f / total : 0.f;
     T* out = static_cast<T*>(a.out.data) + bh / a.heads * a.out.batch_stride + bh % a.heads * a.out.head_stride + i * a.out.token_stride;
     if (lane * 4 < a.dim) {
         uint2 x{tc::pack2<T>(acc[0] * f, acc[1] * f), tc::pack2<T>(acc[2] * f, acc[3] * f)};
         *reinterpret_cast<uint2*>(out + lane * 4) = x;
     }
-    if (lane == 0) a.lse[at] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+    if (lane == 0) a.lse[at] = any ? (top + log2f(total)) * kLn2 : -INFINITY;
 }
 
 // The forward. A CTA owns two tiles of 128 queries of one head; warps 0-3 and 4-7 make their
@@ -462,14 +465,18 @@ __global__ void __launch_bounds__(kFwdThreads, 1) attn_fwd_tc_kernel(const AttnA
         if (ok && mine) ok = tc::bar_wait(o_full(t), kApart ? (mine - 1) & 1 : 0, failed);
         if (ok) {
             tc::fence_after();
-            const bool live = asked && m != -INFINITY;
             const int64_t at = (w.b * a.heads + h) * a.q_len + row;
-            const float f = live ? 1.f / l : 0.f;
             if (a.splits > 1) {
                 const int64_t to = split * (a.batch * a.heads * a.q_len) + at;
+                const bool live = asked && m != -INFINITY;
+                const float f = live ? 1.f / l : 0.f;
                 store_part<D>(a.part_out + to * a.dim, o_at, f, a.dim, mine_to_write && live, mine > 0);
                 if (mine_to_write) a.part_lse2[to] = live ? m - kUp + log2f(l) : -INFINITY;
             } else {
+                // seen by the mask: where every score is -inf the sum is zero and the row NaN
+                const bool live = asked && attn_sees_any(w, row);
+                if (l == 0.f) l = NAN;
+                const float f = live ? 1.f / l : 0.f;
                 T* out = static_cast<T*>(a.out.data) + w.b * a.out.batch_stride + h * a.out.head_stride + row * a.out.token_stride;
                 store_row<T, D>(out, o_at, f, a.dim, mine_to_write, live, mine > 0);
                 if (mine_to_write) a.lse[at] = live ? (m - kUp + log2f(l)) * kLn2 : -INFINITY;

@@ -72,6 +72,7 @@ __device__ __forceinline__ AttnHead attn_head(const AttnArgs& a, int64_t h, int6
 __device__ __forceinline__ bool attn_sees(const AttnHead& w, int64_t i, int64_t j) {
     return i < w.q_len && j < w.kv_len && j <= i + w.ahead;
 }
+__device__ __forceinline__ bool attn_sees_any(const AttnHead& w, int64_t i) { return attn_sees(w, i, 0); }
 // The end of the keys that any query before `i_end` sees.
 __device__ __forceinline__ int64_t attn_keys_end(const AttnHead& w, int64_t i_end) {
     const int64_t last = (i_end < w.q_len ? i_end : w.q_len) - 1;

@@ -2,7 +2,7 @@
 
 softmax of scores among which one is NaN or +inf, or of which all are -inf, is NaN, and so is its
 log-sum and every gradient that such a row takes part in. Only a query that sees no key has output 0
-and log-sum -inf. A key that a query does not see has weight 0, whatever its value. Rows that see
+and log-sum -inf. A key that a query does not see has weight 0, whatever its finite value. Rows that see
 only finite scores keep the definition's values, within the bounds of test_network_attention_gpu.
 """
 import math
@@ -146,3 +146,36 @@ def test_a_key_that_is_not_finite_shows_at_every_place(value, d, lk, dtype):
 @pytest.mark.parametrize("d", [64, 128])
 def test_a_nan_query_shows_in_the_keys_gradients_at_every_place(d, dtype):
     _query_in_the_keys_gradients(d, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("shape", [(1, 96, 96, 2, 2, 64), (1, 200, 300, 2, 1, 128), (1, 1, 8000, 4, 4, 128),
+                                   (1, 5, 3000, 8, 2, 64)], ids=_name)
+def test_scores_of_minus_infinity(shape, dtype):
+    """A key whose score is -inf has weight 0 beside finite ones; where all are -inf the row is NaN
+    (0 / 0), unlike a row that sees no key."""
+    import torch
+    from splatx_cuda import network
+    b, lq, lk, h, hk, d = shape
+    q, k, v, g = _inputs(d + lk, *shape, dtype)
+    q[..., 0] = 1
+    k[..., 0] = 0
+    k[:, ::7, :, 0] = -INF
+    out, lse = network.attention_fwd(q, k, v)
+    keep = torch.ones(lk, dtype=torch.bool, device="cuda")
+    keep[::7] = False
+    seen = _seen(b, lq, int(keep.sum()), False, None, None)
+    want = _definition(q, k[:, keep], v[:, keep], g, None, seen, d ** -0.5, ROUND[dtype])
+    _check("out", out.transpose(1, 2), *want["out"])
+    _check("lse", lse, *want["lse"])
+    k[..., 0] = -INF
+    out, lse, (v_q, v_k, v_v) = _fwd_bwd(q, k, v, g)
+    _all_nan(out=out, lse=lse, v_q=v_q, v_k=v_k, v_v=v_v)
+    none = torch.zeros(b, dtype=torch.int32, device="cuda")
+    out, lse = network.attention_fwd(q, k, v, kv_lens=none)
+    assert not out.any() and bool((lse == -INF).all())
+    # the first tokens' queries before any key, the last one behind one of them
+    few = torch.full((b,), 1, dtype=torch.int32, device="cuda")
+    out, lse = network.attention_fwd(q, k, v, kv_lens=few, causal=True)
+    assert not out[:, :-1].any() and bool((lse[:, :, :-1] == -INF).all())
+    _all_nan(out=out[:, -1:], lse=lse[:, :, -1:])
