@@ -292,7 +292,9 @@ _TENSOR = np.dtype(_nat.SxAdamwTensor)
 
 
 class AdamW:
-    """AdamW (decoupled weight decay, bias correction) over all parameters in one launch.
+    """AdamW (decoupled weight decay, bias correction) over all parameters in one launch. Each parameter
+    counts its own steps, which its bias correction goes by: one without a gradient is skipped and does
+    not count. (Parameters with different counts take a launch for each count.)
 
     params: tensors, or dicts {"params": [...], "lr": ..., "weight_decay": ...} for groups with a
     rate or decay of their own. They must be contiguous CUDA tensors of one device. Moments are held
@@ -301,7 +303,8 @@ class AdamW:
 
     state: moments to go on from, {"exp_avg": [...], "exp_avg_sq": [...], "step": n} and, with 8
     bits, "exp_avg_scale" and "exp_avg_sq_scale", one tensor per parameter in order; the tensors are
-    used and updated in place. ``state()`` returns them."""
+    used and updated in place. n: the steps taken, one number or one per parameter. ``state()`` returns
+    them."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, *,
                  state_bits=32, state=None):
@@ -349,9 +352,11 @@ class AdamW:
             kinds["exp_avg_scale"] = kinds["exp_avg_sq_scale"] = torch.float32
         if state is not None and set(state) != {*kinds, "step"}:
             raise ValueError(f"{what}: state needs {sorted({*kinds, 'step'})}")
-        self._cfg.step = 0 if state is None else int(state["step"])
-        if self._cfg.step < 0:
-            raise ValueError(f"{what}: negative step")
+        taken = 0 if state is None else state["step"]
+        taken = list(taken) if isinstance(taken, (list, tuple)) else [taken] * len(self.params)
+        if len(taken) != len(self.params) or any(int(t) < 0 for t in taken):
+            raise ValueError(f"{what}: step must be a number of at least 0, or one per parameter")
+        self._steps = np.array([int(t) for t in taken], dtype=np.int64)
         mine = {}
         for key, dtype in kinds.items():
             sizes = [-(-p.numel() // RUN) if key.endswith("scale") else p.numel()
@@ -375,8 +380,10 @@ class AdamW:
         return [[p.numel() for p in ps], [p.dtype for p in ps], [p.get_device() for p in ps]]
 
     def state(self) -> dict:
-        """The moments and the number of steps taken, as the constructor takes them."""
-        return {**self._state, "step": int(self._cfg.step)}
+        """The moments and the number of steps taken, as the constructor takes them: one number where it
+        is the same for every parameter, else one per parameter."""
+        taken = self._steps.tolist()
+        return {**self._state, "step": taken[0] if len(set(taken)) == 1 else taken}
 
     def set_lr(self, lr):
         """The learning rate of the next steps: a number, or one per parameter."""
@@ -405,13 +412,19 @@ class AdamW:
                              "tensor of its parameter's shape and device")
         table["grad"], table["grad_dtype"] = [g.data_ptr() for g in grads], kinds
         self._cfg.grad_scale = float(grad_scale)
-        self._cfg.step += 1
-        try:
-            with _at(self.device) as stream:
-                check(_nat.lib().sxcuda_adamw_step(table.ctypes.data, len(table),
-                                                   C.byref(self._cfg), stream))
-        except Exception:
-            self._cfg.step -= 1
-            raise
-        # autograd's check of saved tensors sees that the parameters are no longer what they were
-        torch.autograd.graph.increment_version(params)
+        there = np.array(there, dtype=np.intp)
+        numbers = self._steps[there] + 1
+        order = sorted(set(numbers.tolist()))
+        if len(order) > 1 and not (np.isfinite(table["lr"]) & np.isfinite(table["weight_decay"])).all():
+            raise ValueError(f"{what}: lr and weight_decay must be finite")  # before the first launch
+        with _at(self.device) as stream:
+            for number in order:
+                mine = np.flatnonzero(numbers == number)
+                some = len(mine) < len(table)
+                rows = np.ascontiguousarray(table[mine]) if some else table
+                self._cfg.step = number
+                check(_nat.lib().sxcuda_adamw_step(rows.ctypes.data, len(rows), C.byref(self._cfg),
+                                                   stream))
+                self._steps[there[mine]] = number
+                # autograd's check of saved tensors sees that the parameters are not what they were
+                torch.autograd.graph.increment_version([params[i] for i in mine] if some else params)

@@ -1,0 +1,88 @@
+"""AdamW over a program's whole life: parameters whose gradients come late, groups, memory that is
+shared or moves, divisors at the ends of the range. CFG and the numpy step are those of
+test_network_norm_adamw_gpu, which give every bit."""
+import math
+
+import numpy as np
+import pytest
+
+from test_network_norm_adamw_gpu import CFG, F, _np, _numpy_step
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_each_parameter_counts_its_own_steps(bits):
+    """A parameter whose first gradient comes after 50 steps of others takes a fresh optimiser's first
+    step, one without a gradient in between goes on with its own count, and so does an optimiser made
+    from the state."""
+    import torch
+    from splatx_cuda.network import AdamW
+    gen = torch.Generator().manual_seed(bits)
+    t = lambda n: torch.randn(n, generator=gen).cuda()  # noqa: E731
+    early, late, never = t(3000), t(700), t(5)
+    new, kept = late.clone(), never.clone()
+    opt = AdamW([early, late, never], state_bits=bits, **CFG)
+    for _ in range(50):
+        opt.step([t(3000), None, None])
+    assert torch.equal(late, new) and opt.state()["step"] == [50, 0, 0]
+    g = [t(700) for _ in range(3)]
+    opt.step([t(3000), g[0], None])
+    fresh = AdamW([new], state_bits=bits, **CFG)
+    fresh.step([g[0]])
+    assert torch.equal(late, new)
+    if bits == 32:
+        was = np.zeros(700, F)
+        first = torch.zeros(700, device="cuda")
+        AdamW([first], **CFG).step([g[0]])
+        assert np.array_equal(_np(first), _numpy_step(was, _np(g[0]), was, was, 1)[0])
+    opt.step([None, g[1], None])
+    fresh.step([g[1]])
+    assert torch.equal(late, new) and opt.state()["step"] == [51, 2, 0]
+    opt.step([None, None, None])
+    assert opt.state()["step"] == [51, 2, 0] and torch.equal(never, kept)
+    state = {k: v if k == "step" else [x.clone() for x in v] for k, v in opt.state().items()}
+    copy = [x.clone() for x in (early, late, never)]
+    other = AdamW(copy, state_bits=bits, state=state, **CFG)
+    ge = t(3000)
+    opt.step([ge, g[2], None])
+    other.step([ge, g[2], None])
+    fresh.step([g[2]])
+    assert torch.equal(late, new) and all(torch.equal(x, y) for x, y in zip((early, late, never), copy))
+    assert other.state()["step"] == [52, 3, 0] and fresh.state()["step"] == 3
+
+
+def test_counts_of_steps_are_checked():
+    import torch
+    from splatx_cuda.network import AdamW
+    a, b = torch.zeros(8, device="cuda"), torch.zeros(4, device="cuda")
+    moments = lambda: [torch.zeros(8, device="cuda"), torch.zeros(4, device="cuda")]  # noqa: E731
+    for bad in ([1], [1, 2, 3], [1, -1], -1):
+        with pytest.raises(ValueError):
+            AdamW([a, b], state={"step": bad, "exp_avg": moments(), "exp_avg_sq": moments()})
+    for good, shown in ((7, 7), ([7, 7], 7), ([7, 0], [7, 0])):
+        opt = AdamW([a, b], state={"step": good, "exp_avg": moments(), "exp_avg_sq": moments()})
+        assert opt.state()["step"] == shown
+
+
+def test_a_bad_rate_stops_every_launch():
+    import torch
+    from splatx_cuda.network import AdamW
+    a, b = torch.zeros(8, device="cuda"), torch.zeros(4, device="cuda")
+    opt = AdamW([a, b], **CFG)
+    opt.step([torch.ones_like(a), None])
+    was = a.clone()
+    for lr in ([1e-3, np.nan], [np.inf, 1e-3]):
+        opt.set_lr(lr)
+        with pytest.raises(ValueError):
+            opt.step([torch.ones_like(a), torch.ones_like(b)])
+    assert torch.equal(a, was) and not b.any() and opt.state()["step"] == [1, 0]
+
+
+def test_a_step_shows_in_the_versions_of_what_it_updates():
+    import torch
+    from splatx_cuda.network import AdamW
+    a, b = (torch.zeros(8, device="cuda") for _ in range(2))
+    versions = a._version, b._version
+    AdamW([a, b], **CFG).step([torch.ones_like(a), None])
+    assert a._version > versions[0] and b._version == versions[1]
