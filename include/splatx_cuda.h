@@ -843,7 +843,7 @@ typedef struct SxAdamwTensor {
 typedef struct SxAdamwConfig {
     double b1, b2, eps; /* 0 <= b < 1, eps >= 0 */
     double grad_scale;
-    int64_t step;       /* this step's number, from 1 */
+    int64_t step;       /* this step's number, from 1; a graph that captures the call replays this number */
     int32_t state_bits; /* 32 or 8 */
 } SxAdamwConfig;
 

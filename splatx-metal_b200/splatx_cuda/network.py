@@ -391,7 +391,8 @@ class AdamW:
 
     def step(self, grads=None, *, grad_scale=1.0):
         """One step on `grads` (one per parameter) or on the parameters' .grad; parameters whose
-        gradient is None stay as they are. grad_scale multiplies every gradient."""
+        gradient is None stay as they are. grad_scale multiplies every gradient. Not to be captured in
+        a graph (RuntimeError): a step's number and bias corrections are arguments of its launch."""
         what = "AdamW.step"
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
@@ -418,6 +419,9 @@ class AdamW:
         if len(order) > 1 and not (np.isfinite(table["lr"]) & np.isfinite(table["weight_decay"])).all():
             raise ValueError(f"{what}: lr and weight_decay must be finite")  # before the first launch
         with _at(self.device) as stream:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"{what}: a step cannot be captured in a graph: every replay would "
+                                   "be the same step, with its bias corrections")
             for number in order:
                 mine = np.flatnonzero(numbers == number)
                 some = len(mine) < len(table)

@@ -86,3 +86,25 @@ def test_a_step_shows_in_the_versions_of_what_it_updates():
     versions = a._version, b._version
     AdamW([a, b], **CFG).step([torch.ones_like(a), None])
     assert a._version > versions[0] and b._version == versions[1]
+
+
+def test_refused_while_a_graph_is_captured():
+    """A captured step would take the same step number, with the same bias corrections, in every
+    replay."""
+    import torch
+    from splatx_cuda.network import AdamW
+    p, g = torch.ones(300, device="cuda"), torch.ones(300, device="cuda")
+    opt = AdamW([p], **CFG)
+    opt.step([g])
+    was = p.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        p * 2
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.step([g])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p, was) and opt.state()["step"] == 1
+    opt.step([g])
+    assert opt.state()["step"] == 2 and not torch.equal(p, was)
