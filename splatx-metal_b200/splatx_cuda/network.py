@@ -297,9 +297,9 @@ class AdamW:
     not count. (Parameters with different counts take a launch for each count.)
 
     params: tensors, or dicts {"params": [...], "lr": ..., "weight_decay": ...} for groups with a
-    rate or decay of their own. They must be contiguous CUDA tensors of one device. Moments are held
-    in 32 bits, or with state_bits=8 as e4m3 codes of m and of sqrt(v) with a float32 scale for
-    every 256 values (2.03 bytes for a value's two moments in place of 8).
+    rate or decay of their own (other keys are refused). They must be contiguous CUDA tensors of
+    one device. Moments are held in 32 bits, or with state_bits=8 as e4m3 codes of m and of sqrt(v)
+    with a float32 scale for every 256 values (2.03 bytes for a value's two moments in place of 8).
 
     state: moments to go on from, {"exp_avg": [...], "exp_avg_sq": [...], "step": n} and, with 8
     bits, "exp_avg_scale" and "exp_avg_sq_scale", one tensor per parameter in order; the tensors are
@@ -311,11 +311,19 @@ class AdamW:
         what = "AdamW"
         if state_bits not in (8, 32):
             raise ValueError(f"{what}: state_bits must be 8 or 32")
-        params = list(params)
-        groups = params if params and isinstance(params[0], dict) else [{"params": params}]
+        groups = [] if isinstance(params, (torch.Tensor, dict)) else list(params)
+        if groups and not any(isinstance(g, dict) for g in groups):
+            groups = [{"params": groups}]
         self.params, rates, decays = [], [], []
         for g in groups:
-            mine = list(g["params"])
+            if not isinstance(g, dict) or "params" not in g:
+                raise ValueError(f"{what}: params are tensors, or dicts that each have 'params'")
+            if unknown := set(g) - {"params", "lr", "weight_decay"}:
+                raise ValueError(f"{what}: a group has an lr and a weight_decay of its own, no "
+                                 f"{', '.join(map(str, unknown))}")
+            mine = [None] if isinstance(g["params"], torch.Tensor) else list(g["params"])
+            if not all(isinstance(p, torch.Tensor) for p in mine):
+                raise ValueError(f"{what}: params must be a sequence of tensors")
             self.params += mine
             rates += [float(g.get("lr", lr))] * len(mine)
             decays += [float(g.get("weight_decay", weight_decay))] * len(mine)

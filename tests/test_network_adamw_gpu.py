@@ -108,3 +108,18 @@ def test_refused_while_a_graph_is_captured():
     assert torch.equal(p, was) and opt.state()["step"] == 1
     opt.step([g])
     assert opt.state()["step"] == 2 and not torch.equal(p, was)
+
+
+def test_groups_take_rate_and_decay_and_nothing_else():
+    """betas and eps are one for all parameters: a group's own, or a name with a slip, is refused
+    instead of dropped."""
+    import torch
+    from splatx_cuda.network import AdamW
+    p, o = torch.zeros(8, device="cuda"), torch.zeros(4, device="cuda")
+    AdamW([{"params": [p], "lr": 0.1, "weight_decay": 0.0}, {"params": iter([o])}, {"params": []}])
+    for bad in ({"betas": (0.5, 0.9)}, {"eps": 1e-4}, {"weigth_decay": 0.0}):
+        with pytest.raises(ValueError, match=next(iter(bad))):
+            AdamW([{"params": [p], **bad}])
+    for bad in ([{"lr": 0.1}], [{"params": [p]}, o], [o, {"params": [p]}], [{"params": p}], ["p"], p, {"params": [p]}):
+        with pytest.raises(ValueError):
+            AdamW(bad)
