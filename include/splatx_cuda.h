@@ -847,7 +847,8 @@ typedef struct SxAdamwConfig {
     int32_t state_bits; /* 32 or 8 */
 } SxAdamwConfig;
 
-/* tensors: HOST array of n_tensors, read before the call returns. */
+/* tensors: HOST array of n_tensors, read before the call returns. What is updated (parameters, moments,
+ * scales) must not overlap: its order within a launch is not defined. */
 int32_t sxcuda_adamw_step(const SxAdamwTensor* tensors, int64_t n_tensors,
                           const SxAdamwConfig* cfg, sxcuda_stream_t stream);
 

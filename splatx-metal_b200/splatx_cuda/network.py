@@ -335,15 +335,13 @@ class AdamW:
             _dtype(p, what)
             if not p.is_contiguous():
                 raise ValueError(f"{what}: parameters must be contiguous")
-        # two updates of one tensor in a launch would race
-        at = [p.data_ptr() for p in self.params if p.numel()]
-        if len(set(at)) != len(at):
-            raise ValueError(f"{what}: a parameter is given more than once")
         self._kept = self._facts()
         self.bits = state_bits
         self._cfg = _nat.SxAdamwConfig(float(betas[0]), float(betas[1]), float(eps), 1.0, 0,
                                        state_bits)
         self._state = self._bind(what, state)
+        self._at = [p.data_ptr() for p in self.params]
+        self._apart(what)
         n = len(self.params)
         self._table = np.zeros(n, dtype=_TENSOR)
         self._table["n"] = [p.numel() for p in self.params]
@@ -382,6 +380,14 @@ class AdamW:
                                      "parameters' sizes and device")
         return mine
 
+    def _apart(self, what):
+        """Refuses parameters and moments that share memory: CTAs would update it without order."""
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+                       for ts in (self.params, *self._state.values()) for t in ts if t.numel())
+        if any(start < end for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError(f"{what}: parameters or moments overlap in memory, or one is given more "
+                             "than once")
+
     def _facts(self) -> list:
         """What a step relies on of the parameters, which may have been given other memory since."""
         ps = self.params
@@ -408,8 +414,11 @@ class AdamW:
         params = self.params
         if self._facts() != self._kept or not all([p.is_contiguous() for p in params]):
             raise ValueError(f"{what}: a parameter's size, dtype, device or layout has changed")
-        table = self._table
-        table["param"] = [p.data_ptr() for p in params]
+        table, at = self._table, [p.data_ptr() for p in params]
+        if at != self._at:
+            self._apart(what)
+            self._at = at
+        table["param"] = at
         there = [i for i, g in enumerate(grads) if g is not None]
         if len(there) < len(grads):
             params, grads = [params[i] for i in there], [grads[i] for i in there]

@@ -123,3 +123,36 @@ def test_groups_take_rate_and_decay_and_nothing_else():
     for bad in ([{"lr": 0.1}], [{"params": [p]}, o], [o, {"params": [p]}], [{"params": p}], ["p"], p, {"params": [p]}):
         with pytest.raises(ValueError):
             AdamW(bad)
+
+
+def test_memory_that_is_updated_twice_is_refused():
+    """Parameters and moments whose bytes overlap, whatever their starts, when the optimiser is made and
+    when a parameter is given other memory later: two CTAs would read and write them without order."""
+    import torch
+    from splatx_cuda.network import AdamW
+    flat, m, v = (torch.zeros(1024, device="cuda") for _ in range(3))
+    state = lambda m0, m1, v0, v1: {"step": 0, "exp_avg": [m0, m1], "exp_avg_sq": [v0, v1]}  # noqa: E731
+    m0, m1, v0, v1 = m[:512], m[512:], v[:512], v[512:]
+    AdamW([flat[:512], flat[512:]], state=state(m0, m1, v0, v1))
+    for params, st in (([flat[:512], flat[256:768]], None), ([flat[256:768], flat[:512]], None),
+                       ([flat, flat[1000:1001]], None), ([flat[:512], flat[512:]], state(m0, m0, v0, v1)),
+                       ([flat[:512], flat[512:]], state(m0, m1, v0, m1)),
+                       ([flat[:512], flat[512:]], state(m0, m1, v[:512], v[511:1023])),
+                       ([flat[:512], flat[512:]], state(m0, m1, v0, flat[512:])),
+                       ([flat[:512].bfloat16(), flat.view(torch.float16)[:1], flat], None)):
+        with pytest.raises(ValueError, match="overlap|more than once"):
+            AdamW(params, state=st)
+    a, b = (torch.nn.Parameter(torch.randn(600, device="cuda")) for _ in range(2))
+    g = torch.randn(600, device="cuda")
+    opt = AdamW([a, b], **CFG)
+    opt.step([g, g])
+    own = b.data
+    for tied in (a.data, opt.state()["exp_avg"][0]):
+        b.data = tied
+        was = a.detach().clone(), [t.clone() for t in opt.state()["exp_avg"]]
+        with pytest.raises(ValueError, match="overlap"):
+            opt.step([g, g])
+        assert torch.equal(a, was[0]) and all(torch.equal(x, y) for x, y in zip(opt.state()["exp_avg"], was[1]))
+    b.data = own
+    opt.step([g, g])
+    assert opt.state()["step"] == 2
