@@ -378,6 +378,9 @@ class AdamW:
                         t.device != self.device:
                     raise ValueError(f"{what}: {key} needs contiguous {dtype} tensors of the "
                                      "parameters' sizes and device")
+            # the kernel has their addresses: tensors of the optimiser's own hold that memory, whatever
+            # the caller gives its own tensors or lists later
+            mine[key] = [t.detach() for t in mine[key]]
         return mine
 
     def _apart(self, what):
@@ -394,10 +397,12 @@ class AdamW:
         return [[p.numel() for p in ps], [p.dtype for p in ps], [p.get_device() for p in ps]]
 
     def state(self) -> dict:
-        """The moments and the number of steps taken, as the constructor takes them: one number where it
-        is the same for every parameter, else one per parameter."""
+        """The moments (views of what the next step updates) and the number of steps taken, as the
+        constructor takes them: one number where it is the same for every parameter, else one per
+        parameter."""
         taken = self._steps.tolist()
-        return {**self._state, "step": taken[0] if len(set(taken)) == 1 else taken}
+        return {**{key: [t.detach() for t in ts] for key, ts in self._state.items()},
+                "step": taken[0] if len(set(taken)) == 1 else taken}
 
     def set_lr(self, lr):
         """The learning rate of the next steps: a number, or one per parameter."""

@@ -156,3 +156,34 @@ def test_memory_that_is_updated_twice_is_refused():
     b.data = own
     opt.step([g, g])
     assert opt.state()["step"] == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_moments_stay_the_optimisers_own(bits):
+    """What state() hands out, and what the constructor was given, may be replaced or given other memory
+    without changing where the next step reads and writes its moments."""
+    import torch
+    from splatx_cuda.network import AdamW
+    gen = torch.Generator().manual_seed(3)
+    t = lambda: torch.randn(900, generator=gen).cuda()  # noqa: E731
+    p, grads = t(), [t() for _ in range(4)]
+    q = p.clone()
+    want, opt = AdamW([q], state_bits=bits, **CFG), AdamW([p], state_bits=bits, **CFG)
+    want.step([grads[0]])
+    opt.step([grads[0]])
+    given = opt.state()
+    opt = AdamW([p], state_bits=bits, state=given, **CFG)
+    for i, g in enumerate(grads[1:]):
+        want.step([g])
+        for shown in (given, opt.state()) if i else ():
+            for key in shown:
+                if key != "step":
+                    shown[key][0].data = torch.empty_like(shown[key][0])  # as when moments are moved away
+                    shown[key][0] = None
+                    shown[key].clear()
+        given = opt.state()
+        opt.step([g])
+        assert torch.equal(p, q), i
+    for key, tensors in want.state().items():
+        if key != "step":
+            assert torch.equal(opt.state()[key][0].view(torch.uint8), tensors[0].view(torch.uint8))
