@@ -363,6 +363,7 @@ class AdamW:
         if len(taken) != len(self.params) or any(int(t) < 0 for t in taken):
             raise ValueError(f"{what}: step must be a number of at least 0, or one per parameter")
         self._steps = np.array([int(t) for t in taken], dtype=np.int64)
+        self._even = bool((self._steps == self._steps[0]).all())  # one count, which a step need not sort
         mine = {}
         for key, dtype in kinds.items():
             sizes = [-(-p.numel() // RUN) if key.endswith("scale") else p.numel()
@@ -393,8 +394,7 @@ class AdamW:
 
     def _facts(self) -> list:
         """What a step relies on of the parameters, which may have been given other memory since."""
-        ps = self.params
-        return [[p.numel() for p in ps], [p.dtype for p in ps], [p.get_device() for p in ps]]
+        return [[p.numel() for p in self.params], [p.dtype for p in self.params]]
 
     def state(self) -> dict:
         """The moments (views of what the next step updates) and the number of steps taken, as the
@@ -420,7 +420,8 @@ class AdamW:
         if self._facts() != self._kept or not all([p.is_contiguous() for p in params]):
             raise ValueError(f"{what}: a parameter's size, dtype, device or layout has changed")
         table, at = self._table, [p.data_ptr() for p in params]
-        if at != self._at:
+        if at != self._at:  # an address says which device it is on, too
+            _on(self.device, what, *params)
             self._apart(what)
             self._at = at
         table["param"] = at
@@ -435,22 +436,25 @@ class AdamW:
                              "tensor of its parameter's shape and device")
         table["grad"], table["grad_dtype"] = [g.data_ptr() for g in grads], kinds
         self._cfg.grad_scale = float(grad_scale)
-        there = np.array(there, dtype=np.intp)
-        numbers = self._steps[there] + 1
-        order = sorted(set(numbers.tolist()))
-        if len(order) > 1 and not (np.isfinite(table["lr"]) & np.isfinite(table["weight_decay"])).all():
-            raise ValueError(f"{what}: lr and weight_decay must be finite")  # before the first launch
+        if self._even and len(there) == len(self.params):
+            launches = {int(self._steps[0]) + 1: slice(None)}
+        else:
+            numbers, there = self._steps[there] + 1, np.array(there, dtype=np.intp)
+            launches = {n: np.flatnonzero(numbers == n) for n in sorted(set(numbers.tolist()))}
+            if len(launches) > 1 and not np.isfinite([table["lr"], table["weight_decay"]]).all():
+                raise ValueError(f"{what}: lr and weight_decay must be finite")  # before the first
+            self._even = False
         with _at(self.device) as stream:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError(f"{what}: a step cannot be captured in a graph: every replay would "
                                    "be the same step, with its bias corrections")
-            for number in order:
-                mine = np.flatnonzero(numbers == number)
-                some = len(mine) < len(table)
+            for number, mine in launches.items():
+                some = len(launches) > 1
                 rows = np.ascontiguousarray(table[mine]) if some else table
                 self._cfg.step = number
                 check(_nat.lib().sxcuda_adamw_step(rows.ctypes.data, len(rows), C.byref(self._cfg),
                                                    stream))
-                self._steps[there[mine]] = number
+                self._steps[slice(None) if self._even else there[mine]] = number
                 # autograd's check of saved tensors sees that the parameters are not what they were
                 torch.autograd.graph.increment_version([params[i] for i in mine] if some else params)
+        self._even = self._even or bool((self._steps == self._steps[0]).all())

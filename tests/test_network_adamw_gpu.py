@@ -187,3 +187,19 @@ def test_the_moments_stay_the_optimisers_own(bits):
     for key, tensors in want.state().items():
         if key != "step":
             assert torch.equal(opt.state()[key][0].view(torch.uint8), tensors[0].view(torch.uint8))
+
+
+def test_a_parameter_moved_off_the_device_is_refused():
+    import torch
+    from splatx_cuda.network import AdamW
+    p = torch.nn.Parameter(torch.zeros(8, device="cuda"))
+    opt = AdamW([p], **CFG)
+    opt.step([torch.ones(8, device="cuda")])
+    was, p.data = p.data, p.data.cpu()
+    with pytest.raises(ValueError):
+        opt.step([torch.ones(8)])
+    with pytest.raises(ValueError):
+        opt.step([torch.ones(8, device="cuda")])
+    p.data = was
+    opt.step([torch.ones(8, device="cuda")])
+    assert opt.state()["step"] == 2
