@@ -205,14 +205,14 @@ void validate_adamw(const SxAdamwTensor* t, int64_t n, const SxAdamwConfig* c, c
     if (c->step < 1) throw_invalid(w, "step counts from 1");
     if (!(c->b1 >= 0.0 && c->b1 < 1.0) || !(c->b2 >= 0.0 && c->b2 < 1.0))
         throw_invalid(w, "b1 and b2 must be in [0, 1)");
-    if (!(c->eps >= 0.0) || !std::isfinite(c->eps)) throw_invalid(w, "eps must be finite and not negative");
-    if (!std::isfinite(c->grad_scale)) throw_invalid(w, "grad_scale must be finite");
+    const auto finite = [](double x) { return std::isfinite(static_cast<float>(x)); };  // as the kernel has it
+    if (!(c->eps >= 0.0) || !finite(c->eps)) throw_invalid(w, "eps must be finite and not negative");
+    if (!finite(c->grad_scale)) throw_invalid(w, "grad_scale must be finite");
     for (int64_t i = 0; i < n; ++i) {
         if (t[i].n < 0) throw_invalid(w, "negative n");
         validate_dtype(t[i].param_dtype, w, "param_dtype");
         validate_dtype(t[i].grad_dtype, w, "grad_dtype");
-        if (!std::isfinite(t[i].lr) || !std::isfinite(t[i].weight_decay))
-            throw_invalid(w, "lr and weight_decay must be finite");
+        if (!finite(t[i].lr) || !finite(t[i].weight_decay)) throw_invalid(w, "lr and weight_decay must be finite");
         if (t[i].n == 0) continue;
         validate_pointer(t[i].param, t[i].param_dtype, w, "param");
         validate_pointer(t[i].grad, t[i].grad_dtype, w, "grad");

@@ -203,3 +203,39 @@ def test_a_parameter_moved_off_the_device_is_refused():
     p.data = was
     opt.step([torch.ones(8, device="cuda")])
     assert opt.state()["step"] == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [8192, 700])
+@pytest.mark.parametrize("eps", [0.0, 1e-40, 1e-38, 1e-30, 1e30, 3e38])
+def test_divisors_at_the_ends_of_the_range(eps, n, bits):
+    """Values without a gradient beside others: m / (0 + eps) is 0 for every eps above zero, also for one
+    that 32 bits hold below 2^-126, and not a number for none; a divisor near the largest value leaves
+    the weights as they are. In chunks of the fast path and in tails."""
+    import torch
+    from splatx_cuda.network import AdamW
+    rng = np.random.default_rng(n)
+    g = rng.standard_normal(n).astype(F)
+    g[::3] = 0
+    was = rng.standard_normal(n).astype(F)
+    p = torch.from_numpy(was).cuda()
+    cfg = {**CFG, "eps": eps}
+    AdamW([p], state_bits=bits, **cfg).step([torch.from_numpy(g).cuda()])
+    with np.errstate(invalid="ignore"):
+        b1, b2 = CFG["betas"]
+        m, v = g * F(1 - b1), (g * g) * F(1 - b2)
+        d = np.sqrt(v) * F(1 / math.sqrt(1 - b2)) + F(eps)
+        want = was * F(1 - CFG["lr"] * CFG["weight_decay"]) - m / d * F(CFG["lr"] / (1 - b1))
+    assert np.array_equal(_np(p), want, equal_nan=True)
+    assert np.isnan(want).any() == (eps == 0.0)
+
+
+def test_numbers_that_32_bits_do_not_hold_are_refused():
+    import torch
+    from splatx_cuda.network import AdamW
+    p, g = torch.zeros(8, device="cuda"), torch.zeros(8, device="cuda")
+    for f in (lambda: AdamW([p], eps=1e39).step([g]), lambda: AdamW([p], lr=-1e39).step([g]),
+              lambda: AdamW([p], weight_decay=1e39).step([g]), lambda: AdamW([p]).step([g], grad_scale=1e39)):
+        with pytest.raises(ValueError):
+            f()
+    assert not p.any()
