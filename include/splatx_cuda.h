@@ -821,7 +821,8 @@ int32_t sxcuda_layer_norm_bwd(const SxLayerNormInputs* in, const SxLayerNormGrad
  * 400 of them:
  *   g' = g * grad_scale            m' = b1 m + (1 - b1) g'        v' = b2 v + (1 - b2) g'^2
  *   p' = p (1 - lr weight_decay) - lr / (1 - b1^step) * m' / (sqrt(v' / (1 - b2^step)) + eps)
- * evaluated in 32 bits, every operation rounded by itself. (sxcuda_fused_adam is the reference's
+ * evaluated in 32 bits, every operation rounded by itself (but for a quotient whose m' is below 2^-100: it
+ * may be off by its last bit, and differ so with the value's place in its tensor). (sxcuda_fused_adam is the reference's
  * Adam without bias correction, over one tensor.)
  * 8-bit moments: m and sqrt(v) are held as e4m3 codes, each run of 256 consecutive values with
  * one 32-bit scale (largest magnitude / 448); a value above zero of sqrt(v) keeps at least the

@@ -239,3 +239,22 @@ def test_numbers_that_32_bits_do_not_hold_are_refused():
         with pytest.raises(ValueError):
             f()
     assert not p.any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("n", [1 << 16, 1000])
+def test_quotients_of_small_moments(n, bits):
+    """Every bit from a moment of 2^-100 on; below that the quotient's last bit may be off, which moves
+    the weight (zero before) by that much of itself, and a unit of the smallest numbers."""
+    import torch
+    from splatx_cuda.network import AdamW
+    rng = np.random.default_rng(n)
+    g = (rng.choice([-1, 1], n) * rng.uniform(1, 2, n) * 2.0 ** rng.uniform(-135, -60, n)).astype(F)
+    p = torch.zeros(n, device="cuda")
+    AdamW([p], state_bits=bits, **CFG).step([torch.from_numpy(g).cuda()])
+    zero = np.zeros(n, F)
+    want, m, _ = _numpy_step(zero, g, zero, zero, 1)
+    exact = np.abs(m) >= 2.0 ** -100
+    assert exact.any() and not exact.all() and np.array_equal(_np(p)[exact], want[exact])
+    off = np.abs(_np(p).astype(np.float64) - want)
+    assert np.all(off <= 2.0 ** -22 * np.abs(want.astype(np.float64)) + 2.0 ** -149)
