@@ -199,9 +199,10 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     }
 }
 
-// The largest magnitudes of the output's gradient and of v below the lengths, per batch entry and key
-// head, as the bits of a float, which order like unsigned numbers (so the atomics' order does not
-// matter). A CTA per 64 rows of a head: the first `g_blocks` for the gradient, the others for v.
+// The largest squared norms of the rows of the output's gradient and of v below the lengths, per batch
+// entry and key head, as the bits of a float, which order like unsigned numbers (so the atomics' order does
+// not matter). A CTA per 64 rows of a head, 16 lanes a row: the first `g_blocks` for the gradient, the
+// others for v.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, uint32_t g_blocks) {
     const bool is_g = blockIdx.x < g_blocks;
@@ -209,18 +210,23 @@ __global__ void __launch_bounds__(256) attn_largest_kernel(const AttnArgs a, uin
     const uint32_t block = is_g ? blockIdx.x : blockIdx.x - g_blocks;
     const int64_t len = is_g ? a.q_len : a.kv_len;
     const int heads = is_g ? a.heads : a.kv_heads, per_head = static_cast<int>((len + 63) / 64);
-    const int64_t bh = block / per_head, b = bh / heads, r0 = static_cast<int64_t>(block % per_head) * 64;
-    const int64_t end = min(attn_length(is_g ? a.q_lens : a.kv_lens, b, len), r0 + 64);
-    const T* p = static_cast<const T*>(v.data) + b * v.batch_stride + bh % heads * v.head_stride;
+    const int64_t bh = block / per_head, b = bh / heads, r0 = static_cast<int64_t>(block % per_head) * 64 + threadIdx.x / 16;
+    const int64_t end = attn_length(is_g ? a.q_lens : a.kv_lens, b, len);
+    const int c = threadIdx.x % 16 * 8;
+    const T* p = static_cast<const T*>(v.data) + b * v.batch_stride + bh % heads * v.head_stride + c;
     float top = 0.f;
-    for (int64_t r = r0 + threadIdx.x / 16; r < end; r += 16)
-        for (int c = threadIdx.x % 16 * 8; c < a.dim; c += 128) {
-            const Pack<T, 8> x = *reinterpret_cast<const Pack<T, 8>*>(p + r * v.token_stride + c);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(to_f32(x.v[e])));
+    for (int i = 0; i < 4; ++i) {
+        const int64_t r = r0 + i * 16;
+        float s = 0.f;
+        if (r < end && c < a.dim) {
+            const Pack<T, 8> x = *reinterpret_cast<const Pack<T, 8>*>(p + r * v.token_stride);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s = fmaf(to_f32(x.v[e]), to_f32(x.v[e]), s);
         }
-#pragma unroll
-    for (int off = 16; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, off));
+        top = fmaxf(top, sum16(s));
+    }
+    top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 16));
     if (threadIdx.x % 32 == 0 && top > 0.f) {
         const int64_t hk = is_g ? bh % heads / a.group : bh % heads;
         atomicMax(a.largest + 2 * (b * a.kv_heads + hk) + !is_g, __float_as_uint(top));

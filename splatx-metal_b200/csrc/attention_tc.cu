@@ -574,10 +574,11 @@ struct Loaded {
 };
 
 // float16 keeps 11 bits only above 2^-14: p and ds are held times powers of two, so that what a
-// gradient is summed from does not vanish before the sum. p is at most 1; for ds
-// |p (g v - delta)| <= 2 dim max|g| max|v|, which `ds` times takes to at most 2^15. The maxima are those
-// of the heads that share a key head (whose gradient is one sum), so that no other head's or batch
-// entry's magnitudes take bits away.
+// gradient is summed from does not vanish before the sum. p is at most 1; for ds, out being a mean of rows
+// of v, |p (g v - delta)| <= 2 max|g| max|v| with the rows' norms, which `ds` times takes to at most 2^14.
+// What ds holds is then off by at most 2^-25 / `ds`, 2^-38 of that bound, where its own 11 bits end. The
+// maxima are those of the heads that share a key head (whose gradient is one sum), so that no other head's
+// or batch entry's magnitudes take bits away.
 struct HalfScale {
     float p = 1.f, ds = 1.f;
 };
@@ -586,7 +587,7 @@ __device__ __forceinline__ HalfScale half_scale(const AttnArgs& a, int64_t b, in
     HalfScale h;
     if constexpr (std::is_same_v<T, __half>) {
         const uint32_t* largest = a.largest + 2 * (b * a.kv_heads + hk);
-        const float bound = 2.f * a.dim * __uint_as_float(largest[0]) * __uint_as_float(largest[1]);
+        const float bound = 2.f * sqrtf(__uint_as_float(largest[0])) * sqrtf(__uint_as_float(largest[1]));
         h.p = 1.f / exp2f(kHalfShift);
         if (bound > 0x1p-80f && bound < 0x1p80f) h.ds = exp2f(14.f - ceilf(log2f(bound)));
     }

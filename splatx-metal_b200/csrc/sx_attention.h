@@ -22,8 +22,8 @@ struct AttnArgs {
     float* minus_lse2;   // [batch, heads, q_pad]: minus the log-sums in base 2, -inf where nothing is seen
     float* minus_delta;  // [batch, heads, q_pad]
     // float16 on the tensor cores: probabilities are held times 2^p_shift, and ds times a power of two
-    // taken from the largest magnitudes of the output's gradient and of v: [batch, kv_heads, 2], the
-    // bits of a float each.
+    // taken from the largest squared norms of the rows of the output's gradient and of v: [batch,
+    // kv_heads, 2], the bits of a float each.
     float p_shift;
     uint32_t* largest;
     int64_t batch, q_len, kv_len, q_pad;
