@@ -605,7 +605,6 @@ __device__ __forceinline__ void set_pair(uint32_t (&r)[32], int i, tc::Two x) {
 // and causal 2 x 16 (4) x 4096 x 128 bf16: 3 of them 190.4 and 449.6 us, 4 194.8 and 451.4, 5 191.8 and
 // 451.3.
 constexpr int kPolyBwd = 3;
-template <typename T>
 __device__ __forceinline__ void exp_pair(uint32_t (&r)[32], int i, tc::Two x) {
     float lo, hi;
     if (i / 2 % 16 * kPolyBwd % 16 < kPolyBwd) {
@@ -788,8 +787,8 @@ __device__ __forceinline__ Loaded bwd_kv_tile(const AttnArgs& a, const TcMaps& m
 #pragma unroll
                 for (int e = 0; e < 32; e += 4) {
                     const ulonglong2 x = lse[c * 8 + e / 4];
-                    exp_pair<T>(r[c], e, tc::fma2(pair(r[c], e), times, tc::Two{x.x}));
-                    exp_pair<T>(r[c], e + 2, tc::fma2(pair(r[c], e + 2), times, tc::Two{x.y}));
+                    exp_pair(r[c], e, tc::fma2(pair(r[c], e), times, tc::Two{x.x}));
+                    exp_pair(r[c], e + 2, tc::fma2(pair(r[c], e + 2), times, tc::Two{x.y}));
                 }
                 if (cut) keep_columns(r[c], lo - c * 32, hi - c * 32);
                 uint32_t p[16];
@@ -945,7 +944,7 @@ __device__ __forceinline__ Loaded bwd_q_tile(const AttnArgs& a, const TcMaps& ma
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) exp_pair<T>(r[c], e, tc::fma2(pair(r[c], e), times, lse));
+                for (int e = 0; e < 32; e += 2) exp_pair(r[c], e, tc::fma2(pair(r[c], e), times, lse));
             ok = tc::bar_wait(bars.w_full(), j & 1, failed);
             if (!ok) break;
             tc::fence_after();

@@ -311,7 +311,6 @@ __global__ void __launch_bounds__(kThreads<LANES>, kBwdPerSm<LANES>) norm_bwd_ke
 
 // Columns too many for registers: a CTA per row, read again for each pass (from L2 as a rule), and
 // the column sums by a thread per column over a slice of the rows.
-template <typename T>
 __device__ __forceinline__ float cta_sum(float x, float* buf, int& phase) {
     float s[1] = {x};
     group_sum<kNormThreads, 1>(s, buf, phase);
@@ -326,13 +325,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_wide_kernel(const NormA
         const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
         float s = 0.f;
         for (int c = threadIdx.x; c < a.cols; c += kNormThreads) s += to_f32(x[c]);
-        const float mean = cta_sum<T>(s, buf, phase) * inv_c;
+        const float mean = cta_sum(s, buf, phase) * inv_c;
         s = 0.f;
         for (int c = threadIdx.x; c < a.cols; c += kNormThreads) {
             const float d = to_f32(x[c]) - mean;
             s = fmaf(d, d, s);
         }
-        const float rstd = 1.f / sqrtf(fmaf(cta_sum<T>(s, buf, phase), inv_c, a.eps));
+        const float rstd = 1.f / sqrtf(fmaf(cta_sum(s, buf, phase), inv_c, a.eps));
         T* y = static_cast<T*>(a.y) + row * a.y_stride;
         for (int c = threadIdx.x; c < a.cols; c += kNormThreads)
             y[c] = from_f32<T>(fmaf((to_f32(x[c]) - mean) * rstd, param_at(a.w, a.param_dtype, c, 1.f),

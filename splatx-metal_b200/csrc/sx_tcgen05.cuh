@@ -115,12 +115,6 @@ __device__ __forceinline__ void tmem_load32(uint32_t (&r)[32], uint32_t at) {
         : SX_R8(r, 0), SX_R8(r, 8), SX_R8(r, 16), SX_R8(r, 24)
         : "r"(at));
 }
-__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-        : SX_R8(r, 0), SX_R8(r, 8)
-        : "r"(at));
-}
 __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -138,7 +132,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&r)[16
 #define SX_T8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
 // Waits for the thread's loads. The registers are named as changed behind the wait, so that the
 // compiler moves no use of them before it.
-__device__ __forceinline__ void changed(uint32_t (&r)[16]) { asm volatile("" : SX_T8(r, 0), SX_T8(r, 8)); }
 __device__ __forceinline__ void changed(uint32_t (&r)[32]) {
     asm volatile("" : SX_T8(r, 0), SX_T8(r, 8));
     asm volatile("" : SX_T8(r, 16), SX_T8(r, 24));
