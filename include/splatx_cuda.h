@@ -858,7 +858,9 @@ int32_t sxcuda_adamw_step(const SxAdamwTensor* tensors, int64_t n_tensors,
  * Query i of batch b sees key j where i < q_lens[b], j < kv_lens[b] and, when causal,
  * j <= i + kv_lens[b] - q_lens[b] (without lengths: q_len and kv_len). A query that sees none has
  * output 0, log-sum -inf and gradient 0; a key that none sees has gradient 0. Rows at or beyond
- * the lengths may hold anything, NaN among it. */
+ * the lengths may hold anything, NaN among it. Below them, a query that sees a score of NaN or +inf, or
+ * only scores of -inf, is NaN with its log-sum and the gradients it takes part in; and since 0 * NaN is
+ * NaN, a k or v that is not finite may also reach queries whose causal mask hides it. */
 typedef struct SxAttentionView {
     void* data;           /* [batch, tokens, heads, head_dim], head_dim contiguous */
     int64_t batch_stride; /* elements */

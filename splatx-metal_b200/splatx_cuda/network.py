@@ -140,7 +140,8 @@ def attention_fwd(q, k, v, *, scale=None, causal=False, q_lens=None, kv_lens=Non
     axis contiguous. scale defaults to 1 / sqrt(head_dim). q_lens, kv_lens: int32 [batch] token
     counts of a padded batch; what lies beyond them is not used. causal: query i sees key j where
     j <= i + kv_len - q_len (the lengths of its batch entry). A query that sees no key gets output 0
-    and log-sum -inf."""
+    and log-sum -inf; one that sees a score of NaN or +inf, or only -inf, is NaN. A k or v that is
+    not finite may also reach queries whose causal mask hides it (0 * NaN is NaN)."""
     q, k, v, ins, device = _attention_inputs("attention_fwd", q, k, v, scale, causal, q_lens, kv_lens)
     b, n, h, _ = q.shape
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
