@@ -10,8 +10,8 @@
 // query heads that share the key-value head), one owns a tile of queries and passes over the keys.
 // That computes s and g v^T twice, and needs neither atomics nor partial sums in memory, so results
 // do not change between calls. These kernels are bound by the multiply-adds and the shared-memory
-// reads that feed them (four rows and four columns a thread); causal bf16 16 heads x 8192 x 128 takes
-// them 12.1 ms, the tensor-core forward 0.21 ms.
+// reads that feed them (four rows and four columns a thread): causal 16 heads (4 key-value) x 8192 x 128
+// in 32 bits takes the forward 12.0 ms, 23 TFLOP/s (bf16 on the tensor cores 0.22 ms).
 #include "sx_attention.h"
 
 namespace sx {

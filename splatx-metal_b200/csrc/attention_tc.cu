@@ -10,9 +10,11 @@
 // With 128 columns the products and shared memory bound the forward, with 64 the exponentials and the
 // path through them (score, maximum, probability and back, some 2000 cycles of latency per tile, which
 // two tiles in turn hide in part). Measured, bf16: forward, causal, 16 heads (4 key-value) x 8192 x 128:
-// 212 us, 1297 TFLOP/s of the needed products, 0.78 of the measured rate of large matrix products
-// (1657); x 64: 182 us. Backward, causal, 2 x 16 (4) x 4096 x 128: 380 us, 904 TFLOP/s counting the five
-// products that the gradient needs; 8 x 16 x 1024 x 64: 188 us (456).
+// 216 us in short runs, 1272 TFLOP/s of the needed products, 0.77 of the measured rate of large matrix
+// products (1657); in a steady run, under the power limit, 254 us, 1082 TFLOP/s, 0.77 of the rate that
+// those products sustain (1414). x 64: 191 us. Backward, causal, 2 x 16 (4) x 4096 x 128: 389 us, steady
+// 457 us (884 and 752 TFLOP/s counting the five products that the gradient needs); 8 x 16 x 1024 x 64: 191
+// us, steady 195 (450 and 441).
 // Kept out, measured: one CTA per SM that takes tiles by ticket (short sequences 5% faster, long ones
 // 7-13% slower: the loops of both kinds of tile then share too few registers); two warps that issue the
 // forward's products (64 columns 5% faster, 128 20% slower); sixteen softmax warps (12% slower).

@@ -12,10 +12,11 @@
 // cost: a thread holds 64 bytes of a row (half of that in the backward, whose column sums take two
 // registers a value), so that the groups' sums are spread over many values; the arithmetic is done two
 // values at a time; and the weights lie in shared memory, in the order the lanes read them, which
-// leaves registers for more rows. bf16 32768 x 1024: forward 24.8 us (5.4 TB/s), backward 42.8 us
-// (4.7 TB/s); with the weights in registers and 32 values a thread the forward took 47 us (8 warps an
-// SM), with 8 values a thread 39 us (twice the instructions a row). The backward's bound is its
-// instructions and the rows that 128 registers a thread leave in flight.
+// leaves registers for more rows. bf16 32768 x 1024: forward 24.8 us (5.4 TB/s), backward 43.5 us
+// (4.6 TB/s); with the weights in registers and 32 values a thread the forward took 47 us (8 warps an
+// SM), with 8 values a thread 39 us (twice the instructions a row). Of the backward's time 37.8 us are
+// the first kernel's without its partial rows (5.3 TB/s, with the rows that 128 registers a thread leave
+// in flight), 5.7 us the partial rows and the second kernel.
 // The grid is what the SMs hold; each group takes every n-th row, so the backward's column sums stay
 // in registers until the group is done. They then go, one partial row per CTA, to the workspace, and a
 // second kernel adds the partial rows in order: the result does not depend on timing.
