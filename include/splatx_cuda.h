@@ -906,6 +906,114 @@ int32_t sxcuda_attention_bwd(const SxAttentionInputs* in, const SxAttentionGrads
  * the device. */
 int32_t sxcuda_attention_status(uint32_t* status);
 
+/* y = act(x weight^T + bias) + residual: a layer's matrix product with what follows it. The sums, the bias,
+ * the activation and the residual are taken in 32 bits and rounded once. rows 0 is a no-op (the
+ * backward then writes zero weight and bias gradients). */
+#define SXCUDA_ACT_NONE 0
+#define SXCUDA_ACT_RELU 1
+#define SXCUDA_ACT_SILU 2      /* z / (1 + exp(-z)) */
+#define SXCUDA_ACT_GELU 3      /* z Phi(z), Phi the normal distribution function */
+#define SXCUDA_ACT_GELU_TANH 4 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+
+typedef struct SxLinearInputs {
+    const void* x;      /* [rows, in_features], dtype, rows x_stride elements apart */
+    const void* weight; /* [out_features, in_features], dtype, rows weight_stride elements apart */
+    const void* bias;   /* [out_features], bias_dtype; NULL = zeros (the backward does not read it) */
+    int64_t rows, in_features, out_features; /* features 1..2^30 - 1, rows 0..2^30 - 1 */
+    int64_t x_stride, weight_stride;         /* >= in_features unless there is one row at most */
+    int32_t dtype, bias_dtype;
+    int32_t activation;
+} SxLinearInputs;
+
+/* residual: [rows, out_features] of dtype, or NULL. y and pre (x weight^T + bias before the activation,
+ * which the backward of an activation reads; NULL where that is not wanted): [rows, out_features] of
+ * dtype. residual may be y itself. Workspace query protocol (the size may be 0; a non-NULL workspace
+ * pointer is then not read); x's and weight's addresses and strides count for the size. */
+typedef struct SxLinearOutputs {
+    const void* residual;
+    int64_t residual_stride;
+    void* y;
+    int64_t y_stride;
+    void* pre;
+    int64_t pre_stride;
+} SxLinearOutputs;
+int32_t sxcuda_linear_fwd(const SxLinearInputs* in, const SxLinearOutputs* out, void* workspace,
+                          size_t* workspace_bytes, sxcuda_stream_t stream);
+
+typedef struct SxLinearGradsIn {
+    const void* v_y; /* [rows, out_features], dtype: gradient of y (and, unchanged, of residual) */
+    int64_t v_y_stride;
+    const void* pre; /* of the forward; NULL without an activation */
+    int64_t pre_stride;
+} SxLinearGradsIn;
+
+typedef struct SxLinearGrads {
+    void* v_x; /* [rows, in_features], dtype, or NULL */
+    int64_t v_x_stride;
+    void* v_weight; /* [out_features, in_features], dtype, or NULL */
+    int64_t v_weight_stride;
+    void* v_bias; /* [out_features], bias_dtype, or NULL */
+} SxLinearGrads;
+
+/* v_z = v_y act'(pre), held in dtype; v_x = v_z weight, v_weight = v_z^T x, v_bias = the sum of v_z over
+ * the rows before v_z is rounded. Sums in a fixed order: the result is the same in every call. Workspace query
+ * protocol; the query reads gin and out, too. */
+int32_t sxcuda_linear_bwd(const SxLinearInputs* in, const SxLinearGradsIn* gin, const SxLinearGrads* out,
+                          void* workspace, size_t* workspace_bytes, sxcuda_stream_t stream);
+
+/* Status bits of the linear kernels of the current device, as sxcuda_attention_status. */
+int32_t sxcuda_linear_status(uint32_t* status);
+
+/* Queries and keys normalised per head and rotated by the positions of their tokens:
+ *   u = x / sqrt(mean x^2 + eps) * weight  (without norm: u = x)
+ *   (u1, u2) -> (u1 cos - u2 sin, u1 sin + u2 cos) for every pair of a head's values, at the angle of its
+ *   axis' position times the pair's frequency.
+ * Axis a has axis_dims[a] values, half as many pairs; the pairs of axis 0 come first in freqs. Which values
+ * are a pair: SXCUDA_PAIRS_AXIS: value j of the axis' own run and value j + axis_dims[a] / 2 of it;
+ * SXCUDA_PAIRS_WHOLE: values i and i + (sum of axis_dims) / 2, i the pair's number over all axes;
+ * SXCUDA_PAIRS_NEIGHBOURS: values 2 i and 2 i + 1. Values behind the sum of axis_dims are not rotated.
+ * Angles are taken in 64 bits, whole turns off; norms, sines and products in 32 bits, rounded once. */
+#define SXCUDA_PAIRS_AXIS 0
+#define SXCUDA_PAIRS_WHOLE 1
+#define SXCUDA_PAIRS_NEIGHBOURS 2
+#define SXCUDA_POS_F32 0
+#define SXCUDA_POS_I32 1
+#define SXCUDA_POS_I64 2
+
+typedef struct SxRotaryInputs {
+    SxAttentionView q;     /* [batch, tokens, q_heads, head_dim] */
+    SxAttentionView k;     /* [batch, tokens, k_heads, head_dim]; not read where k_heads is 0 */
+    const void* positions; /* [batch, tokens, axes] of pos_dtype; strides in elements, 0 = shared */
+    int64_t pos_batch_stride, pos_token_stride, pos_axis_stride;
+    const double* freqs;   /* HOST array, sum of axis_dims / 2, finite; read before the call returns */
+    const void* q_weight;  /* [head_dim], param_dtype; NULL = ones (and without norm) */
+    const void* k_weight;
+    int64_t batch, tokens;
+    int32_t q_heads, k_heads;
+    int32_t head_dim;      /* 1..256 */
+    int32_t axes;          /* 1..4 */
+    int32_t axis_dims[4];  /* even, >= 0, their sum at most head_dim */
+    int32_t pairs, dtype, param_dtype, pos_dtype;
+    int32_t norm;          /* 0 or 1 */
+    float eps;             /* finite, >= 0 */
+} SxRotaryInputs;
+
+/* q_out like q, k_out like k; each may be its input (the same data and strides). */
+int32_t sxcuda_qk_norm_rotary_fwd(const SxRotaryInputs* in, const SxAttentionView* q_out,
+                                  const SxAttentionView* k_out, sxcuda_stream_t stream);
+
+typedef struct SxRotaryGrads {
+    SxAttentionView v_q_out, v_k_out; /* gradients of the outputs */
+    SxAttentionView v_q, v_k;         /* written */
+    void* v_q_weight;                 /* [head_dim], param_dtype, or NULL; NULL without norm */
+    void* v_k_weight;
+} SxRotaryGrads;
+
+/* q and k (of the forward's inputs) are read only with norm. Positions get no gradient. Workspace query
+ * protocol. The weights' sums are taken in a fixed order. */
+int32_t sxcuda_qk_norm_rotary_bwd(const SxRotaryInputs* in, const SxRotaryGrads* grads, void* workspace,
+                                  size_t* workspace_bytes, sxcuda_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -252,6 +252,71 @@ void validate_attention(const SxAttentionInputs* in, const char* w) {
     validate_view(in->v, *in, in->kv_len, in->kv_heads, false, w, "v");
 }
 
+void validate_matrix(const void* p, int64_t stride, int64_t rows, int64_t cols, int32_t dtype, const char* w, const char* what) {
+    if (rows == 0) return;
+    validate_pointer(p, dtype, w, what);
+    if (rows > 1 && stride < cols) throw_invalid(w, std::string(what) + ": rows overlap (stride < columns)");
+}
+void validate_linear(const SxLinearInputs* in, const char* w) {
+    if (!in) throw_invalid(w, "null inputs");
+    validate_dtype(in->dtype, w, "dtype");
+    validate_dtype(in->bias_dtype, w, "bias_dtype");
+    if (in->activation < SXCUDA_ACT_NONE || in->activation > SXCUDA_ACT_GELU_TANH) throw_invalid(w, "unknown activation");
+    if (in->rows < 0 || in->rows > INT32_MAX / 2) throw_invalid(w, "rows must be 0..2^30 - 1");
+    if (in->in_features < 1 || in->in_features > INT32_MAX / 2 || in->out_features < 1 || in->out_features > INT32_MAX / 2)
+        throw_invalid(w, "in_features and out_features must be 1..2^30 - 1");
+    validate_matrix(in->x, in->x_stride, in->rows, in->in_features, in->dtype, w, "x");
+    validate_matrix(in->weight, in->weight_stride, in->out_features, in->in_features, in->dtype, w, "weight");
+    if (in->bias) validate_pointer(in->bias, in->bias_dtype, w, "bias");
+}
+
+void validate_head_view(const SxAttentionView& v, const SxRotaryInputs& in, int32_t heads, bool written, const char* w, const char* what) {
+    if (in.batch == 0 || in.tokens == 0 || heads == 0) return;
+    validate_pointer(v.data, in.dtype, w, what);
+    if (v.batch_stride < 0 || v.token_stride < 0 || v.head_stride < 0)
+        throw_invalid(w, std::string(what) + ": negative stride");
+    if (written && ((in.batch > 1 && v.batch_stride == 0) || (in.tokens > 1 && v.token_stride < in.head_dim) ||
+                    (heads > 1 && v.head_stride < in.head_dim)))
+        throw_invalid(w, std::string(what) + ": rows that are written overlap");
+}
+void validate_rotary(const SxRotaryInputs* in, bool reads, const char* w) {
+    if (!in) throw_invalid(w, "null inputs");
+    validate_dtype(in->dtype, w, "dtype");
+    validate_dtype(in->param_dtype, w, "param_dtype");
+    if (in->pos_dtype < SXCUDA_POS_F32 || in->pos_dtype > SXCUDA_POS_I64) throw_invalid(w, "unknown pos_dtype");
+    if (in->pairs < SXCUDA_PAIRS_AXIS || in->pairs > SXCUDA_PAIRS_NEIGHBOURS) throw_invalid(w, "unknown pairs");
+    if (in->batch < 0 || in->tokens < 0 || in->batch > INT32_MAX / 2 || in->tokens > INT32_MAX / 2)
+        throw_invalid(w, "batch and tokens must be 0..2^30 - 1");
+    if (in->q_heads < 1 || in->q_heads > 65535 || in->k_heads < 0 || in->k_heads > 65535)
+        throw_invalid(w, "q_heads must be 1..65535 and k_heads 0..65535");
+    if (in->head_dim < 1 || in->head_dim > 256) throw_invalid(w, "head_dim must be 1..256");
+    if (in->axes < 1 || in->axes > 4) throw_invalid(w, "there must be 1..4 axes");
+    int64_t rotated = 0;
+    for (int i = 0; i < in->axes; ++i) {
+        if (in->axis_dims[i] < 0 || in->axis_dims[i] % 2 != 0) throw_invalid(w, "axis_dims must be even and not negative");
+        rotated += in->axis_dims[i];
+    }
+    if (rotated > in->head_dim) throw_invalid(w, "the axes have more values than a head");
+    if (rotated && !in->freqs) throw_invalid(w, "null freqs");
+    for (int64_t i = 0; i < rotated / 2; ++i)
+        if (!std::isfinite(in->freqs[i])) throw_invalid(w, "freqs must be finite");
+    if (!(in->eps >= 0.0f) || !std::isfinite(in->eps)) throw_invalid(w, "eps must be finite and not negative");
+    if (in->norm != 0 && in->norm != 1) throw_invalid(w, "norm must be 0 or 1");
+    if (!in->norm && (in->q_weight || in->k_weight)) throw_invalid(w, "weights need norm");
+    if (in->q_weight) validate_pointer(in->q_weight, in->param_dtype, w, "q_weight");
+    if (in->k_weight) validate_pointer(in->k_weight, in->param_dtype, w, "k_weight");
+    if (in->batch && in->tokens) {
+        if (!in->positions) throw_invalid(w, "null positions");
+        const uintptr_t size = in->pos_dtype == SXCUDA_POS_I64 ? 8 : 4;
+        if (reinterpret_cast<uintptr_t>(in->positions) % size != 0) throw_invalid(w, "positions is not aligned to its element");
+        if (in->pos_batch_stride < 0 || in->pos_token_stride < 0 || in->pos_axis_stride < 0)
+            throw_invalid(w, "positions: negative stride");
+    }
+    if (!reads) return;
+    validate_head_view(in->q, *in, in->q_heads, false, w, "q");
+    validate_head_view(in->k, *in, in->k_heads, false, w, "k");
+}
+
 void validate_raster(const SxRasterizeFwdInputs* in, const char* w) {
     if (!in) throw_invalid(w, "null inputs");
     if (!in->means2d || !in->conics || !in->colors || !in->opacities || !in->isect_offsets)
@@ -1129,6 +1194,79 @@ int32_t sxcuda_attention_status(uint32_t* status) {
     return guarded([&] {
         if (!status) throw_invalid("attention_status", "null status");
         *status = attention_status();
+    });
+}
+
+int32_t sxcuda_linear_fwd(const SxLinearInputs* in, const SxLinearOutputs* out, void* ws, size_t* ws_bytes, sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "linear_fwd";
+        validate_linear(in, w);
+        if (workspace_query(ws, ws_bytes, linear_fwd_workspace(*in), w)) return;
+        if (!out) throw_invalid(w, "null outputs");
+        validate_matrix(out->y, out->y_stride, in->rows, in->out_features, in->dtype, w, "y");
+        if (out->pre) validate_matrix(out->pre, out->pre_stride, in->rows, in->out_features, in->dtype, w, "pre");
+        if (out->residual) validate_matrix(out->residual, out->residual_stride, in->rows, in->out_features, in->dtype, w, "residual");
+        if (*ws_bytes && reinterpret_cast<uintptr_t>(ws) % 16 != 0) throw_invalid(w, "workspace must be 16-byte aligned");
+        launch_linear_fwd(*in, *out, ws, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_linear_bwd(const SxLinearInputs* in, const SxLinearGradsIn* g, const SxLinearGrads* out, void* ws,
+                          size_t* ws_bytes, sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "linear_bwd";
+        validate_linear(in, w);
+        if (!g || !out) throw_invalid(w, "null gradients");
+        validate_matrix(g->v_y, g->v_y_stride, in->rows, in->out_features, in->dtype, w, "v_y");
+        if ((in->activation == SXCUDA_ACT_NONE) != (g->pre == nullptr) && in->rows)
+            throw_invalid(w, "pre is needed with an activation, and only then");
+        if (g->pre) validate_matrix(g->pre, g->pre_stride, in->rows, in->out_features, in->dtype, w, "pre");
+        if (out->v_x) validate_matrix(out->v_x, out->v_x_stride, in->rows, in->in_features, in->dtype, w, "v_x");
+        if (out->v_weight) validate_matrix(out->v_weight, out->v_weight_stride, in->out_features, in->in_features, in->dtype, w, "v_weight");
+        if (out->v_bias) validate_pointer(out->v_bias, in->bias_dtype, w, "v_bias");
+        if (workspace_query(ws, ws_bytes, linear_bwd_workspace(*in, *g, *out), w)) return;
+        if (*ws_bytes && reinterpret_cast<uintptr_t>(ws) % 16 != 0) throw_invalid(w, "workspace must be 16-byte aligned");
+        launch_linear_bwd(*in, *g, *out, ws, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_linear_status(uint32_t* status) {
+    return guarded([&] {
+        if (!status) throw_invalid("linear_status", "null status");
+        *status = linear_status();
+    });
+}
+
+int32_t sxcuda_qk_norm_rotary_fwd(const SxRotaryInputs* in, const SxAttentionView* q_out, const SxAttentionView* k_out,
+                                  sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "qk_norm_rotary_fwd";
+        validate_rotary(in, true, w);
+        if (!q_out || (in->k_heads && !k_out)) throw_invalid(w, "null outputs");
+        validate_head_view(*q_out, *in, in->q_heads, true, w, "q_out");
+        const SxAttentionView none{};
+        if (in->k_heads) validate_head_view(*k_out, *in, in->k_heads, true, w, "k_out");
+        launch_qk_norm_rotary_fwd(*in, *q_out, in->k_heads ? *k_out : none, as_stream(stream));
+    });
+}
+
+int32_t sxcuda_qk_norm_rotary_bwd(const SxRotaryInputs* in, const SxRotaryGrads* g, void* ws, size_t* ws_bytes,
+                                  sxcuda_stream_t stream) {
+    return guarded([&] {
+        const char* w = "qk_norm_rotary_bwd";
+        validate_rotary(in, in && in->norm, w);
+        if (workspace_query(ws, ws_bytes, qk_norm_rotary_bwd_workspace(*in), w)) return;
+        if (!g) throw_invalid(w, "null gradients");
+        validate_head_view(g->v_q_out, *in, in->q_heads, false, w, "v_q_out");
+        validate_head_view(g->v_q, *in, in->q_heads, true, w, "v_q");
+        validate_head_view(g->v_k_out, *in, in->k_heads, false, w, "v_k_out");
+        validate_head_view(g->v_k, *in, in->k_heads, true, w, "v_k");
+        if (!in->norm && (g->v_q_weight || g->v_k_weight)) throw_invalid(w, "weights need norm");
+        if (!in->k_heads && g->v_k_weight) throw_invalid(w, "v_k_weight needs k");
+        if (g->v_q_weight) validate_pointer(g->v_q_weight, in->param_dtype, w, "v_q_weight");
+        if (g->v_k_weight) validate_pointer(g->v_k_weight, in->param_dtype, w, "v_k_weight");
+        if (*ws_bytes && reinterpret_cast<uintptr_t>(ws) % 16 != 0) throw_invalid(w, "workspace must be 16-byte aligned");
+        launch_qk_norm_rotary_bwd(*in, *g, ws, as_stream(stream));
     });
 }
 

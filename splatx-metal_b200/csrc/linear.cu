@@ -1,0 +1,374 @@
+// linear.cu — y = act(x W^T + b) + residual and its gradients: products on the multiply-add pipes, the sums
+// over parts of a tile, the gradient of the activation, and the host's part.
+//
+//   z = x W^T + b;  y = act(z) + r;   v_z = v_y act'(z);  v_x = v_z W;  v_W = v_z^T x;  v_b = sum of v_z's rows.
+// Three products of one kind, C = A B^T over an axis K along which either operand's rows or columns run.
+#include <algorithm>
+
+#include "sx_linear.h"
+
+namespace sx {
+namespace {
+
+// ---- products on the multiply-add pipes ----
+// A CTA takes 128 x 128 values of C, a thread 8 x 8 of them as 2 x 2 blocks of 4 x 4; 16 of K at a time go
+// through shared memory, the next 16 are on their way in registers meanwhile.
+constexpr int kTile = 128, kDepth = 16, kThreads = 256;
+constexpr int kPitch = kTile + 4;
+
+// The thread's 8 values of a 128 x 16 block of an operand: along K for row `tid / 2`, or along the rows for
+// K value `tid / 16`.
+template <typename T>
+struct Staged {
+    float x[8];
+    __device__ void load(const LinearOperand& o, int64_t row0, int64_t rows, int64_t k0, int64_t k_end, bool wide) {
+        const bool along_k = o.k_stride == 1;
+        const int t = threadIdx.x;
+        const int64_t row = row0 + (along_k ? t / 2 : t % 16 * 8), k = k0 + (along_k ? t % 2 * 8 : t / 16);
+        const T* p = static_cast<const T*>(o.data) + row * o.row_stride + k * o.k_stride;
+        const int64_t left = (along_k ? row < rows : k < k_end) ? (along_k ? k_end - k : rows - row) : 0;
+        constexpr int N = sizeof(T) == 4 ? 4 : 8;
+        if (wide && left >= 8) {
+#pragma unroll
+            for (int i = 0; i < 8; i += N) {
+                const auto v = *reinterpret_cast<const Pack<T, N>*>(p + i);
+#pragma unroll
+                for (int j = 0; j < N; ++j) x[i + j] = to_f32(v.v[j]);
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = i < left ? to_f32(p[i]) : 0.f;
+    }
+    __device__ void store(const LinearOperand& o, float (&to)[kDepth][kPitch]) const {
+        const int t = threadIdx.x;
+        if (o.k_stride == 1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) to[t % 2 * 8 + i][t / 2] = x[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<float4*>(&to[t / 16][t % 16 * 8 + i]) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        }
+    }
+};
+
+// The epilogue for `n` (at most N) consecutive columns of a row.
+template <typename T, int N>
+__device__ __forceinline__ void linear_finish(const LinearProduct& p, int64_t row, int64_t col, float (&z)[N], int n) {
+    T pre[N], y[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i >= n) break;
+        z[i] += linear_param(p.bias, p.bias_dtype, col + i);
+        pre[i] = from_f32<T>(z[i]);
+        float v = linear_act(p.act, z[i]);
+        if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[row * p.residual_stride + col + i]);
+        y[i] = from_f32<T>(v);
+    }
+    T* to = static_cast<T*>(p.y) + row * p.y_stride + col;
+    T* keep = static_cast<T*>(p.pre) + row * p.pre_stride + col;
+    const auto fits = [](const T* a) { return reinterpret_cast<uintptr_t>(a) % (N * sizeof(T)) == 0; };
+    if (n == N && fits(to) && (!p.pre || fits(keep))) {
+        *reinterpret_cast<Pack<T, N>*>(to) = *reinterpret_cast<Pack<T, N>*>(y);
+        if (p.pre) *reinterpret_cast<Pack<T, N>*>(keep) = *reinterpret_cast<Pack<T, N>*>(pre);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i >= n) break;
+        to[i] = y[i];
+        if (p.pre) keep[i] = pre[i];
+    }
+}
+
+// Where a part of a tile lies: [columns / 8][rows][8].
+__device__ __forceinline__ float* part_at(const LinearProduct& p, int64_t slot, int row, int col) {
+    return p.parts + slot * p.plan.slot_values() + (static_cast<int64_t>(col / 8) * p.plan.tile_m + row) * 8 + col % 8;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant__ LinearProduct p, bool a_wide, bool b_wide) {
+    __shared__ float as[2][kDepth][kPitch], bs[2][kDepth][kPitch];
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    LinearWalk walk(p.plan, blockIdx.x);
+    LinearPiece piece;
+    while (walk.next(p.plan, piece)) {
+        const LinearTile tile = linear_tile(p.plan, piece.tile);
+        const int64_t m0 = tile.m * kTile, n0 = tile.n * kTile, end = min(static_cast<int64_t>(piece.k1) * kDepth, p.k);
+        float c[8][8] = {};
+        Staged<T> a, b;
+        a.load(p.a, m0, p.m, static_cast<int64_t>(piece.k0) * kDepth, end, a_wide);
+        b.load(p.b, n0, p.n, static_cast<int64_t>(piece.k0) * kDepth, end, b_wide);
+        for (int k = piece.k0; k < piece.k1; ++k) {
+            const int at = k & 1;
+            a.store(p.a, as[at]);
+            b.store(p.b, bs[at]);
+            __syncthreads();
+            if (k + 1 < piece.k1) {
+                a.load(p.a, m0, p.m, static_cast<int64_t>(k + 1) * kDepth, end, a_wide);
+                b.load(p.b, n0, p.n, static_cast<int64_t>(k + 1) * kDepth, end, b_wide);
+            }
+#pragma unroll
+            for (int d = 0; d < kDepth; ++d) {
+                float x[8], y[8];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    *reinterpret_cast<float4*>(x + 4 * h) = *reinterpret_cast<const float4*>(&as[at][d][ty * 4 + h * 64]);
+                    *reinterpret_cast<float4*>(y + 4 * h) = *reinterpret_cast<const float4*>(&bs[at][d][tx * 4 + h * 64]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) c[i][j] = fmaf(x[i], y[j], c[i][j]);
+            }
+        }
+        __syncthreads();  // the next piece's first stores
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int row = ty * 4 + i % 4 + i / 4 * 64, col = tx * 4 + h * 64;
+                const int64_t n = min(p.n - n0 - col, static_cast<int64_t>(4));
+                if (m0 + row >= p.m || n <= 0) continue;
+                float z[4] = {c[i][4 * h], c[i][4 * h + 1], c[i][4 * h + 2], c[i][4 * h + 3]};
+                if (piece.slot < 0) linear_finish<T, 4>(p, m0 + row, n0 + col, z, static_cast<int>(n));
+                else *reinterpret_cast<float4*>(part_at(p, piece.slot, row, col)) = make_float4(z[0], z[1], z[2], z[3]);
+            }
+    }
+}
+
+// Adds the parts of the tiles that cuts go through, in the order of K, and finishes them. A thread has 8
+// columns of a row; blockIdx.y counts the tiles behind the whole ones.
+template <typename T>
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinearProduct p) {
+    const LinearPlan& plan = p.plan;
+    const int64_t t = blockIdx.y;
+    const int64_t w0 = plan.worker_of(t * plan.kblocks), w1 = plan.worker_of((t + 1) * plan.kblocks - 1);
+    if (w0 == w1) return;  // no cut goes through it
+    const LinearTile tile = linear_tile(plan, plan.whole + t);
+    const int64_t m0 = tile.m * plan.tile_m, n0 = tile.n * plan.tile_n;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(plan.tile_m), p.m - m0)), groups = plan.tile_n / 8;
+    const int i = blockIdx.x * 256 + threadIdx.x, row = i / groups, col = i % groups * 8;
+    const int64_t n = min(p.n - n0 - col, static_cast<int64_t>(8));
+    if (row >= rows || n <= 0) return;
+    float z[8] = {};
+    for (int64_t w = w0; w <= w1; ++w) {
+        const float4* part = reinterpret_cast<const float4*>(part_at(p, 2 * w + (w == w0), row, col));
+        const float4 x = part[0], y = part[1];
+        z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w;
+        z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
+    }
+    linear_finish<T, 8>(p, m0 + row, n0 + col, z, static_cast<int>(n));
+}
+
+bool linear_wide(const LinearOperand& o, int64_t size) {
+    const int64_t other = o.k_stride == 1 ? o.row_stride : o.k_stride;
+    return reinterpret_cast<uintptr_t>(o.data) % 16 == 0 && other * size % 16 == 0;
+}
+
+// Whole tiles, but for those of the last turns where workers would go without: the cut costs a launch and
+// its parts' way through memory, and a piece has at least `least` K blocks.
+LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, int depth, int64_t workers, int64_t least) {
+    LinearPlan p;
+    p.tile_m = tile_m, p.tile_n = tile_n;
+    p.tiles_m = (m + tile_m - 1) / tile_m, p.tiles_n = (n + tile_n - 1) / tile_n;
+    p.kblocks = (k + depth - 1) / depth;
+    const int64_t tiles = p.tiles(), turns = tiles / workers;
+    p.workers = static_cast<int32_t>(std::min(tiles, workers));
+    p.whole = tiles;
+    if (tiles % workers == 0) return p;
+    const int64_t whole = turns > 0 ? (turns - 1) * workers : 0, units = (tiles - whole) * p.kblocks;
+    const int64_t used = std::min(workers, std::max<int64_t>(units / least, 1));
+    const int64_t now = p.kblocks * ((tiles - whole + workers - 1) / workers), then = (units + used - 1) / used;
+    if (now - then < 2 * least) return p;
+    p.whole = whole;
+    p.units = units;
+    p.workers = static_cast<int32_t>(used);
+    return p;
+}
+
+constexpr int kPerSm = 2;
+
+LinearPlan product_plan(int64_t m, int64_t n, int64_t k) {
+    return linear_plan(m, n, k, kTile, kTile, kDepth, static_cast<int64_t>(sm_count()) * kPerSm, 8);
+}
+
+void launch_product(const LinearProduct& p, cudaStream_t s) {
+    by_dtype(p.dtype, [&](auto t) {
+        using T = decltype(t);
+        const auto kernel = linear_kernel<T>;
+        SX_LAUNCH(kernel, static_cast<unsigned>(p.plan.workers), kThreads, 0, s, p, linear_wide(p.a, sizeof(T)), linear_wide(p.b, sizeof(T)));
+        if (!p.plan.cut()) return;
+        const auto join = linear_join_kernel<T>;
+        const int64_t rows = std::min<int64_t>(p.m, p.plan.tile_m);
+        SX_LAUNCH(join, dim3(blocks_for(rows * (p.plan.tile_n / 8), 256), static_cast<unsigned>(p.plan.tiles() - p.plan.whole)), 256, 0, s, p);
+    });
+}
+
+// ---- v_z = v_y act'(pre), and the sum of its rows ----
+// A CTA has 32 V columns (a warp's lanes V each) and a slice of the rows, which its warps take in turn.
+constexpr int kSlopeWarps = 8;
+struct SlopeArgs {
+    const void* v_y;
+    const void* pre;
+    void* v_z;    // NULL: v_y itself
+    float* sums;  // [slices, cols] or NULL
+    int64_t v_y_stride, pre_stride, v_z_stride, rows, cols, slice;
+    int32_t act;
+};
+template <typename T, int V>
+__global__ void __launch_bounds__(kSlopeWarps * 32) linear_slope_kernel(const SlopeArgs a) {
+    __shared__ float part[kSlopeWarps][32 * V];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * V;
+    const int64_t r0 = blockIdx.y * a.slice, r1 = min(r0 + a.slice, a.rows);
+    float sum[V] = {};
+    if (c < a.cols)
+        for (int64_t r = r0 + warp; r < r1; r += kSlopeWarps) {
+            const auto g = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.v_y) + r * a.v_y_stride + c);
+            Pack<T, V> z{}, to;
+            if (a.pre) z = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.pre) + r * a.pre_stride + c);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float x = to_f32(g.v[i]);
+                if (a.pre) x *= linear_slope(a.act, to_f32(z.v[i]));
+                sum[i] += x;
+                to.v[i] = from_f32<T>(x);
+            }
+            if (a.v_z) *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.v_z) + r * a.v_z_stride + c) = to;
+        }
+    if (!a.sums) return;
+#pragma unroll
+    for (int i = 0; i < V; ++i) part[warp][lane * V + i] = sum[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * V; i += kSlopeWarps * 32) {
+        const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 * V + i;
+        float x = 0.f;
+        for (int w = 0; w < kSlopeWarps; ++w) x += part[w][i];
+        if (col < a.cols) a.sums[blockIdx.y * a.cols + col] = x;
+    }
+}
+__global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int64_t slices, int64_t cols, void* v_bias, int32_t dtype) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (c >= cols) return;
+    float x = 0.f;
+    for (int64_t i = 0; i < slices; ++i) x += sums[i * cols + c];
+    if (dtype == SXCUDA_F32) static_cast<float*>(v_bias)[c] = x;
+    else if (dtype == SXCUDA_F16) static_cast<__half*>(v_bias)[c] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16*>(v_bias)[c] = __float2bfloat16_rn(x);
+}
+
+struct SlopePlan {
+    int v;
+    int64_t strips, slices, slice;
+};
+SlopePlan slope_plan(const SxLinearInputs& in, const SxLinearGradsIn& g) {
+    const int64_t size = dtype_bytes(in.dtype), most = 16 / size;
+    const auto wide = [&](const void* p, int64_t stride) {
+        return reinterpret_cast<uintptr_t>(p) % 16 == 0 && (in.rows <= 1 || stride % most == 0);
+    };
+    SlopePlan p;
+    p.v = in.out_features % most == 0 && wide(g.v_y, g.v_y_stride) && wide(g.pre, g.pre_stride) ? static_cast<int>(most) : 1;
+    p.strips = (in.out_features + 32 * p.v - 1) / (32 * p.v);
+    const int64_t want = std::max<int64_t>(static_cast<int64_t>(sm_count()) * 8 / p.strips, 1);
+    p.slice = std::max<int64_t>((in.rows + want - 1) / want, 4 * kSlopeWarps);
+    p.slices = (in.rows + p.slice - 1) / p.slice;
+    return p;
+}
+
+size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
+
+// The backward's workspace: v_z (where it is not v_y), the bias' sums, the products' parts.
+struct BwdSpace {
+    size_t v_z = 0, sums = 0, parts = 0, bytes = 0;
+};
+BwdSpace bwd_space(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out) {
+    BwdSpace w;
+    if (in.rows == 0) return w;
+    w.v_z = 0;
+    size_t at = g.pre ? aligned(static_cast<size_t>(in.rows) * in.out_features * dtype_bytes(in.dtype)) : 0;
+    w.sums = at;
+    if (out.v_bias) at += aligned(static_cast<size_t>(slope_plan(in, g).slices) * in.out_features * 4);
+    w.parts = at;
+    size_t parts = 0;
+    if (out.v_x) parts = std::max(parts, product_plan(in.rows, in.in_features, in.out_features).workspace());
+    if (out.v_weight) parts = std::max(parts, product_plan(in.out_features, in.in_features, in.rows).workspace());
+    w.bytes = at + parts;
+    return w;
+}
+
+}  // namespace
+
+uint32_t linear_status() { return 0; }
+
+size_t linear_fwd_workspace(const SxLinearInputs& in) {
+    return in.rows ? product_plan(in.rows, in.out_features, in.in_features).workspace() : 0;
+}
+
+void launch_linear_fwd(const SxLinearInputs& in, const SxLinearOutputs& out, void* ws, cudaStream_t s) {
+    if (in.rows == 0) return;
+    LinearProduct p{};
+    p.a = {in.x, in.x_stride, 1};
+    p.b = {in.weight, in.weight_stride, 1};
+    p.m = in.rows, p.n = in.out_features, p.k = in.in_features;
+    p.dtype = in.dtype, p.bias_dtype = in.bias_dtype, p.act = in.activation;
+    p.bias = in.bias;
+    p.residual = out.residual, p.residual_stride = out.residual_stride;
+    p.y = out.y, p.y_stride = out.y_stride;
+    p.pre = out.pre, p.pre_stride = out.pre_stride;
+    p.parts = static_cast<float*>(ws);
+    p.plan = product_plan(p.m, p.n, p.k);
+    launch_product(p, s);
+}
+
+size_t linear_bwd_workspace(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out) {
+    return bwd_space(in, g, out).bytes;
+}
+
+void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out, void* ws, cudaStream_t s) {
+    const int64_t size = dtype_bytes(in.dtype);
+    if (in.rows == 0) {
+        if (out.v_weight)
+            cuda_check(cudaMemset2DAsync(out.v_weight, out.v_weight_stride * size, 0, in.in_features * size, in.out_features, s), "linear_bwd");
+        if (out.v_bias) cuda_check(cudaMemsetAsync(out.v_bias, 0, in.out_features * dtype_bytes(in.bias_dtype), s), "linear_bwd");
+        return;
+    }
+    const BwdSpace space = bwd_space(in, g, out);
+    uint8_t* at = static_cast<uint8_t*>(ws);
+    LinearOperand v_z{g.v_y, g.v_y_stride, 1};  // [rows, out_features]
+    if (g.pre || out.v_bias) {
+        const SlopePlan plan = slope_plan(in, g);
+        SlopeArgs a{g.v_y, g.pre, nullptr, nullptr, g.v_y_stride, g.pre_stride, in.out_features, in.rows, in.out_features, plan.slice, in.activation};
+        if (g.pre) v_z = {a.v_z = at + space.v_z, in.out_features, 1};
+        if (out.v_bias) a.sums = reinterpret_cast<float*>(at + space.sums);
+        by_dtype(in.dtype, [&](auto t) {
+            using T = decltype(t);
+            const auto kernel = plan.v == 1 ? linear_slope_kernel<T, 1> : linear_slope_kernel<T, 16 / sizeof(T)>;
+            SX_LAUNCH(kernel, dim3(static_cast<unsigned>(plan.strips), static_cast<unsigned>(plan.slices)), kSlopeWarps * 32, 0, s, a);
+        });
+        if (out.v_bias)
+            SX_LAUNCH(linear_bias_kernel, blocks_for(in.out_features, 256), 256, 0, s, a.sums, plan.slices, in.out_features, out.v_bias, in.bias_dtype);
+    }
+    LinearProduct p{};
+    p.dtype = in.dtype;
+    p.parts = reinterpret_cast<float*>(at + space.parts);
+    if (out.v_x) {
+        p.a = v_z;
+        p.b = {in.weight, 1, in.weight_stride};
+        p.m = in.rows, p.n = in.in_features, p.k = in.out_features;
+        p.y = out.v_x, p.y_stride = out.v_x_stride;
+        p.plan = product_plan(p.m, p.n, p.k);
+        launch_product(p, s);
+    }
+    if (out.v_weight) {
+        p.a = {v_z.data, 1, v_z.row_stride};
+        p.b = {in.x, 1, in.x_stride};
+        p.m = in.out_features, p.n = in.in_features, p.k = in.rows;
+        p.y = out.v_weight, p.y_stride = out.v_weight_stride;
+        p.plan = product_plan(p.m, p.n, p.k);
+        launch_product(p, s);
+    }
+}
+
+}  // namespace sx

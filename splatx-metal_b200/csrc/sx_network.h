@@ -1,5 +1,5 @@
 // sx_network.h — launchers of the network operators (layer norm, AdamW over many tensors,
-// attention) and the element-type helpers they share. Every launcher enqueues on `stream` and
+// attention, linear layers, norm and rotation of queries and keys) and the element-type helpers they share. Every launcher enqueues on `stream` and
 // throws sx::RuntimeError on a launch failure; arguments are validated by the C entry points.
 #pragma once
 
@@ -64,5 +64,18 @@ void launch_attention_fwd(const SxAttentionInputs& in, const SxAttentionView& ou
 size_t attention_bwd_workspace(const SxAttentionInputs& in);
 void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn& g,
                           const SxAttentionGrads& out, void* ws, cudaStream_t s);
+
+// The linear kernels' status word of the current device, read and cleared (synchronises).
+uint32_t linear_status();
+size_t linear_fwd_workspace(const SxLinearInputs& in);
+void launch_linear_fwd(const SxLinearInputs& in, const SxLinearOutputs& out, void* ws, cudaStream_t s);
+size_t linear_bwd_workspace(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out);
+void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out, void* ws,
+                       cudaStream_t s);
+
+void launch_qk_norm_rotary_fwd(const SxRotaryInputs& in, const SxAttentionView& q_out, const SxAttentionView& k_out,
+                               cudaStream_t s);
+size_t qk_norm_rotary_bwd_workspace(const SxRotaryInputs& in);
+void launch_qk_norm_rotary_bwd(const SxRotaryInputs& in, const SxRotaryGrads& g, void* ws, cudaStream_t s);
 
 }  // namespace sx

@@ -244,6 +244,43 @@ class SxAttentionGrads(C.Structure):
     _fields_ = [("v_q", SxAttentionView), ("v_k", SxAttentionView), ("v_v", SxAttentionView)]
 
 
+class SxLinearInputs(C.Structure):
+    _fields_ = [("x", vp), ("weight", vp), ("bias", vp), ("rows", C.c_int64),
+                ("in_features", C.c_int64), ("out_features", C.c_int64), ("x_stride", C.c_int64),
+                ("weight_stride", C.c_int64), ("dtype", C.c_int32), ("bias_dtype", C.c_int32),
+                ("activation", C.c_int32)]
+
+
+class SxLinearOutputs(C.Structure):
+    _fields_ = [("residual", vp), ("residual_stride", C.c_int64), ("y", vp), ("y_stride", C.c_int64),
+                ("pre", vp), ("pre_stride", C.c_int64)]
+
+
+class SxLinearGradsIn(C.Structure):
+    _fields_ = [("v_y", vp), ("v_y_stride", C.c_int64), ("pre", vp), ("pre_stride", C.c_int64)]
+
+
+class SxLinearGrads(C.Structure):
+    _fields_ = [("v_x", vp), ("v_x_stride", C.c_int64), ("v_weight", vp),
+                ("v_weight_stride", C.c_int64), ("v_bias", vp)]
+
+
+class SxRotaryInputs(C.Structure):
+    _fields_ = [("q", SxAttentionView), ("k", SxAttentionView), ("positions", vp),
+                ("pos_batch_stride", C.c_int64), ("pos_token_stride", C.c_int64),
+                ("pos_axis_stride", C.c_int64), ("freqs", vp), ("q_weight", vp), ("k_weight", vp),
+                ("batch", C.c_int64), ("tokens", C.c_int64), ("q_heads", C.c_int32),
+                ("k_heads", C.c_int32), ("head_dim", C.c_int32), ("axes", C.c_int32),
+                ("axis_dims", C.c_int32 * 4), ("pairs", C.c_int32), ("dtype", C.c_int32),
+                ("param_dtype", C.c_int32), ("pos_dtype", C.c_int32), ("norm", C.c_int32),
+                ("eps", C.c_float)]
+
+
+class SxRotaryGrads(C.Structure):
+    _fields_ = [("v_q_out", SxAttentionView), ("v_k_out", SxAttentionView), ("v_q", SxAttentionView),
+                ("v_k", SxAttentionView), ("v_q_weight", vp), ("v_k_weight", vp)]
+
+
 P = C.POINTER
 _SIGNATURES = {
     "sxcuda_last_error": (C.c_char_p, []),
@@ -348,6 +385,13 @@ _SIGNATURES = {
     "sxcuda_attention_bwd": (C.c_int32, [P(SxAttentionInputs), P(SxAttentionGradsIn),
                                          P(SxAttentionGrads), vp, c_size_p, vp]),
     "sxcuda_attention_status": (C.c_int32, [c_uint32_p]),
+    "sxcuda_linear_fwd": (C.c_int32, [P(SxLinearInputs), P(SxLinearOutputs), vp, c_size_p, vp]),
+    "sxcuda_linear_bwd": (C.c_int32, [P(SxLinearInputs), P(SxLinearGradsIn), P(SxLinearGrads), vp,
+                                      c_size_p, vp]),
+    "sxcuda_linear_status": (C.c_int32, [c_uint32_p]),
+    "sxcuda_qk_norm_rotary_fwd": (C.c_int32, [P(SxRotaryInputs), P(SxAttentionView),
+                                              P(SxAttentionView), vp]),
+    "sxcuda_qk_norm_rotary_bwd": (C.c_int32, [P(SxRotaryInputs), P(SxRotaryGrads), vp, c_size_p, vp]),
 }
 
 _lib = None

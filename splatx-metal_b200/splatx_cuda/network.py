@@ -1,4 +1,5 @@
-"""Operators for training a network beside the splats: attention, layer norm, AdamW.
+"""Operators for training a network beside the splats: attention, the norm and rotation of its queries
+and keys, linear layers, layer norm, AdamW.
 
 The reference has no counterpart: its trainer updates the Gaussians themselves. A network that
 predicts, refines or conditions them (tokens of splats or of image patches) trains with these.
@@ -10,10 +11,13 @@ not synchronise. Contract violations raise ``ValueError``, device failures ``Run
     v_q, v_k, v_v = attention_bwd(v_out, q, k, v, out, lse, causal=True)
     y, mean, rstd = layer_norm_fwd(x, weight, bias)
     v_x, v_weight, v_bias = layer_norm_bwd(v_y, x, weight, mean, rstd)
+    y, pre = linear_fwd(x, weight, bias, activation="gelu", keep=True)
+    v_x, v_weight, v_bias = linear_bwd(v_y, x, weight, bias, pre, activation="gelu")
+    q, k = qk_norm_rotary_fwd(q, k, positions, axes=(32, 48, 48))  # [batch, tokens, axes]
     AdamW(params, lr=1e-3, state_bits=8).step()              # params with .grad, or step(grads)
 
-``attention`` and ``layer_norm`` are the same with torch's autograd (first derivatives; a second one
-raises ``RuntimeError``).
+``attention``, ``linear``, ``qk_norm_rotary`` and ``layer_norm`` are the same with torch's autograd
+(first derivatives; a second one raises ``RuntimeError``).
 """
 from __future__ import annotations
 
@@ -285,6 +289,275 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
     """layer_norm_fwd's y, differentiable in x, weight and bias."""
     return _LayerNorm.apply(x, weight, bias, float(eps))
+
+
+# ---------------------------------------------------------------- linear layers
+
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+
+def linear_status() -> int:
+    """Status bits the linear kernels of the current device have set since the last call (0: all is
+    well; 1: a bounded wait inside a kernel ran out and its outputs are invalid). Synchronises."""
+    st = C.c_uint32(0)
+    check(_nat.lib().sxcuda_linear_status(C.byref(st)))
+    return int(st.value)
+
+
+def _linear_inputs(what, x, weight, bias, activation):
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be one of {list(_ACTIVATIONS)}, got {activation!r}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"{what}: x [..., in] and weight [out, in] needed, got {tuple(x.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if weight.dtype != x.dtype:
+        raise ValueError(f"{what}: x and weight must have one dtype, got {x.dtype} and {weight.dtype}")
+    device, code = x.device, _dtype(x, what)
+    n, cols = weight.shape
+    _on(device, what, weight, bias)
+    if bias is not None and (bias.shape != (n,) or not bias.is_contiguous()):
+        raise ValueError(f"{what}: bias must be a contiguous tensor of [{n}]")
+    flat, rows, x_stride = _rows(x, cols)
+    w, _, w_stride = _rows(weight, cols)
+    ins = _nat.SxLinearInputs(
+        flat.data_ptr(), w.data_ptr(), None if bias is None else bias.data_ptr(), rows, cols, n, x_stride,
+        w_stride, code, 0 if bias is None else _dtype(bias, what), _ACTIVATIONS[activation])
+    return flat, w, ins, device
+
+
+def linear_fwd(x, weight, bias=None, *, activation=None, residual=None, keep=False):
+    """act(x weight^T + bias) + residual: (y [..., out], pre).
+
+    x: [..., in]; weight: [out, in] of x's dtype (float32, float16 or bfloat16); bias: [out] of any of
+    them; residual: like y. activation: None, "relu", "silu", "gelu" (with the normal distribution
+    function) or "gelu_tanh" (its tanh form). Sums, bias, activation and residual are taken in 32 bits
+    and rounded once. pre is x weight^T + bias rounded to x's dtype, which linear_bwd needs where there
+    is an activation; None unless keep. 16-bit types run on the tensor cores."""
+    what = "linear_fwd"
+    flat, w, ins, device = _linear_inputs(what, x, weight, bias, activation)
+    n = weight.shape[0]
+    y = x.new_empty((*x.shape[:-1], n))
+    pre = torch.empty_like(y) if keep else None
+    out = _nat.SxLinearOutputs(None, 0, y.data_ptr(), n, pre.data_ptr() if keep else None, n)
+    if residual is not None:
+        if residual.shape != y.shape or residual.dtype != y.dtype:
+            raise ValueError(f"{what}: residual must be like y, {y.dtype} of {tuple(y.shape)}")
+        _on(device, what, residual)
+        r, _, out.residual_stride = _rows(residual, n)
+        out.residual = r.data_ptr()
+    entry = _nat.lib().sxcuda_linear_fwd
+    with _at(device) as stream:
+        ws, at, nbytes = _space(device, entry, C.byref(ins), C.byref(out))
+        check(entry(C.byref(ins), C.byref(out), at, C.byref(nbytes), stream))
+    return y, pre
+
+
+def _space(device, entry, *args):
+    nbytes = C.c_size_t(0)
+    check(entry(*args, None, C.byref(nbytes), None))
+    if not nbytes.value:
+        return None, 16, nbytes
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), nbytes
+
+
+def linear_bwd(v_y, x, weight, bias=None, pre=None, *, activation=None, needs_x=True, needs_weight=True):
+    """Gradients (v_x, v_weight, v_bias) of linear_fwd for the gradient v_y of its y (which is also the
+    residual's). pre is the forward's, needed with an activation and only then. v_bias is like bias, None
+    without one; v_x and v_weight are None where they are not needed. Deterministic."""
+    what = "linear_bwd"
+    flat, w, ins, device = _linear_inputs(what, x, weight, bias, activation)
+    n = weight.shape[0]
+    if v_y.shape != (*x.shape[:-1], n) or v_y.dtype != x.dtype:
+        raise ValueError(f"{what}: v_y must be {x.dtype} of {(*x.shape[:-1], n)}")
+    if (pre is None) != (activation is None):
+        raise ValueError(f"{what}: pre is needed with an activation, and only then")
+    _on(device, what, v_y, pre)
+    g, _, g_stride = _rows(v_y, n)
+    gin = _nat.SxLinearGradsIn(g.data_ptr(), g_stride, None, n)
+    if pre is not None:
+        if pre.shape != v_y.shape or pre.dtype != v_y.dtype:
+            raise ValueError(f"{what}: pre must be like v_y")
+        z, _, gin.pre_stride = _rows(pre, n)
+        gin.pre = z.data_ptr()
+    v_x = torch.empty_like(x, memory_format=torch.contiguous_format) if needs_x else None
+    v_w = torch.empty_like(weight, memory_format=torch.contiguous_format) if needs_weight else None
+    v_b = None if bias is None else torch.empty_like(bias)
+    cols = weight.shape[1]
+    out = _nat.SxLinearGrads(v_x.data_ptr() if needs_x else None, cols,
+                             v_w.data_ptr() if needs_weight else None, cols,
+                             None if v_b is None else v_b.data_ptr())
+    entry = _nat.lib().sxcuda_linear_bwd
+    with _at(device) as stream:
+        ws, at, nbytes = _space(device, entry, C.byref(ins), C.byref(gin), C.byref(out))
+        check(entry(C.byref(ins), C.byref(gin), C.byref(out), at, C.byref(nbytes), stream))
+    return v_x, v_w, v_b
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        keep = activation is not None and any(ctx.needs_input_grad[:3])
+        y, pre = linear_fwd(x, weight, bias, activation=activation, residual=residual, keep=keep)
+        ctx.save_for_backward(x, weight, bias, pre)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, v_y):
+        x, weight, bias, pre = ctx.saved_tensors
+        needs = ctx.needs_input_grad
+        v_x = v_w = v_b = None
+        if any(needs[:3]):
+            v_x, v_w, v_b = linear_bwd(v_y, x, weight, bias if needs[2] else None, pre,
+                                       activation=ctx.activation, needs_x=needs[0], needs_weight=needs[1])
+        return v_x, v_w, v_b, v_y if needs[3] else None, None
+
+
+def linear(x, weight, bias=None, *, activation=None, residual=None):
+    """linear_fwd's y, differentiable in x, weight, bias and residual."""
+    return _Linear.apply(x, weight, bias, residual, activation)
+
+
+# ---------------------------------------------------------------- norm and rotation of queries and keys
+
+_PAIRS = {"axis": 0, "whole": 1, "neighbours": 2}
+_POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
+
+
+def _ladder(what, axes, base, freqs):
+    """The pairs' frequencies as a C array: given ones, or base^(-2 j / dim) for pair j of an axis."""
+    if freqs is None:
+        if not (isinstance(base, (int, float)) and base > 0 and math.isfinite(base)):
+            raise ValueError(f"{what}: base must be a number above zero")
+        freqs = [float(base) ** (-2.0 * j / d) for d in axes for j in range(d // 2)]
+    elif len(freqs) != sum(axes) // 2:
+        raise ValueError(f"{what}: {sum(axes) // 2} freqs needed, got {len(freqs)}")
+    return (C.c_double * max(len(freqs), 1))(*[float(f) for f in freqs])
+
+
+def _head_rows(t, what):
+    if t.dim() != 4:
+        raise ValueError(f"{what}: [batch, tokens, heads, head_dim] needed, got {tuple(t.shape)}")
+    return t.contiguous() if t.stride(3) != 1 and t.shape[3] != 1 else t
+
+
+def _rotary_inputs(what, q, k, positions, axes, base, freqs, pairs, norm, q_weight, k_weight, eps):
+    q = _head_rows(q, what)
+    b, n, h, d = q.shape
+    code, device = _dtype(q, what), q.device
+    if k is not None:
+        k = _head_rows(k, what)
+        if k.dtype != q.dtype or k.shape[:2] != q.shape[:2] or k.shape[3] != d:
+            raise ValueError(f"{what}: k must be {q.dtype} of [{b}, {n}, heads, {d}], got {k.dtype} of "
+                             f"{tuple(k.shape)}")
+    elif k_weight is not None:
+        raise ValueError(f"{what}: k_weight needs k")
+    if pairs not in _PAIRS:
+        raise ValueError(f"{what}: pairs must be one of {list(_PAIRS)}")
+    axes = tuple(int(a) for a in axes)
+    if not 1 <= len(axes) <= 4 or any(a < 0 or a % 2 for a in axes) or sum(axes) > d:
+        raise ValueError(f"{what}: axes must be 1 to 4 even numbers of values, at most {d} together, got {axes}")
+    code_at = _POSITIONS.get(positions.dtype)
+    if code_at is None:
+        raise ValueError(f"{what}: positions must be float32, int32 or int64, got {positions.dtype}")
+    if positions.requires_grad:
+        raise ValueError(f"{what}: positions get no gradient: detach() them")
+    if positions.shape not in ((b, n, len(axes)), (n, len(axes))):
+        raise ValueError(f"{what}: positions must be [{b}, {n}, {len(axes)}] or [{n}, {len(axes)}], got "
+                         f"{tuple(positions.shape)}")
+    first = k_weight if q_weight is None else q_weight
+    for w in (q_weight, k_weight):
+        if w is not None and (not norm or w.shape != (d,) or not w.is_contiguous() or w.dtype != first.dtype):
+            raise ValueError(f"{what}: q_weight and k_weight need norm and must be contiguous tensors of "
+                             f"[{d}] with one dtype")
+    _on(device, what, k, positions, q_weight, k_weight)
+    at = positions.stride()
+    table = _ladder(what, axes, base, freqs)
+    ins = _nat.SxRotaryInputs(
+        _view(q), _view(q) if k is None else _view(k), positions.data_ptr(), at[0] if len(at) == 3 else 0,
+        at[-2], at[-1], C.addressof(table), None if q_weight is None else q_weight.data_ptr(),
+        None if k_weight is None else k_weight.data_ptr(), b, n, h, 0 if k is None else k.shape[2], d,
+        len(axes), (C.c_int32 * 4)(*axes), _PAIRS[pairs], code, 0 if first is None else _dtype(first, what),
+        code_at, bool(norm), eps)
+    return q, k, ins, device, table
+
+
+def qk_norm_rotary_fwd(q, k, positions, *, axes, base=10000.0, freqs=None, pairs="axis", norm=True,
+                       q_weight=None, k_weight=None, eps=1e-6):
+    """Queries and keys normalised per head, x / sqrt(mean x^2 + eps) * weight, and rotated by the
+    positions of their tokens: (q, k) as new tensors.
+
+    q: [batch, tokens, heads, head_dim]; k: the same with heads of its own, or None; float32, float16 or
+    bfloat16, head_dim up to 256, any strides with the last axis contiguous (views of a joint projection).
+    positions: [batch, tokens, axes] or [tokens, axes] in float32, int32 or int64: places in an image
+    (row, column), a video (time, row, column), a scene (x, y, z), or one number; they get no gradient.
+    axes: how many values of a head each axis rotates, in pairs; those behind the sum are not rotated.
+    Pair j of an axis with d values turns by position * base^(-2 j / d), or by position * freqs[i], i
+    counting the pairs of all axes. pairs: which values are one: "axis": j and j + d / 2 of the axis' own
+    run of values; "whole": i and i + sum(axes) / 2; "neighbours": 2 i and 2 i + 1. norm=False only
+    rotates. q_weight, k_weight: [head_dim], None for ones."""
+    what = "qk_norm_rotary_fwd"
+    q, k, ins, device, table = _rotary_inputs(what, q, k, positions, axes, base, freqs, pairs, norm,
+                                              q_weight, k_weight, eps)
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    qv = _nat.SxAttentionView(*_view(q_out))
+    kv = None if k is None else C.byref(_nat.SxAttentionView(*_view(k_out)))
+    with _at(device) as stream:
+        check(_nat.lib().sxcuda_qk_norm_rotary_fwd(C.byref(ins), C.byref(qv), kv, stream))
+    return q_out, k_out
+
+
+def qk_norm_rotary_bwd(v_q_out, v_k_out, q, k, positions, *, axes, base=10000.0, freqs=None, pairs="axis",
+                       norm=True, q_weight=None, k_weight=None, eps=1e-6):
+    """Gradients (v_q, v_k, v_q_weight, v_k_weight) of qk_norm_rotary_fwd for the gradients of its
+    outputs; None for what was not given. Deterministic."""
+    what = "qk_norm_rotary_bwd"
+    q, k, ins, device, table = _rotary_inputs(what, q, k, positions, axes, base, freqs, pairs, norm,
+                                              q_weight, k_weight, eps)
+    if (v_k_out is None) != (k is None):
+        raise ValueError(f"{what}: v_k_out is needed with k, and only then")
+    grads = []
+    for name, g, t in (("v_q_out", v_q_out, q), ("v_k_out", v_k_out, k)):
+        if t is not None and (g.shape != t.shape or g.dtype != t.dtype):
+            raise ValueError(f"{what}: {name} must be {t.dtype} of {tuple(t.shape)}")
+        grads.append(None if t is None else _head_rows(g, what))
+    _on(device, what, *grads)
+    outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k)]
+    v_w = [None if w is None else torch.empty_like(w) for w in (q_weight, k_weight)]
+    none = (None, 0, 0, 0)
+    g = _nat.SxRotaryGrads(*(none if t is None else _view(t) for t in (*grads, *outs)),
+                           *(None if w is None else w.data_ptr() for w in v_w))
+    entry = _nat.lib().sxcuda_qk_norm_rotary_bwd
+    with _at(device) as stream:
+        ws, at, nbytes = _space(device, entry, C.byref(ins), C.byref(g))
+        check(entry(C.byref(ins), C.byref(g), at, C.byref(nbytes), stream))
+    return (*outs, *v_w)
+
+
+class _QkNormRotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, q_weight, k_weight, how):
+        ctx.save_for_backward(q, k, positions, q_weight, k_weight)
+        ctx.how = how
+        return qk_norm_rotary_fwd(q, k, positions, q_weight=q_weight, k_weight=k_weight, **how)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, v_q_out, v_k_out):
+        q, k, positions, q_weight, k_weight = ctx.saved_tensors
+        v_q, v_k, v_qw, v_kw = qk_norm_rotary_bwd(v_q_out, None if k is None else v_k_out, q, k, positions,
+                                                  q_weight=q_weight, k_weight=k_weight, **ctx.how)
+        return v_q, v_k, None, v_qw, v_kw, None
+
+
+def qk_norm_rotary(q, k, positions, *, axes, base=10000.0, freqs=None, pairs="axis", norm=True,
+                   q_weight=None, k_weight=None, eps=1e-6):
+    """qk_norm_rotary_fwd's (q, k), differentiable in q, k and the weights."""
+    how = {"axes": axes, "base": base, "freqs": freqs, "pairs": pairs, "norm": norm, "eps": eps}
+    return _QkNormRotary.apply(q, k, positions, q_weight, k_weight, how)
 
 
 # ---------------------------------------------------------------- AdamW
