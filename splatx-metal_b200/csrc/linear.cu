@@ -22,10 +22,10 @@ template <typename T>
 struct Staged {
     float x[8];
     __device__ void load(const LinearOperand& o, int64_t row0, int64_t rows, int64_t k0, int64_t k_end, bool wide) {
-        const bool along_k = o.k_stride == 1;
+        const bool along_k = !o.across;
         const int t = threadIdx.x;
         const int64_t row = row0 + (along_k ? t / 2 : t % 16 * 8), k = k0 + (along_k ? t % 2 * 8 : t / 16);
-        const T* p = static_cast<const T*>(o.data) + row * o.row_stride + k * o.k_stride;
+        const T* p = static_cast<const T*>(o.data) + (along_k ? row * o.stride + k : k * o.stride + row);
         const int64_t left = (along_k ? row < rows : k < k_end) ? (along_k ? k_end - k : rows - row) : 0;
         constexpr int N = sizeof(T) == 4 ? 4 : 8;
         if (wide && left >= 8) {
@@ -42,7 +42,7 @@ struct Staged {
     }
     __device__ void store(const LinearOperand& o, float (&to)[kDepth][kPitch]) const {
         const int t = threadIdx.x;
-        if (o.k_stride == 1) {
+        if (!o.across) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) to[t % 2 * 8 + i][t / 2] = x[i];
         } else {
@@ -62,7 +62,7 @@ __device__ __forceinline__ void linear_finish(const LinearProduct& p, int64_t ro
         if (i >= n) break;
         z[i] += linear_param(p.bias, p.bias_dtype, col + i);
         pre[i] = from_f32<T>(z[i]);
-        float v = linear_act(p.act, z[i]);
+        float v = act_of<T>(p.act, z[i]);
         if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[row * p.residual_stride + col + i]);
         y[i] = from_f32<T>(v);
     }
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant_
     LinearPiece piece;
     while (walk.next(p.plan, piece)) {
         const LinearTile tile = linear_tile(p.plan, piece.tile);
-        const int64_t m0 = tile.m * kTile, n0 = tile.n * kTile, end = min(static_cast<int64_t>(piece.k1) * kDepth, p.k);
+        const int64_t m0 = static_cast<int64_t>(tile.m) * kTile, n0 = static_cast<int64_t>(tile.n) * kTile, end = min(static_cast<int64_t>(piece.k1) * kDepth, p.k);
         float c[8][8] = {};
         Staged<T> a, b;
         a.load(p.a, m0, p.m, static_cast<int64_t>(piece.k0) * kDepth, end, a_wide);
@@ -146,8 +146,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
     const int64_t t = blockIdx.y;
     const int64_t w0 = plan.worker_of(t * plan.kblocks), w1 = plan.worker_of((t + 1) * plan.kblocks - 1);
     if (w0 == w1) return;  // no cut goes through it
-    const LinearTile tile = linear_tile(plan, plan.whole + t);
-    const int64_t m0 = tile.m * plan.tile_m, n0 = tile.n * plan.tile_n;
+    const LinearTile tile = linear_tile(plan, plan.whole + static_cast<int32_t>(t));
+    const int64_t m0 = static_cast<int64_t>(tile.m) * plan.tile_m, n0 = static_cast<int64_t>(tile.n) * plan.tile_n;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.tile_m), p.m - m0)), groups = plan.tile_n / 8;
     const int i = blockIdx.x * 256 + threadIdx.x, row = i / groups, col = i % groups * 8;
     const int64_t n = min(p.n - n0 - col, static_cast<int64_t>(8));
@@ -163,48 +163,83 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
 }
 
 bool linear_wide(const LinearOperand& o, int64_t size) {
-    const int64_t other = o.k_stride == 1 ? o.row_stride : o.k_stride;
-    return reinterpret_cast<uintptr_t>(o.data) % 16 == 0 && other * size % 16 == 0;
+    return reinterpret_cast<uintptr_t>(o.data) % 16 == 0 && o.stride * size % 16 == 0;
 }
 
-// Whole tiles, but for those of the last turns where workers would go without: the cut costs a launch and
-// its parts' way through memory, and a piece has at least `least` K blocks.
+}  // namespace
+
 LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, int depth, int64_t workers, int64_t least) {
     LinearPlan p;
     p.tile_m = tile_m, p.tile_n = tile_n;
-    p.tiles_m = (m + tile_m - 1) / tile_m, p.tiles_n = (n + tile_n - 1) / tile_n;
-    p.kblocks = (k + depth - 1) / depth;
-    const int64_t tiles = p.tiles(), turns = tiles / workers;
+    const int64_t tiles_m = (m + tile_m - 1) / tile_m, tiles_n = (n + tile_n - 1) / tile_n, tiles = tiles_m * tiles_n;
+    if (tiles > INT32_MAX / kLinearBand) throw_invalid("linear", "too many tiles");
+    p.tiles_m = static_cast<int32_t>(tiles_m), p.tiles_n = static_cast<int32_t>(tiles_n);
+    p.kblocks = static_cast<int32_t>((k + depth - 1) / depth);
+    const int64_t turns = tiles / workers;
     p.workers = static_cast<int32_t>(std::min(tiles, workers));
-    p.whole = tiles;
+    p.whole = static_cast<int32_t>(tiles);
     if (tiles % workers == 0) return p;
     const int64_t whole = turns > 0 ? (turns - 1) * workers : 0, units = (tiles - whole) * p.kblocks;
     const int64_t used = std::min(workers, std::max<int64_t>(units / least, 1));
     const int64_t now = p.kblocks * ((tiles - whole + workers - 1) / workers), then = (units + used - 1) / used;
     if (now - then < 2 * least) return p;
-    p.whole = whole;
+    p.whole = static_cast<int32_t>(whole);
     p.units = units;
     p.workers = static_cast<int32_t>(used);
     return p;
 }
 
+namespace {
+
 constexpr int kPerSm = 2;
 
-LinearPlan product_plan(int64_t m, int64_t n, int64_t k) {
-    return linear_plan(m, n, k, kTile, kTile, kDepth, static_cast<int64_t>(sm_count()) * kPerSm, 8);
+LinearPlan product_plan(int32_t dtype, int64_t m, int64_t n, int64_t k) {
+    return dtype == SXCUDA_F32 ? linear_plan(m, n, k, kTile, kTile, kDepth, static_cast<int64_t>(sm_count()) * kPerSm, 8)
+                               : linear_tc_plan(m, n, k);
 }
 
 void launch_product(const LinearProduct& p, cudaStream_t s) {
+    if (p.dtype == SXCUDA_F32)
+        SX_LAUNCH(linear_kernel<float>, static_cast<unsigned>(p.plan.workers), kThreads, 0, s, p, linear_wide(p.a, 4), linear_wide(p.b, 4));
+    else launch_linear_tc(p, s);
+    if (!p.plan.cut()) return;
     by_dtype(p.dtype, [&](auto t) {
-        using T = decltype(t);
-        const auto kernel = linear_kernel<T>;
-        SX_LAUNCH(kernel, static_cast<unsigned>(p.plan.workers), kThreads, 0, s, p, linear_wide(p.a, sizeof(T)), linear_wide(p.b, sizeof(T)));
-        if (!p.plan.cut()) return;
-        const auto join = linear_join_kernel<T>;
+        const auto join = linear_join_kernel<decltype(t)>;
         const int64_t rows = std::min<int64_t>(p.m, p.plan.tile_m);
         SX_LAUNCH(join, dim3(blocks_for(rows * (p.plan.tile_n / 8), 256), static_cast<unsigned>(p.plan.tiles() - p.plan.whole)), 256, 0, s, p);
     });
 }
+
+// ---- rows that tensor maps do not take, copied to rows that they do ----
+__global__ void __launch_bounds__(256) linear_pack_kernel(const uint16_t* from, int64_t stride, int64_t rows, int32_t cols, uint16_t* to,
+                                                          int32_t pitch) {
+    const int64_t pieces = pitch / 8, i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, row = i / pieces;
+    const int32_t c = static_cast<int32_t>(i - row * pieces) * 8;
+    if (row >= rows) return;
+    Pack<uint16_t, 8> x;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x.v[j] = c + j < cols ? from[row * stride + c + j] : 0;
+    *reinterpret_cast<Pack<uint16_t, 8>*>(to + row * pitch + c) = x;
+}
+int64_t pitch_of(int64_t cols) { return (cols + 7) / 8 * 8; }
+
+// A matrix of the call as the products read it: itself, or its copy at `at` in the workspace.
+struct Matrix {
+    const void* data;
+    int64_t stride, rows, cols;
+    bool copied(int32_t dtype) const { return dtype != SXCUDA_F32 && !linear_tc_takes(data, stride, rows); }
+    size_t bytes(int32_t dtype) const { return copied(dtype) ? aligned_bytes(static_cast<size_t>(rows) * pitch_of(cols) * 2) : 0; }
+    static size_t aligned_bytes(size_t n) { return (n + 255) / 256 * 256; }
+    Matrix ready(int32_t dtype, uint8_t* at, cudaStream_t s) const {
+        if (!copied(dtype)) return *this;
+        const int64_t pitch = pitch_of(cols);
+        SX_LAUNCH(linear_pack_kernel, blocks_for(rows * (pitch / 8), 256), 256, 0, s, static_cast<const uint16_t*>(data), stride, rows,
+                  static_cast<int32_t>(cols), reinterpret_cast<uint16_t*>(at), static_cast<int32_t>(pitch));
+        return {at, pitch, rows, cols};
+    }
+    LinearOperand along_k() const { return {data, stride, false}; }  // its rows are the operand's
+    LinearOperand across_k() const { return {data, stride, true}; }  // its columns are
+};
 
 // ---- v_z = v_y act'(pre), and the sum of its rows ----
 // A CTA has 32 V columns (a warp's lanes V each) and a slice of the rows, which its warps take in turn.
@@ -232,7 +267,7 @@ __global__ void __launch_bounds__(kSlopeWarps * 32) linear_slope_kernel(const Sl
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 float x = to_f32(g.v[i]);
-                if (a.pre) x *= linear_slope(a.act, to_f32(z.v[i]));
+                if (a.pre) x *= slope_of<T>(a.act, to_f32(z.v[i]));
                 sum[i] += x;
                 to.v[i] = from_f32<T>(x);
             }
@@ -277,53 +312,59 @@ SlopePlan slope_plan(const SxLinearInputs& in, const SxLinearGradsIn& g) {
     return p;
 }
 
-size_t aligned(size_t n) { return (n + 255) / 256 * 256; }
-
-// The backward's workspace: v_z (where it is not v_y), the bias' sums, the products' parts.
+// The backward's workspace: v_z where it is not v_y, copies of x and weight, the bias' sums, the products' parts.
 struct BwdSpace {
-    size_t v_z = 0, sums = 0, parts = 0, bytes = 0;
+    Matrix x, weight, v_y;
+    bool v_z = false;  // made
+    size_t x_at = 0, weight_at = 0, v_z_at = 0, sums_at = 0, parts_at = 0, bytes = 0;
+    BwdSpace(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out)
+        : x{in.x, in.x_stride, in.rows, in.in_features}, weight{in.weight, in.weight_stride, in.out_features, in.in_features},
+          v_y{g.v_y, g.v_y_stride, in.rows, in.out_features} {
+        if (in.rows == 0) return;
+        const auto take = [&](size_t& at, size_t n) {
+            at = bytes;
+            bytes += Matrix::aligned_bytes(n);
+        };
+        v_z = g.pre || ((out.v_x || out.v_weight) && v_y.copied(in.dtype));
+        if (v_z) take(v_z_at, static_cast<size_t>(in.rows) * pitch_of(in.out_features) * dtype_bytes(in.dtype));
+        if (out.v_weight) take(x_at, x.bytes(in.dtype));
+        if (out.v_x) take(weight_at, weight.bytes(in.dtype));
+        if (out.v_bias) take(sums_at, static_cast<size_t>(slope_plan(in, g).slices) * in.out_features * 4);
+        size_t parts = 0;
+        if (out.v_x) parts = product_plan(in.dtype, in.rows, in.in_features, in.out_features).workspace();
+        if (out.v_weight) parts = std::max(parts, product_plan(in.dtype, in.out_features, in.in_features, in.rows).workspace());
+        take(parts_at, parts);
+    }
 };
-BwdSpace bwd_space(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out) {
-    BwdSpace w;
-    if (in.rows == 0) return w;
-    w.v_z = 0;
-    size_t at = g.pre ? aligned(static_cast<size_t>(in.rows) * in.out_features * dtype_bytes(in.dtype)) : 0;
-    w.sums = at;
-    if (out.v_bias) at += aligned(static_cast<size_t>(slope_plan(in, g).slices) * in.out_features * 4);
-    w.parts = at;
-    size_t parts = 0;
-    if (out.v_x) parts = std::max(parts, product_plan(in.rows, in.in_features, in.out_features).workspace());
-    if (out.v_weight) parts = std::max(parts, product_plan(in.out_features, in.in_features, in.rows).workspace());
-    w.bytes = at + parts;
-    return w;
-}
 
 }  // namespace
 
-uint32_t linear_status() { return 0; }
-
 size_t linear_fwd_workspace(const SxLinearInputs& in) {
-    return in.rows ? product_plan(in.rows, in.out_features, in.in_features).workspace() : 0;
+    if (in.rows == 0) return 0;
+    const Matrix x{in.x, in.x_stride, in.rows, in.in_features}, w{in.weight, in.weight_stride, in.out_features, in.in_features};
+    return x.bytes(in.dtype) + w.bytes(in.dtype) + product_plan(in.dtype, in.rows, in.out_features, in.in_features).workspace();
 }
 
 void launch_linear_fwd(const SxLinearInputs& in, const SxLinearOutputs& out, void* ws, cudaStream_t s) {
     if (in.rows == 0) return;
+    uint8_t* at = static_cast<uint8_t*>(ws);
+    const Matrix x{in.x, in.x_stride, in.rows, in.in_features}, w{in.weight, in.weight_stride, in.out_features, in.in_features};
     LinearProduct p{};
-    p.a = {in.x, in.x_stride, 1};
-    p.b = {in.weight, in.weight_stride, 1};
+    p.a = x.ready(in.dtype, at, s).along_k();
+    p.b = w.ready(in.dtype, at += x.bytes(in.dtype), s).along_k();
     p.m = in.rows, p.n = in.out_features, p.k = in.in_features;
     p.dtype = in.dtype, p.bias_dtype = in.bias_dtype, p.act = in.activation;
     p.bias = in.bias;
     p.residual = out.residual, p.residual_stride = out.residual_stride;
     p.y = out.y, p.y_stride = out.y_stride;
     p.pre = out.pre, p.pre_stride = out.pre_stride;
-    p.parts = static_cast<float*>(ws);
-    p.plan = product_plan(p.m, p.n, p.k);
+    p.parts = reinterpret_cast<float*>(at + w.bytes(in.dtype));
+    p.plan = product_plan(in.dtype, p.m, p.n, p.k);
     launch_product(p, s);
 }
 
 size_t linear_bwd_workspace(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out) {
-    return bwd_space(in, g, out).bytes;
+    return BwdSpace(in, g, out).bytes;
 }
 
 void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out, void* ws, cudaStream_t s) {
@@ -334,14 +375,14 @@ void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const
         if (out.v_bias) cuda_check(cudaMemsetAsync(out.v_bias, 0, in.out_features * dtype_bytes(in.bias_dtype), s), "linear_bwd");
         return;
     }
-    const BwdSpace space = bwd_space(in, g, out);
+    const BwdSpace space(in, g, out);
     uint8_t* at = static_cast<uint8_t*>(ws);
-    LinearOperand v_z{g.v_y, g.v_y_stride, 1};  // [rows, out_features]
-    if (g.pre || out.v_bias) {
+    Matrix v_z = space.v_y;
+    if (space.v_z || out.v_bias) {
         const SlopePlan plan = slope_plan(in, g);
-        SlopeArgs a{g.v_y, g.pre, nullptr, nullptr, g.v_y_stride, g.pre_stride, in.out_features, in.rows, in.out_features, plan.slice, in.activation};
-        if (g.pre) v_z = {a.v_z = at + space.v_z, in.out_features, 1};
-        if (out.v_bias) a.sums = reinterpret_cast<float*>(at + space.sums);
+        SlopeArgs a{g.v_y, g.pre, nullptr, nullptr, g.v_y_stride, g.pre_stride, pitch_of(in.out_features), in.rows, in.out_features, plan.slice, in.activation};
+        if (space.v_z) v_z = {a.v_z = at + space.v_z_at, a.v_z_stride, in.rows, in.out_features};
+        if (out.v_bias) a.sums = reinterpret_cast<float*>(at + space.sums_at);
         by_dtype(in.dtype, [&](auto t) {
             using T = decltype(t);
             const auto kernel = plan.v == 1 ? linear_slope_kernel<T, 1> : linear_slope_kernel<T, 16 / sizeof(T)>;
@@ -352,21 +393,21 @@ void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const
     }
     LinearProduct p{};
     p.dtype = in.dtype;
-    p.parts = reinterpret_cast<float*>(at + space.parts);
+    p.parts = reinterpret_cast<float*>(at + space.parts_at);
     if (out.v_x) {
-        p.a = v_z;
-        p.b = {in.weight, 1, in.weight_stride};
+        p.a = v_z.along_k();
+        p.b = space.weight.ready(in.dtype, at + space.weight_at, s).across_k();
         p.m = in.rows, p.n = in.in_features, p.k = in.out_features;
         p.y = out.v_x, p.y_stride = out.v_x_stride;
-        p.plan = product_plan(p.m, p.n, p.k);
+        p.plan = product_plan(in.dtype, p.m, p.n, p.k);
         launch_product(p, s);
     }
     if (out.v_weight) {
-        p.a = {v_z.data, 1, v_z.row_stride};
-        p.b = {in.x, 1, in.x_stride};
+        p.a = v_z.across_k();
+        p.b = space.x.ready(in.dtype, at + space.x_at, s).across_k();
         p.m = in.out_features, p.n = in.in_features, p.k = in.rows;
         p.y = out.v_weight, p.y_stride = out.v_weight_stride;
-        p.plan = product_plan(p.m, p.n, p.k);
+        p.plan = product_plan(in.dtype, p.m, p.n, p.k);
         launch_product(p, s);
     }
 }

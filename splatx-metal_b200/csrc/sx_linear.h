@@ -7,10 +7,12 @@
 
 namespace sx {
 
-// Rows of an operand: element (row, k) at data[row * row_stride + k * k_stride]; one of the strides is 1.
+// An operand of a product: element (row, k) at data[row * stride + k], or, with its rows across K, at
+// data[k * stride + row].
 struct LinearOperand {
     const void* data;
-    int64_t row_stride, k_stride;
+    int64_t stride;
+    bool across;
 };
 
 // How a product's output tiles are worked on. Tiles below `whole` go round the workers; the K blocks of
@@ -18,11 +20,9 @@ struct LinearOperand {
 // of them end together. A tile that a cut goes through is left in parts in the workspace, 32-bit sums,
 // which a second kernel adds in order.
 struct LinearPlan {
-    int32_t tile_m = 0, tile_n = 0;
-    int64_t tiles_m = 0, tiles_n = 0, kblocks = 0;
-    int64_t whole = 0, units = 0;
-    int32_t workers = 0;
-    __host__ __device__ int64_t tiles() const { return tiles_m * tiles_n; }
+    int32_t tile_m = 0, tile_n = 0, tiles_m = 0, tiles_n = 0, kblocks = 0, whole = 0, workers = 0;
+    int64_t units = 0;
+    __host__ __device__ int32_t tiles() const { return tiles_m * tiles_n; }
     __host__ __device__ bool cut() const { return units > 0; }
     __host__ __device__ int64_t start(int64_t worker) const { return worker * units / workers; }
     __host__ __device__ int64_t worker_of(int64_t unit) const { return ((unit + 1) * workers - 1) / units; }
@@ -50,41 +50,38 @@ struct LinearProduct {
 
 // One stretch of a tile's K blocks; slot: of the part it is left in, -1 where it is the whole tile.
 struct LinearPiece {
-    int64_t tile;
-    int32_t k0, k1;
-    int64_t slot;
+    int32_t tile, k0, k1, slot;
 };
 
 // The pieces of one worker, in order.
 struct LinearWalk {
-    int64_t tile, unit, end;
-    int32_t worker;
-    __device__ LinearWalk(const LinearPlan& p, int32_t w) : tile(w), unit(p.cut() ? p.start(w) : 0), end(p.cut() ? p.start(w + 1) : 0), worker(w) {}
+    int64_t unit, end;
+    int32_t tile, worker;
+    __device__ LinearWalk(const LinearPlan& p, int32_t w) : unit(p.cut() ? p.start(w) : 0), end(p.cut() ? p.start(w + 1) : 0), tile(w), worker(w) {}
     __device__ bool next(const LinearPlan& p, LinearPiece& piece) {
         if (tile < p.whole) {
-            piece = {tile, 0, static_cast<int32_t>(p.kblocks), -1};
+            piece = {tile, 0, p.kblocks, -1};
             tile += p.workers;
             return true;
         }
         if (unit >= end) return false;
-        const int64_t t = unit / p.kblocks, k0 = unit - t * p.kblocks;
-        const int64_t k1 = k0 + end - unit < p.kblocks ? k0 + end - unit : p.kblocks;
-        const bool all = k0 == 0 && k1 == p.kblocks;
-        piece = {p.whole + t, static_cast<int32_t>(k0), static_cast<int32_t>(k1), all ? -1 : 2 * static_cast<int64_t>(worker) + (k0 == 0)};
+        const int32_t t = static_cast<int32_t>(unit / p.kblocks), k0 = static_cast<int32_t>(unit - static_cast<int64_t>(t) * p.kblocks);
+        const int32_t k1 = static_cast<int32_t>(min(k0 + (end - unit), static_cast<int64_t>(p.kblocks)));
+        piece = {p.whole + t, k0, k1, k0 == 0 && k1 == p.kblocks ? -1 : 2 * worker + (k0 == 0)};
         unit += k1 - k0;
         return true;
     }
 };
 
-// Which tile a number stands for: bands of kBand rows of tiles, in each the rows fastest, so that the tiles
-// that are worked on at the same time share their operands in L2.
+// Which tile a number stands for: bands of kLinearBand rows of tiles, in each the rows fastest, so that the
+// tiles that are worked on at the same time share their operands in L2.
 constexpr int kLinearBand = 8;
 struct LinearTile {
-    int64_t m, n;
+    int32_t m, n;
 };
-__host__ __device__ inline LinearTile linear_tile(const LinearPlan& p, int64_t t) {
-    const int64_t band = t / (kLinearBand * p.tiles_n), first = band * kLinearBand;
-    const int64_t rows = p.tiles_m - first < kLinearBand ? p.tiles_m - first : kLinearBand, r = t - first * p.tiles_n;
+__device__ inline LinearTile linear_tile(const LinearPlan& p, int32_t t) {
+    const int32_t band = t / (kLinearBand * p.tiles_n), first = band * kLinearBand;
+    const int32_t rows = min(p.tiles_m - first, kLinearBand), r = t - first * p.tiles_n;
     return {first + r % rows, r / rows};
 }
 
@@ -132,5 +129,86 @@ __device__ __forceinline__ float linear_slope(int32_t act, float z) {
         default: return 1.f;
     }
 }
+
+// ---- the same for 16-bit results: within 2^-16 of the value, at two instructions of the special-function unit ----
+// The normal distribution's tail: Phi(-a) = t P(t) exp(-a^2 / 2) with t = 1 / (1 + 0.3 a); P fitted for the least
+// relative error over a = 0..14 (8.2e-6).
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2Of = 1.4426950408889634f;  // of e
+struct Normal {
+    float below, density;  // Phi(z), and exp(-z^2 / 2)
+};
+__device__ __forceinline__ Normal normal_fast(float z) {
+    const float a = fabsf(z), t = rcp_fast(fmaf(0.3f, a, 1.f)), e = exp2_fast(-0.5f * kLog2Of * a * a);
+    float p = fmaf(-0x1.3bca6ap-4f, t, 0x1.ba7182p-3f);
+    p = fmaf(p, t, -0x1.15ac44p-6f);
+    p = fmaf(p, t, 0x1.27505cp-3f);
+    p = fmaf(p, t, 0x1.d1e316p-4f);
+    p = fmaf(p, t, 0x1.ebd2f4p-4f);
+    const float tail = p * t * e;
+    return {z < 0.f ? tail : 1.f - tail, e};
+}
+__device__ __forceinline__ float gate_fast(float z) { return rcp_fast(1.f + exp2_fast(-kLog2Of * z)); }
+template <int ACT>
+__device__ __forceinline__ float act_fast(float z) {
+    if constexpr (ACT == SXCUDA_ACT_RELU) return z < 0.f ? 0.f : z;
+    if constexpr (ACT == SXCUDA_ACT_SILU) return z * gate_fast(z);
+    if constexpr (ACT == SXCUDA_ACT_GELU) return z * normal_fast(z).below;
+    if constexpr (ACT == SXCUDA_ACT_GELU_TANH) return z * gate_fast(tanh_gate_at(z));
+    return z;
+}
+__device__ __forceinline__ float slope_fast(int32_t act, float z) {
+    z = fabsf(z) > 1e4f ? copysignf(1e4f, z) : z;
+    switch (act) {
+        case SXCUDA_ACT_RELU: return z > 0.f ? 1.f : z != z ? z : 0.f;
+        case SXCUDA_ACT_SILU: {
+            const float g = gate_fast(z);
+            return fmaf(z * g, 1.f - g, g);
+        }
+        case SXCUDA_ACT_GELU: {
+            const Normal n = normal_fast(z);
+            return fmaf(z * 0.3989422804014327f, n.density, n.below);
+        }
+        case SXCUDA_ACT_GELU_TANH: {
+            const float g = gate_fast(tanh_gate_at(z));
+            return fmaf(z * g * (1.f - g), kGeluTanh * fmaf(3.f * kGeluCube * z, z, 1.f), g);
+        }
+        default: return 1.f;
+    }
+}
+template <typename T>
+__device__ __forceinline__ float act_of(int32_t act, float z) {
+    if constexpr (sizeof(T) == 4) return linear_act(act, z);
+    switch (act) {
+        case SXCUDA_ACT_RELU: return act_fast<SXCUDA_ACT_RELU>(z);
+        case SXCUDA_ACT_SILU: return act_fast<SXCUDA_ACT_SILU>(z);
+        case SXCUDA_ACT_GELU: return act_fast<SXCUDA_ACT_GELU>(z);
+        case SXCUDA_ACT_GELU_TANH: return act_fast<SXCUDA_ACT_GELU_TANH>(z);
+        default: return z;
+    }
+}
+template <typename T>
+__device__ __forceinline__ float slope_of(int32_t act, float z) {
+    if constexpr (sizeof(T) == 4) return linear_slope(act, z);
+    else return slope_fast(act, z);
+}
+
+// ---- products on the tensor cores (linear_tc.cu), of operands that tensor maps take ----
+bool linear_tc_takes(const void* data, int64_t stride, int64_t rows);
+LinearPlan linear_tc_plan(int64_t m, int64_t n, int64_t k);
+void launch_linear_tc(const LinearProduct& p, cudaStream_t s);
+
+// Whole tiles, but for those of the last turns where workers would go without: the cut costs a launch and
+// its parts' way through memory, and a piece has at least `least` K blocks.
+LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, int depth, int64_t workers, int64_t least);
 
 }  // namespace sx
