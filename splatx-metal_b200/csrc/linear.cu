@@ -82,9 +82,8 @@ __device__ __forceinline__ void linear_finish(const LinearProduct& p, int64_t ro
     }
 }
 
-// Where a part of a tile lies: [columns / 8][rows][8].
 __device__ __forceinline__ float* part_at(const LinearProduct& p, int64_t slot, int row, int col) {
-    return p.parts + slot * p.plan.slot_values() + (static_cast<int64_t>(col / 8) * p.plan.tile_m + row) * 8 + col % 8;
+    return p.parts + slot * p.plan.slot_values() + row * p.plan.tile_n + col;
 }
 
 template <typename T>
@@ -138,23 +137,22 @@ __global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant_
     }
 }
 
-// Adds the parts of the tiles that cuts go through, in the order of K, and finishes them. A thread has 8
-// columns of a row; blockIdx.y counts the tiles behind the whole ones.
+// Adds the parts of the tiles that are cut, in the order of K, and finishes them. A thread has 8 columns of
+// a row; blockIdx.y is the tile's number among them.
 template <typename T>
 __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinearProduct p) {
     const LinearPlan& plan = p.plan;
-    const int64_t t = blockIdx.y;
-    const int64_t w0 = plan.worker_of(t * plan.kblocks), w1 = plan.worker_of((t + 1) * plan.kblocks - 1);
-    if (w0 == w1) return;  // no cut goes through it
-    const LinearTile tile = linear_tile(plan, plan.whole + static_cast<int32_t>(t));
+    const int32_t t = static_cast<int32_t>(blockIdx.y), parts = plan.parts(t);
+    const LinearTile tile = linear_tile(plan, plan.whole + t);
     const int64_t m0 = static_cast<int64_t>(tile.m) * plan.tile_m, n0 = static_cast<int64_t>(tile.n) * plan.tile_n;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.tile_m), p.m - m0)), groups = plan.tile_n / 8;
-    const int i = blockIdx.x * 256 + threadIdx.x, row = i / groups, col = i % groups * 8;
+    const int at = blockIdx.x * 256 + threadIdx.x, row = at / groups, col = at % groups * 8;
     const int64_t n = min(p.n - n0 - col, static_cast<int64_t>(8));
     if (row >= rows || n <= 0) return;
     float z[8] = {};
-    for (int64_t w = w0; w <= w1; ++w) {
-        const float4* part = reinterpret_cast<const float4*>(part_at(p, 2 * w + (w == w0), row, col));
+#pragma unroll 4
+    for (int i = 0; i < parts; ++i) {
+        const float4* part = reinterpret_cast<const float4*>(part_at(p, t * plan.slots + i, row, col));
         const float4 x = part[0], y = part[1];
         z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w;
         z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
@@ -168,24 +166,30 @@ bool linear_wide(const LinearOperand& o, int64_t size) {
 
 }  // namespace
 
-LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, int depth, int64_t workers, int64_t least) {
+LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, int depth, int64_t workers, int64_t least,
+                       int64_t gain) {
     LinearPlan p;
     p.tile_m = tile_m, p.tile_n = tile_n;
     const int64_t tiles_m = (m + tile_m - 1) / tile_m, tiles_n = (n + tile_n - 1) / tile_n, tiles = tiles_m * tiles_n;
     if (tiles > INT32_MAX / kLinearBand) throw_invalid("linear", "too many tiles");
+    const int64_t kblocks = (k + depth - 1) / depth, rest = tiles % workers;
     p.tiles_m = static_cast<int32_t>(tiles_m), p.tiles_n = static_cast<int32_t>(tiles_n);
-    p.kblocks = static_cast<int32_t>((k + depth - 1) / depth);
-    const int64_t turns = tiles / workers;
+    p.kblocks = static_cast<int32_t>(kblocks);
     p.workers = static_cast<int32_t>(std::min(tiles, workers));
     p.whole = static_cast<int32_t>(tiles);
-    if (tiles % workers == 0) return p;
-    const int64_t whole = turns > 0 ? (turns - 1) * workers : 0, units = (tiles - whole) * p.kblocks;
-    const int64_t used = std::min(workers, std::max<int64_t>(units / least, 1));
-    const int64_t now = p.kblocks * ((tiles - whole + workers - 1) / workers), then = (units + used - 1) / used;
-    if (now - then < 2 * least) return p;
-    p.whole = static_cast<int32_t>(whole);
-    p.units = units;
-    p.workers = static_cast<int32_t>(used);
+    if (rest == 0) return p;
+    const int64_t share = std::max(least, (rest * kblocks + workers - 1) / workers);
+    if (kblocks - share < gain || rest * kblocks > INT32_MAX) return p;
+    const int64_t main = std::min(workers / rest, kblocks / share), tail = kblocks - main * share, others = workers - main * rest;
+    const int64_t tail_share = tail ? std::max(std::min(least, tail), (rest * tail + others - 1) / others) : 1;
+    p.whole = static_cast<int32_t>(tiles - rest);
+    p.rest = static_cast<int32_t>(rest);
+    p.main = static_cast<int32_t>(main);
+    p.share = static_cast<int32_t>(share);
+    p.tail = static_cast<int32_t>(tail);
+    p.tail_share = static_cast<int32_t>(tail_share);
+    p.slots = static_cast<int32_t>(main + (tail ? (tail + tail_share - 1) / tail_share + 1 : 0));
+    p.workers = static_cast<int32_t>(p.whole ? workers : main * rest + (rest * tail + tail_share - 1) / tail_share);
     return p;
 }
 
@@ -194,7 +198,7 @@ namespace {
 constexpr int kPerSm = 2;
 
 LinearPlan product_plan(int32_t dtype, int64_t m, int64_t n, int64_t k) {
-    return dtype == SXCUDA_F32 ? linear_plan(m, n, k, kTile, kTile, kDepth, static_cast<int64_t>(sm_count()) * kPerSm, 8)
+    return dtype == SXCUDA_F32 ? linear_plan(m, n, k, kTile, kTile, kDepth, static_cast<int64_t>(sm_count()) * kPerSm, 8, 32)
                                : linear_tc_plan(m, n, k);
 }
 
@@ -206,7 +210,7 @@ void launch_product(const LinearProduct& p, cudaStream_t s) {
     by_dtype(p.dtype, [&](auto t) {
         const auto join = linear_join_kernel<decltype(t)>;
         const int64_t rows = std::min<int64_t>(p.m, p.plan.tile_m);
-        SX_LAUNCH(join, dim3(blocks_for(rows * (p.plan.tile_n / 8), 256), static_cast<unsigned>(p.plan.tiles() - p.plan.whole)), 256, 0, s, p);
+        SX_LAUNCH(join, dim3(blocks_for(rows * (p.plan.tile_n / 8), 256), static_cast<unsigned>(p.plan.rest)), 256, 0, s, p);
     });
 }
 
@@ -284,14 +288,30 @@ __global__ void __launch_bounds__(kSlopeWarps * 32) linear_slope_kernel(const Sl
         if (col < a.cols) a.sums[blockIdx.y * a.cols + col] = x;
     }
 }
-__global__ void __launch_bounds__(256) linear_bias_kernel(const float* sums, int64_t slices, int64_t cols, void* v_bias, int32_t dtype) {
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-    if (c >= cols) return;
-    float x = 0.f;
-    for (int64_t i = 0; i < slices; ++i) x += sums[i * cols + c];
-    if (dtype == SXCUDA_F32) static_cast<float*>(v_bias)[c] = x;
-    else if (dtype == SXCUDA_F16) static_cast<__half*>(v_bias)[c] = __float2half_rn(x);
-    else static_cast<__nv_bfloat16*>(v_bias)[c] = __float2bfloat16_rn(x);
+// Adds the slices' sums of 32 columns: warp w takes every 32nd slice, eight in flight, then the warps are
+// added in order.
+__global__ void __launch_bounds__(1024) linear_bias_kernel(const float* part, int64_t slices, int64_t cols, void* v_bias, int32_t dtype) {
+    __shared__ float sums[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+    float s = 0.f;
+    if (c < cols)
+        for (int64_t r = warp; r < slices; r += 8 * 32) {
+            float x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = r + i * 32 < slices ? part[(r + i * 32) * cols + c] : 0.f;
+            s += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+        }
+    sums[warp][lane] = s;
+    __syncthreads();
+    s = sums[lane][warp];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 + warp;
+    if (lane || at >= cols) return;
+    if (dtype == SXCUDA_F32) static_cast<float*>(v_bias)[at] = s;
+    else if (dtype == SXCUDA_F16) static_cast<__half*>(v_bias)[at] = __float2half_rn(s);
+    else static_cast<__nv_bfloat16*>(v_bias)[at] = __float2bfloat16_rn(s);
 }
 
 struct SlopePlan {
@@ -389,7 +409,7 @@ void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const
             SX_LAUNCH(kernel, dim3(static_cast<unsigned>(plan.strips), static_cast<unsigned>(plan.slices)), kSlopeWarps * 32, 0, s, a);
         });
         if (out.v_bias)
-            SX_LAUNCH(linear_bias_kernel, blocks_for(in.out_features, 256), 256, 0, s, a.sums, plan.slices, in.out_features, out.v_bias, in.bias_dtype);
+            SX_LAUNCH(linear_bias_kernel, blocks_for(in.out_features, 32), 1024, 0, s, a.sums, plan.slices, in.out_features, out.v_bias, in.bias_dtype);
     }
     LinearProduct p{};
     p.dtype = in.dtype;

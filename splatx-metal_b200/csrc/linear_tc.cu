@@ -108,6 +108,13 @@ __host__ __device__ constexpr uint32_t pair_shape(int n, bool a_across, bool b_a
            static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(kTileM >> 4) << 24;
 }
 
+// The columns that a tile's products have: half of them where the product's last ones need no more.
+template <int TN>
+__device__ __forceinline__ int columns(const LinearProduct& p, const LinearTile& tile) {
+    if constexpr (TN == 256) return p.n - static_cast<int64_t>(tile.n) * TN <= TN / 2 ? TN / 2 : TN;
+    return TN;
+}
+
 // ---- loads ----
 template <int ROWS, bool ACROSS>  // ROWS rows from `row` and 64 values of K from `k`
 __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* map, int row, int k, uint32_t bar) {
@@ -150,7 +157,7 @@ __device__ __forceinline__ void store_values(T* p, bool wide, const float (&x)[1
 template <int ACT>
 __device__ __forceinline__ void activate(float (&x)[16]) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = act_fast<ACT>(x[i]);
+    for (int i = 0; i < 16; i += 2) act_pair<ACT>(x[i], x[i + 1]);
 }
 
 // How the rows of y, pre and residual are reached: 32 or 16 bytes at a time, or value by value.
@@ -220,9 +227,9 @@ __device__ __forceinline__ void finish(const LinearProduct& p, Reach reach, cons
     }
 }
 __device__ __forceinline__ void leave(const LinearProduct& p, int slot, int row, int col, uint32_t (&r)[32]) {
-    float* part = p.parts + slot * p.plan.slot_values() + (static_cast<int64_t>(col / 8) * kTileM + row) * 8;
+    float* part = p.parts + slot * p.plan.slot_values() + row * p.plan.tile_n + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tc::store32(part + i * kTileM * 8, *reinterpret_cast<uint32_t(*)[8]>(r + 8 * i));
+    for (int i = 0; i < 4; ++i) tc::store32(part + 8 * i, *reinterpret_cast<uint32_t(*)[8]>(r + 8 * i));
 }
 
 template <typename T, int TN, bool A_ACROSS, bool B_ACROSS>
@@ -264,7 +271,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         bool ok = true;
         while (ok && walk.next(p.plan, piece)) {
             const LinearTile tile = linear_tile(p.plan, piece.tile);
-            const int m = tile.m * kTileM + static_cast<int>(rank) * kRows, n = tile.n * TN + static_cast<int>(rank) * (TN / 2);
+            const int m = tile.m * kTileM + static_cast<int>(rank) * kRows, n = tile.n * TN + static_cast<int>(rank) * (columns<TN>(p, tile) / 2);
             for (int k = piece.k0; k < piece.k1; ++k) {
                 if (asked >= kStages) ok = tc::bar_wait(bars.empty(slot), parity ^ 1, failed);
                 if (!ok) break;
@@ -284,12 +291,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     } else if (warp == 9) {
         if (rank == 0) {
             const uint32_t one = tc::elect();
-            constexpr uint32_t shape = pair_shape<T>(TN, A_ACROSS, B_ACROSS);
             int slot = 0, count = 0;
             uint32_t parity = 0;
             bool ok = true;
             for (; ok && walk.next(p.plan, piece); ++count) {
                 const uint32_t d = tmem + (count & 1) * TN;
+                const uint32_t shape = pair_shape<T>(columns<TN>(p, linear_tile(p.plan, piece.tile)), A_ACROSS, B_ACROSS);
                 if (count >= 2) ok = tc::bar_wait(bars.acc_empty(count & 1), ((count >> 1) & 1) ^ 1, failed);
                 tc::fence_after();
                 for (int k = piece.k0; ok && k < piece.k1; ++k) {
@@ -431,8 +438,9 @@ bool linear_tc_takes(const void* data, int64_t stride, int64_t rows) {
 
 LinearPlan linear_tc_plan(int64_t m, int64_t n, int64_t k) {
     const int64_t pairs = sm_count() / 2;
-    const bool narrow = n <= 128 || (m + kTileM - 1) / kTileM * ((n + 255) / 256) < pairs;
-    return linear_plan(m, n, k, kTileM, narrow ? 128 : 256, kDepth, pairs, 4);
+    const int64_t tiles = (m + kTileM - 1) / kTileM * ((n + 255) / 256);
+    const bool narrow = n <= 128 || (tiles < pairs && tiles * ((k + kDepth - 1) / kDepth) < 16 * pairs);
+    return linear_plan(m, n, k, kTileM, narrow ? 128 : 256, kDepth, pairs, 4, 24);
 }
 
 void launch_linear_tc(const LinearProduct& p, cudaStream_t s) {

@@ -9,9 +9,10 @@
 // Bound by memory: each value is read once and written once. A row (one head of one token) belongs to a
 // group of lanes of a warp; a thread holds V first values of pairs and their V partners, so that the rotation
 // needs no other lane, and 16-byte accesses where the pairs' layout allows them (V = 8 values of 16 bits).
-// A warp takes one token at a time: its lanes share the token's sines and cosines (through shared memory,
-// once for all heads), which then stay in registers, as the weights do for the whole kernel: a CTA works
-// on queries only or on keys only. The next row and the next token's position are on their way meanwhile.
+// A warp takes one token at a time, its queries and then its keys: its lanes make the token's sines and
+// cosines once for all heads, in shared memory, in the order in which lanes read them; the weights lie there
+// in the same way. Groups of a warp read the same entries at the same time, so that a read is one pass of
+// shared memory, and registers are left for warps and for rows that are on their way.
 // Angles: position x frequency in turns in 64 bits, the nearest quarter turn taken off there; what is left
 // is at most an eighth, and its 32 bits are exact to 2^-28 of a turn however far the position.
 #include <algorithm>
@@ -19,6 +20,7 @@
 
 #include "sx_internal.h"
 #include "sx_network.h"
+#include "sx_two.cuh"
 
 namespace sx {
 namespace {
@@ -34,16 +36,15 @@ struct RotHalf {  // the queries or the keys
     int64_t x_batch, x_token, x_head, g_batch, g_token, g_head, out_batch, out_token, out_head;
     const void* weight;
     float* part;  // [blocks, dim]: the CTAs' sums for the weight's gradient
-    int32_t heads, chunk, chunks;  // heads; those of a unit of work; units a token
-    int32_t blocks;
-    int64_t units;
+    int32_t heads, turns;  // turns: of a warp's groups until all heads are done
 };
 
 struct RotArgs {
     RotHalf half[2];
     const void* positions;
     int64_t pos_batch, pos_token, pos_axis;
-    int64_t tokens;
+    int64_t tokens, units;
+    int32_t chunk, chunks;  // turns of a unit of work, units of a token
     int32_t pos_dtype, param_dtype, axes, dim, pairs, slots, lanes;  // slots: V pairs each; lanes: of a row's group
     int32_t mode, norm;
     int32_t axis_dims[4];
@@ -89,21 +90,43 @@ struct Row {
     Pack<T, V> first[NV], second[NV];
 };
 
-// The thread's part of one kernel: which rows, pairs and weights are its own.
+// V values in pairs that one instruction works on.
+template <int V>
+struct Values {
+    static constexpr int N = (V + 1) / 2;
+    tc::Two v[N];
+};
+
+extern __shared__ double rot_smem[];
+
+// The thread's part of a kernel.
 template <typename T, int V, bool NB, int NV>
 struct Rot {
-    static constexpr int W = V < 4 ? V : 4;  // values of a table access
+    static constexpr int W = V < 4 ? V : 4;      // values of a table access
+    static constexpr int N = Values<V>::N;
     const RotArgs& a;
-    const RotHalf& h;
-    float* table;  // [2 V / W][slots][W]: cosines, then sines, in the order in which lanes read them
-    const double* turns;
-    const uint8_t* axis;
+    double* turns;
+    float* weights;  // of queries, then of keys: [2][2 V / W][slots][W], first values and partners
+    float* table;    // [2 V / W][slots][W]: cosines, then sines of the warp's token
+    uint8_t* axis;
     int lane, group, in_group, rows;  // rows: groups of a warp
     Slot at[NV];
     bool mine[NV];
 
-    __device__ Rot(const RotArgs& a, const RotHalf& h, float* table, const double* turns, const uint8_t* axis)
-        : a(a), h(h), table(table), turns(turns), axis(axis), lane(threadIdx.x & 31) {
+    __device__ explicit Rot(const RotArgs& a) : a(a), turns(rot_smem), lane(threadIdx.x & 31) {
+        const int width = 2 * a.slots * V;
+        weights = reinterpret_cast<float*>(rot_smem + (a.pairs + 1) / 2 * 2);
+        table = weights + (2 + (threadIdx.x >> 5)) * width;
+        axis = reinterpret_cast<uint8_t*>(weights + (2 + kRotWarps) * width);
+        for (int i = threadIdx.x; i < a.pairs; i += kRotThreads) turns[i] = a.turns[i], axis[i] = a.axis[i];
+        for (int i = threadIdx.x; i < 2 * a.slots * V; i += kRotThreads) {
+            const int k = i >= a.slots * V, pair = i - k * a.slots * V;
+            const Slot s = slot_at<V>(a, pair / V);
+            const RotHalf& h = a.half[k];
+            const int one = place(s, pair % V, 0), two = place(s, pair % V, 1);
+            *entry(weights + k * width, pair, 0) = rot_param(h.weight, a.param_dtype, one);
+            *entry(weights + k * width, pair, V) = two < 0 ? 0.f : rot_param(h.weight, a.param_dtype, two);
+        }
         group = lane / a.lanes;
         in_group = lane % a.lanes;
         rows = 32 / a.lanes;
@@ -113,23 +136,42 @@ struct Rot {
             mine[n] = slot < a.slots;
             at[n] = mine[n] ? slot_at<V>(a, slot) : Slot{0, -1};
         }
-        for (int i = lane; i < a.slots * V; i += 32) *entry(i, 0) = 1.f, *entry(i, V) = 0.f;  // not rotated
-        __syncwarp();
+        for (int i = lane; i < a.slots * V; i += 32) *entry(table, i, 0) = 1.f, *entry(table, i, V) = 0.f;  // not rotated
+        __syncthreads();
     }
-    __device__ float* entry(int pair, int skip) const {
+    static size_t smem_bytes(const RotArgs& a) {
+        return (a.pairs + 1) / 2 * 2 * 8 + static_cast<size_t>(2 + kRotWarps) * 2 * a.slots * V * 4 + a.pairs;
+    }
+    __device__ float* entry(float* t, int pair, int skip) const {
         const int slot = pair / V, e = pair % V + skip;
-        return table + ((e / W) * a.slots + slot) * W + e % W;
+        return t + ((e / W) * a.slots + slot) * W + e % W;
+    }
+    // The entries of the thread's slot n: V of them from `skip`.
+    __device__ Values<V> entries(const float* t, int n, int skip) const {
+        const int slot = mine[n] ? in_group + n * a.lanes : 0;
+        Values<V> r;
+#pragma unroll
+        for (int e = 0; e < V; e += W) {
+            const auto x = reinterpret_cast<const Pack<float, W>*>(t)[((skip + e) / W) * a.slots + slot];
+            if constexpr (W == 1) {
+                r.v[0] = tc::two(x.v[0], 0.f);
+            } else {
+#pragma unroll
+                for (int k = 0; k < W; k += 2) r.v[(e + k) / 2] = tc::two(x.v[k], x.v[k + 1]);
+            }
+        }
+        return r;
     }
     // Lane i's position along axis i.
     __device__ double position(int64_t unit) const {
-        if (lane >= a.axes || unit >= h.units) return 0.;
-        const int64_t token = unit / h.chunks, b = token / a.tokens;
-        const int64_t i = b * a.pos_batch + (token - b * a.tokens) * a.pos_token + lane * a.pos_axis;
+        if (lane >= a.axes || unit >= a.units) return 0.;
+        const Token t = token_of(unit);
+        const int64_t i = t.batch * a.pos_batch + t.token * a.pos_token + lane * a.pos_axis;
         if (a.pos_dtype == SXCUDA_POS_F32) return static_cast<const float*>(a.positions)[i];
         if (a.pos_dtype == SXCUDA_POS_I32) return static_cast<const int32_t*>(a.positions)[i];
         return static_cast<double>(static_cast<const int64_t*>(a.positions)[i]);
     }
-    __device__ void angles(double mine_position, float (&c)[NV][V], float (&s)[NV][V]) const {
+    __device__ void angles(double mine_position) const {
         __syncwarp();
         for (int i = lane; i - lane < a.pairs; i += 32) {
             const int j = i < a.pairs ? i : 0;
@@ -141,33 +183,64 @@ struct Rot {
             const int q = static_cast<int>(static_cast<long long>(fabs(quarters) < 9e15 ? quarters : 0.) & 3);
             const float cc = q & 1 ? sine : cosine, ss = q & 1 ? cosine : sine;
             if (i < a.pairs) {
-                *entry(i, 0) = q == 1 || q == 2 ? -cc : cc;
-                *entry(i, V) = q >= 2 ? -ss : ss;
+                *entry(table, i, 0) = q == 1 || q == 2 ? -cc : cc;
+                *entry(table, i, V) = q >= 2 ? -ss : ss;
             }
         }
         __syncwarp();
-#pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const int slot = mine[n] ? in_group + n * a.lanes : 0;
-#pragma unroll
-            for (int e = 0; e < V; e += W) {
-                const auto x = reinterpret_cast<const Pack<float, W>*>(table)[(e / W) * a.slots + slot];
-                const auto y = reinterpret_cast<const Pack<float, W>*>(table)[((V + e) / W) * a.slots + slot];
-#pragma unroll
-                for (int k = 0; k < W; ++k) c[n][e + k] = x.v[k], s[n][e + k] = y.v[k];
-            }
+    }
+    struct Token {
+        int64_t batch, token;
+        int chunk;
+    };
+    __device__ Token token_of(int64_t unit) const {
+        if (a.units <= INT32_MAX) {  // 64-bit divisions take some hundred instructions
+            const uint32_t u = static_cast<uint32_t>(unit), t = u / static_cast<uint32_t>(a.chunks);
+            const uint32_t n = static_cast<uint32_t>(a.tokens), b = t / n;
+            return {b, t - b * n, static_cast<int>(u - t * a.chunks)};
         }
+        const int64_t t = unit / a.chunks, b = t / a.tokens;
+        return {b, t - b * a.tokens, static_cast<int>(unit - t * a.chunks)};
     }
-    // The group's head of a unit in its turn `it`; -1: none left.
-    __device__ int head_of(int64_t unit, int it) const {
-        const int in_chunk = it * rows + group, head = static_cast<int>(unit % h.chunks) * h.chunk + in_chunk;
-        return unit < h.units && in_chunk < h.chunk && head < h.heads ? head : -1;
+    // A turn of the warp's groups: where the group's row is, and whether there is one.
+    struct Turn {
+        int64_t unit, x, g, out;
+        int number;  // of the token's turns: first the queries', then the keys'
+        int end;     // the unit's last one, and one
+        bool there;
+    };
+    __device__ Turn first_turn(int64_t unit) const {
+        if (unit >= a.units) return {unit, 0, 0, 0, 0, 0, false};
+        const Token t = token_of(unit);
+        Turn r{unit, t.batch, t.token, 0, t.chunk * a.chunk, 0, false};
+        r.end = min(r.number + a.chunk, a.half[0].turns + a.half[1].turns);
+        return head_of(r, t.batch, t.token);
     }
-    __device__ int64_t offset(int64_t unit, int head, int64_t batch, int64_t token, int64_t head_stride) const {
-        const int64_t t = unit / h.chunks, b = t / a.tokens;
-        return b * batch + (t - b * a.tokens) * token + head * head_stride;
+    __device__ Turn head_of(Turn r, int64_t batch, int64_t token) const {
+        const int k = r.number >= a.half[0].turns;
+        const RotHalf& h = a.half[k];
+        const int head = (r.number - (k ? a.half[0].turns : 0)) * rows + group;
+        r.there = head < h.heads;
+        r.x = batch * h.x_batch + token * h.x_token + head * h.x_head;
+        r.g = batch * h.g_batch + token * h.g_token + head * h.g_head;
+        r.out = batch * h.out_batch + token * h.out_token + head * h.out_head;
+        return r;
     }
-    __device__ void load(Row<T, V, NV>& r, const T* row, bool there) const {
+    __device__ Turn next_turn(Turn r, int64_t step) const {
+        if (++r.number == r.end) return first_turn(r.unit + step);
+        if (r.number == a.half[0].turns) {  // from the queries to the keys
+            const Token t = token_of(r.unit);
+            return head_of(r, t.batch, t.token);
+        }
+        const int k = r.number >= a.half[0].turns;
+        const RotHalf& h = a.half[k];
+        r.x += rows * h.x_head, r.g += rows * h.g_head, r.out += rows * h.out_head;
+        r.there = (r.number - (k ? a.half[0].turns : 0)) * rows + group < h.heads;
+        return r;
+    }
+    __device__ bool keys(const Turn& r) const { return r.number >= a.half[0].turns; }
+    __device__ void load(Row<T, V, NV>& r, const void* base, int64_t offset, bool there) const {
+        const T* row = static_cast<const T*>(base) + offset;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             r.first[n] = r.second[n] = Pack<T, V>{};
@@ -177,13 +250,22 @@ struct Rot {
             }
         }
     }
-    __device__ void store(T* row, const float (&p)[NV][V], const float (&q)[NV][V]) const {
+    __device__ void store(void* base, int64_t offset, const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
+        T* row = static_cast<T*>(base) + offset;
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             if (!mine[n]) continue;
             Pack<T, V> x, y;
 #pragma unroll
-            for (int e = 0; e < V; ++e) *value(x, y, e, 0) = from_f32<T>(p[n][e]), *value(x, y, e, 1) = from_f32<T>(q[n][e]);
+            for (int e = 0; e < V; e += 2) {
+                float lo, hi;
+                tc::split(p[n].v[e / 2], lo, hi);
+                *value(x, y, e, 0) = from_f32<T>(lo);
+                if constexpr (V > 1) *value(x, y, e + 1, 0) = from_f32<T>(hi);
+                tc::split(q[n].v[e / 2], lo, hi);
+                *value(x, y, e, 1) = from_f32<T>(lo);
+                if constexpr (V > 1) *value(x, y, e + 1, 1) = from_f32<T>(hi);
+            }
             *reinterpret_cast<Pack<T, V>*>(row + at[n].first) = x;
             if (at[n].second >= 0) *reinterpret_cast<Pack<T, V>*>(row + at[n].second) = y;
         }
@@ -198,222 +280,223 @@ struct Rot {
             return second ? &y.v[e] : &x.v[e];
         }
     }
-    // The place in the head of the first (second) value of pair e of slot n.
-    __device__ int place(int n, int e, int second) const {
+    // The place in the head of the first (second) value of a slot's pair e; -1: there is none.
+    static __device__ int place(const Slot& s, int e, int second) {
         if constexpr (NB) {
             const int i = 2 * e + second;
-            return i < V ? at[n].first + i : at[n].second < 0 ? -1 : at[n].second + i - V;
+            return i < V ? s.first + i : s.second < 0 ? -1 : s.second + i - V;
         } else {
-            return second ? (at[n].second < 0 ? -1 : at[n].second + e) : at[n].first + e;
+            return second ? (s.second < 0 ? -1 : s.second + e) : s.first + e;
         }
     }
-    __device__ void unpack(const Row<T, V, NV>& r, float (&p)[NV][V], float (&q)[NV][V]) const {
+    static __device__ void unpack(const Row<T, V, NV>& r, Values<V> (&p)[NV], Values<V> (&q)[NV]) {
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
-            for (int e = 0; e < V; ++e)
-                p[n][e] = to_f32(*value(r.first[n], r.second[n], e, 0)), q[n][e] = to_f32(*value(r.first[n], r.second[n], e, 1));
-    }
-    __device__ float group_sum(float x) const {
-        for (int o = a.lanes / 2; o; o >>= 1) x += __shfl_xor_sync(kFullMask, x, o);
-        return x;
-    }
-    __device__ void weights(float (&p)[NV][V], float (&q)[NV][V]) const {
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const int i = place(n, e, 0), j = place(n, e, 1);
-                p[n][e] = mine[n] ? rot_param(h.weight, a.param_dtype, i) : 0.f;
-                q[n][e] = mine[n] && j >= 0 ? rot_param(h.weight, a.param_dtype, j) : 0.f;
+            for (int e = 0; e < V; e += 2) {
+                const auto get = [&](int i, int second) { return i < V ? to_f32(*value(r.first[n], r.second[n], i, second)) : 0.f; };
+                p[n].v[e / 2] = tc::two(get(e, 0), get(e + 1, 0));
+                q[n].v[e / 2] = tc::two(get(e, 1), get(e + 1, 1));
             }
     }
-    __device__ float rstd(const float (&p)[NV][V], const float (&q)[NV][V]) const {
-        float ss = 0.f;
+    __device__ float group_sum(tc::Two x) const {
+        float lo, hi;
+        tc::split(x, lo, hi);
+        lo += hi;
+        for (int o = a.lanes / 2; o; o >>= 1) lo += __shfl_xor_sync(kFullMask, lo, o);
+        return lo;
+    }
+    __device__ float rstd(const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
+        tc::Two ss = tc::two(0.f, 0.f);
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
-            for (int e = 0; e < V; ++e) ss = fmaf(p[n][e], p[n][e], fmaf(q[n][e], q[n][e], ss));
+            for (int e = 0; e < N; ++e) ss = tc::fma2(p[n].v[e], p[n].v[e], tc::fma2(q[n].v[e], q[n].v[e], ss));
         return __frsqrt_rn(fmaf(group_sum(ss), a.inv_dim, a.eps));
     }
 };
 
-extern __shared__ double rot_smem[];
-
-// The CTA's half, its number among that half's CTAs, and the tables in shared memory.
-struct RotPlace {
-    const RotHalf* half;
-    int block;
-    double* turns;
-    uint8_t* axis;
-    float* table;
-};
-__device__ __forceinline__ RotPlace rot_place(const RotArgs& a, int width) {
-    const int k = blockIdx.x >= a.half[0].blocks;
-    RotPlace p{&a.half[k], static_cast<int>(blockIdx.x) - (k ? a.half[0].blocks : 0), rot_smem, nullptr, nullptr};
-    p.table = reinterpret_cast<float*>(rot_smem + (a.pairs + 1) / 2 * 2) + (threadIdx.x >> 5) * 2 * width;
-    p.axis = reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(rot_smem + (a.pairs + 1) / 2 * 2) + kRotWarps * 2 * width);
-    for (int i = threadIdx.x; i < a.pairs; i += kRotThreads) p.turns[i] = a.turns[i], p.axis[i] = a.axis[i];
-    __syncthreads();
-    return p;
-}
-size_t rot_smem_bytes(const RotArgs& a, int v) {
-    return (a.pairs + 1) / 2 * 2 * 8 + static_cast<size_t>(kRotWarps) * 2 * a.slots * v * 4 + a.pairs;
-}
-
 template <typename T, int V, bool NB, int NV>
-__global__ void __launch_bounds__(kRotThreads) rotary_fwd_kernel(const __grid_constant__ RotArgs a) {
-    const RotPlace at = rot_place(a, a.slots * V);
-    const Rot<T, V, NB, NV> me(a, *at.half, at.table, at.turns, at.axis);
-    const RotHalf& h = me.h;
-    const int64_t step = static_cast<int64_t>(h.blocks) * kRotWarps;
-    const int turns = (h.chunk + me.rows - 1) / me.rows;
-    float w0[NV][V], w1[NV][V], c[NV][V], s[NV][V];
-    me.weights(w0, w1);
-    int64_t unit = static_cast<int64_t>(at.block) * kRotWarps + (threadIdx.x >> 5);
-    int it = 0;
-    const auto fetch = [&](Row<T, V, NV>& r, int64_t u, int i) {
-        const int head = me.head_of(u, i);
-        me.load(r, static_cast<const T*>(h.x) + (head < 0 ? 0 : me.offset(u, head, h.x_batch, h.x_token, h.x_head)), head >= 0);
-    };
+__global__ void __launch_bounds__(kRotThreads, V == 1 ? 2 : 7) rotary_fwd_kernel(const __grid_constant__ RotArgs a) {
+    const Rot<T, V, NB, NV> me(a);
+    using Me = Rot<T, V, NB, NV>;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRotWarps;
+    const tc::Two minus = tc::two(-1.f, -1.f);
+    auto turn = me.first_turn(static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5));
     Row<T, V, NV> row;
-    fetch(row, unit, 0);
-    double position = me.position(unit);
-    while (unit < h.units) {
-        const bool last = it + 1 == turns;
-        const int64_t next_unit = last ? unit + step : unit;
-        const int next_it = last ? 0 : it + 1;
-        Row<T, V, NV> next;
-        fetch(next, next_unit, next_it);
-        if (it == 0) {
-            me.angles(position, c, s);
+    me.load(row, a.half[me.keys(turn)].x, turn.x, turn.there);
+    double position = me.position(turn.unit);
+    int64_t unit = -1;
+    while (turn.unit < a.units) {
+        const auto next = me.next_turn(turn, step);
+        Row<T, V, NV> next_row;
+        me.load(next_row, a.half[me.keys(next)].x, next.x, next.there);
+        if (turn.unit != unit) {
+            me.angles(position);
+            unit = turn.unit;
             position = me.position(unit + step);
         }
-        float p[NV][V], q[NV][V];
-        me.unpack(row, p, q);
-        const float r = a.norm ? me.rstd(p, q) : 1.f;
+        Values<V> p[NV], q[NV];
+        Me::unpack(row, p, q);
+        const bool k = me.keys(turn);
+        if (a.norm) {
+            const float r = me.rstd(p, q);
+            const tc::Two rr = tc::two(r, r);
+            const float* w = me.weights + (k ? 2 * a.slots * V : 0);
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
+            for (int n = 0; n < NV; ++n) {
+                const Values<V> w0 = me.entries(w, n, 0), w1 = me.entries(w, n, V);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float u1 = p[n][e] * r * w0[n][e], u2 = q[n][e] * r * w1[n][e];
-                p[n][e] = fmaf(u1, c[n][e], -u2 * s[n][e]);
-                q[n][e] = fmaf(u1, s[n][e], u2 * c[n][e]);
+                for (int e = 0; e < Me::N; ++e) {
+                    p[n].v[e] = tc::mul2(tc::mul2(p[n].v[e], rr), w0.v[e]);
+                    q[n].v[e] = tc::mul2(tc::mul2(q[n].v[e], rr), w1.v[e]);
+                }
             }
-        const int head = me.head_of(unit, it);
-        if (head >= 0) me.store(static_cast<T*>(h.out) + me.offset(unit, head, h.out_batch, h.out_token, h.out_head), p, q);
-        row = next;
-        unit = next_unit;
-        it = next_it;
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
+#pragma unroll
+            for (int e = 0; e < Me::N; ++e) {
+                const tc::Two u1 = p[n].v[e], u2 = q[n].v[e];
+                p[n].v[e] = tc::fma2(u1, c.v[e], tc::mul2(tc::mul2(u2, minus), s.v[e]));
+                q[n].v[e] = tc::fma2(u1, s.v[e], tc::mul2(u2, c.v[e]));
+            }
+        }
+        if (turn.there) me.store(a.half[k].out, turn.out, p, q);
+        row = next_row;
+        turn = next;
     }
 }
 
 template <typename T, int V, bool NB, int NV>
-__global__ void __launch_bounds__(kRotThreads) rotary_bwd_kernel(const __grid_constant__ RotArgs a) {
-    const RotPlace at = rot_place(a, a.slots * V);
-    const Rot<T, V, NB, NV> me(a, *at.half, at.table, at.turns, at.axis);
-    const RotHalf& h = me.h;
-    const int64_t step = static_cast<int64_t>(h.blocks) * kRotWarps;
-    const int turns = (h.chunk + me.rows - 1) / me.rows;
-    float w0[NV][V], w1[NV][V], c[NV][V], s[NV][V], sum0[NV][V] = {}, sum1[NV][V] = {};
-    me.weights(w0, w1);
-    int64_t unit = static_cast<int64_t>(at.block) * kRotWarps + (threadIdx.x >> 5);
-    int it = 0;
-    const auto fetch = [&](Row<T, V, NV>& x, Row<T, V, NV>& g, int64_t u, int i) {
-        const int head = me.head_of(u, i);
-        me.load(g, static_cast<const T*>(h.g) + (head < 0 ? 0 : me.offset(u, head, h.g_batch, h.g_token, h.g_head)), head >= 0);
-        me.load(x, static_cast<const T*>(h.x) + (head < 0 ? 0 : me.offset(u, head, h.x_batch, h.x_token, h.x_head)),
-                head >= 0 && a.norm);
-    };
+__global__ void __launch_bounds__(kRotThreads, V == 1 ? 2 : 4) rotary_bwd_kernel(const __grid_constant__ RotArgs a) {
+    const Rot<T, V, NB, NV> me(a);
+    using Me = Rot<T, V, NB, NV>;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRotWarps;
+    const tc::Two minus = tc::two(-1.f, -1.f);
+    Values<V> sum[2][2][NV];  // of queries and keys, first values and partners
+#pragma unroll
+    for (int i = 0; i < 4 * NV; ++i)
+#pragma unroll
+        for (int e = 0; e < Me::N; ++e) sum[i / NV / 2][i / NV % 2][i % NV].v[e] = tc::two(0.f, 0.f);
+    auto turn = me.first_turn(static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5));
     Row<T, V, NV> x_row, g_row;
-    fetch(x_row, g_row, unit, 0);
-    double position = me.position(unit);
-    while (unit < h.units) {
-        const bool last = it + 1 == turns;
-        const int64_t next_unit = last ? unit + step : unit;
-        const int next_it = last ? 0 : it + 1;
+    me.load(g_row, a.half[me.keys(turn)].g, turn.g, turn.there);
+    me.load(x_row, a.half[me.keys(turn)].x, turn.x, turn.there && a.norm);
+    double position = me.position(turn.unit);
+    int64_t unit = -1;
+    while (turn.unit < a.units) {
+        const auto next = me.next_turn(turn, step);
         Row<T, V, NV> x_next, g_next;
-        fetch(x_next, g_next, next_unit, next_it);
-        if (it == 0) {
-            me.angles(position, c, s);
+        me.load(g_next, a.half[me.keys(next)].g, next.g, next.there);
+        me.load(x_next, a.half[me.keys(next)].x, next.x, next.there && a.norm);
+        if (turn.unit != unit) {
+            me.angles(position);
+            unit = turn.unit;
             position = me.position(unit + step);
         }
-        const int head = me.head_of(unit, it);
-        float p[NV][V], q[NV][V];
-        me.unpack(g_row, p, q);
+        const bool k = me.keys(turn);
+        Values<V> p[NV], q[NV];
+        Me::unpack(g_row, p, q);
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
+        for (int n = 0; n < NV; ++n) {
+            const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float g1 = p[n][e], g2 = q[n][e];
-                p[n][e] = fmaf(g1, c[n][e], g2 * s[n][e]);
-                q[n][e] = fmaf(g2, c[n][e], -g1 * s[n][e]);
+            for (int e = 0; e < Me::N; ++e) {
+                const tc::Two g1 = p[n].v[e], g2 = q[n].v[e];
+                p[n].v[e] = tc::fma2(g1, c.v[e], tc::mul2(g2, s.v[e]));
+                q[n].v[e] = tc::fma2(g2, c.v[e], tc::mul2(tc::mul2(g1, minus), s.v[e]));
             }
+        }
         if (a.norm) {
-            float x0[NV][V], x1[NV][V];
-            me.unpack(x_row, x0, x1);
+            Values<V> x0[NV], x1[NV];
+            Me::unpack(x_row, x0, x1);
             const float r = me.rstd(x0, x1);
-            float dot = 0.f;
+            const tc::Two rr = tc::two(r, r);
+            const float* w = me.weights + (k ? 2 * a.slots * V : 0);
+            tc::Two dot = tc::two(0.f, 0.f);
+            const auto add = [&](Values<V> (&sums)[2][NV]) {
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
+                for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    x0[n][e] *= r, x1[n][e] *= r;
-                    if (head >= 0) {  // of a group without a row r may be infinite
-                        sum0[n][e] = fmaf(p[n][e], x0[n][e], sum0[n][e]);
-                        sum1[n][e] = fmaf(q[n][e], x1[n][e], sum1[n][e]);
+                    for (int e = 0; e < Me::N; ++e) {
+                        sums[0][n].v[e] = tc::fma2(p[n].v[e], x0[n].v[e], sums[0][n].v[e]);
+                        sums[1][n].v[e] = tc::fma2(q[n].v[e], x1[n].v[e], sums[1][n].v[e]);
                     }
-                    p[n][e] *= w0[n][e], q[n][e] *= w1[n][e];
-                    dot = fmaf(p[n][e], x0[n][e], fmaf(q[n][e], x1[n][e], dot));
-                }
-            dot = me.group_sum(dot) * a.inv_dim;
+            };
 #pragma unroll
             for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    p[n][e] = fmaf(-x0[n][e], dot, p[n][e]) * r;
-                    q[n][e] = fmaf(-x1[n][e], dot, q[n][e]) * r;
+                for (int e = 0; e < Me::N; ++e) x0[n].v[e] = tc::mul2(x0[n].v[e], rr), x1[n].v[e] = tc::mul2(x1[n].v[e], rr);
+            if (turn.there) {  // of a group without a row r may be infinite
+                if (k) add(sum[1]);
+                else add(sum[0]);
+            }
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const Values<V> w0 = me.entries(w, n, 0), w1 = me.entries(w, n, V);
+#pragma unroll
+                for (int e = 0; e < Me::N; ++e) {
+                    p[n].v[e] = tc::mul2(p[n].v[e], w0.v[e]), q[n].v[e] = tc::mul2(q[n].v[e], w1.v[e]);
+                    dot = tc::fma2(p[n].v[e], x0[n].v[e], tc::fma2(q[n].v[e], x1[n].v[e], dot));
+                }
+            }
+            const float m = -me.group_sum(dot) * a.inv_dim;
+            const tc::Two mm = tc::two(m, m);
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int e = 0; e < Me::N; ++e) {
+                    p[n].v[e] = tc::mul2(tc::fma2(x0[n].v[e], mm, p[n].v[e]), rr);
+                    q[n].v[e] = tc::mul2(tc::fma2(x1[n].v[e], mm, q[n].v[e]), rr);
                 }
         }
-        if (head >= 0) me.store(static_cast<T*>(h.out) + me.offset(unit, head, h.out_batch, h.out_token, h.out_head), p, q);
+        if (turn.there) me.store(a.half[k].out, turn.out, p, q);
         x_row = x_next;
         g_row = g_next;
-        unit = next_unit;
-        it = next_it;
+        turn = next;
     }
-    if (!h.part) return;
+    if (!a.half[0].part && !a.half[1].part) return;
     // the warp's groups, then the CTA's warps, in order
-    __syncthreads();
     float* sums = reinterpret_cast<float*>(rot_smem);  // [warps, dim], over the tables
 #pragma unroll
-    for (int n = 0; n < NV; ++n)
+    for (int k = 0; k < 2; ++k) {
+        if (!a.half[k].part) continue;
+        __syncthreads();
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            float x = sum0[n][e], y = sum1[n][e];
-            for (int o = 16; o >= a.lanes; o >>= 1) x += __shfl_xor_sync(kFullMask, x, o), y += __shfl_xor_sync(kFullMask, y, o);
-            if (me.group == 0 && me.mine[n]) {
-                const int i = me.place(n, e, 0), j = me.place(n, e, 1);
-                sums[(threadIdx.x >> 5) * a.dim + i] = x;
-                if (j >= 0) sums[(threadIdx.x >> 5) * a.dim + j] = y;
+        for (int n = 0; n < NV; ++n)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float x[2], lo, hi;
+                tc::split(sum[k][0][n].v[e / 2], lo, hi);
+                x[0] = e % 2 ? hi : lo;
+                tc::split(sum[k][1][n].v[e / 2], lo, hi);
+                x[1] = e % 2 ? hi : lo;
+                for (int o = 16; o >= a.lanes; o >>= 1)
+                    x[0] += __shfl_xor_sync(kFullMask, x[0], o), x[1] += __shfl_xor_sync(kFullMask, x[1], o);
+                if (me.group == 0 && me.mine[n]) {
+                    const int i = Me::place(me.at[n], e, 0), j = Me::place(me.at[n], e, 1);
+                    sums[(threadIdx.x >> 5) * a.dim + i] = x[0];
+                    if (j >= 0) sums[(threadIdx.x >> 5) * a.dim + j] = x[1];
+                }
             }
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.dim; i += kRotThreads) {
+            float x = 0.f;
+            for (int w = 0; w < kRotWarps; ++w) x += sums[w * a.dim + i];
+            a.half[k].part[static_cast<int64_t>(blockIdx.x) * a.dim + i] = x;
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.dim; i += kRotThreads) {
-        float x = 0.f;
-        for (int w = 0; w < kRotWarps; ++w) x += sums[w * a.dim + i];
-        h.part[static_cast<int64_t>(at.block) * a.dim + i] = x;
     }
 }
 
 // Adds the CTAs' sums of 32 values: warp w takes every 32nd row, then the warps are added in order.
-__global__ void __launch_bounds__(1024) rotary_sums_kernel(const float* q_part, int64_t q_rows, const float* k_part, int64_t k_rows,
-                                                           int32_t dim, void* v_qw, void* v_kw, int32_t param_dtype) {
+__global__ void __launch_bounds__(1024) rotary_sums_kernel(const float* q_part, const float* k_part, int64_t rows, int32_t dim, void* v_qw, void* v_kw, int32_t param_dtype) {
     __shared__ float sums[32][33];
     const bool k = blockIdx.y;
     const float* part = k ? k_part : q_part;
     void* to = k ? v_kw : v_qw;
     if (!to) return;
-    const int64_t rows = k ? k_rows : q_rows;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
     float s = 0.f;
     if (c < dim)
@@ -433,11 +516,7 @@ __global__ void __launch_bounds__(1024) rotary_sums_kernel(const float* q_part, 
 }
 
 // ---- host ----
-struct RotPlan {
-    RotArgs a;
-    int v = 1;
-};
-
+constexpr int kRotMostPerSm = 8;
 bool view_fits(const SxAttentionView& x, int64_t size, int64_t bytes) {
     const auto fits = [&](int64_t n) { return n * size % bytes == 0; };
     return reinterpret_cast<uintptr_t>(x.data) % bytes == 0 && fits(x.batch_stride) && fits(x.token_stride) && fits(x.head_stride);
@@ -491,19 +570,20 @@ RotArgs rot_args(const SxRotaryInputs& in, int v) {
     return a;
 }
 
-// Units of work and CTAs. A unit is a token with all its heads, so that its sines are taken once; where there
-// are fewer tokens than half the warps that fit, a unit is as many heads as a warp has groups.
-void rot_divide(RotArgs& a, int64_t tokens, int per_sm) {
-    const int64_t most = static_cast<int64_t>(sm_count()) * per_sm;
-    const int rows = 32 / a.lanes, heads = a.half[0].heads + a.half[1].heads;
-    for (RotHalf& h : a.half) {
-        if (!h.heads) continue;
-        h.chunk = tokens * 2 >= most * kRotWarps ? h.heads : std::min(rows, h.heads);
-        h.chunks = (h.heads + h.chunk - 1) / h.chunk;
-        h.units = tokens * h.chunks;
-        const int64_t share = std::max<int64_t>(most * h.heads / heads, 1);
-        h.blocks = static_cast<int32_t>(std::min(share, (h.units + kRotWarps - 1) / kRotWarps));
-    }
+// Units of work: a token with all its heads, so that its sines are taken once; where there are fewer tokens
+// than half the warps that fit, one turn of a warp's groups.
+template <typename K>
+int rot_divide(RotArgs& a, int64_t tokens, K kernel, size_t smem) {
+    int per_sm = 0;
+    cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kRotThreads, smem), "qk_norm_rotary");
+    const int64_t most = static_cast<int64_t>(sm_count()) * std::min(std::max(per_sm, 1), kRotMostPerSm);
+    const int rows = 32 / a.lanes;
+    for (RotHalf& h : a.half) h.turns = (h.heads + rows - 1) / rows;
+    const int turns = a.half[0].turns + a.half[1].turns;
+    a.chunk = tokens * 2 >= most * kRotWarps ? turns : 1;
+    a.chunks = (turns + a.chunk - 1) / a.chunk;
+    a.units = tokens * a.chunks;
+    return static_cast<int>(std::min(most, (a.units + kRotWarps - 1) / kRotWarps));
 }
 
 // Calls f(element, pairs a thread, neighbours, slots a thread).
@@ -524,8 +604,6 @@ void by_layout(const SxRotaryInputs& in, int v, F&& f) {
     });
 }
 
-constexpr int kRotFwdPerSm = 6, kRotBwdPerSm = 4;
-
 }  // namespace
 
 void launch_qk_norm_rotary_fwd(const SxRotaryInputs& in, const SxAttentionView& q_out, const SxAttentionView& k_out, cudaStream_t s) {
@@ -538,16 +616,18 @@ void launch_qk_norm_rotary_fwd(const SxRotaryInputs& in, const SxAttentionView& 
     };
     set(a.half[0], q_out);
     if (in.k_heads) set(a.half[1], k_out);
-    rot_divide(a, tokens, kRotFwdPerSm);
     by_layout(in, v, [&](auto t, auto n, auto nb, auto slots) {
         constexpr int V = decltype(n)::value, NV = decltype(slots)::value;
-        const auto kernel = rotary_fwd_kernel<decltype(t), V, decltype(nb)::value, NV>;
-        SX_LAUNCH(kernel, static_cast<unsigned>(a.half[0].blocks + a.half[1].blocks), kRotThreads, rot_smem_bytes(a, V), s, a);
+        constexpr bool NB = decltype(nb)::value;
+        const auto kernel = rotary_fwd_kernel<decltype(t), V, NB, NV>;
+        const size_t smem = Rot<decltype(t), V, NB, NV>::smem_bytes(a);
+        const int blocks = rot_divide(a, tokens, kernel, smem);
+        SX_LAUNCH(kernel, blocks, kRotThreads, smem, s, a);
     });
 }
 
 size_t qk_norm_rotary_bwd_workspace(const SxRotaryInputs& in) {
-    return in.norm ? static_cast<size_t>(sm_count()) * kRotBwdPerSm * in.head_dim * 4 + 2 * in.head_dim * 4 : 0;
+    return in.norm ? static_cast<size_t>(sm_count()) * kRotMostPerSm * 2 * in.head_dim * 4 : 0;
 }
 
 void launch_qk_norm_rotary_bwd(const SxRotaryInputs& in, const SxRotaryGrads& g, void* ws, cudaStream_t s) {
@@ -571,19 +651,20 @@ void launch_qk_norm_rotary_bwd(const SxRotaryInputs& in, const SxRotaryGrads& g,
     };
     set(a.half[0], g.v_q_out, g.v_q);
     if (in.k_heads) set(a.half[1], g.v_k_out, g.v_k);
-    rot_divide(a, tokens, kRotBwdPerSm);
-    float* part = static_cast<float*>(ws);
-    if (g.v_q_weight) a.half[0].part = part;
-    if (g.v_k_weight) a.half[1].part = part + static_cast<int64_t>(a.half[0].blocks) * in.head_dim;
     by_layout(in, v, [&](auto t, auto n, auto nb, auto slots) {
         constexpr int V = decltype(n)::value, NV = decltype(slots)::value;
-        const auto kernel = rotary_bwd_kernel<decltype(t), V, decltype(nb)::value, NV>;
-        const size_t smem = std::max<size_t>(rot_smem_bytes(a, V), static_cast<size_t>(kRotWarps) * in.head_dim * 4);
-        SX_LAUNCH(kernel, static_cast<unsigned>(a.half[0].blocks + a.half[1].blocks), kRotThreads, smem, s, a);
+        constexpr bool NB = decltype(nb)::value;
+        const auto kernel = rotary_bwd_kernel<decltype(t), V, NB, NV>;
+        const size_t smem = std::max<size_t>(Rot<decltype(t), V, NB, NV>::smem_bytes(a), static_cast<size_t>(kRotWarps) * in.head_dim * 4);
+        const int blocks = rot_divide(a, tokens, kernel, smem);
+        float* part = static_cast<float*>(ws);
+        if (g.v_q_weight) a.half[0].part = part;
+        if (g.v_k_weight) a.half[1].part = part + static_cast<int64_t>(blocks) * in.head_dim;
+        SX_LAUNCH(kernel, blocks, kRotThreads, smem, s, a);
+        if (g.v_q_weight || g.v_k_weight)
+            SX_LAUNCH(rotary_sums_kernel, dim3(blocks_for(in.head_dim, 32), 2), 1024, 0, s, a.half[0].part, a.half[1].part, blocks,
+                      in.head_dim, g.v_q_weight, g.v_k_weight, in.param_dtype);
     });
-    if (g.v_q_weight || g.v_k_weight)
-        SX_LAUNCH(rotary_sums_kernel, dim3(blocks_for(in.head_dim, 32), 2), 1024, 0, s, a.half[0].part, a.half[0].blocks,
-                  a.half[1].part, a.half[1].blocks, in.head_dim, g.v_q_weight, g.v_k_weight, in.param_dtype);
 }
 
 }  // namespace sx

@@ -4,6 +4,7 @@
 
 #include "sx_internal.h"
 #include "sx_network.h"
+#include "sx_two.cuh"
 
 namespace sx {
 
@@ -15,21 +16,21 @@ struct LinearOperand {
     bool across;
 };
 
-// How a product's output tiles are worked on. Tiles below `whole` go round the workers; the K blocks of
-// the others are one line of units that is cut into as many equal pieces as there are workers, so that all
-// of them end together. A tile that a cut goes through is left in parts in the workspace, 32-bit sums,
-// which a second kernel adds in order.
+// How a product's output tiles are worked on. Tiles below `whole` go round the workers. The `rest`, fewer
+// than there are workers, are cut along K so that all workers end together: worker t + j rest takes the K
+// blocks [j share, (j + 1) share) of rest tile t for each j < main, so that those who run at the same time
+// read the same K blocks; the tails behind main * share make one line of rest * tail blocks that the
+// other workers divide, tail_share each. A cut tile is left in parts in the workspace, 32-bit sums, which a
+// second kernel adds in the order of K.
 struct LinearPlan {
     int32_t tile_m = 0, tile_n = 0, tiles_m = 0, tiles_n = 0, kblocks = 0, whole = 0, workers = 0;
-    int64_t units = 0;
+    int32_t rest = 0, main = 0, share = 0, tail = 0, tail_share = 1, slots = 0;  // slots: of a tile's parts
     __host__ __device__ int32_t tiles() const { return tiles_m * tiles_n; }
-    __host__ __device__ bool cut() const { return units > 0; }
-    __host__ __device__ int64_t start(int64_t worker) const { return worker * units / workers; }
-    __host__ __device__ int64_t worker_of(int64_t unit) const { return ((unit + 1) * workers - 1) / units; }
-    // Every worker may leave a part that begins in its tile's middle (slot 2 w) and one that begins at its
-    // tile's start (slot 2 w + 1).
+    __host__ __device__ bool cut() const { return rest > 0; }
+    __host__ __device__ int32_t first_tail(int32_t t) const { return t * tail / tail_share; }
+    __host__ __device__ int32_t parts(int32_t t) const { return main + (tail ? ((t + 1) * tail - 1) / tail_share - first_tail(t) + 1 : 0); }
     __host__ __device__ int64_t slot_values() const { return static_cast<int64_t>(tile_m) * tile_n; }
-    size_t workspace() const { return cut() ? static_cast<size_t>(2 * workers * slot_values()) * 4 : 0; }
+    size_t workspace() const { return static_cast<size_t>(rest) * slots * slot_values() * 4; }
 };
 
 // A product C = A B^T over K, [m, n], and its epilogue y = act(C + bias) + residual.
@@ -55,20 +56,28 @@ struct LinearPiece {
 
 // The pieces of one worker, in order.
 struct LinearWalk {
-    int64_t unit, end;
-    int32_t tile, worker;
-    __device__ LinearWalk(const LinearPlan& p, int32_t w) : unit(p.cut() ? p.start(w) : 0), end(p.cut() ? p.start(w + 1) : 0), tile(w), worker(w) {}
+    int32_t tile, main, unit, end;  // main: the piece of a rest tile that is this worker's, -1: none left
+    __device__ LinearWalk(const LinearPlan& p, int32_t w) : tile(w), main(-1), unit(0), end(0) {
+        if (!p.cut()) return;
+        if (w < p.main * p.rest) main = w;
+        else unit = (w - p.main * p.rest) * p.tail_share, end = min(unit + p.tail_share, p.rest * p.tail);
+    }
     __device__ bool next(const LinearPlan& p, LinearPiece& piece) {
         if (tile < p.whole) {
             piece = {tile, 0, p.kblocks, -1};
             tile += p.workers;
             return true;
         }
+        if (main >= 0) {
+            const int32_t t = main % p.rest, j = main / p.rest;
+            piece = {p.whole + t, j * p.share, (j + 1) * p.share, t * p.slots + j};
+            main = -1;
+            return true;
+        }
         if (unit >= end) return false;
-        const int32_t t = static_cast<int32_t>(unit / p.kblocks), k0 = static_cast<int32_t>(unit - static_cast<int64_t>(t) * p.kblocks);
-        const int32_t k1 = static_cast<int32_t>(min(k0 + (end - unit), static_cast<int64_t>(p.kblocks)));
-        piece = {p.whole + t, k0, k1, k0 == 0 && k1 == p.kblocks ? -1 : 2 * worker + (k0 == 0)};
-        unit += k1 - k0;
+        const int32_t t = unit / p.tail, at = unit - t * p.tail, n = min(end - unit, p.tail - at), k0 = p.main * p.share + at;
+        piece = {p.whole + t, k0, k0 + n, t * p.slots + p.main + unit / p.tail_share - p.first_tail(t)};
+        unit += n;
         return true;
     }
 };
@@ -185,6 +194,40 @@ __device__ __forceinline__ float slope_fast(int32_t act, float z) {
         default: return 1.f;
     }
 }
+// act_fast of two values, by instructions that work on two where there are such.
+template <int ACT>
+__device__ __forceinline__ void act_pair(float& x, float& y) {
+    using namespace tc;
+    if constexpr (ACT == SXCUDA_ACT_GELU) {
+        // max(z, 0) - |z| Phi(-|z|); beyond 64 the tail is zero, and infinity times zero would be NaN
+        float a, b;
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(fabsf(x)), "f"(64.f));
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(fabsf(y)), "f"(64.f));
+        const Two z = two(a, b);
+        float u, v;
+        split(fma2(z, two(0.3f, 0.3f), two(1.f, 1.f)), u, v);
+        const Two t = two(rcp_fast(u), rcp_fast(v));
+        split(mul2(mul2(z, two(-0.5f * kLog2Of, -0.5f * kLog2Of)), z), u, v);
+        const Two e = two(exp2_fast(u), exp2_fast(v));
+        Two p = fma2(two(0x1.3bca6ap-4f, 0x1.3bca6ap-4f), t, two(-0x1.ba7182p-3f, -0x1.ba7182p-3f));
+        p = fma2(p, t, two(0x1.15ac44p-6f, 0x1.15ac44p-6f));
+        p = fma2(p, t, two(-0x1.27505cp-3f, -0x1.27505cp-3f));
+        p = fma2(p, t, two(-0x1.d1e316p-4f, -0x1.d1e316p-4f));
+        p = fma2(p, t, two(-0x1.ebd2f4p-4f, -0x1.ebd2f4p-4f));  // all signs turned
+        split(fma2(mul2(mul2(p, t), e), z, two(fmaxf(x, 0.f), fmaxf(y, 0.f))), x, y);
+    } else if constexpr (ACT == SXCUDA_ACT_SILU || ACT == SXCUDA_ACT_GELU_TANH) {
+        const Two z = two(x, y);
+        Two u = z;
+        if constexpr (ACT == SXCUDA_ACT_GELU_TANH) u = mul2(z, fma2(mul2(z, z), two(kGeluCube, kGeluCube), two(1.f, 1.f)));
+        constexpr float k = ACT == SXCUDA_ACT_SILU ? -kLog2Of : -kLog2Of * kGeluTanh;
+        float a, b;
+        split(mul2(u, two(k, k)), a, b);
+        split(add2(two(exp2_fast(a), exp2_fast(b)), two(1.f, 1.f)), a, b);
+        split(mul2(z, two(rcp_fast(a), rcp_fast(b))), x, y);
+    } else {
+        x = act_fast<ACT>(x), y = act_fast<ACT>(y);
+    }
+}
 template <typename T>
 __device__ __forceinline__ float act_of(int32_t act, float z) {
     if constexpr (sizeof(T) == 4) return linear_act(act, z);
@@ -207,8 +250,9 @@ bool linear_tc_takes(const void* data, int64_t stride, int64_t rows);
 LinearPlan linear_tc_plan(int64_t m, int64_t n, int64_t k);
 void launch_linear_tc(const LinearProduct& p, cudaStream_t s);
 
-// Whole tiles, but for those of the last turns where workers would go without: the cut costs a launch and
-// its parts' way through memory, and a piece has at least `least` K blocks.
-LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, int depth, int64_t workers, int64_t least);
+// Cuts the last turn's tiles where that saves at least `gain` K blocks of it: the cut costs a launch and
+// its parts' way through memory. A piece has at least `least` K blocks.
+LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, int depth, int64_t workers, int64_t least,
+                       int64_t gain);
 
 }  // namespace sx
