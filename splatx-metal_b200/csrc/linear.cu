@@ -82,10 +82,6 @@ __device__ __forceinline__ void linear_finish(const LinearProduct& p, int64_t ro
     }
 }
 
-__device__ __forceinline__ float* part_at(const LinearProduct& p, int64_t slot, int row, int col) {
-    return p.parts + slot * p.plan.slot_values() + row * p.plan.tile_n + col;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant__ LinearProduct p, bool a_wide, bool b_wide) {
     __shared__ float as[2][kDepth][kPitch], bs[2][kDepth][kPitch];
@@ -132,7 +128,7 @@ __global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant_
                 if (m0 + row >= p.m || n <= 0) continue;
                 float z[4] = {c[i][4 * h], c[i][4 * h + 1], c[i][4 * h + 2], c[i][4 * h + 3]};
                 if (piece.slot < 0) linear_finish<T, 4>(p, m0 + row, n0 + col, z, static_cast<int>(n));
-                else *reinterpret_cast<float4*>(part_at(p, piece.slot, row, col)) = make_float4(z[0], z[1], z[2], z[3]);
+                else *reinterpret_cast<float4*>(linear_part(p, piece.slot, row, col)) = make_float4(z[0], z[1], z[2], z[3]);
             }
     }
 }
@@ -146,13 +142,15 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
     const LinearTile tile = linear_tile(plan, plan.whole + t);
     const int64_t m0 = static_cast<int64_t>(tile.m) * plan.tile_m, n0 = static_cast<int64_t>(tile.n) * plan.tile_n;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.tile_m), p.m - m0)), groups = plan.tile_n / 8;
-    const int at = blockIdx.x * 256 + threadIdx.x, row = at / groups, col = at % groups * 8;
+    // a warp has 8 rows and 4 times 8 columns: 256 bytes of a part side by side, 64 of a row of y
+    const int at = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int row = at / (groups / 4) * 8 + lane % 8, col = (at % (groups / 4) * 4 + lane / 8) * 8;
     const int64_t n = min(p.n - n0 - col, static_cast<int64_t>(8));
     if (row >= rows || n <= 0) return;
     float z[8] = {};
 #pragma unroll 4
     for (int i = 0; i < parts; ++i) {
-        const float4* part = reinterpret_cast<const float4*>(part_at(p, t * plan.slots + i, row, col));
+        const float4* part = reinterpret_cast<const float4*>(linear_part(p, t * plan.slots + i, row, col));
         const float4 x = part[0], y = part[1];
         z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w;
         z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
@@ -210,7 +208,7 @@ void launch_product(const LinearProduct& p, cudaStream_t s) {
     by_dtype(p.dtype, [&](auto t) {
         const auto join = linear_join_kernel<decltype(t)>;
         const int64_t rows = std::min<int64_t>(p.m, p.plan.tile_m);
-        SX_LAUNCH(join, dim3(blocks_for(rows * (p.plan.tile_n / 8), 256), static_cast<unsigned>(p.plan.rest)), 256, 0, s, p);
+        SX_LAUNCH(join, dim3(blocks_for((rows + 7) / 8 * (p.plan.tile_n / 32), 8), static_cast<unsigned>(p.plan.rest)), 256, 0, s, p);
     });
 }
 

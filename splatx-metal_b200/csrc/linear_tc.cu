@@ -1,14 +1,14 @@
 // linear_tc.cu — C = A B^T on the tensor cores for 16-bit operands, with the linear layer's epilogue.
 //
 // Two CTAs of a cluster make one tile of 256 x TN values: each holds 128 rows of A and half of B's rows in
-// shared memory (TMA, 64 values of K a stage), the leader's warp 9 issues products over both (cta_group::2),
+// shared memory (TMA, 64 values of K a stage), one warp of the leader issues products over both (cta_group::2),
 // and each CTA has the sums of its own 128 rows in its tensor memory, twice, so that one tile's epilogue runs
 // under the next one's products. Rows of an operand may run along K or across it (the gradients' products
 // read weight, x and v_z across): the tensor cores take either from shared memory.
 //
-//   warps 0-7: epilogue, a thread a row and half of the columns
-//   warp 8:    asks for the CTA's part of the tiles, on the leader's barriers
-//   warp 9:    allocates tensor memory; in the leader issues the products
+//   the first warps: epilogue, a thread a row and its share of the columns
+//   the loader:      asks for the CTA's part of the tiles, on the leader's barriers
+//   the issuer:      allocates tensor memory; in the leader issues the products
 #include <cuda.h>
 
 #include <algorithm>
@@ -33,21 +33,25 @@ namespace {
 
 constexpr int kRows = 128, kTileM = 2 * kRows, kDepth = 64;
 constexpr int kPanel = kDepth * 128;  // bytes of 64 values of K for 64 rows that lie across K
-constexpr int kEpilogueWarps = 8, kThreads = 320;
+constexpr int kPatches = 16;      // of a CTA
+
+constexpr int kTurnPitch = 9;    // words of 16 values' row, and one
+constexpr int kPatchCols = 32;   // a warp's unit of the epilogue: 32 rows and so many columns
+constexpr int kPatch = 32 * kPatchCols * 2;
 constexpr long long kLanding = 4000000;  // cycles in which any copy has landed (2 ms)
 
 struct LinearMaps {
-    CUtensorMap a, b;
+    CUtensorMap a, b, y, pre, residual;
 };
 
 template <int TN>
 struct Smem {
     static constexpr int kA = kRows * 128, kB = TN / 2 * 128, kStage = kA + kB;
     static constexpr int kStages = TN == 256 ? 6 : 8;
-    static constexpr int kBias = kStages * kStage;                     // [warps][TN / 2] floats
-    static constexpr int kTurn = kBias + kEpilogueWarps * TN / 2 * 4;  // [warps][32][17] floats
-    static constexpr int kBars = kTurn + kEpilogueWarps * 32 * 17 * 4;
-    static constexpr int kBytes = kBars + (2 * kStages + 5) * 8 + 16;
+    static constexpr int kPatchesAt = kStages * kStage;
+    static constexpr int kBias = kPatchesAt + kPatches * kPatch;  // [2][TN] floats
+    static constexpr int kBars = kBias + 2 * TN * 4;
+    static constexpr int kBytes = kBars + (2 * kStages + 5 + kPatches) * 8 + 16;
     static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -59,6 +63,7 @@ struct Bars {
     __device__ uint32_t acc_full(int i) const { return base + (2 * STAGES + i) * 8; }  // each CTA's
     __device__ uint32_t acc_empty(int i) const { return base + (2 * STAGES + 2 + i) * 8; }  // the leader's
     __device__ uint32_t drained() const { return base + (2 * STAGES + 4) * 8; }
+    __device__ uint32_t residual(int warp) const { return base + (2 * STAGES + 5 + warp) * 8; }
 };
 
 // ---- what a pair of CTAs needs ----
@@ -71,7 +76,7 @@ __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ void arrive_in(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 // A box of a 2-axis map into this CTA's shared memory, counted on a barrier of either CTA.
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t cluster_bar) {
@@ -80,6 +85,18 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(cluster_bar)
         : "memory");
 }
+__device__ __forceinline__ void load_own(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                 "l"(map), "r"(x), "r"(y), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y), "r"(src) : "memory");
+}
+__device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int N>  // all but the last N groups of the thread's stores have left shared memory
+__device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void pair_alloc(uint32_t to_smem, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to_smem), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -127,15 +144,18 @@ __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap* ma
 }
 
 // ---- epilogue ----
+__device__ __forceinline__ void tmem_load16(uint32_t (&r)[16], uint32_t at) {  // 16 consecutive columns of the thread's lane
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : SX_R8(r, 0), SX_R8(r, 8)
+        : "r"(at));
+}
+__device__ __forceinline__ void wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+    asm volatile("" : SX_T8(r, 0), SX_T8(r, 8));
+}
 template <typename T>
-__device__ __forceinline__ void load_values(const T* p, bool wide, float (&x)[16]) {  // 16-byte aligned, `wide`: 32
-    uint32_t w[8];
-    if (wide) {
-        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];" : SX_R8(w, 0) : "l"(p) : "memory");
-    } else {
-        *reinterpret_cast<uint4*>(w) = reinterpret_cast<const uint4*>(p)[0];
-        *reinterpret_cast<uint4*>(w + 4) = reinterpret_cast<const uint4*>(p)[1];
-    }
+__device__ __forceinline__ void unpack(const uint32_t (&w)[8], float (&x)[16]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const auto v = *reinterpret_cast<const Pack<T, 2>*>(&w[i]);
@@ -143,16 +163,9 @@ __device__ __forceinline__ void load_values(const T* p, bool wide, float (&x)[16
     }
 }
 template <typename T>
-__device__ __forceinline__ void store_values(T* p, bool wide, const float (&x)[16]) {
-    uint32_t w[8];
+__device__ __forceinline__ void pack(const float (&x)[16], uint32_t (&w)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[i] = tc::pack2<T>(x[2 * i], x[2 * i + 1]);
-    if (wide) {
-        tc::store32(p, w);
-    } else {
-        reinterpret_cast<uint4*>(p)[0] = *reinterpret_cast<uint4*>(w);
-        reinterpret_cast<uint4*>(p)[1] = *reinterpret_cast<uint4*>(w + 4);
-    }
 }
 template <int ACT>
 __device__ __forceinline__ void activate(float (&x)[16]) {
@@ -160,86 +173,141 @@ __device__ __forceinline__ void activate(float (&x)[16]) {
     for (int i = 0; i < 16; i += 2) act_pair<ACT>(x[i], x[i + 1]);
 }
 
-// How the rows of y, pre and residual are reached: 32 or 16 bytes at a time, or value by value.
-struct Reach {
-    bool vectors, wide;
-};
-
-// 16 columns of the thread's row, whole, at addresses of 16 bytes.
 template <typename T>
-__device__ __forceinline__ void finish_row(const LinearProduct& p, Reach reach, int64_t row, int64_t col, float (&x)[16]) {
-    if (p.pre) store_values(static_cast<T*>(p.pre) + row * p.pre_stride + col, reach.wide, x);
-    switch (p.act) {
+__device__ __forceinline__ void epilogue_act(int32_t act, float (&x)[16]) {
+    switch (act) {
         case SXCUDA_ACT_RELU: activate<SXCUDA_ACT_RELU>(x); break;
         case SXCUDA_ACT_SILU: activate<SXCUDA_ACT_SILU>(x); break;
         case SXCUDA_ACT_GELU: activate<SXCUDA_ACT_GELU>(x); break;
         case SXCUDA_ACT_GELU_TANH: activate<SXCUDA_ACT_GELU_TANH>(x); break;
         default: break;
     }
+}
+__device__ __forceinline__ void add_bias(const uint32_t* r, const float* bias, float (&x)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + i);
+        x[i] = __uint_as_float(r[i]) + b.x, x[i + 1] = __uint_as_float(r[i + 1]) + b.y;
+        x[i + 2] = __uint_as_float(r[i + 2]) + b.z, x[i + 3] = __uint_as_float(r[i + 3]) + b.w;
+    }
+}
+
+// A patch in shared memory as the copies have its rows, with their swizzle: 16 bytes of a lane's row.
+__device__ __forceinline__ uint4* patch_at(uint8_t* patch, int lane, int i) {
+    return reinterpret_cast<uint4*>(patch + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4));
+}
+__device__ __forceinline__ void to_patch(uint8_t* patch, int lane, int i, const uint32_t (&w)[8]) {
+    *patch_at(patch, lane, i) = uint4{w[0], w[1], w[2], w[3]};
+    *patch_at(patch, lane, i + 1) = uint4{w[4], w[5], w[6], w[7]};
+}
+__device__ __forceinline__ void from_patch(uint8_t* patch, int lane, int i, uint32_t (&w)[8]) {
+    const uint4 a = *patch_at(patch, lane, i), b = *patch_at(patch, lane, i + 1);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+}
+
+// The epilogue of 16 columns of a patch, those from 16 h on, a thread a row: r are its sums. The residual is
+// in the patch; pre goes to it (if it is wanted, y to `w` alone), or y does.
+template <typename T>
+__device__ __forceinline__ void finish_patch(const LinearProduct& p, const uint32_t (&r)[16], const float* bias, uint8_t* patch, int lane, int h,
+                                             uint32_t (&w)[8]) {
+    float x[16];
+    add_bias(r, bias, x);
+    uint32_t z[8];
+    if (p.residual) from_patch(patch, lane, 2 * h, z);
+    if (p.pre) {
+        pack<T>(x, w);
+        to_patch(patch, lane, 2 * h, w);
+    }
+    epilogue_act<T>(p.act, x);
     if (p.residual) {
-        float r[16];
-        load_values(static_cast<const T*>(p.residual) + row * p.residual_stride + col, reach.wide, r);
+        float v[16];
+        unpack<T>(z, v);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] += r[i];
+        for (int i = 0; i < 16; ++i) x[i] += v[i];
     }
-    store_values(static_cast<T*>(p.y) + row * p.y_stride + col, reach.wide, x);
+    pack<T>(x, w);
+    if (!p.pre) to_patch(patch, lane, 2 * h, w);
 }
 
-// 16 columns of the warp's 32 rows, value by value: turned in shared memory, so that lanes stand side by side
-// in a row.
+// The same where copies do not reach the rows of y, pre or residual: 16 columns at a time are turned in shared
+// memory, so that lanes stand side by side in a row, and go value by value.
+struct Turn {
+    int lane, rows, cols;  // rows and columns that there are
+    uint32_t* words;       // [32][kTurnPitch]
+};
 template <typename T>
-__device__ __forceinline__ void finish_turned(const LinearProduct& p, float (*turn)[17], int64_t row0, int64_t col0, int lane, const float (&x)[16]) {
+__device__ __forceinline__ void put(const Turn& at, T* first, int64_t stride, const float (&x)[16]) {
+    uint32_t w[8];
+    pack<T>(x, w);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) turn[lane][i] = x[i];
+    for (int i = 0; i < 8; ++i) at.words[at.lane * kTurnPitch + i] = w[i];
     __syncwarp();
-    const int64_t col = col0 + lane % 16;
-    for (int i = lane / 16; i < 32; i += 2) {
-        const int64_t row = row0 + i;
-        if (row >= p.m || col >= p.n) continue;
-        const float z = turn[i][lane % 16];
-        if (p.pre) static_cast<T*>(p.pre)[row * p.pre_stride + col] = from_f32<T>(z);
-        float y = act_of<T>(p.act, z);
-        if (p.residual) y += to_f32(static_cast<const T*>(p.residual)[row * p.residual_stride + col]);
-        static_cast<T*>(p.y)[row * p.y_stride + col] = from_f32<T>(y);
-    }
+    const int half = at.lane / 16, col = at.lane % 16;
+    const T* from = reinterpret_cast<const T*>(at.words) + half * 2 * kTurnPitch + col;
+    T* to = first + half * stride + col;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (2 * i + half < at.rows && col < at.cols) to[2 * i * stride] = from[2 * i * 2 * kTurnPitch];
     __syncwarp();
 }
-
-// 32 columns of a tile's row: the epilogue, or what is left of a part of the tile.
 template <typename T>
-__device__ __forceinline__ void finish(const LinearProduct& p, Reach reach, const float* bias, float (*turn)[17], int64_t row, int64_t col0,
-                                       int lane, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void get(const Turn& at, const T* first, int64_t stride, float (&x)[16]) {
+    const int half = at.lane / 16, col = at.lane % 16;
+    const T* from = first + half * stride + col;
+    T* to = reinterpret_cast<T*>(at.words) + half * 2 * kTurnPitch + col;
+    T v[16];
 #pragma unroll
-    for (int h = 0; h < 32; h += 16) {
-        const int64_t col = col0 + h;
-        float x[16];
+    for (int i = 0; i < 16; ++i) v[i] = 2 * i + half < at.rows && col < at.cols ? from[2 * i * stride] : from_f32<T>(0.f);
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            const float4 b = *reinterpret_cast<const float4*>(bias + h + i);
-            x[i] = __uint_as_float(r[h + i]) + b.x, x[i + 1] = __uint_as_float(r[h + i + 1]) + b.y;
-            x[i + 2] = __uint_as_float(r[h + i + 2]) + b.z, x[i + 3] = __uint_as_float(r[h + i + 3]) + b.w;
-        }
-        if (reach.vectors && col + 16 <= p.n) {
-            if (row < p.m) finish_row<T>(p, reach, row, col, x);
-        } else if (col < p.n) {
-            finish_turned<T>(p, turn, row - lane, col, lane, x);
-        }
-    }
+    for (int i = 0; i < 16; ++i) to[2 * i * 2 * kTurnPitch] = v[i];
+    __syncwarp();
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = at.words[at.lane * kTurnPitch + i];
+    __syncwarp();
+    unpack<T>(w, x);
 }
-__device__ __forceinline__ void leave(const LinearProduct& p, int slot, int row, int col, uint32_t (&r)[32]) {
-    float* part = p.parts + slot * p.plan.slot_values() + row * p.plan.tile_n + col;
+template <typename T>
+__device__ __forceinline__ void finish_turned(const LinearProduct& p, const uint32_t (&r)[16], const float* bias, uint32_t* words, int lane, int rows,
+                                              int64_t row, int64_t col) {
+    const Turn at{lane, rows, static_cast<int>(min(p.n - col, static_cast<int64_t>(16))), words};
+    if (at.cols <= 0) return;
+    float x[16];
+    add_bias(r, bias, x);
+    if (p.pre) put(at, static_cast<T*>(p.pre) + row * p.pre_stride + col, p.pre_stride, x);
+    epilogue_act<T>(p.act, x);
+    if (p.residual) {
+        float y[16];
+        get(at, static_cast<const T*>(p.residual) + row * p.residual_stride + col, p.residual_stride, y);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tc::store32(part + 8 * i, *reinterpret_cast<uint32_t(*)[8]>(r + 8 * i));
+        for (int i = 0; i < 16; ++i) x[i] += y[i];
+    }
+    put(at, static_cast<T*>(p.y) + row * p.y_stride + col, p.y_stride, x);
 }
 
-template <typename T, int TN, bool A_ACROSS, bool B_ACROSS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-    linear_tc_kernel(const __grid_constant__ LinearProduct p, const __grid_constant__ LinearMaps maps, Reach reach) {
+// Part of a cut tile, as [columns / 8][rows][8]: a warp's rows side by side.
+__device__ __forceinline__ void leave(const LinearProduct& p, int slot, int row, int col, uint32_t (&r)[16]) {
+    float* part = linear_part(p, slot, row, col);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) tc::store32(part + i * kTileM * 8, *reinterpret_cast<uint32_t(*)[8]>(r + 8 * i));
+}
+
+// The warps of the epilogue: sixteen where there is an activation, a residual, a second result; eight for the
+// gradients, whose epilogue only rounds (measured in us, eight and sixteen: 32768 x 1024 x 4096 with gelu and pre
+// 245 and 230, without either 177 and 182).
+template <bool B_ACROSS>
+constexpr int kEpilogueWarps = B_ACROSS ? 8 : 16;
+template <bool B_ACROSS>
+constexpr int kThreads = 32 * (kEpilogueWarps<B_ACROSS> + 2);
+
+template <typename T, int TN, bool A_ACROSS, bool B_ACROSS, bool COPIES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<B_ACROSS>, 1)
+    linear_tc_kernel(const __grid_constant__ LinearProduct p, const __grid_constant__ LinearMaps maps) {
     using S = Smem<TN>;
-    constexpr int kStages = S::kStages;
+    constexpr int kStages = S::kStages, kWarps = kEpilogueWarps<B_ACROSS>, kLoader = kWarps, kIssuer = kWarps + 1;
     extern __shared__ __align__(1024) uint8_t smem[];
     const Bars<kStages> bars{tc::smem_addr(smem) + S::kBars};
-    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(smem + S::kBars + (2 * kStages + 5) * 8);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(smem + S::kBytes - 16);
     uint32_t* tmem_at = const_cast<uint32_t*>(failed) + 1;
     const uint32_t base = tc::smem_addr(smem);
     const int warp = __shfl_sync(kFullMask, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -248,24 +316,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     LinearPiece piece;
     int asked = 0;  // stages that this warp has asked for
 
-    if (warp == 8 && lane == 0) {
+    if (warp == kLoader && lane == 0) {
         tc::prefetch_map(&maps.a);
         tc::prefetch_map(&maps.b);
         for (int s = 0; s < kStages; ++s) tc::bar_init(bars.full(s), 1), tc::bar_init(bars.empty(s), 1);
-        for (int i = 0; i < 2; ++i) tc::bar_init(bars.acc_full(i), 1), tc::bar_init(bars.acc_empty(i), 2 * kEpilogueWarps);
+        for (int i = 0; i < 2; ++i) tc::bar_init(bars.acc_full(i), 1), tc::bar_init(bars.acc_empty(i), 2 * kWarps);
         tc::bar_init(bars.drained(), 1);
+        for (int i = 0; i < kWarps; ++i) tc::bar_init(bars.residual(i), 1);
         tc::bar_init_fence();
         *failed = 0;
     }
     __syncwarp();
-    if (warp == 9) pair_alloc(tc::smem_addr(tmem_at), 2 * TN);
+    if (warp == kIssuer) pair_alloc(tc::smem_addr(tmem_at), 2 * TN);
     tc::fence_before();
     __syncthreads();
     cluster_sync();
     tc::fence_after();
     const uint32_t tmem = __shfl_sync(kFullMask, *tmem_at, 0);
 
-    if (warp == 8) {
+    if (warp == kLoader) {
         int slot = 0;
         uint32_t parity = 0;
         bool ok = true;
@@ -288,7 +357,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         // the products' last arrivals, without which this CTA's memory must not go
         for (int i = max(0, asked - kStages); ok && i < asked; ++i) ok = tc::bar_wait(bars.empty(i % kStages), (i / kStages) & 1, failed);
-    } else if (warp == 9) {
+    } else if (warp == kIssuer) {
         if (rank == 0) {
             const uint32_t one = tc::elect();
             int slot = 0, count = 0;
@@ -314,38 +383,125 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
         }
     } else {
-        constexpr int kCols = TN / 2;
-        const int half = warp >> 2, in_tile = static_cast<int>(rank) * kRows + (warp & 3) * 32 + lane;
+        constexpr int kCols = TN / (kWarps / 4), kOwn = kPatches / kWarps;  // columns and patches of a warp
+        const int part = warp >> 2, in_tile = static_cast<int>(rank) * kRows + (warp & 3) * 32;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        float* bias = reinterpret_cast<float*>(smem + S::kBias) + warp * kCols;
-        float(*turn)[17] = reinterpret_cast<float(*)[17]>(smem + S::kTurn) + warp * 32;
-        bool ok = true;
-        for (int count = 0; ok && walk.next(p.plan, piece); ++count) {
+        uint8_t* patch = smem + S::kPatchesAt + warp * kOwn * kPatch;
+        uint32_t patch_in = tc::smem_addr(patch);
+        // two patches in turn where a patch holds nothing else
+        const bool in_turn = kOwn == 2 && !p.residual && !p.pre;
+        uint32_t turn = 0;  // parity of the residuals' barrier
+        bool due = false;   // a residual's copy is on its way
+        const auto ask = [&](int row, int col) {
+            if (lane == 0) {
+                stores_read<0>();
+                tc::bar_expect(bars.residual(warp), kPatch);
+                load_own(patch_in, &maps.residual, col, row, bars.residual(warp));
+            }
+            due = true;
+            __syncwarp();
+        };
+        const auto send = [&](const CUtensorMap* map, int row, int col) {
+            tc::fence_smem_to_async();
+            __syncwarp();
+            if (lane == 0) {
+                store_box(map, col, row, patch_in);
+                stores_commit();
+            }
+        };
+        // where a piece is, and its bias: taken a tile ahead. Four warps have the same columns.
+        struct Place {
+            int row, col, rows, slot;
+            float bias;
+        };
+        const int bias_at = part * kCols + (warp & 3) * (kCols / 4) + lane;
+        const auto place = [&]() {
             const LinearTile tile = linear_tile(p.plan, piece.tile);
-            const int64_t row = static_cast<int64_t>(tile.m) * kTileM + in_tile, n0 = static_cast<int64_t>(tile.n) * TN + half * kCols;
-            __syncwarp();
-            for (int i = lane; i < kCols; i += 32) bias[i] = n0 + i < p.n ? linear_param(p.bias, p.bias_dtype, n0 + i) : 0.f;
-            __syncwarp();
+            Place r{tile.m * kTileM + in_tile, tile.n * TN + part * kCols, 0, piece.slot, 0.f};
+            r.rows = static_cast<int>(max(min(p.m - r.row, static_cast<int64_t>(32)), static_cast<int64_t>(0)));
+            const int col = tile.n * TN + bias_at;
+            if (lane < kCols / 4 && col < p.n) r.bias = linear_param(p.bias, p.bias_dtype, col);
+            return r;
+        };
+        bool more = walk.next(p.plan, piece), ok = true;
+        Place next{};
+        if (more) next = place();
+        for (int count = 0; ok && more; ++count) {
+            const Place here = next;
+            const int row = here.row, n0 = here.col, rows = here.rows;
+            const bool finishes = here.slot < 0 && rows > 0;
+            float* bias = reinterpret_cast<float*>(smem + S::kBias) + (count & 1) * TN;
+            if (lane < kCols / 4) bias[bias_at] = here.bias;
+            bias += part * kCols;
+            asm volatile("bar.sync %0, 128;" ::"r"(part + 1) : "memory");
+            more = walk.next(p.plan, piece);
+            if (more) next = place();
+            if (COPIES && finishes && p.residual && n0 < p.n) ask(row, n0);
             ok = tc::bar_wait(bars.acc_full(count & 1), (count >> 1) & 1, failed);
             if (!ok) break;
             tc::fence_after();
-            const uint32_t at = tmem + lanes + (count & 1) * TN + half * kCols;
-#pragma unroll 1
-            for (int c = 0; c < kCols; c += 32) {
-                uint32_t r[32];
-                __syncwarp();
-                tc::tmem_load32(r, at + c);
-                tc::wait_ld(r);
-                if (c + 32 == kCols) {
+            const uint32_t at = tmem + lanes + (count & 1) * TN + part * kCols;
+            uint32_t sums[2][16];  // 16 columns, and the next ones on their way
+            tmem_load16(sums[0], at);
+            const auto take = [&](int col) {  // those from `col` on are there, the next ones asked for, or all are read
+                wait_ld16(sums[col / 16 & 1]);
+                if (col + 16 < kCols) {
+                    __syncwarp();
+                    tmem_load16(sums[(col / 16 & 1) ^ 1], at + col + 16);
+                } else {
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) arrive_in(in_cta(bars.acc_empty(count & 1), 0));
                 }
-                if (n0 + c >= p.n) continue;  // the same for the whole warp
-                if (piece.slot < 0) finish<T>(p, reach, bias + c, turn, row, n0 + c, lane, r);
-                else if (row < p.m) leave(p, piece.slot, in_tile, half * kCols + c, r);
+            };
+#pragma unroll 1
+            for (int c = 0; c < kCols; c += kPatchCols) {
+                const bool some = n0 + c < p.n && rows > 0;  // the same for the whole warp
+                const bool patched = COPIES && some && finishes;
+                if (patched) {
+                    if (p.residual) {
+                        ok = tc::bar_wait(bars.residual(warp), turn, failed);
+                        if (!ok) break;
+                        turn ^= 1;
+                        due = false;
+                    } else if (lane == 0) {
+                        if (in_turn) stores_read<1>();
+                        else stores_read<0>();
+                    }
+                    __syncwarp();
+                }
+                uint32_t y[2][8];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    take(c + 16 * h);
+                    uint32_t(&r)[16] = sums[h];
+                    if (!some) continue;
+                    if (!finishes) {
+                        if (lane < rows) leave(p, here.slot, in_tile + lane, part * kCols + c + 16 * h, r);
+                    } else if constexpr (COPIES) {
+                        finish_patch<T>(p, r, bias + c + 16 * h, patch, lane, h, y[h]);
+                    } else {
+                        finish_turned<T>(p, r, bias + c + 16 * h, reinterpret_cast<uint32_t*>(patch), lane, rows, row, n0 + c + 16 * h);
+                    }
+                }
+                if (!patched) continue;
+                if (p.pre) {
+                    send(&maps.pre, row, n0 + c);
+                    if (lane == 0) stores_read<0>();
+                    __syncwarp();
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) to_patch(patch, lane, 2 * h, y[h]);
+                }
+                send(&maps.y, row, n0 + c);
+                if (in_turn) {
+                    const int to = patch_in == tc::smem_addr(smem + S::kPatchesAt + warp * kOwn * kPatch) ? kPatch : -kPatch;
+                    patch += to, patch_in += to;
+                }
+                if (p.residual && c + kPatchCols < kCols && n0 + c + kPatchCols < p.n) ask(row, n0 + c + kPatchCols);
             }
         }
+        if (due) tc::bar_drain(bars.residual(warp), turn);
+        if (lane == 0) stores_done();
     }
 
     tc::fence_before();
@@ -355,12 +511,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     cluster_sync();
     if (*failed) {  // nothing may land in the pair's memory after it has gone
-        if (warp == 8) {
+        if (warp == kLoader) {
             if (rank == 0)
                 for (int i = max(0, asked - kStages); i < asked; ++i) tc::bar_drain(bars.full(i % kStages), (i / kStages) & 1);
             for (const long long start = clock64(); clock64() - start < kLanding;) {
             }
-        } else if (warp == 9 && rank == 0) {
+        } else if (warp == kIssuer && rank == 0) {
             const uint32_t one = tc::elect();
             asm volatile(
                 "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
@@ -372,7 +528,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         cluster_sync();
         if (threadIdx.x == 0) atomicOr(&g_linear_status, 1u);
     }
-    if (warp == 9) pair_free(tmem, 2 * TN);
+    if (warp == kIssuer) pair_free(tmem, 2 * TN);
 }
 
 // ---- host ----
@@ -390,6 +546,15 @@ EncodeFn encode_fn() {
     return fn;
 }
 
+void encode(CUtensorMap* m, int32_t dtype, const void* data, const cuuint64_t (&dims)[2], const cuuint64_t (&strides)[1], int cols, int rows,
+            CUtensorMapSwizzle swizzle) {
+    const cuuint32_t box[2] = {static_cast<cuuint32_t>(cols), static_cast<cuuint32_t>(rows)}, step[2] = {1, 1};
+    const CUresult r = encode_fn()(m, dtype == SXCUDA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
+                                   const_cast<void*>(data), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) throw RuntimeError("linear: cuTensorMapEncodeTiled failed with " + std::to_string(static_cast<int>(r)));
+}
+
 // The operand's memory as [outer][inner], inner contiguous: K is the inner axis, or the rows are (across). Boxes
 // of 64 inner values; what lies beyond the operand reads as zero.
 CUtensorMap make_map(const LinearOperand& o, int64_t rows, int64_t k, int box_rows, int32_t dtype) {
@@ -398,30 +563,36 @@ CUtensorMap make_map(const LinearOperand& o, int64_t rows, int64_t k, int box_ro
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
     // one row may have any stride: a length that fits stands for it
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(2 * (outer > 1 ? o.stride : (inner + 7) / 8 * 8))};
-    const cuuint32_t box[2] = {64, static_cast<cuuint32_t>(o.across ? kDepth : box_rows)}, step[2] = {1, 1};
-    const CUresult r = encode_fn()(&m, dtype == SXCUDA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                                   const_cast<void*>(o.data), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) throw RuntimeError("linear: cuTensorMapEncodeTiled failed with " + std::to_string(static_cast<int>(r)));
+    encode(&m, dtype, o.data, dims, strides, 64, o.across ? kDepth : box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
     return m;
 }
 
-Reach reach_of(const LinearProduct& p) {
-    const auto fits = [&](const void* x, int64_t stride, int64_t bytes) {
-        return !x || (reinterpret_cast<uintptr_t>(x) % bytes == 0 && (p.m <= 1 || stride * 2 % bytes == 0));
-    };
-    const auto all = [&](int64_t bytes) {
-        return fits(p.y, p.y_stride, bytes) && fits(p.pre, p.pre_stride, bytes) && fits(p.residual, p.residual_stride, bytes);
-    };
-    return {all(16), all(32)};
+// The epilogue's patches of y, pre and residual.
+CUtensorMap patch_map(const LinearProduct& p, const void* data, int64_t stride) {
+    CUtensorMap m{};
+    if (!data) return m;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.n), static_cast<cuuint64_t>(p.m)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(2 * (p.m > 1 ? stride : (p.n + 7) / 8 * 8))};
+    encode(&m, p.dtype, data, dims, strides, kPatchCols, 32, CU_TENSOR_MAP_SWIZZLE_64B);
+    return m;
 }
 
 template <typename T, int TN, bool A_ACROSS, bool B_ACROSS>
 void launch_tile(const LinearProduct& p, cudaStream_t s) {
-    const auto kernel = linear_tc_kernel<T, TN, A_ACROSS, B_ACROSS>;
-    smem_limit_once(reinterpret_cast<const void*>(kernel), Smem<TN>::kBytes, "linear");
-    const LinearMaps maps{make_map(p.a, p.m, p.k, kRows, p.dtype), make_map(p.b, p.n, p.k, TN / 2, p.dtype)};
-    SX_LAUNCH(kernel, static_cast<unsigned>(2 * p.plan.workers), kThreads, Smem<TN>::kBytes, s, p, maps, reach_of(p));
+    LinearMaps maps{make_map(p.a, p.m, p.k, kRows, p.dtype), make_map(p.b, p.n, p.k, TN / 2, p.dtype), {}, {}, {}};
+    const auto run = [&](auto kernel) {
+        smem_limit_once(reinterpret_cast<const void*>(kernel), Smem<TN>::kBytes, "linear");
+        SX_LAUNCH(kernel, static_cast<unsigned>(2 * p.plan.workers), kThreads<B_ACROSS>, Smem<TN>::kBytes, s, p, maps);
+    };
+    const auto reached = [&](const void* x, int64_t stride) { return !x || linear_tc_takes(x, stride, p.m); };
+    if (reached(p.y, p.y_stride) && reached(p.pre, p.pre_stride) && reached(p.residual, p.residual_stride)) {
+        maps.y = patch_map(p, p.y, p.y_stride);
+        maps.pre = patch_map(p, p.pre, p.pre_stride);
+        maps.residual = patch_map(p, p.residual, p.residual_stride);
+        run(linear_tc_kernel<T, TN, A_ACROSS, B_ACROSS, true>);
+    } else {
+        run(linear_tc_kernel<T, TN, A_ACROSS, B_ACROSS, false>);
+    }
 }
 template <typename T, int TN>
 void launch_across(const LinearProduct& p, cudaStream_t s) {

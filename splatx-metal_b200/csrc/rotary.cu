@@ -202,73 +202,49 @@ struct Rot {
         const int64_t t = unit / a.chunks, b = t / a.tokens;
         return {b, t - b * a.tokens, static_cast<int>(unit - t * a.chunks)};
     }
-    // A turn of the warp's groups: where the group's row is, and whether there is one.
-    struct Turn {
-        int64_t unit, x, g, out;
-        int number;  // of the token's turns: first the queries', then the keys'
-        int end;     // the unit's last one, and one
-        bool there;
-    };
-    __device__ Turn first_turn(int64_t unit) const {
-        if (unit >= a.units) return {unit, 0, 0, 0, 0, 0, false};
-        const Token t = token_of(unit);
-        Turn r{unit, t.batch, t.token, 0, t.chunk * a.chunk, 0, false};
-        r.end = min(r.number + a.chunk, a.half[0].turns + a.half[1].turns);
-        return head_of(r, t.batch, t.token);
-    }
-    __device__ Turn head_of(Turn r, int64_t batch, int64_t token) const {
-        const int k = r.number >= a.half[0].turns;
-        const RotHalf& h = a.half[k];
-        const int head = (r.number - (k ? a.half[0].turns : 0)) * rows + group;
-        r.there = head < h.heads;
-        r.x = batch * h.x_batch + token * h.x_token + head * h.x_head;
-        r.g = batch * h.g_batch + token * h.g_token + head * h.g_head;
-        r.out = batch * h.out_batch + token * h.out_token + head * h.out_head;
-        return r;
-    }
-    __device__ Turn next_turn(Turn r, int64_t step) const {
-        if (++r.number == r.end) return first_turn(r.unit + step);
-        if (r.number == a.half[0].turns) {  // from the queries to the keys
-            const Token t = token_of(r.unit);
-            return head_of(r, t.batch, t.token);
-        }
-        const int k = r.number >= a.half[0].turns;
-        const RotHalf& h = a.half[k];
-        r.x += rows * h.x_head, r.g += rows * h.g_head, r.out += rows * h.out_head;
-        r.there = (r.number - (k ? a.half[0].turns : 0)) * rows + group < h.heads;
-        return r;
-    }
-    __device__ bool keys(const Turn& r) const { return r.number >= a.half[0].turns; }
-    __device__ void load(Row<T, V, NV>& r, const void* base, int64_t offset, bool there) const {
-        const T* row = static_cast<const T*>(base) + offset;
+    // A slot that is not the thread's own keeps the zeros it started with.
+    __device__ void load(Row<T, V, NV>& r, const T* row, bool there) const {
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            r.first[n] = r.second[n] = Pack<T, V>{};
+        for (int n = 0; n < NV; ++n)
             if (there && mine[n]) {
                 r.first[n] = *reinterpret_cast<const Pack<T, V>*>(row + at[n].first);
-                if (at[n].second >= 0) r.second[n] = *reinterpret_cast<const Pack<T, V>*>(row + at[n].second);
+                if (V > 1 || at[n].second >= 0) r.second[n] = *reinterpret_cast<const Pack<T, V>*>(row + at[n].second);
             }
-        }
     }
-    __device__ void store(void* base, int64_t offset, const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
-        T* row = static_cast<T*>(base) + offset;
+    __device__ void store(T* row, const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             if (!mine[n]) continue;
             Pack<T, V> x, y;
+            if constexpr (V == 1) {
+                float lo, none;
+                tc::split(p[n].v[0], lo, none);
+                x.v[0] = from_f32<T>(lo);
+                tc::split(q[n].v[0], lo, none);
+                y.v[0] = from_f32<T>(lo);
+            } else {
 #pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                float lo, hi;
-                tc::split(p[n].v[e / 2], lo, hi);
-                *value(x, y, e, 0) = from_f32<T>(lo);
-                if constexpr (V > 1) *value(x, y, e + 1, 0) = from_f32<T>(hi);
-                tc::split(q[n].v[e / 2], lo, hi);
-                *value(x, y, e, 1) = from_f32<T>(lo);
-                if constexpr (V > 1) *value(x, y, e + 1, 1) = from_f32<T>(hi);
+                for (int e = 0; e < V; e += 2) {
+                    float a0, a1, b0, b1;
+                    tc::split(p[n].v[e / 2], a0, a1);
+                    tc::split(q[n].v[e / 2], b0, b1);
+                    if constexpr (NB) {  // pair e is the values 2 e and 2 e + 1
+                        two_to(2 * e < V ? x : y, 2 * e % V, a0, b0);
+                        two_to(2 * e + 2 < V ? x : y, (2 * e + 2) % V, a1, b1);
+                    } else {
+                        two_to(x, e, a0, a1);
+                        two_to(y, e, b0, b1);
+                    }
+                }
             }
             *reinterpret_cast<Pack<T, V>*>(row + at[n].first) = x;
-            if (at[n].second >= 0) *reinterpret_cast<Pack<T, V>*>(row + at[n].second) = y;
+            if (V > 1 || at[n].second >= 0) *reinterpret_cast<Pack<T, V>*>(row + at[n].second) = y;
         }
+    }
+    static __device__ __forceinline__ void two_to(Pack<T, V>& x, int i, float lo, float hi) {
+        if constexpr (std::is_same_v<T, __half>) reinterpret_cast<__half2*>(x.v)[i / 2] = __floats2half2_rn(lo, hi);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) reinterpret_cast<__nv_bfloat162*>(x.v)[i / 2] = __floats2bfloat162_rn(lo, hi);
+        else x.v[i] = lo, x.v[i + 1] = hi;
     }
     // The first (second) value of pair e among a slot's.
     template <typename P>
@@ -316,56 +292,76 @@ struct Rot {
     }
 };
 
+// Calls f(half, base of the token's rows as offsets, first turn, end) for the queries' and the keys' turns of a unit.
+template <typename F>
+__device__ __forceinline__ void rot_halves(const RotArgs& a, int chunk, F&& f) {
+    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.half[0].turns + a.half[1].turns), q = a.half[0].turns;
+    if (begin < q) f(std::integral_constant<int, 0>{}, begin, min(end, q));
+    if (end > q) f(std::integral_constant<int, 1>{}, max(begin, q) - q, end - q);
+}
+
+constexpr int kFwdAhead = 4, kBwdAhead = 2;  // rows of a group that are asked for at once
+
 template <typename T, int V, bool NB, int NV>
-__global__ void __launch_bounds__(kRotThreads, V == 1 ? 2 : 7) rotary_fwd_kernel(const __grid_constant__ RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, V == 1 ? 2 : 5) rotary_fwd_kernel(const __grid_constant__ RotArgs a) {
     const Rot<T, V, NB, NV> me(a);
     using Me = Rot<T, V, NB, NV>;
     const int64_t step = static_cast<int64_t>(gridDim.x) * kRotWarps;
     const tc::Two minus = tc::two(-1.f, -1.f);
-    auto turn = me.first_turn(static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5));
-    Row<T, V, NV> row;
-    me.load(row, a.half[me.keys(turn)].x, turn.x, turn.there);
-    double position = me.position(turn.unit);
-    int64_t unit = -1;
-    while (turn.unit < a.units) {
-        const auto next = me.next_turn(turn, step);
-        Row<T, V, NV> next_row;
-        me.load(next_row, a.half[me.keys(next)].x, next.x, next.there);
-        if (turn.unit != unit) {
-            me.angles(position);
-            unit = turn.unit;
-            position = me.position(unit + step);
-        }
-        Values<V> p[NV], q[NV];
-        Me::unpack(row, p, q);
-        const bool k = me.keys(turn);
-        if (a.norm) {
-            const float r = me.rstd(p, q);
-            const tc::Two rr = tc::two(r, r);
-            const float* w = me.weights + (k ? 2 * a.slots * V : 0);
+    Row<T, V, NV> row[kFwdAhead] = {};
+    int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5);
+    double position = me.position(unit);
+    for (; unit < a.units; unit += step) {
+        const auto token = me.token_of(unit);
+        bool made = false;
+        rot_halves(a, token.chunk, [&](auto k, int turn, int end) {
+            const RotHalf& h = a.half[k];
+            const T* x = static_cast<const T*>(h.x) + token.batch * h.x_batch + token.token * h.x_token + (turn * me.rows + me.group) * h.x_head;
+            T* out = static_cast<T*>(h.out) + token.batch * h.out_batch + token.token * h.out_token + (turn * me.rows + me.group) * h.out_head;
+            const int64_t x_step = me.rows * h.x_head, out_step = me.rows * h.out_head;
+            const float* weights = me.weights + k * 2 * a.slots * V;
+            int left = h.heads - turn * me.rows - me.group;
+            for (; turn < end; turn += kFwdAhead) {
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                const Values<V> w0 = me.entries(w, n, 0), w1 = me.entries(w, n, V);
-#pragma unroll
-                for (int e = 0; e < Me::N; ++e) {
-                    p[n].v[e] = tc::mul2(tc::mul2(p[n].v[e], rr), w0.v[e]);
-                    q[n].v[e] = tc::mul2(tc::mul2(q[n].v[e], rr), w1.v[e]);
+                for (int i = 0; i < kFwdAhead; ++i, x += x_step) me.load(row[i], x, turn + i < end && left > i * me.rows);
+                if (!made) {
+                    me.angles(position);
+                    position = me.position(unit + step);
+                    made = true;
                 }
-            }
-        }
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
+                for (int i = 0; i < kFwdAhead; ++i, out += out_step) {
+                    if (turn + i >= end) break;
+                    Values<V> p[NV], q[NV];
+                    Me::unpack(row[i], p, q);
+                    if (a.norm) {
+                        const float r = me.rstd(p, q);
+                        const tc::Two rr = tc::two(r, r);
 #pragma unroll
-            for (int e = 0; e < Me::N; ++e) {
-                const tc::Two u1 = p[n].v[e], u2 = q[n].v[e];
-                p[n].v[e] = tc::fma2(u1, c.v[e], tc::mul2(tc::mul2(u2, minus), s.v[e]));
-                q[n].v[e] = tc::fma2(u1, s.v[e], tc::mul2(u2, c.v[e]));
+                        for (int n = 0; n < NV; ++n) {
+                            const Values<V> w0 = me.entries(weights, n, 0), w1 = me.entries(weights, n, V);
+#pragma unroll
+                            for (int e = 0; e < Me::N; ++e) {
+                                p[n].v[e] = tc::mul2(tc::mul2(p[n].v[e], rr), w0.v[e]);
+                                q[n].v[e] = tc::mul2(tc::mul2(q[n].v[e], rr), w1.v[e]);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NV; ++n) {
+                        const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
+#pragma unroll
+                        for (int e = 0; e < Me::N; ++e) {
+                            const tc::Two u1 = p[n].v[e], u2 = q[n].v[e];
+                            p[n].v[e] = tc::fma2(u1, c.v[e], tc::mul2(tc::mul2(u2, minus), s.v[e]));
+                            q[n].v[e] = tc::fma2(u1, s.v[e], tc::mul2(u2, c.v[e]));
+                        }
+                    }
+                    if (left > i * me.rows) me.store(out, p, q);
+                }
+                left -= kFwdAhead * me.rows;
             }
-        }
-        if (turn.there) me.store(a.half[k].out, turn.out, p, q);
-        row = next_row;
-        turn = next;
+        });
     }
 }
 
@@ -380,82 +376,84 @@ __global__ void __launch_bounds__(kRotThreads, V == 1 ? 2 : 4) rotary_bwd_kernel
     for (int i = 0; i < 4 * NV; ++i)
 #pragma unroll
         for (int e = 0; e < Me::N; ++e) sum[i / NV / 2][i / NV % 2][i % NV].v[e] = tc::two(0.f, 0.f);
-    auto turn = me.first_turn(static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5));
-    Row<T, V, NV> x_row, g_row;
-    me.load(g_row, a.half[me.keys(turn)].g, turn.g, turn.there);
-    me.load(x_row, a.half[me.keys(turn)].x, turn.x, turn.there && a.norm);
-    double position = me.position(turn.unit);
-    int64_t unit = -1;
-    while (turn.unit < a.units) {
-        const auto next = me.next_turn(turn, step);
-        Row<T, V, NV> x_next, g_next;
-        me.load(g_next, a.half[me.keys(next)].g, next.g, next.there);
-        me.load(x_next, a.half[me.keys(next)].x, next.x, next.there && a.norm);
-        if (turn.unit != unit) {
-            me.angles(position);
-            unit = turn.unit;
-            position = me.position(unit + step);
-        }
-        const bool k = me.keys(turn);
-        Values<V> p[NV], q[NV];
-        Me::unpack(g_row, p, q);
+    Row<T, V, NV> x_row[kBwdAhead] = {}, g_row[kBwdAhead] = {};
+    int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5);
+    double position = me.position(unit);
+    for (; unit < a.units; unit += step) {
+        const auto token = me.token_of(unit);
+        bool made = false;
+        rot_halves(a, token.chunk, [&](auto k, int turn, int end) {
+            const RotHalf& h = a.half[k];
+            const int head = turn * me.rows + me.group;
+            const T* x = static_cast<const T*>(h.x) + token.batch * h.x_batch + token.token * h.x_token + head * h.x_head;
+            const T* g = static_cast<const T*>(h.g) + token.batch * h.g_batch + token.token * h.g_token + head * h.g_head;
+            T* out = static_cast<T*>(h.out) + token.batch * h.out_batch + token.token * h.out_token + head * h.out_head;
+            const int64_t x_step = me.rows * h.x_head, g_step = me.rows * h.g_head, out_step = me.rows * h.out_head;
+            const float* weights = me.weights + k * 2 * a.slots * V;
+            int left = h.heads - head;
+            for (; turn < end; turn += kBwdAhead) {
 #pragma unroll
-        for (int n = 0; n < NV; ++n) {
-            const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
+                for (int i = 0; i < kBwdAhead; ++i, x += x_step, g += g_step) {
+                    const bool there = turn + i < end && left > i * me.rows;
+                    me.load(g_row[i], g, there);
+                    me.load(x_row[i], x, there && a.norm);
+                }
+                if (!made) {
+                    me.angles(position);
+                    position = me.position(unit + step);
+                    made = true;
+                }
 #pragma unroll
-            for (int e = 0; e < Me::N; ++e) {
-                const tc::Two g1 = p[n].v[e], g2 = q[n].v[e];
-                p[n].v[e] = tc::fma2(g1, c.v[e], tc::mul2(g2, s.v[e]));
-                q[n].v[e] = tc::fma2(g2, c.v[e], tc::mul2(tc::mul2(g1, minus), s.v[e]));
-            }
-        }
-        if (a.norm) {
-            Values<V> x0[NV], x1[NV];
-            Me::unpack(x_row, x0, x1);
-            const float r = me.rstd(x0, x1);
-            const tc::Two rr = tc::two(r, r);
-            const float* w = me.weights + (k ? 2 * a.slots * V : 0);
-            tc::Two dot = tc::two(0.f, 0.f);
-            const auto add = [&](Values<V> (&sums)[2][NV]) {
+                for (int i = 0; i < kBwdAhead; ++i, out += out_step) {
+                    if (turn + i >= end) break;
+                    const bool there = left > i * me.rows;
+                    Values<V> p[NV], q[NV];
+                    Me::unpack(g_row[i], p, q);
 #pragma unroll
-                for (int n = 0; n < NV; ++n)
+                    for (int n = 0; n < NV; ++n) {
+                        const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
 #pragma unroll
-                    for (int e = 0; e < Me::N; ++e) {
-                        sums[0][n].v[e] = tc::fma2(p[n].v[e], x0[n].v[e], sums[0][n].v[e]);
-                        sums[1][n].v[e] = tc::fma2(q[n].v[e], x1[n].v[e], sums[1][n].v[e]);
+                        for (int e = 0; e < Me::N; ++e) {
+                            const tc::Two g1 = p[n].v[e], g2 = q[n].v[e];
+                            p[n].v[e] = tc::fma2(g1, c.v[e], tc::mul2(g2, s.v[e]));
+                            q[n].v[e] = tc::fma2(g2, c.v[e], tc::mul2(tc::mul2(g1, minus), s.v[e]));
+                        }
                     }
-            };
+                    if (a.norm) {
+                        Values<V> x0[NV], x1[NV];
+                        Me::unpack(x_row[i], x0, x1);
+                        const float r = me.rstd(x0, x1);
+                        const tc::Two rr = tc::two(r, r);
+                        tc::Two dot = tc::two(0.f, 0.f);
 #pragma unroll
-            for (int n = 0; n < NV; ++n)
+                        for (int n = 0; n < NV; ++n) {
+                            const Values<V> w0 = me.entries(weights, n, 0), w1 = me.entries(weights, n, V);
 #pragma unroll
-                for (int e = 0; e < Me::N; ++e) x0[n].v[e] = tc::mul2(x0[n].v[e], rr), x1[n].v[e] = tc::mul2(x1[n].v[e], rr);
-            if (turn.there) {  // of a group without a row r may be infinite
-                if (k) add(sum[1]);
-                else add(sum[0]);
-            }
+                            for (int e = 0; e < Me::N; ++e) {
+                                x0[n].v[e] = tc::mul2(x0[n].v[e], rr), x1[n].v[e] = tc::mul2(x1[n].v[e], rr);
+                                if (there) {  // of a group without a row r may be infinite
+                                    sum[k][0][n].v[e] = tc::fma2(p[n].v[e], x0[n].v[e], sum[k][0][n].v[e]);
+                                    sum[k][1][n].v[e] = tc::fma2(q[n].v[e], x1[n].v[e], sum[k][1][n].v[e]);
+                                }
+                                p[n].v[e] = tc::mul2(p[n].v[e], w0.v[e]), q[n].v[e] = tc::mul2(q[n].v[e], w1.v[e]);
+                                dot = tc::fma2(p[n].v[e], x0[n].v[e], tc::fma2(q[n].v[e], x1[n].v[e], dot));
+                            }
+                        }
+                        const float m = -me.group_sum(dot) * a.inv_dim;
+                        const tc::Two mm = tc::two(m, m);
 #pragma unroll
-            for (int n = 0; n < NV; ++n) {
-                const Values<V> w0 = me.entries(w, n, 0), w1 = me.entries(w, n, V);
+                        for (int n = 0; n < NV; ++n)
 #pragma unroll
-                for (int e = 0; e < Me::N; ++e) {
-                    p[n].v[e] = tc::mul2(p[n].v[e], w0.v[e]), q[n].v[e] = tc::mul2(q[n].v[e], w1.v[e]);
-                    dot = tc::fma2(p[n].v[e], x0[n].v[e], tc::fma2(q[n].v[e], x1[n].v[e], dot));
+                            for (int e = 0; e < Me::N; ++e) {
+                                p[n].v[e] = tc::mul2(tc::fma2(x0[n].v[e], mm, p[n].v[e]), rr);
+                                q[n].v[e] = tc::mul2(tc::fma2(x1[n].v[e], mm, q[n].v[e]), rr);
+                            }
+                    }
+                    if (there) me.store(out, p, q);
                 }
+                left -= kBwdAhead * me.rows;
             }
-            const float m = -me.group_sum(dot) * a.inv_dim;
-            const tc::Two mm = tc::two(m, m);
-#pragma unroll
-            for (int n = 0; n < NV; ++n)
-#pragma unroll
-                for (int e = 0; e < Me::N; ++e) {
-                    p[n].v[e] = tc::mul2(tc::fma2(x0[n].v[e], mm, p[n].v[e]), rr);
-                    q[n].v[e] = tc::mul2(tc::fma2(x1[n].v[e], mm, q[n].v[e]), rr);
-                }
-        }
-        if (turn.there) me.store(a.half[k].out, turn.out, p, q);
-        x_row = x_next;
-        g_row = g_next;
-        turn = next;
+        });
     }
     if (!a.half[0].part && !a.half[1].part) return;
     // the warp's groups, then the CTA's warps, in order

@@ -49,6 +49,11 @@ struct LinearProduct {
     LinearPlan plan;
 };
 
+// Where a part of a tile lies: [columns / 8][rows][8].
+__device__ __forceinline__ float* linear_part(const LinearProduct& p, int slot, int row, int col) {
+    return p.parts + slot * p.plan.slot_values() + (col / 8 * p.plan.tile_m + row) * 8 + col % 8;
+}
+
 // One stretch of a tile's K blocks; slot: of the part it is left in, -1 where it is the whole tile.
 struct LinearPiece {
     int32_t tile, k0, k1, slot;
@@ -199,14 +204,13 @@ template <int ACT>
 __device__ __forceinline__ void act_pair(float& x, float& y) {
     using namespace tc;
     if constexpr (ACT == SXCUDA_ACT_GELU) {
-        // max(z, 0) - |z| Phi(-|z|); beyond 64 the tail is zero, and infinity times zero would be NaN
-        float a, b;
-        asm("min.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(fabsf(x)), "f"(64.f));
-        asm("min.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(fabsf(y)), "f"(64.f));
-        const Two z = two(a, b);
+        // max(z, 0) - |z| Phi(-|z|). Beyond 64 the tail is zero, which infinity must not multiply; a NaN comes
+        // back by exp(-z^2 / 2) alone. One reciprocal for two: of 1 .. 20.2, so that their product is as good.
+        const Two a = two(fminf(fabsf(x), 64.f), fminf(fabsf(y), 64.f));
         float u, v;
-        split(fma2(z, two(0.3f, 0.3f), two(1.f, 1.f)), u, v);
-        const Two t = two(rcp_fast(u), rcp_fast(v));
+        split(fma2(a, two(0.3f, 0.3f), two(1.f, 1.f)), u, v);
+        const float both = rcp_fast(u * v);
+        const Two t = mul2(two(both, both), two(v, u)), z = two(x, y);
         split(mul2(mul2(z, two(-0.5f * kLog2Of, -0.5f * kLog2Of)), z), u, v);
         const Two e = two(exp2_fast(u), exp2_fast(v));
         Two p = fma2(two(0x1.3bca6ap-4f, 0x1.3bca6ap-4f), t, two(-0x1.ba7182p-3f, -0x1.ba7182p-3f));
@@ -214,7 +218,7 @@ __device__ __forceinline__ void act_pair(float& x, float& y) {
         p = fma2(p, t, two(-0x1.27505cp-3f, -0x1.27505cp-3f));
         p = fma2(p, t, two(-0x1.d1e316p-4f, -0x1.d1e316p-4f));
         p = fma2(p, t, two(-0x1.ebd2f4p-4f, -0x1.ebd2f4p-4f));  // all signs turned
-        split(fma2(mul2(mul2(p, t), e), z, two(fmaxf(x, 0.f), fmaxf(y, 0.f))), x, y);
+        split(fma2(mul2(mul2(p, t), a), e, two(fmaxf(x, 0.f), fmaxf(y, 0.f))), x, y);
     } else if constexpr (ACT == SXCUDA_ACT_SILU || ACT == SXCUDA_ACT_GELU_TANH) {
         const Two z = two(x, y);
         Two u = z;
