@@ -961,7 +961,7 @@ typedef struct SxLinearGrads {
 int32_t sxcuda_linear_bwd(const SxLinearInputs* in, const SxLinearGradsIn* gin, const SxLinearGrads* out,
                           void* workspace, size_t* workspace_bytes, sxcuda_stream_t stream);
 
-/* Status bits of the linear kernels of the current device, as sxcuda_attention_status. */
+/* Status bits of the linear and qk_norm_rotary kernels of the current device, as sxcuda_attention_status. */
 int32_t sxcuda_linear_status(uint32_t* status);
 
 /* Queries and keys normalised per head and rotated by the positions of their tokens:

@@ -26,7 +26,7 @@ uint32_t linear_status() {
     cuda_check(cudaDeviceSynchronize(), "linear_status");
     cuda_check(cudaMemcpyFromSymbol(&st, g_linear_status, sizeof(st)), "linear_status");
     if (st) cuda_check(cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(zero)), "linear_status");
-    return st;
+    return st | rotary_status();
 }
 
 namespace {

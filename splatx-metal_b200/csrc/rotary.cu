@@ -12,7 +12,10 @@
 // A warp takes one token at a time, its queries and then its keys: its lanes make the token's sines and
 // cosines once for all heads, in shared memory, in the order in which lanes read them; the weights lie there
 // in the same way. Groups of a warp read the same entries at the same time, so that a read is one pass of
-// shared memory, and registers are left for warps and for rows that are on their way.
+// shared memory. The token's rows come to shared memory by bulk copies, the next token's while one is worked
+// on, and leave from their place there by bulk copies: the loops then have no addresses of memory and no
+// registers for rows on their way. Rows that such copies do not reach (16 bytes) are read and written value by
+// value.
 // Angles: position x frequency in turns in 64 bits, the nearest quarter turn taken off there; what is left
 // is at most an eighth, and its 32 bits are exact to 2^-28 of a turn however far the position.
 #include <algorithm>
@@ -20,9 +23,21 @@
 
 #include "sx_internal.h"
 #include "sx_network.h"
-#include "sx_two.cuh"
+#include "sx_tcgen05.cuh"
 
 namespace sx {
+
+__device__ uint32_t g_rotary_status;
+
+uint32_t rotary_status() {
+    uint32_t st = 0;
+    const uint32_t zero = 0;
+    cuda_check(cudaDeviceSynchronize(), "rotary_status");
+    cuda_check(cudaMemcpyFromSymbol(&st, g_rotary_status, sizeof(st)), "rotary_status");
+    if (st) cuda_check(cudaMemcpyToSymbol(g_rotary_status, &zero, sizeof(zero)), "rotary_status");
+    return st;
+}
+
 namespace {
 
 constexpr int kRotThreads = 128;
@@ -45,6 +60,7 @@ struct RotArgs {
     int64_t pos_batch, pos_token, pos_axis;
     int64_t tokens, units;
     int32_t chunk, chunks;  // turns of a unit of work, units of a token
+    int32_t stage;          // bytes of a unit's rows of one kind in shared memory
     int32_t pos_dtype, param_dtype, axes, dim, pairs, slots, lanes;  // slots: V pairs each; lanes: of a row's group
     int32_t mode, norm;
     int32_t axis_dims[4];
@@ -85,11 +101,6 @@ __device__ __forceinline__ Slot slot_at(const RotArgs& a, int slot) {
     return {start + j, start + j + a.axis_dims[axis] / 2};  // the run starts at value 2 start
 }
 
-template <typename T, int V, int NV>
-struct Row {
-    Pack<T, V> first[NV], second[NV];
-};
-
 // V values in pairs that one instruction works on.
 template <int V>
 struct Values {
@@ -97,35 +108,38 @@ struct Values {
     tc::Two v[N];
 };
 
-extern __shared__ double rot_smem[];
+constexpr int kTable = 2 * kRotMostPairs;  // floats of a table: V first entries and V seconds of up to 128 / V slots
+
+struct RotShared {
+    alignas(16) float weights[2][kTable];       // of queries and keys
+    alignas(16) float angles[kRotWarps][kTable];  // cosines and sines of each warp's token
+    double turns[kRotMostPairs];
+    uint64_t full[kRotWarps][2];  // barriers of the stages
+    uint8_t axis[kRotMostPairs];
+    uint32_t failed;
+};
 
 // The thread's part of a kernel.
 template <typename T, int V, bool NB, int NV>
 struct Rot {
-    static constexpr int W = V < 4 ? V : 4;      // values of a table access
+    static constexpr int W = V < 4 ? V : 4;                   // values of a table access
+    static constexpr int kPiece = kRotMostPairs / V * W;      // floats from an access' entries to the slots' next ones
     static constexpr int N = Values<V>::N;
     const RotArgs& a;
-    double* turns;
-    float* weights;  // of queries, then of keys: [2][2 V / W][slots][W], first values and partners
-    float* table;    // [2 V / W][slots][W]: cosines, then sines of the warp's token
-    uint8_t* axis;
+    RotShared& sh;
+    float* table;
     int lane, group, in_group, rows;  // rows: groups of a warp
-    Slot at[NV];
-    bool mine[NV];
+    int first[NV], second[NV];        // where the slots are in a head; 0 where the slot is not the thread's own
+    bool mine[NV], pair[NV];
 
-    __device__ explicit Rot(const RotArgs& a) : a(a), turns(rot_smem), lane(threadIdx.x & 31) {
-        const int width = 2 * a.slots * V;
-        weights = reinterpret_cast<float*>(rot_smem + (a.pairs + 1) / 2 * 2);
-        table = weights + (2 + (threadIdx.x >> 5)) * width;
-        axis = reinterpret_cast<uint8_t*>(weights + (2 + kRotWarps) * width);
-        for (int i = threadIdx.x; i < a.pairs; i += kRotThreads) turns[i] = a.turns[i], axis[i] = a.axis[i];
+    __device__ Rot(const RotArgs& a, RotShared& sh) : a(a), sh(sh), table(sh.angles[threadIdx.x >> 5]), lane(threadIdx.x & 31) {
+        for (int i = threadIdx.x; i < a.pairs; i += kRotThreads) sh.turns[i] = a.turns[i], sh.axis[i] = a.axis[i];
         for (int i = threadIdx.x; i < 2 * a.slots * V; i += kRotThreads) {
-            const int k = i >= a.slots * V, pair = i - k * a.slots * V;
-            const Slot s = slot_at<V>(a, pair / V);
-            const RotHalf& h = a.half[k];
-            const int one = place(s, pair % V, 0), two = place(s, pair % V, 1);
-            *entry(weights + k * width, pair, 0) = rot_param(h.weight, a.param_dtype, one);
-            *entry(weights + k * width, pair, V) = two < 0 ? 0.f : rot_param(h.weight, a.param_dtype, two);
+            const int k = i >= a.slots * V, at = i - k * a.slots * V;
+            const Slot s = slot_at<V>(a, at / V);
+            const int one = place(s.first, s.second, at % V, 0), two = place(s.first, s.second, at % V, 1);
+            *entry(sh.weights[k], at, 0) = rot_param(a.half[k].weight, a.param_dtype, one);
+            *entry(sh.weights[k], at, V) = two < 0 ? 0.f : rot_param(a.half[k].weight, a.param_dtype, two);
         }
         group = lane / a.lanes;
         in_group = lane % a.lanes;
@@ -134,25 +148,25 @@ struct Rot {
         for (int n = 0; n < NV; ++n) {
             const int slot = in_group + n * a.lanes;
             mine[n] = slot < a.slots;
-            at[n] = mine[n] ? slot_at<V>(a, slot) : Slot{0, -1};
+            const Slot s = mine[n] ? slot_at<V>(a, slot) : Slot{0, 0};
+            pair[n] = V > 1 || s.second >= 0;
+            first[n] = s.first, second[n] = pair[n] ? s.second : 0;
         }
         for (int i = lane; i < a.slots * V; i += 32) *entry(table, i, 0) = 1.f, *entry(table, i, V) = 0.f;  // not rotated
         __syncthreads();
     }
-    static size_t smem_bytes(const RotArgs& a) {
-        return (a.pairs + 1) / 2 * 2 * 8 + static_cast<size_t>(2 + kRotWarps) * 2 * a.slots * V * 4 + a.pairs;
-    }
-    __device__ float* entry(float* t, int pair, int skip) const {
+    static __device__ float* entry(float* t, int pair, int skip) {
         const int slot = pair / V, e = pair % V + skip;
-        return t + ((e / W) * a.slots + slot) * W + e % W;
+        return t + e / W * kPiece + slot * W + e % W;
     }
     // The entries of the thread's slot n: V of them from `skip`.
-    __device__ Values<V> entries(const float* t, int n, int skip) const {
+    __device__ __forceinline__ Values<V> entries(const float* t, int n, int skip) const {
         const int slot = mine[n] ? in_group + n * a.lanes : 0;
+        const float* from = t + slot * W;
         Values<V> r;
 #pragma unroll
         for (int e = 0; e < V; e += W) {
-            const auto x = reinterpret_cast<const Pack<float, W>*>(t)[((skip + e) / W) * a.slots + slot];
+            const auto x = *reinterpret_cast<const Pack<float, W>*>(from + (skip + e) / W * kPiece);
             if constexpr (W == 1) {
                 r.v[0] = tc::two(x.v[0], 0.f);
             } else {
@@ -161,33 +175,6 @@ struct Rot {
             }
         }
         return r;
-    }
-    // Lane i's position along axis i.
-    __device__ double position(int64_t unit) const {
-        if (lane >= a.axes || unit >= a.units) return 0.;
-        const Token t = token_of(unit);
-        const int64_t i = t.batch * a.pos_batch + t.token * a.pos_token + lane * a.pos_axis;
-        if (a.pos_dtype == SXCUDA_POS_F32) return static_cast<const float*>(a.positions)[i];
-        if (a.pos_dtype == SXCUDA_POS_I32) return static_cast<const int32_t*>(a.positions)[i];
-        return static_cast<double>(static_cast<const int64_t*>(a.positions)[i]);
-    }
-    __device__ void angles(double mine_position) const {
-        __syncwarp();
-        for (int i = lane; i - lane < a.pairs; i += 32) {
-            const int j = i < a.pairs ? i : 0;
-            const double p = __shfl_sync(kFullMask, mine_position, axis[j]);
-            const double t = p * turns[j], quarters = rint(4. * t);
-            // of a product beyond 2^53 no digit of a turn is left: it stands at 0 (of an infinity NaN is left)
-            float sine, cosine;
-            sincospif(static_cast<float>(2. * fma(-0.25, quarters, t)), &sine, &cosine);
-            const int q = static_cast<int>(static_cast<long long>(fabs(quarters) < 9e15 ? quarters : 0.) & 3);
-            const float cc = q & 1 ? sine : cosine, ss = q & 1 ? cosine : sine;
-            if (i < a.pairs) {
-                *entry(table, i, 0) = q == 1 || q == 2 ? -cc : cc;
-                *entry(table, i, V) = q >= 2 ? -ss : ss;
-            }
-        }
-        __syncwarp();
     }
     struct Token {
         int64_t batch, token;
@@ -202,16 +189,65 @@ struct Rot {
         const int64_t t = unit / a.chunks, b = t / a.tokens;
         return {b, t - b * a.tokens, static_cast<int>(unit - t * a.chunks)};
     }
-    // A slot that is not the thread's own keeps the zeros it started with.
-    __device__ void load(Row<T, V, NV>& r, const T* row, bool there) const {
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-            if (there && mine[n]) {
-                r.first[n] = *reinterpret_cast<const Pack<T, V>*>(row + at[n].first);
-                if (V > 1 || at[n].second >= 0) r.second[n] = *reinterpret_cast<const Pack<T, V>*>(row + at[n].second);
-            }
+    // Lane i's position along axis i.
+    __device__ double position(const Token& t) const {
+        if (lane >= a.axes) return 0.;
+        const int64_t i = t.batch * a.pos_batch + t.token * a.pos_token + lane * a.pos_axis;
+        if (a.pos_dtype == SXCUDA_POS_F32) return static_cast<const float*>(a.positions)[i];
+        if (a.pos_dtype == SXCUDA_POS_I32) return static_cast<const int32_t*>(a.positions)[i];
+        return static_cast<double>(static_cast<const int64_t*>(a.positions)[i]);
     }
-    __device__ void store(T* row, const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
+    __device__ void angles(double mine_position) const {
+        __syncwarp();
+        for (int i = lane; i - lane < a.pairs; i += 32) {
+            const int j = i < a.pairs ? i : 0;
+            const double p = __shfl_sync(kFullMask, mine_position, sh.axis[j]);
+            const double t = p * sh.turns[j], quarters = rint(4. * t);
+            // of a product beyond 2^51 no quarter of a turn is left: it stands at 0 (of an infinity NaN is left)
+            float sine, cosine;
+            sincospif(static_cast<float>(2. * fma(-0.25, quarters, t)), &sine, &cosine);
+            const int q = fabs(quarters) < 2251799813685248. ? __double2loint(quarters + 6755399441055744.) & 3 : 0;  // its low bits
+            const float cc = q & 1 ? sine : cosine, ss = q & 1 ? cosine : sine;
+            if (i < a.pairs) {
+                *entry(table, i, 0) = q == 1 || q == 2 ? -cc : cc;
+                *entry(table, i, V) = q >= 2 ? -ss : ss;
+            }
+        }
+        __syncwarp();
+    }
+    // The place in the head of the first (second) value of a slot's pair e; -1: there is none.
+    static __device__ int place(int first, int second, int e, int which) {
+        if constexpr (NB) {
+            const int i = 2 * e + which;
+            return i < V ? first + i : second < 0 ? -1 : second + i - V;
+        } else {
+            return which ? (second < 0 ? -1 : second + e) : first + e;
+        }
+    }
+    // A row's values, first ones and partners. A slot that is not the thread's own is zeros.
+    __device__ __forceinline__ void load(const T* row, Values<V> (&p)[NV], Values<V> (&q)[NV]) const {
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const auto x = *reinterpret_cast<const Pack<T, V>*>(row + first[n]), y = *reinterpret_cast<const Pack<T, V>*>(row + second[n]);
+            if constexpr (V == 1) {
+                p[n].v[0] = tc::two(mine[n] ? to_f32(x.v[0]) : 0.f, 0.f);
+                q[n].v[0] = tc::two(mine[n] && pair[n] ? to_f32(y.v[0]) : 0.f, 0.f);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e += 2) {
+                    if constexpr (NB) {  // pair e is the values 2 e and 2 e + 1
+                        const float2 one = two_of(2 * e < V ? x : y, 2 * e % V), other = two_of(2 * e + 2 < V ? x : y, (2 * e + 2) % V);
+                        p[n].v[e / 2] = tc::two(one.x, other.x), q[n].v[e / 2] = tc::two(one.y, other.y);
+                    } else {
+                        const float2 one = two_of(x, e), other = two_of(y, e);
+                        p[n].v[e / 2] = tc::two(one.x, one.y), q[n].v[e / 2] = tc::two(other.x, other.y);
+                    }
+                }
+                if (!mine[n]) p[n] = q[n] = Values<V>{};
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* row, const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             if (!mine[n]) continue;
@@ -228,7 +264,7 @@ struct Rot {
                     float a0, a1, b0, b1;
                     tc::split(p[n].v[e / 2], a0, a1);
                     tc::split(q[n].v[e / 2], b0, b1);
-                    if constexpr (NB) {  // pair e is the values 2 e and 2 e + 1
+                    if constexpr (NB) {
                         two_to(2 * e < V ? x : y, 2 * e % V, a0, b0);
                         two_to(2 * e + 2 < V ? x : y, (2 * e + 2) % V, a1, b1);
                     } else {
@@ -237,43 +273,19 @@ struct Rot {
                     }
                 }
             }
-            *reinterpret_cast<Pack<T, V>*>(row + at[n].first) = x;
-            if (V > 1 || at[n].second >= 0) *reinterpret_cast<Pack<T, V>*>(row + at[n].second) = y;
+            *reinterpret_cast<Pack<T, V>*>(row + first[n]) = x;
+            if (pair[n]) *reinterpret_cast<Pack<T, V>*>(row + second[n]) = y;
         }
+    }
+    static __device__ __forceinline__ float2 two_of(const Pack<T, V>& x, int i) {
+        if constexpr (std::is_same_v<T, __half>) return __half22float2(reinterpret_cast<const __half2*>(x.v)[i / 2]);
+        else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(x.v)[i / 2]);
+        else return {x.v[i], x.v[i + 1]};
     }
     static __device__ __forceinline__ void two_to(Pack<T, V>& x, int i, float lo, float hi) {
         if constexpr (std::is_same_v<T, __half>) reinterpret_cast<__half2*>(x.v)[i / 2] = __floats2half2_rn(lo, hi);
         else if constexpr (std::is_same_v<T, __nv_bfloat16>) reinterpret_cast<__nv_bfloat162*>(x.v)[i / 2] = __floats2bfloat162_rn(lo, hi);
         else x.v[i] = lo, x.v[i + 1] = hi;
-    }
-    // The first (second) value of pair e among a slot's.
-    template <typename P>
-    static __device__ __forceinline__ auto* value(P& x, P& y, int e, int second) {
-        if constexpr (NB) {
-            const int i = 2 * e + second;
-            return i < V ? &x.v[i] : &y.v[i - V];
-        } else {
-            return second ? &y.v[e] : &x.v[e];
-        }
-    }
-    // The place in the head of the first (second) value of a slot's pair e; -1: there is none.
-    static __device__ int place(const Slot& s, int e, int second) {
-        if constexpr (NB) {
-            const int i = 2 * e + second;
-            return i < V ? s.first + i : s.second < 0 ? -1 : s.second + i - V;
-        } else {
-            return second ? (s.second < 0 ? -1 : s.second + e) : s.first + e;
-        }
-    }
-    static __device__ void unpack(const Row<T, V, NV>& r, Values<V> (&p)[NV], Values<V> (&q)[NV]) {
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-#pragma unroll
-            for (int e = 0; e < V; e += 2) {
-                const auto get = [&](int i, int second) { return i < V ? to_f32(*value(r.first[n], r.second[n], i, second)) : 0.f; };
-                p[n].v[e / 2] = tc::two(get(e, 0), get(e + 1, 0));
-                q[n].v[e / 2] = tc::two(get(e, 1), get(e + 1, 1));
-            }
     }
     __device__ float group_sum(tc::Two x) const {
         float lo, hi;
@@ -288,204 +300,283 @@ struct Rot {
         for (int n = 0; n < NV; ++n)
 #pragma unroll
             for (int e = 0; e < N; ++e) ss = tc::fma2(p[n].v[e], p[n].v[e], tc::fma2(q[n].v[e], q[n].v[e], ss));
-        return __frsqrt_rn(fmaf(group_sum(ss), a.inv_dim, a.eps));
+        return rsqrtf(fmaf(group_sum(ss), a.inv_dim, a.eps));  // within 2 units of the last place
+    }
+
+    // A row of the group's, forward: from `x` to `out` where there is one.
+    __device__ __forceinline__ void forward(const T* x, T* out, int k, bool there) const {
+        const tc::Two minus = tc::two(-1.f, -1.f);
+        Values<V> p[NV], q[NV];
+        load(x, p, q);
+        if (a.norm) {
+            const float r = rstd(p, q);
+            const tc::Two rr = tc::two(r, r);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const Values<V> w0 = entries(sh.weights[k], n, 0), w1 = entries(sh.weights[k], n, V);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    p[n].v[e] = tc::mul2(tc::mul2(p[n].v[e], rr), w0.v[e]);
+                    q[n].v[e] = tc::mul2(tc::mul2(q[n].v[e], rr), w1.v[e]);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const Values<V> c = entries(table, n, 0), s = entries(table, n, V);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const tc::Two u1 = p[n].v[e], u2 = q[n].v[e];
+                p[n].v[e] = tc::fma2(u1, c.v[e], tc::mul2(tc::mul2(u2, minus), s.v[e]));
+                q[n].v[e] = tc::fma2(u1, s.v[e], tc::mul2(u2, c.v[e]));
+            }
+        }
+        if (there) store(out, p, q);
+    }
+    // The same backward, from the gradient `g` (and x, with norm) to `out`; adds to the weight's sums.
+    __device__ __forceinline__ void backward(const T* x, const T* g, T* out, int k, bool there, Values<V> (&sum)[2][NV]) const {
+        const tc::Two minus = tc::two(-1.f, -1.f);
+        Values<V> p[NV], q[NV];
+        load(g, p, q);
+#pragma unroll
+        for (int n = 0; n < NV; ++n) {
+            const Values<V> c = entries(table, n, 0), s = entries(table, n, V);
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const tc::Two g1 = p[n].v[e], g2 = q[n].v[e];
+                p[n].v[e] = tc::fma2(g1, c.v[e], tc::mul2(g2, s.v[e]));
+                q[n].v[e] = tc::fma2(g2, c.v[e], tc::mul2(tc::mul2(g1, minus), s.v[e]));
+            }
+        }
+        if (a.norm) {
+            Values<V> x0[NV], x1[NV];
+            load(x, x0, x1);
+            const float r = rstd(x0, x1);
+            const tc::Two rr = tc::two(r, r);
+            tc::Two dot = tc::two(0.f, 0.f);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const Values<V> w0 = entries(sh.weights[k], n, 0), w1 = entries(sh.weights[k], n, V);
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    x0[n].v[e] = tc::mul2(x0[n].v[e], rr), x1[n].v[e] = tc::mul2(x1[n].v[e], rr);
+                    if (there) {  // what a group without a row has read is nothing
+                        sum[0][n].v[e] = tc::fma2(p[n].v[e], x0[n].v[e], sum[0][n].v[e]);
+                        sum[1][n].v[e] = tc::fma2(q[n].v[e], x1[n].v[e], sum[1][n].v[e]);
+                    }
+                    p[n].v[e] = tc::mul2(p[n].v[e], w0.v[e]), q[n].v[e] = tc::mul2(q[n].v[e], w1.v[e]);
+                    dot = tc::fma2(p[n].v[e], x0[n].v[e], tc::fma2(q[n].v[e], x1[n].v[e], dot));
+                }
+            }
+            const float m = -group_sum(dot) * a.inv_dim;
+            const tc::Two mm = tc::two(m, m);
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int e = 0; e < N; ++e) {
+                    p[n].v[e] = tc::mul2(tc::fma2(x0[n].v[e], mm, p[n].v[e]), rr);
+                    q[n].v[e] = tc::mul2(tc::fma2(x1[n].v[e], mm, q[n].v[e]), rr);
+                }
+        }
+        if (there) store(out, p, q);
+    }
+    // The CTA's sums for the weights' gradients: its warps' groups, then its warps, in order.
+    __device__ void leave(const Values<V> (&sum)[2][2][NV]) const {
+        float* sums = sh.angles[0];  // [warps, dim], over the tables
+        static_assert(sizeof(sh.angles) >= kRotWarps * 256 * 4);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (!a.half[k].part) continue;
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < NV; ++n)
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    float x[2], lo, hi;
+                    tc::split(sum[k][0][n].v[e / 2], lo, hi);
+                    x[0] = e % 2 ? hi : lo;
+                    tc::split(sum[k][1][n].v[e / 2], lo, hi);
+                    x[1] = e % 2 ? hi : lo;
+                    for (int o = 16; o >= a.lanes; o >>= 1)
+                        x[0] += __shfl_xor_sync(kFullMask, x[0], o), x[1] += __shfl_xor_sync(kFullMask, x[1], o);
+                    if (group == 0 && mine[n]) {
+                        const int i = place(first[n], second[n], e, 0), j = place(first[n], second[n], e, 1);
+                        sums[(threadIdx.x >> 5) * a.dim + i] = x[0];
+                        if (pair[n]) sums[(threadIdx.x >> 5) * a.dim + j] = x[1];
+                    }
+                }
+            __syncthreads();
+            for (int i = threadIdx.x; i < a.dim; i += kRotThreads) {
+                float x = 0.f;
+                for (int w = 0; w < kRotWarps; ++w) x += sums[w * a.dim + i];
+                a.half[k].part[static_cast<int64_t>(blockIdx.x) * a.dim + i] = x;
+            }
+        }
     }
 };
 
-// Calls f(half, base of the token's rows as offsets, first turn, end) for the queries' and the keys' turns of a unit.
-template <typename F>
-__device__ __forceinline__ void rot_halves(const RotArgs& a, int chunk, F&& f) {
-    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.half[0].turns + a.half[1].turns), q = a.half[0].turns;
-    if (begin < q) f(std::integral_constant<int, 0>{}, begin, min(end, q));
-    if (end > q) f(std::integral_constant<int, 1>{}, max(begin, q) - q, end - q);
-}
-
-constexpr int kFwdAhead = 4, kBwdAhead = 2;  // rows of a group that are asked for at once
-
-template <typename T, int V, bool NB, int NV>
-__global__ void __launch_bounds__(kRotThreads, V == 1 ? 2 : 5) rotary_fwd_kernel(const __grid_constant__ RotArgs a) {
-    const Rot<T, V, NB, NV> me(a);
-    using Me = Rot<T, V, NB, NV>;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kRotWarps;
-    const tc::Two minus = tc::two(-1.f, -1.f);
-    Row<T, V, NV> row[kFwdAhead] = {};
-    int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5);
-    double position = me.position(unit);
-    for (; unit < a.units; unit += step) {
-        const auto token = me.token_of(unit);
-        bool made = false;
-        rot_halves(a, token.chunk, [&](auto k, int turn, int end) {
-            const RotHalf& h = a.half[k];
-            const T* x = static_cast<const T*>(h.x) + token.batch * h.x_batch + token.token * h.x_token + (turn * me.rows + me.group) * h.x_head;
-            T* out = static_cast<T*>(h.out) + token.batch * h.out_batch + token.token * h.out_token + (turn * me.rows + me.group) * h.out_head;
-            const int64_t x_step = me.rows * h.x_head, out_step = me.rows * h.out_head;
-            const float* weights = me.weights + k * 2 * a.slots * V;
-            int left = h.heads - turn * me.rows - me.group;
-            for (; turn < end; turn += kFwdAhead) {
-#pragma unroll
-                for (int i = 0; i < kFwdAhead; ++i, x += x_step) me.load(row[i], x, turn + i < end && left > i * me.rows);
-                if (!made) {
-                    me.angles(position);
-                    position = me.position(unit + step);
-                    made = true;
-                }
-#pragma unroll
-                for (int i = 0; i < kFwdAhead; ++i, out += out_step) {
-                    if (turn + i >= end) break;
-                    Values<V> p[NV], q[NV];
-                    Me::unpack(row[i], p, q);
-                    if (a.norm) {
-                        const float r = me.rstd(p, q);
-                        const tc::Two rr = tc::two(r, r);
-#pragma unroll
-                        for (int n = 0; n < NV; ++n) {
-                            const Values<V> w0 = me.entries(weights, n, 0), w1 = me.entries(weights, n, V);
-#pragma unroll
-                            for (int e = 0; e < Me::N; ++e) {
-                                p[n].v[e] = tc::mul2(tc::mul2(p[n].v[e], rr), w0.v[e]);
-                                q[n].v[e] = tc::mul2(tc::mul2(q[n].v[e], rr), w1.v[e]);
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int n = 0; n < NV; ++n) {
-                        const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
-#pragma unroll
-                        for (int e = 0; e < Me::N; ++e) {
-                            const tc::Two u1 = p[n].v[e], u2 = q[n].v[e];
-                            p[n].v[e] = tc::fma2(u1, c.v[e], tc::mul2(tc::mul2(u2, minus), s.v[e]));
-                            q[n].v[e] = tc::fma2(u1, s.v[e], tc::mul2(u2, c.v[e]));
-                        }
-                    }
-                    if (left > i * me.rows) me.store(out, p, q);
-                }
-                left -= kFwdAhead * me.rows;
-            }
-        });
-    }
-}
-
-template <typename T, int V, bool NB, int NV>
-__global__ void __launch_bounds__(kRotThreads, V == 1 ? 2 : 4) rotary_bwd_kernel(const __grid_constant__ RotArgs a) {
-    const Rot<T, V, NB, NV> me(a);
-    using Me = Rot<T, V, NB, NV>;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kRotWarps;
-    const tc::Two minus = tc::two(-1.f, -1.f);
-    Values<V> sum[2][2][NV];  // of queries and keys, first values and partners
+template <int V, int NV>
+__device__ __forceinline__ void no_sums(Values<V> (&sum)[2][2][NV]) {
 #pragma unroll
     for (int i = 0; i < 4 * NV; ++i)
 #pragma unroll
-        for (int e = 0; e < Me::N; ++e) sum[i / NV / 2][i / NV % 2][i % NV].v[e] = tc::two(0.f, 0.f);
-    Row<T, V, NV> x_row[kBwdAhead] = {}, g_row[kBwdAhead] = {};
-    int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5);
-    double position = me.position(unit);
-    for (; unit < a.units; unit += step) {
+        for (int e = 0; e < Values<V>::N; ++e) sum[i / NV / 2][i / NV % 2][i % NV].v[e] = tc::two(0.f, 0.f);
+}
+
+// A unit's rows of queries or keys: heads from `head` on, `n` of them, row `at` of the unit's first.
+struct RotRun {
+    int head, n, at;
+};
+__device__ __forceinline__ RotRun rot_run(const RotArgs& a, int rows, int chunk, int k) {
+    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.half[0].turns + a.half[1].turns), q = a.half[0].turns;
+    const int from = k ? max(begin, q) - q : begin, to = k ? end - q : min(end, q);
+    return {from * rows, max(min(to * rows, a.half[k].heads) - from * rows, 0), k ? (max(begin, q) - begin) * rows : 0};
+}
+
+// Rows value by value.
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(kRotThreads) rotary_plain_kernel(const __grid_constant__ RotArgs a) {
+    __shared__ RotShared sh;
+    const Rot<T, 1, false, 4> me(a, sh);
+    Values<1> sum[2][2][4];
+    no_sums(sum);
+    for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5); unit < a.units;
+         unit += static_cast<int64_t>(gridDim.x) * kRotWarps) {
         const auto token = me.token_of(unit);
-        bool made = false;
-        rot_halves(a, token.chunk, [&](auto k, int turn, int end) {
+        me.angles(me.position(token));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
             const RotHalf& h = a.half[k];
-            const int head = turn * me.rows + me.group;
-            const T* x = static_cast<const T*>(h.x) + token.batch * h.x_batch + token.token * h.x_token + head * h.x_head;
-            const T* g = static_cast<const T*>(h.g) + token.batch * h.g_batch + token.token * h.g_token + head * h.g_head;
-            T* out = static_cast<T*>(h.out) + token.batch * h.out_batch + token.token * h.out_token + head * h.out_head;
-            const int64_t x_step = me.rows * h.x_head, g_step = me.rows * h.g_head, out_step = me.rows * h.out_head;
-            const float* weights = me.weights + k * 2 * a.slots * V;
-            int left = h.heads - head;
-            for (; turn < end; turn += kBwdAhead) {
-#pragma unroll
-                for (int i = 0; i < kBwdAhead; ++i, x += x_step, g += g_step) {
-                    const bool there = turn + i < end && left > i * me.rows;
-                    me.load(g_row[i], g, there);
-                    me.load(x_row[i], x, there && a.norm);
-                }
-                if (!made) {
-                    me.angles(position);
-                    position = me.position(unit + step);
-                    made = true;
-                }
-#pragma unroll
-                for (int i = 0; i < kBwdAhead; ++i, out += out_step) {
-                    if (turn + i >= end) break;
-                    const bool there = left > i * me.rows;
-                    Values<V> p[NV], q[NV];
-                    Me::unpack(g_row[i], p, q);
-#pragma unroll
-                    for (int n = 0; n < NV; ++n) {
-                        const Values<V> c = me.entries(me.table, n, 0), s = me.entries(me.table, n, V);
-#pragma unroll
-                        for (int e = 0; e < Me::N; ++e) {
-                            const tc::Two g1 = p[n].v[e], g2 = q[n].v[e];
-                            p[n].v[e] = tc::fma2(g1, c.v[e], tc::mul2(g2, s.v[e]));
-                            q[n].v[e] = tc::fma2(g2, c.v[e], tc::mul2(tc::mul2(g1, minus), s.v[e]));
-                        }
-                    }
-                    if (a.norm) {
-                        Values<V> x0[NV], x1[NV];
-                        Me::unpack(x_row[i], x0, x1);
-                        const float r = me.rstd(x0, x1);
-                        const tc::Two rr = tc::two(r, r);
-                        tc::Two dot = tc::two(0.f, 0.f);
-#pragma unroll
-                        for (int n = 0; n < NV; ++n) {
-                            const Values<V> w0 = me.entries(weights, n, 0), w1 = me.entries(weights, n, V);
-#pragma unroll
-                            for (int e = 0; e < Me::N; ++e) {
-                                x0[n].v[e] = tc::mul2(x0[n].v[e], rr), x1[n].v[e] = tc::mul2(x1[n].v[e], rr);
-                                if (there) {  // of a group without a row r may be infinite
-                                    sum[k][0][n].v[e] = tc::fma2(p[n].v[e], x0[n].v[e], sum[k][0][n].v[e]);
-                                    sum[k][1][n].v[e] = tc::fma2(q[n].v[e], x1[n].v[e], sum[k][1][n].v[e]);
-                                }
-                                p[n].v[e] = tc::mul2(p[n].v[e], w0.v[e]), q[n].v[e] = tc::mul2(q[n].v[e], w1.v[e]);
-                                dot = tc::fma2(p[n].v[e], x0[n].v[e], tc::fma2(q[n].v[e], x1[n].v[e], dot));
-                            }
-                        }
-                        const float m = -me.group_sum(dot) * a.inv_dim;
-                        const tc::Two mm = tc::two(m, m);
-#pragma unroll
-                        for (int n = 0; n < NV; ++n)
-#pragma unroll
-                            for (int e = 0; e < Me::N; ++e) {
-                                p[n].v[e] = tc::mul2(tc::fma2(x0[n].v[e], mm, p[n].v[e]), rr);
-                                q[n].v[e] = tc::mul2(tc::fma2(x1[n].v[e], mm, q[n].v[e]), rr);
-                            }
-                    }
-                    if (there) me.store(out, p, q);
-                }
-                left -= kBwdAhead * me.rows;
+            const RotRun run = rot_run(a, me.rows, token.chunk, k);
+            for (int i = 0; i < run.n; i += me.rows) {
+                const bool there = i + me.group < run.n;
+                const int64_t head = run.head + (there ? i + me.group : i);
+                const auto row = [&](const void* p, int64_t batch, int64_t tokens, int64_t heads) {
+                    return static_cast<const T*>(p) + token.batch * batch + token.token * tokens + head * heads;
+                };
+                const T* x = row(h.x, h.x_batch, h.x_token, h.x_head);
+                T* out = const_cast<T*>(row(h.out, h.out_batch, h.out_token, h.out_head));
+                if constexpr (BACK) me.backward(x, row(h.g, h.g_batch, h.g_token, h.g_head), out, k, there, sum[k]);
+                else me.forward(x, out, k, there);
             }
-        });
-    }
-    if (!a.half[0].part && !a.half[1].part) return;
-    // the warp's groups, then the CTA's warps, in order
-    float* sums = reinterpret_cast<float*>(rot_smem);  // [warps, dim], over the tables
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        if (!a.half[k].part) continue;
-        __syncthreads();
-#pragma unroll
-        for (int n = 0; n < NV; ++n)
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                float x[2], lo, hi;
-                tc::split(sum[k][0][n].v[e / 2], lo, hi);
-                x[0] = e % 2 ? hi : lo;
-                tc::split(sum[k][1][n].v[e / 2], lo, hi);
-                x[1] = e % 2 ? hi : lo;
-                for (int o = 16; o >= a.lanes; o >>= 1)
-                    x[0] += __shfl_xor_sync(kFullMask, x[0], o), x[1] += __shfl_xor_sync(kFullMask, x[1], o);
-                if (me.group == 0 && me.mine[n]) {
-                    const int i = Me::place(me.at[n], e, 0), j = Me::place(me.at[n], e, 1);
-                    sums[(threadIdx.x >> 5) * a.dim + i] = x[0];
-                    if (j >= 0) sums[(threadIdx.x >> 5) * a.dim + j] = x[1];
-                }
-            }
-        __syncthreads();
-        for (int i = threadIdx.x; i < a.dim; i += kRotThreads) {
-            float x = 0.f;
-            for (int w = 0; w < kRotWarps; ++w) x += sums[w * a.dim + i];
-            a.half[k].part[static_cast<int64_t>(blockIdx.x) * a.dim + i] = x;
         }
     }
+    if constexpr (BACK) me.leave(sum);
+}
+
+// Rows by bulk copies: each warp has two stages for a unit's rows (backward: of the gradient, then of x).
+__device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
+}
+
+template <typename T, int V, bool NB, int NV, bool BACK>
+__global__ void __launch_bounds__(kRotThreads, V > 2 ? (BACK ? 4 : 7) : (BACK ? 2 : 3)) rotary_kernel(const __grid_constant__ RotArgs a) {
+    __shared__ RotShared sh;
+    extern __shared__ __align__(128) uint8_t stages[];
+    const int warp = threadIdx.x >> 5;
+    const uint32_t bars = tc::smem_addr(sh.full[warp]);
+    if (threadIdx.x % 32 == 0) {
+        tc::bar_init(bars, 1);
+        tc::bar_init(bars + 8, 1);
+        tc::bar_init_fence();
+    }
+    if (threadIdx.x == 0) sh.failed = 0;
+    const Rot<T, V, NB, NV> me(a, sh);
+    volatile uint32_t* failed = &sh.failed;
+    const int bytes = a.dim * static_cast<int>(sizeof(T)), stage = a.stage * (BACK ? 2 : 1);
+    uint8_t* mine = stages + static_cast<size_t>(warp) * 2 * stage;
+    Values<V> sum[2][2][NV];
+    no_sums(sum);
+    const auto rows_of = [&](const auto& token, const void* p, int64_t batch, int64_t tokens, int64_t heads, int head) {
+        return static_cast<const T*>(p) + token.batch * batch + token.token * tokens + head * heads;
+    };
+    // Asks for a unit's rows: run by run where its heads lie side by side, else a lane a head.
+    const auto ask = [&](const typename Rot<T, V, NB, NV>::Token& token, int s) {
+        const uint32_t to = tc::smem_addr(mine + s * stage), bar = bars + 8 * s;
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // each lane's own: the stage's last rows have left
+        __syncwarp();
+        if (me.lane == 0) {
+            int n = 0;
+            for (int k = 0; k < 2; ++k) n += rot_run(a, me.rows, token.chunk, k).n;
+            tc::bar_expect(bar, n * bytes * (BACK && a.norm ? 2 : 1));
+        }
+        __syncwarp();
+        const auto copy = [&](const T* from, int64_t heads, const RotRun& run, uint32_t at) {
+            if (heads == a.dim) {
+                if (me.lane == 0) tc::bulk_load(at, from, run.n * bytes, bar);
+            } else {
+                for (int i = me.lane; i < run.n; i += 32) tc::bulk_load(at + i * bytes, from + i * heads, bytes, bar);
+            }
+        };
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const RotHalf& h = a.half[k];
+            const RotRun run = rot_run(a, me.rows, token.chunk, k);
+            if (run.n == 0) continue;
+            if (BACK) copy(rows_of(token, h.g, h.g_batch, h.g_token, h.g_head, run.head), h.g_head, run, to + run.at * bytes);
+            if (!BACK || a.norm)
+                copy(rows_of(token, h.x, h.x_batch, h.x_token, h.x_head, run.head), h.x_head, run, to + (BACK ? a.stage : 0) + run.at * bytes);
+        }
+    };
+    const int64_t step = static_cast<int64_t>(gridDim.x) * kRotWarps;
+    int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp;
+    bool ok = true;
+    typename Rot<T, V, NB, NV>::Token token{}, next{};
+    double position = 0.;
+    int asked = 0;
+    if (unit < a.units) {
+        token = me.token_of(unit);
+        ask(token, 0);
+        asked = 1;
+        position = me.position(token);
+    }
+    for (int count = 0; unit < a.units; ++count) {
+        const int s = count & 1;
+        const bool more = unit + step < a.units;
+        me.angles(position);
+        if (more) {
+            next = me.token_of(unit + step);
+            ask(next, s ^ 1);  // its last rows have left while the angles were made
+            ++asked;
+            position = me.position(next);
+        }
+        ok = tc::bar_wait(bars + 8 * s, count >> 1 & 1, failed);
+        if (!ok) break;
+        T* rows = reinterpret_cast<T*>(mine + s * stage);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const RotRun run = rot_run(a, me.rows, token.chunk, k);
+            T* row = rows + (run.at + me.group) * a.dim;
+            for (int i = 0; i < run.n; i += me.rows, row += me.rows * a.dim) {
+                const bool there = i + me.group < run.n;
+                if constexpr (BACK) me.backward(row + a.stage / static_cast<int>(sizeof(T)), row, row, k, there, sum[k]);
+                else me.forward(row, row, k, there);
+            }
+        }
+        tc::fence_smem_to_async();
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const RotHalf& h = a.half[k];
+            const RotRun run = rot_run(a, me.rows, token.chunk, k);
+            T* to = const_cast<T*>(rows_of(token, h.out, h.out_batch, h.out_token, h.out_head, run.head));
+            const uint32_t from = tc::smem_addr(rows) + run.at * bytes;
+            if (h.out_head == a.dim) {
+                if (me.lane == 0 && run.n) bulk_store(to, from, run.n * bytes);
+            } else {
+                for (int i = me.lane; i < run.n; i += 32) bulk_store(to + i * h.out_head, from + i * bytes, bytes);
+            }
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        token = next;
+        unit += step;
+    }
+    if (!ok) {  // nothing may land in this CTA's memory after it has gone
+        for (int i = max(0, asked - 2); i < asked; ++i) tc::bar_drain(bars + 8 * (i & 1), i >> 1 & 1);
+        if (me.lane == 0) atomicOr(&g_rotary_status, 1u);
+    }
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if constexpr (BACK) me.leave(sum);
 }
 
 // Adds the CTAs' sums of 32 values: warp w takes every 32nd row, then the warps are added in order.
@@ -520,21 +611,25 @@ bool view_fits(const SxAttentionView& x, int64_t size, int64_t bytes) {
     return reinterpret_cast<uintptr_t>(x.data) % bytes == 0 && fits(x.batch_stride) && fits(x.token_stride) && fits(x.head_stride);
 }
 
+// Rows that bulk copies reach.
+bool bulk_fits(const SxRotaryInputs& in, const SxAttentionView& x) {
+    return in.head_dim * dtype_bytes(in.dtype) % 16 == 0 && view_fits(x, dtype_bytes(in.dtype), 16);
+}
+
 // The most pairs a thread can take at once: runs of pairs, of their partners and of what is not rotated are
-// multiples of it, and so are the views' strides and addresses.
-int most_pairs(const SxRotaryInputs& in, std::initializer_list<SxAttentionView> views) {
-    const int64_t size = dtype_bytes(in.dtype);
+// multiples of it.
+int most_pairs(const SxRotaryInputs& in) {
     int pairs = 0;
     for (int i = 0; i < in.axes; ++i) pairs += in.axis_dims[i] / 2;
     const int rest = in.head_dim - 2 * pairs;
-    int v = in.dtype == SXCUDA_F32 ? 4 : 8;
     const auto holds = [&](int n) {
         if (rest % 2 || rest / 2 % n || pairs % n) return false;
         if (in.pairs == SXCUDA_PAIRS_AXIS)
             for (int i = 0; i < in.axes; ++i)
                 if (in.axis_dims[i] / 2 % n) return false;
-        return std::all_of(views.begin(), views.end(), [&](const SxAttentionView& x) { return view_fits(x, size, n * size); });
+        return true;
     };
+    int v = in.dtype == SXCUDA_F32 ? 4 : 8;
     while (v > 1 && !holds(v)) v /= 2;
     return v;
 }
@@ -568,20 +663,34 @@ RotArgs rot_args(const SxRotaryInputs& in, int v) {
     return a;
 }
 
-// Units of work: a token with all its heads, so that its sines are taken once; where there are fewer tokens
-// than half the warps that fit, one turn of a warp's groups.
+// Launches f's kernel. Units of work: a token with all its heads, so that its sines are taken once, as far as a
+// stage holds them; where there are fewer tokens than half the warps that fit, one turn of a warp's groups.
+constexpr int kRotStage = 8192;
 template <typename K>
-int rot_divide(RotArgs& a, int64_t tokens, K kernel, size_t smem) {
-    int per_sm = 0;
-    cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kRotThreads, smem), "qk_norm_rotary");
-    const int64_t most = static_cast<int64_t>(sm_count()) * std::min(std::max(per_sm, 1), kRotMostPerSm);
+int rot_launch(RotArgs& a, int64_t tokens, K kernel, int row_bytes, int kinds, cudaStream_t s, float* part, bool q_part, bool k_part) {
     const int rows = 32 / a.lanes;
     for (RotHalf& h : a.half) h.turns = (h.heads + rows - 1) / rows;
     const int turns = a.half[0].turns + a.half[1].turns;
-    a.chunk = tokens * 2 >= most * kRotWarps ? turns : 1;
-    a.chunks = (turns + a.chunk - 1) / a.chunk;
-    a.units = tokens * a.chunks;
-    return static_cast<int>(std::min(most, (a.units + kRotWarps - 1) / kRotWarps));
+    const int fits = kinds ? std::min(std::max(kRotStage / (rows * row_bytes), 1), turns) : turns;
+    int64_t smem = 0;
+    const auto divide = [&](int chunk) {
+        a.chunk = chunk;
+        a.chunks = (turns + chunk - 1) / chunk;
+        a.units = tokens * a.chunks;
+        a.stage = (chunk * rows * row_bytes + 127) / 128 * 128;
+        smem = static_cast<int64_t>(kRotWarps) * 2 * kinds * a.stage;
+    };
+    divide((turns + (turns + fits - 1) / fits - 1) / ((turns + fits - 1) / fits));
+    if (smem > 16384) smem_limit_once(reinterpret_cast<const void*>(kernel), 4 * kRotWarps * kRotStage, "qk_norm_rotary");
+    int per_sm = 0;
+    cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kRotThreads, smem), "qk_norm_rotary");
+    const int64_t most = static_cast<int64_t>(sm_count()) * std::min(std::max(per_sm, 1), kRotMostPerSm);
+    if (a.units * 2 < most * kRotWarps) divide(1);
+    const int blocks = static_cast<int>(std::min(most, (a.units + kRotWarps - 1) / kRotWarps));
+    if (q_part) a.half[0].part = part;
+    if (k_part) a.half[1].part = part + static_cast<int64_t>(blocks) * a.dim;
+    SX_LAUNCH(kernel, blocks, kRotThreads, smem, s, a);
+    return blocks;
 }
 
 // Calls f(element, pairs a thread, neighbours, slots a thread).
@@ -598,7 +707,7 @@ void by_layout(const SxRotaryInputs& in, int v, F&& f) {
             if (v == 8) return order(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
         if (v == 4) return order(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
         if (v == 2) return order(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
-        order(std::integral_constant<int, 1>{}, std::integral_constant<int, 4>{});
+        f(t, std::integral_constant<int, 1>{}, std::false_type{}, std::integral_constant<int, 4>{});  // no order within one
     });
 }
 
@@ -607,7 +716,8 @@ void by_layout(const SxRotaryInputs& in, int v, F&& f) {
 void launch_qk_norm_rotary_fwd(const SxRotaryInputs& in, const SxAttentionView& q_out, const SxAttentionView& k_out, cudaStream_t s) {
     const int64_t tokens = in.batch * in.tokens;
     if (tokens == 0) return;
-    const int v = in.k_heads ? most_pairs(in, {in.q, in.k, q_out, k_out}) : most_pairs(in, {in.q, q_out});
+    const bool bulk = bulk_fits(in, in.q) && bulk_fits(in, q_out) && (!in.k_heads || (bulk_fits(in, in.k) && bulk_fits(in, k_out)));
+    const int v = bulk ? most_pairs(in) : 1, row = static_cast<int>(in.head_dim * dtype_bytes(in.dtype));
     RotArgs a = rot_args(in, v);
     const auto set = [](RotHalf& h, const SxAttentionView& x) {
         h.out = x.data, h.out_batch = x.batch_stride, h.out_token = x.token_stride, h.out_head = x.head_stride;
@@ -615,12 +725,9 @@ void launch_qk_norm_rotary_fwd(const SxRotaryInputs& in, const SxAttentionView& 
     set(a.half[0], q_out);
     if (in.k_heads) set(a.half[1], k_out);
     by_layout(in, v, [&](auto t, auto n, auto nb, auto slots) {
-        constexpr int V = decltype(n)::value, NV = decltype(slots)::value;
-        constexpr bool NB = decltype(nb)::value;
-        const auto kernel = rotary_fwd_kernel<decltype(t), V, NB, NV>;
-        const size_t smem = Rot<decltype(t), V, NB, NV>::smem_bytes(a);
-        const int blocks = rot_divide(a, tokens, kernel, smem);
-        SX_LAUNCH(kernel, blocks, kRotThreads, smem, s, a);
+        using T = decltype(t);
+        if (bulk) rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, false>, row, 1, s, nullptr, false, false);
+        else if constexpr (decltype(n)::value == 1) rot_launch(a, tokens, rotary_plain_kernel<T, false>, row, 0, s, nullptr, false, false);
     });
 }
 
@@ -640,8 +747,9 @@ void launch_qk_norm_rotary_bwd(const SxRotaryInputs& in, const SxRotaryGrads& g,
     }
     SxRotaryInputs at = in;
     if (!in.norm) at.q = g.v_q_out, at.k = g.v_k_out;  // not read
-    const int v = in.k_heads ? most_pairs(at, {at.q, at.k, g.v_q_out, g.v_k_out, g.v_q, g.v_k})
-                             : most_pairs(at, {at.q, g.v_q_out, g.v_q});
+    const bool bulk = bulk_fits(in, at.q) && bulk_fits(in, g.v_q_out) && bulk_fits(in, g.v_q) &&
+                      (!in.k_heads || (bulk_fits(in, at.k) && bulk_fits(in, g.v_k_out) && bulk_fits(in, g.v_k)));
+    const int v = bulk ? most_pairs(in) : 1, row = static_cast<int>(in.head_dim * dtype_bytes(in.dtype));
     RotArgs a = rot_args(at, v);
     const auto set = [](RotHalf& h, const SxAttentionView& x, const SxAttentionView& y) {
         h.g = x.data, h.g_batch = x.batch_stride, h.g_token = x.token_stride, h.g_head = x.head_stride;
@@ -650,15 +758,14 @@ void launch_qk_norm_rotary_bwd(const SxRotaryInputs& in, const SxRotaryGrads& g,
     set(a.half[0], g.v_q_out, g.v_q);
     if (in.k_heads) set(a.half[1], g.v_k_out, g.v_k);
     by_layout(in, v, [&](auto t, auto n, auto nb, auto slots) {
-        constexpr int V = decltype(n)::value, NV = decltype(slots)::value;
-        constexpr bool NB = decltype(nb)::value;
-        const auto kernel = rotary_bwd_kernel<decltype(t), V, NB, NV>;
-        const size_t smem = std::max<size_t>(Rot<decltype(t), V, NB, NV>::smem_bytes(a), static_cast<size_t>(kRotWarps) * in.head_dim * 4);
-        const int blocks = rot_divide(a, tokens, kernel, smem);
+        using T = decltype(t);
         float* part = static_cast<float*>(ws);
-        if (g.v_q_weight) a.half[0].part = part;
-        if (g.v_k_weight) a.half[1].part = part + static_cast<int64_t>(blocks) * in.head_dim;
-        SX_LAUNCH(kernel, blocks, kRotThreads, smem, s, a);
+        int blocks = 0;
+        if (bulk)
+            blocks = rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, true>, row, 2, s, part,
+                                g.v_q_weight, g.v_k_weight);
+        else if constexpr (decltype(n)::value == 1)
+            blocks = rot_launch(a, tokens, rotary_plain_kernel<T, true>, row, 0, s, part, g.v_q_weight, g.v_k_weight);
         if (g.v_q_weight || g.v_k_weight)
             SX_LAUNCH(rotary_sums_kernel, dim3(blocks_for(in.head_dim, 32), 2), 1024, 0, s, a.half[0].part, a.half[1].part, blocks,
                       in.head_dim, g.v_q_weight, g.v_k_weight, in.param_dtype);

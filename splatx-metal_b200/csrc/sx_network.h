@@ -65,8 +65,9 @@ size_t attention_bwd_workspace(const SxAttentionInputs& in);
 void launch_attention_bwd(const SxAttentionInputs& in, const SxAttentionGradsIn& g,
                           const SxAttentionGrads& out, void* ws, cudaStream_t s);
 
-// The linear kernels' status word of the current device, read and cleared (synchronises).
+// The status words of the linear and rotation kernels of the current device, read and cleared (synchronises).
 uint32_t linear_status();
+uint32_t rotary_status();
 size_t linear_fwd_workspace(const SxLinearInputs& in);
 void launch_linear_fwd(const SxLinearInputs& in, const SxLinearOutputs& out, void* ws, cudaStream_t s);
 size_t linear_bwd_workspace(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out);

@@ -297,8 +297,9 @@ _ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
 def linear_status() -> int:
-    """Status bits the linear kernels of the current device have set since the last call (0: all is
-    well; 1: a bounded wait inside a kernel ran out and its outputs are invalid). Synchronises."""
+    """Status bits the linear and qk_norm_rotary kernels of the current device have set since the last
+    call (0: all is well; 1: a bounded wait inside a kernel ran out and its outputs are invalid).
+    Synchronises."""
     st = C.c_uint32(0)
     check(_nat.lib().sxcuda_linear_status(C.byref(st)))
     return int(st.value)
