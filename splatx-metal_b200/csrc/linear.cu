@@ -11,94 +11,118 @@ namespace sx {
 namespace {
 
 // ---- products on the multiply-add pipes ----
-// A CTA takes 128 x 128 values of C, a thread 8 x 8 of them as 2 x 2 blocks of 4 x 4; 16 of K at a time go
-// through shared memory, the next 16 are on their way in registers meanwhile.
-constexpr int kTile = 128, kDepth = 16, kThreads = 256;
-constexpr int kPitch = kTile + 4;
+// A CTA takes TILE x TILE values of C (128, or 64 where there are few), a thread 8 x 8 of them as 2 x 2 blocks of
+// 4 x 4; 16 of K at a time go through shared memory, the next 16 are on their way in registers meanwhile.
+constexpr int kDepth = 16;
+template <int TILE>
+constexpr int kThreads = TILE * TILE / 64;
 
-// The thread's 8 values of a 128 x 16 block of an operand: along K for row `tid / 2`, or along the rows for
-// K value `tid / 16`.
-template <typename T>
+// The thread's share of a TILE x 16 block of an operand, 8 values at a time: along K for a row, or along the rows
+// for a value of K.
+template <int TILE>
 struct Staged {
-    float x[8];
-    __device__ void load(const LinearOperand& o, int64_t row0, int64_t rows, int64_t k0, int64_t k_end, bool wide) {
-        const bool along_k = !o.across;
-        const int t = threadIdx.x;
-        const int64_t row = row0 + (along_k ? t / 2 : t % 16 * 8), k = k0 + (along_k ? t % 2 * 8 : t / 16);
-        const T* p = static_cast<const T*>(o.data) + (along_k ? row * o.stride + k : k * o.stride + row);
-        const int64_t left = (along_k ? row < rows : k < k_end) ? (along_k ? k_end - k : rows - row) : 0;
-        constexpr int N = sizeof(T) == 4 ? 4 : 8;
-        if (wide && left >= 8) {
+    static constexpr int kPitch = TILE + 4, kTurns = TILE * 2 / kThreads<TILE>;
+    float x[kTurns][8];
+    __device__ __forceinline__ void load(const LinearOperand& o, int64_t row0, int64_t rows, int64_t k0, int64_t k_end, bool wide) {
 #pragma unroll
-            for (int i = 0; i < 8; i += N) {
-                const auto v = *reinterpret_cast<const Pack<T, N>*>(p + i);
+        for (int i = 0; i < kTurns; ++i) {
+            const int t = threadIdx.x + i * kThreads<TILE>;
+            const int64_t row = row0 + (o.across ? t % (TILE / 8) * 8 : t / 2), k = k0 + (o.across ? t / (TILE / 8) : t % 2 * 8);
+            const float* p = static_cast<const float*>(o.data) + (o.across ? k * o.stride + row : row * o.stride + k);
+            const int64_t left = (o.across ? k < k_end : row < rows) ? (o.across ? rows - row : k_end - k) : 0;
+            if (wide && left >= 8) {
+                *reinterpret_cast<float4*>(x[i]) = reinterpret_cast<const float4*>(p)[0];
+                *reinterpret_cast<float4*>(x[i] + 4) = reinterpret_cast<const float4*>(p)[1];
+            } else {
 #pragma unroll
-                for (int j = 0; j < N; ++j) x[i + j] = to_f32(v.v[j]);
+                for (int j = 0; j < 8; ++j) x[i][j] = j < left ? p[j] : 0.f;
             }
-            return;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i < left ? to_f32(p[i]) : 0.f;
     }
-    __device__ void store(const LinearOperand& o, float (&to)[kDepth][kPitch]) const {
-        const int t = threadIdx.x;
-        if (!o.across) {
+    __device__ __forceinline__ void store(const LinearOperand& o, float (&to)[kDepth][kPitch]) const {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[t % 2 * 8 + i][t / 2] = x[i];
-        } else {
+        for (int i = 0; i < kTurns; ++i) {
+            const int t = threadIdx.x + i * kThreads<TILE>;
+            if (o.across) {
+                float* at = &to[t / (TILE / 8)][t % (TILE / 8) * 8];
+                *reinterpret_cast<float4*>(at) = *reinterpret_cast<const float4*>(x[i]);
+                *reinterpret_cast<float4*>(at + 4) = *reinterpret_cast<const float4*>(x[i] + 4);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; i += 4)
-                *reinterpret_cast<float4*>(&to[t / 16][t % 16 * 8 + i]) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+                for (int j = 0; j < 8; ++j) to[t % 2 * 8 + j][t / 2] = x[i][j];
+            }
         }
     }
 };
 
 // The epilogue for `n` (at most N) consecutive columns of a row.
 template <typename T, int N>
-__device__ __forceinline__ void linear_finish(const LinearProduct& p, int64_t row, int64_t col, float (&z)[N], int n) {
-    T pre[N], y[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (i >= n) break;
-        z[i] += linear_param(p.bias, p.bias_dtype, col + i);
-        pre[i] = from_f32<T>(z[i]);
-        float v = act_of<T>(p.act, z[i]);
-        if (p.residual) v += to_f32(static_cast<const T*>(p.residual)[row * p.residual_stride + col + i]);
-        y[i] = from_f32<T>(v);
-    }
+__device__ __forceinline__ void linear_finish(const LinearProduct& p, int64_t row, int64_t col, float (&z)[N], const float (&bias)[N], int n) {
     T* to = static_cast<T*>(p.y) + row * p.y_stride + col;
     T* keep = static_cast<T*>(p.pre) + row * p.pre_stride + col;
+    const T* add = static_cast<const T*>(p.residual) + row * p.residual_stride + col;
     const auto fits = [](const T* a) { return reinterpret_cast<uintptr_t>(a) % (N * sizeof(T)) == 0; };
-    if (n == N && fits(to) && (!p.pre || fits(keep))) {
-        *reinterpret_cast<Pack<T, N>*>(to) = *reinterpret_cast<Pack<T, N>*>(y);
-        if (p.pre) *reinterpret_cast<Pack<T, N>*>(keep) = *reinterpret_cast<Pack<T, N>*>(pre);
+    const bool whole = n == N && fits(to) && (!p.pre || fits(keep)) && (!p.residual || fits(add));
+    Pack<T, N> r{};
+    if (p.residual) {
+        if (whole) {
+            r = *reinterpret_cast<const Pack<T, N>*>(add);
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i < n) r.v[i] = add[i];
+        }
+    }
+    Pack<T, N> pre, y;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        z[i] += bias[i];
+        pre.v[i] = from_f32<T>(z[i]);
+    }
+    if (p.act != SXCUDA_ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) z[i] = act_of<T>(p.act, z[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) y.v[i] = from_f32<T>(p.residual ? z[i] + to_f32(r.v[i]) : z[i]);
+    if (whole) {
+        *reinterpret_cast<Pack<T, N>*>(to) = y;
+        if (p.pre) *reinterpret_cast<Pack<T, N>*>(keep) = pre;
         return;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         if (i >= n) break;
-        to[i] = y[i];
-        if (p.pre) keep[i] = pre[i];
+        to[i] = y.v[i];
+        if (p.pre) keep[i] = pre.v[i];
     }
 }
+template <int N>
+__device__ __forceinline__ void linear_biases(const LinearProduct& p, int64_t col, int n, float (&bias)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) bias[i] = i < n ? linear_param(p.bias, p.bias_dtype, col + i) : 0.f;
+}
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant__ LinearProduct p, bool a_wide, bool b_wide) {
-    __shared__ float as[2][kDepth][kPitch], bs[2][kDepth][kPitch];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+template <int TILE>
+__global__ void __launch_bounds__(kThreads<TILE>, TILE == 128 ? 2 : 8) linear_kernel(const __grid_constant__ LinearProduct p, bool a_wide, bool b_wide) {
+    constexpr int kSide = TILE / 8, kHalf = TILE / 2, kPitch = TILE + 4;
+    __shared__ __align__(16) float smem[2][2][kDepth][kPitch];  // of A, of B; twice
+    const int tx = threadIdx.x % kSide, ty = threadIdx.x / kSide;
     LinearWalk walk(p.plan, blockIdx.x);
     LinearPiece piece;
     while (walk.next(p.plan, piece)) {
         const LinearTile tile = linear_tile(p.plan, piece.tile);
-        const int64_t m0 = static_cast<int64_t>(tile.m) * kTile, n0 = static_cast<int64_t>(tile.n) * kTile, end = min(static_cast<int64_t>(piece.k1) * kDepth, p.k);
-        float c[8][8] = {};
-        Staged<T> a, b;
+        const int64_t m0 = static_cast<int64_t>(tile.m) * TILE, n0 = static_cast<int64_t>(tile.n) * TILE, end = min(static_cast<int64_t>(piece.k1) * kDepth, p.k);
+        tc::Two c[8][4];  // two columns each
+#pragma unroll
+        for (int i = 0; i < 32; ++i) c[i / 4][i % 4] = tc::two(0.f, 0.f);
+        Staged<TILE> a, b;
         a.load(p.a, m0, p.m, static_cast<int64_t>(piece.k0) * kDepth, end, a_wide);
         b.load(p.b, n0, p.n, static_cast<int64_t>(piece.k0) * kDepth, end, b_wide);
         for (int k = piece.k0; k < piece.k1; ++k) {
             const int at = k & 1;
-            a.store(p.a, as[at]);
-            b.store(p.b, bs[at]);
+            a.store(p.a, smem[0][at]);
+            b.store(p.b, smem[1][at]);
             __syncthreads();
             if (k + 1 < piece.k1) {
                 a.load(p.a, m0, p.m, static_cast<int64_t>(k + 1) * kDepth, end, a_wide);
@@ -106,30 +130,49 @@ __global__ void __launch_bounds__(kThreads) linear_kernel(const __grid_constant_
             }
 #pragma unroll
             for (int d = 0; d < kDepth; ++d) {
-                float x[8], y[8];
+                float x[8];
+                tc::Two y[4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    *reinterpret_cast<float4*>(x + 4 * h) = *reinterpret_cast<const float4*>(&as[at][d][ty * 4 + h * 64]);
-                    *reinterpret_cast<float4*>(y + 4 * h) = *reinterpret_cast<const float4*>(&bs[at][d][tx * 4 + h * 64]);
+                    *reinterpret_cast<float4*>(x + 4 * h) = *reinterpret_cast<const float4*>(&smem[0][at][d][ty * 4 + h * kHalf]);
+                    const float4 v = *reinterpret_cast<const float4*>(&smem[1][at][d][tx * 4 + h * kHalf]);
+                    y[2 * h] = tc::two(v.x, v.y), y[2 * h + 1] = tc::two(v.z, v.w);
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) c[i][j] = fmaf(x[i], y[j], c[i][j]);
+                    for (int j = 0; j < 4; ++j) c[i][j] = tc::fma2(tc::two(x[i], x[i]), y[j], c[i][j]);
+            }
+        }
+        // half of the rows at a time through shared memory: then 4 columns of row after row, with little code
+        float(*rows)[kPitch] = reinterpret_cast<float(*)[kPitch]>(smem);
+        const int col = static_cast<int>(threadIdx.x) % (TILE / 4) * 4, n = static_cast<int>(min(p.n - n0 - col, static_cast<int64_t>(4)));
+        float bias[4];
+        linear_biases(p, n0 + col, n, bias);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float4 v;
+                    tc::split(c[4 * h + i][2 * j], v.x, v.y);
+                    tc::split(c[4 * h + i][2 * j + 1], v.z, v.w);
+                    *reinterpret_cast<float4*>(&rows[ty * 4 + i][tx * 4 + j * kHalf]) = v;
+                }
+            __syncthreads();
+#pragma unroll 1
+            for (int r = static_cast<int>(threadIdx.x) / (TILE / 4); r < kHalf; r += kThreads<TILE> / (TILE / 4)) {
+                const int row = r + h * kHalf;
+                if (m0 + row >= p.m || n <= 0) break;
+                const float4 v = *reinterpret_cast<const float4*>(&rows[r][col]);
+                float z[4] = {v.x, v.y, v.z, v.w};
+                if (piece.slot < 0) linear_finish<float, 4>(p, m0 + row, n0 + col, z, bias, n);
+                else *reinterpret_cast<float4*>(linear_part(p, piece.slot, row, col)) = v;
             }
         }
         __syncthreads();  // the next piece's first stores
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = ty * 4 + i % 4 + i / 4 * 64, col = tx * 4 + h * 64;
-                const int64_t n = min(p.n - n0 - col, static_cast<int64_t>(4));
-                if (m0 + row >= p.m || n <= 0) continue;
-                float z[4] = {c[i][4 * h], c[i][4 * h + 1], c[i][4 * h + 2], c[i][4 * h + 3]};
-                if (piece.slot < 0) linear_finish<T, 4>(p, m0 + row, n0 + col, z, static_cast<int>(n));
-                else *reinterpret_cast<float4*>(linear_part(p, piece.slot, row, col)) = make_float4(z[0], z[1], z[2], z[3]);
-            }
     }
 }
 
@@ -155,7 +198,9 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
         z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w;
         z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
     }
-    linear_finish<T, 8>(p, m0 + row, n0 + col, z, static_cast<int>(n));
+    float bias[8];
+    linear_biases(p, n0 + col, static_cast<int>(n), bias);
+    linear_finish<T, 8>(p, m0 + row, n0 + col, z, bias, static_cast<int>(n));
 }
 
 bool linear_wide(const LinearOperand& o, int64_t size) {
@@ -193,23 +238,75 @@ LinearPlan linear_plan(int64_t m, int64_t n, int64_t k, int tile_m, int tile_n, 
 
 namespace {
 
-constexpr int kPerSm = 2;
-
 LinearPlan product_plan(int32_t dtype, int64_t m, int64_t n, int64_t k) {
-    return dtype == SXCUDA_F32 ? linear_plan(m, n, k, kTile, kTile, kDepth, static_cast<int64_t>(sm_count()) * kPerSm, 8, 32)
-                               : linear_tc_plan(m, n, k);
+    if (dtype != SXCUDA_F32) return linear_tc_plan(m, n, k);
+    const int64_t sms = sm_count(), large = (m + 127) / 128 * ((n + 127) / 128);
+    return large >= sms ? linear_plan(m, n, k, 128, 128, kDepth, sms * 2, 8, 32) : linear_plan(m, n, k, 64, 64, kDepth, sms * 8, 4, 12);
 }
 
 void launch_product(const LinearProduct& p, cudaStream_t s) {
-    if (p.dtype == SXCUDA_F32)
-        SX_LAUNCH(linear_kernel<float>, static_cast<unsigned>(p.plan.workers), kThreads, 0, s, p, linear_wide(p.a, 4), linear_wide(p.b, 4));
-    else launch_linear_tc(p, s);
+    const auto run = [&](auto kernel, int threads) {
+        SX_LAUNCH(kernel, static_cast<unsigned>(p.plan.workers), threads, 0, s, p, linear_wide(p.a, 4), linear_wide(p.b, 4));
+    };
+    if (p.dtype != SXCUDA_F32) launch_linear_tc(p, s);
+    else if (p.plan.tile_m == 128) run(linear_kernel<128>, kThreads<128>);
+    else run(linear_kernel<64>, kThreads<64>);
     if (!p.plan.cut()) return;
     by_dtype(p.dtype, [&](auto t) {
         const auto join = linear_join_kernel<decltype(t)>;
         const int64_t rows = std::min<int64_t>(p.m, p.plan.tile_m);
         SX_LAUNCH(join, dim3(blocks_for((rows + 7) / 8 * (p.plan.tile_n / 32), 8), static_cast<unsigned>(p.plan.rest)), 256, 0, s, p);
     });
+}
+
+// ---- a few rows ----
+// A warp has an output feature: its lanes go along the weight's row, V values at a time, and each of up to ROWS
+// rows of x has a sum. The weight is read once, by as many warps as there are features; a product on the tensor
+// cores needs its parts of K joined to read it as widely. 1024 -> 4096 features, this and the tiles, in us: bf16
+// 1 row 3.6 and 12, 4 rows 5.6 and 10, 8 rows 9.3 and 10 (4096 -> 4096: 24 and 19); float32 1 row 4.5 and 27, 8
+// rows 12 and 27.
+constexpr int few_rows_of(int32_t dtype) { return dtype == SXCUDA_F32 ? 8 : 4; }
+template <typename T, int V, int ROWS>
+__global__ void __launch_bounds__(128) linear_few_kernel(const __grid_constant__ LinearProduct p) {
+    const int lane = threadIdx.x & 31;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    if (n >= p.n) return;
+    const T* w = static_cast<const T*>(p.b.data) + n * p.b.stride;
+    float sum[ROWS] = {};
+#pragma unroll 4
+    for (int64_t k = lane * V; k < p.k; k += 32 * V) {
+        const auto v = *reinterpret_cast<const Pack<T, V>*>(w + k);
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            const auto x = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(p.a.data) + (r < p.m ? r : 0) * p.a.stride + k);
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[r] = fmaf(to_f32(v.v[i]), to_f32(x.v[i]), sum[r]);
+        }
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum[r] += __shfl_xor_sync(kFullMask, sum[r], o);
+        if (lane == r) mine = sum[r];
+    }
+    if (lane >= p.m) return;
+    float z[1] = {mine}, bias[1] = {linear_param(p.bias, p.bias_dtype, n)};
+    linear_finish<T, 1>(p, lane, n, z, bias, 1);
+}
+template <typename T>
+void launch_few(const LinearProduct& p, cudaStream_t s) {
+    constexpr int V = 16 / sizeof(T);
+    const auto run = [&](auto kernel) { SX_LAUNCH(kernel, blocks_for(p.n, 4), 128, 0, s, p); };
+    const auto rows = [&](auto v) {
+        constexpr int N = decltype(v)::value;
+        if (p.m == 1) run(linear_few_kernel<T, N, 1>);
+        else if (p.m == 2) run(linear_few_kernel<T, N, 2>);
+        else if (p.m <= 4) run(linear_few_kernel<T, N, 4>);
+        else if constexpr (sizeof(T) == 4) run(linear_few_kernel<T, N, 8>);
+    };
+    if (p.k % V == 0 && linear_wide(p.a, sizeof(T)) && linear_wide(p.b, sizeof(T))) rows(std::integral_constant<int, V>{});
+    else rows(std::integral_constant<int, 1>{});
 }
 
 // ---- rows that tensor maps do not take, copied to rows that they do ----
@@ -244,8 +341,10 @@ struct Matrix {
 };
 
 // ---- v_z = v_y act'(pre), and the sum of its rows ----
-// A CTA has 32 V columns (a warp's lanes V each) and a slice of the rows, which its warps take in turn.
-constexpr int kSlopeWarps = 8;
+// A CTA has 32 V columns (a warp's lanes V each) and a slice of the rows, which its warps take in turn; the grid
+// is what the SMs hold. Bound by memory: gelu over bf16 32768 x 4096 163 us (4.9 TB/s); several rows asked for
+// at once by a warp, with fewer warps, were slower (2 rows 185 us, 4 rows 222 us).
+constexpr int kSlopeWarps = 8, kSlopePerSm = 6;
 struct SlopeArgs {
     const void* v_y;
     const void* pre;
@@ -255,7 +354,7 @@ struct SlopeArgs {
     int32_t act;
 };
 template <typename T, int V>
-__global__ void __launch_bounds__(kSlopeWarps * 32) linear_slope_kernel(const SlopeArgs a) {
+__global__ void __launch_bounds__(kSlopeWarps * 32, kSlopePerSm) linear_slope_kernel(const SlopeArgs a) {
     __shared__ float part[kSlopeWarps][32 * V];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * V;
@@ -266,13 +365,12 @@ __global__ void __launch_bounds__(kSlopeWarps * 32) linear_slope_kernel(const Sl
             const auto g = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.v_y) + r * a.v_y_stride + c);
             Pack<T, V> z{}, to;
             if (a.pre) z = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.pre) + r * a.pre_stride + c);
+            float x[V], at[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float x = to_f32(g.v[i]);
-                if (a.pre) x *= slope_of<T>(a.act, to_f32(z.v[i]));
-                sum[i] += x;
-                to.v[i] = from_f32<T>(x);
-            }
+            for (int i = 0; i < V; ++i) x[i] = to_f32(g.v[i]), at[i] = to_f32(z.v[i]);
+            if (a.pre) times_slopes<T>(a.act, at, x);
+#pragma unroll
+            for (int i = 0; i < V; ++i) sum[i] += x[i], to.v[i] = from_f32<T>(x[i]);
             if (a.v_z) *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.v_z) + r * a.v_z_stride + c) = to;
         }
     if (!a.sums) return;
@@ -324,7 +422,7 @@ SlopePlan slope_plan(const SxLinearInputs& in, const SxLinearGradsIn& g) {
     SlopePlan p;
     p.v = in.out_features % most == 0 && wide(g.v_y, g.v_y_stride) && wide(g.pre, g.pre_stride) ? static_cast<int>(most) : 1;
     p.strips = (in.out_features + 32 * p.v - 1) / (32 * p.v);
-    const int64_t want = std::max<int64_t>(static_cast<int64_t>(sm_count()) * 8 / p.strips, 1);
+    const int64_t want = std::max<int64_t>(static_cast<int64_t>(sm_count()) * kSlopePerSm / p.strips, 1);
     p.slice = std::max<int64_t>((in.rows + want - 1) / want, 4 * kSlopeWarps);
     p.slices = (in.rows + p.slice - 1) / p.slice;
     return p;
@@ -355,10 +453,12 @@ struct BwdSpace {
     }
 };
 
+bool few_rows(const SxLinearInputs& in) { return in.rows <= few_rows_of(in.dtype); }
+
 }  // namespace
 
 size_t linear_fwd_workspace(const SxLinearInputs& in) {
-    if (in.rows == 0) return 0;
+    if (in.rows == 0 || few_rows(in)) return 0;
     const Matrix x{in.x, in.x_stride, in.rows, in.in_features}, w{in.weight, in.weight_stride, in.out_features, in.in_features};
     return x.bytes(in.dtype) + w.bytes(in.dtype) + product_plan(in.dtype, in.rows, in.out_features, in.in_features).workspace();
 }
@@ -367,15 +467,20 @@ void launch_linear_fwd(const SxLinearInputs& in, const SxLinearOutputs& out, voi
     if (in.rows == 0) return;
     uint8_t* at = static_cast<uint8_t*>(ws);
     const Matrix x{in.x, in.x_stride, in.rows, in.in_features}, w{in.weight, in.weight_stride, in.out_features, in.in_features};
+    const bool few = few_rows(in);
     LinearProduct p{};
-    p.a = x.ready(in.dtype, at, s).along_k();
-    p.b = w.ready(in.dtype, at += x.bytes(in.dtype), s).along_k();
+    p.a = (few ? x : x.ready(in.dtype, at, s)).along_k();
+    p.b = (few ? w : w.ready(in.dtype, at += x.bytes(in.dtype), s)).along_k();
     p.m = in.rows, p.n = in.out_features, p.k = in.in_features;
     p.dtype = in.dtype, p.bias_dtype = in.bias_dtype, p.act = in.activation;
     p.bias = in.bias;
     p.residual = out.residual, p.residual_stride = out.residual_stride;
     p.y = out.y, p.y_stride = out.y_stride;
     p.pre = out.pre, p.pre_stride = out.pre_stride;
+    if (few) {
+        by_dtype(in.dtype, [&](auto t) { launch_few<decltype(t)>(p, s); });
+        return;
+    }
     p.parts = reinterpret_cast<float*>(at + w.bytes(in.dtype));
     p.plan = product_plan(in.dtype, p.m, p.n, p.k);
     launch_product(p, s);

@@ -12,8 +12,8 @@
 // A warp takes one token at a time, its queries and then its keys: its lanes make the token's sines and
 // cosines once for all heads, in shared memory, in the order in which lanes read them; the weights lie there
 // in the same way. Groups of a warp read the same entries at the same time, so that a read is one pass of
-// shared memory. The token's rows come to shared memory by bulk copies, the next token's while one is worked
-// on, and leave from their place there by bulk copies: the loops then have no addresses of memory and no
+// shared memory. The token's rows come to shared memory by bulk copies, while other warps work on theirs,
+// and leave from their place there by bulk copies: the loops then have no addresses of memory and no
 // registers for rows on their way. Rows that such copies do not reach (16 bytes) are read and written value by
 // value.
 // Angles: position x frequency in turns in 64 bits, the nearest quarter turn taken off there; what is left
@@ -108,13 +108,23 @@ struct Values {
     tc::Two v[N];
 };
 
+// A unit's rows of queries or keys: heads from `head` on, `n` of them, row `at` of the unit's first.
+struct RotRun {
+    int head, n, at;
+};
+__device__ __forceinline__ RotRun rot_run(const RotArgs& a, int rows, int chunk, int k) {
+    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.half[0].turns + a.half[1].turns), q = a.half[0].turns;
+    const int from = k ? max(begin, q) - q : begin, to = k ? end - q : min(end, q);
+    return {from * rows, max(min(to * rows, a.half[k].heads) - from * rows, 0), k ? (max(begin, q) - begin) * rows : 0};
+}
+
 constexpr int kTable = 2 * kRotMostPairs;  // floats of a table: V first entries and V seconds of up to 128 / V slots
 
 struct RotShared {
     alignas(16) float weights[2][kTable];       // of queries and keys
     alignas(16) float angles[kRotWarps][kTable];  // cosines and sines of each warp's token
     double turns[kRotMostPairs];
-    uint64_t full[kRotWarps][2];  // barriers of the stages
+    uint64_t full[kRotWarps];  // barriers of the stages
     uint8_t axis[kRotMostPairs];
     uint32_t failed;
 };
@@ -176,21 +186,31 @@ struct Rot {
         }
         return r;
     }
-    struct Token {
+    // A unit of work, and what of it are queries' and keys' rows.
+    struct Unit {
         int64_t batch, token;
         int chunk;
+        RotRun run[2];
     };
-    __device__ Token token_of(int64_t unit) const {
-        if (a.units <= INT32_MAX) {  // 64-bit divisions take some hundred instructions
-            const uint32_t u = static_cast<uint32_t>(unit), t = u / static_cast<uint32_t>(a.chunks);
-            const uint32_t n = static_cast<uint32_t>(a.tokens), b = t / n;
-            return {b, t - b * n, static_cast<int>(u - t * a.chunks)};
-        }
+    __device__ Unit first_unit(int64_t unit) const {
         const int64_t t = unit / a.chunks, b = t / a.tokens;
-        return {b, t - b * a.tokens, static_cast<int>(unit - t * a.chunks)};
+        Unit u{b, t - b * a.tokens, static_cast<int>(unit - t * a.chunks), {}};
+        u.run[0] = rot_run(a, rows, u.chunk, 0), u.run[1] = rot_run(a, rows, u.chunk, 1);
+        return u;
+    }
+    __device__ void next_unit(Unit& u, int step) const {  // `step` units on
+        if (a.chunks > 1) {
+            const uint32_t c = static_cast<uint32_t>(u.chunk + step), t = c / static_cast<uint32_t>(a.chunks);
+            u.chunk = static_cast<int>(c - t * a.chunks);
+            u.token += t;
+            u.run[0] = rot_run(a, rows, u.chunk, 0), u.run[1] = rot_run(a, rows, u.chunk, 1);
+        } else {
+            u.token += step;
+        }
+        while (u.token >= a.tokens) u.token -= a.tokens, ++u.batch;
     }
     // Lane i's position along axis i.
-    __device__ double position(const Token& t) const {
+    __device__ double position(const Unit& t) const {
         if (lane >= a.axes) return 0.;
         const int64_t i = t.batch * a.pos_batch + t.token * a.pos_token + lane * a.pos_axis;
         if (a.pos_dtype == SXCUDA_POS_F32) return static_cast<const float*>(a.positions)[i];
@@ -201,19 +221,32 @@ struct Rot {
         __syncwarp();
         for (int i = lane; i - lane < a.pairs; i += 32) {
             const int j = i < a.pairs ? i : 0;
-            const double p = __shfl_sync(kFullMask, mine_position, sh.axis[j]);
-            const double t = p * sh.turns[j], quarters = rint(4. * t);
-            // of a product beyond 2^51 no quarter of a turn is left: it stands at 0 (of an infinity NaN is left)
-            float sine, cosine;
-            sincospif(static_cast<float>(2. * fma(-0.25, quarters, t)), &sine, &cosine);
-            const int q = fabs(quarters) < 2251799813685248. ? __double2loint(quarters + 6755399441055744.) & 3 : 0;  // its low bits
-            const float cc = q & 1 ? sine : cosine, ss = q & 1 ? cosine : sine;
+            const double t = __shfl_sync(kFullMask, mine_position, sh.axis[j]) * sh.turns[j];
+            // t in quarters, rounded to a whole number by the sum: its low bits say which quarter
+            const double magic = 6755399441055744., up = fma(4., t, magic);
+            const int q = __double2loint(up);
+            const float2 cs = eighth(static_cast<float>(fma(-0.25, up - magic, t)));
+            const float c = q & 1 ? cs.y : cs.x, s = q & 1 ? cs.x : cs.y;
             if (i < a.pairs) {
-                *entry(table, i, 0) = q == 1 || q == 2 ? -cc : cc;
-                *entry(table, i, V) = q >= 2 ? -ss : ss;
+                *entry(table, i, 0) = __uint_as_float(__float_as_uint(c) ^ static_cast<uint32_t>(q + 1 & 2) << 30);
+                *entry(table, i, V) = __uint_as_float(__float_as_uint(s) ^ static_cast<uint32_t>(q & 2) << 30);
             }
         }
         __syncwarp();
+    }
+    // Cosine and sine of r turns, |r| <= 1/8, by their series to the 10th and 9th power (1.1e-10 and 2e-9 are left).
+    // Further off a position was too far for a turn to be left of it: it stands at 0 (of an infinity NaN is left).
+    static __device__ __forceinline__ float2 eighth(float r) {
+        r = fabsf(r) > 0.25f ? 0.f : r;
+        const float x = 6.2831853071795865f * r, z = x * x;
+        float c = fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
+        c = fmaf(z, c, -1.3888889e-3f);
+        c = fmaf(z, c, 4.1666667e-2f);
+        c = fmaf(z, c, -0.5f);
+        float s = fmaf(z, 2.7557319e-6f, -1.9841270e-4f);
+        s = fmaf(z, s, 8.3333333e-3f);
+        s = fmaf(z, s, -1.6666667e-1f);
+        return {fmaf(z, c, 1.f), fmaf(x * z, s, x)};
     }
     // The place in the head of the first (second) value of a slot's pair e; -1: there is none.
     static __device__ int place(int first, int second, int e, int which) {
@@ -291,7 +324,9 @@ struct Rot {
         float lo, hi;
         tc::split(x, lo, hi);
         lo += hi;
-        for (int o = a.lanes / 2; o; o >>= 1) lo += __shfl_xor_sync(kFullMask, lo, o);
+#pragma unroll
+        for (int o = 16; o; o >>= 1)
+            if (a.lanes > o) lo += __shfl_xor_sync(kFullMask, lo, o);
         return lo;
     }
     __device__ float rstd(const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
@@ -423,31 +458,27 @@ __device__ __forceinline__ void no_sums(Values<V> (&sum)[2][2][NV]) {
         for (int e = 0; e < Values<V>::N; ++e) sum[i / NV / 2][i / NV % 2][i % NV].v[e] = tc::two(0.f, 0.f);
 }
 
-// A unit's rows of queries or keys: heads from `head` on, `n` of them, row `at` of the unit's first.
-struct RotRun {
-    int head, n, at;
-};
-__device__ __forceinline__ RotRun rot_run(const RotArgs& a, int rows, int chunk, int k) {
-    const int begin = chunk * a.chunk, end = min(begin + a.chunk, a.half[0].turns + a.half[1].turns), q = a.half[0].turns;
-    const int from = k ? max(begin, q) - q : begin, to = k ? end - q : min(end, q);
-    return {from * rows, max(min(to * rows, a.half[k].heads) - from * rows, 0), k ? (max(begin, q) - begin) * rows : 0};
-}
+// CTAs an SM holds by their registers.
+template <int V, bool BACK>
+constexpr int kRotPerSm = V > 2 ? (BACK ? 4 : 7) : V == 2 ? (BACK ? 4 : 6) : (BACK ? 2 : 4);
+constexpr int kRotMostPerSm = 7;
 
 // Rows value by value.
 template <typename T, bool BACK>
-__global__ void __launch_bounds__(kRotThreads) rotary_plain_kernel(const __grid_constant__ RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, kRotPerSm<1, BACK>) rotary_plain_kernel(const __grid_constant__ RotArgs a) {
     __shared__ RotShared sh;
     const Rot<T, 1, false, 4> me(a, sh);
     Values<1> sum[2][2][4];
     no_sums(sum);
-    for (int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5); unit < a.units;
-         unit += static_cast<int64_t>(gridDim.x) * kRotWarps) {
-        const auto token = me.token_of(unit);
+    const int step = static_cast<int>(gridDim.x) * kRotWarps;
+    int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + (threadIdx.x >> 5);
+    auto token = me.first_unit(unit);
+    for (; unit < a.units; unit += step, me.next_unit(token, step)) {
         me.angles(me.position(token));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const RotHalf& h = a.half[k];
-            const RotRun run = rot_run(a, me.rows, token.chunk, k);
+            const RotRun run = token.run[k];
             for (int i = 0; i < run.n; i += me.rows) {
                 const bool there = i + me.group < run.n;
                 const int64_t head = run.head + (there ? i + me.group : i);
@@ -464,88 +495,108 @@ __global__ void __launch_bounds__(kRotThreads) rotary_plain_kernel(const __grid_
     if constexpr (BACK) me.leave(sum);
 }
 
-// Rows by bulk copies: each warp has two stages for a unit's rows (backward: of the gradient, then of x).
+// Rows by bulk copies: each warp has a stage for a unit's rows (backward: of the gradient, then of x). While it
+// fills, other warps work: more warps with a stage each were faster than fewer with two (68 and 72 us for
+// 4 x 8192 tokens, 16 (4) heads x 128; backward of 8 x 4096, 16 heads x 64: 93 and 97 us).
 __device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
 }
 
 template <typename T, int V, bool NB, int NV, bool BACK>
-__global__ void __launch_bounds__(kRotThreads, V > 2 ? (BACK ? 4 : 7) : (BACK ? 2 : 3)) rotary_kernel(const __grid_constant__ RotArgs a) {
+__global__ void __launch_bounds__(kRotThreads, kRotPerSm<V, BACK>) rotary_kernel(const __grid_constant__ RotArgs a) {
     __shared__ RotShared sh;
     extern __shared__ __align__(128) uint8_t stages[];
-    const int warp = threadIdx.x >> 5;
-    const uint32_t bars = tc::smem_addr(sh.full[warp]);
-    if (threadIdx.x % 32 == 0) {
-        tc::bar_init(bars, 1);
-        tc::bar_init(bars + 8, 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bar = tc::smem_addr(&sh.full[warp]);
+    if (lane == 0) {
+        tc::bar_init(bar, 1);
         tc::bar_init_fence();
     }
     if (threadIdx.x == 0) sh.failed = 0;
     const Rot<T, V, NB, NV> me(a, sh);
     volatile uint32_t* failed = &sh.failed;
     const int bytes = a.dim * static_cast<int>(sizeof(T)), stage = a.stage * (BACK ? 2 : 1);
-    uint8_t* mine = stages + static_cast<size_t>(warp) * 2 * stage;
+    uint8_t* mine = stages + static_cast<size_t>(warp) * stage;
+    const uint32_t mine_at = tc::smem_addr(mine);
     Values<V> sum[2][2][NV];
     no_sums(sum);
-    const auto rows_of = [&](const auto& token, const void* p, int64_t batch, int64_t tokens, int64_t heads, int head) {
-        return static_cast<const T*>(p) + token.batch * batch + token.token * tokens + head * heads;
+    // Where a head's rows lie side by side, lane 0 has the queries' copies and lane 1 the keys'; else a lane has a
+    // head's. Each lane's own half, as the first case needs it:
+    const RotHalf& own = a.half[lane & 1];
+    const bool joined = a.half[0].x_head == a.dim && a.half[0].out_head == a.dim && (!BACK || a.half[0].g_head == a.dim) &&
+                        (a.half[1].heads == 0 || (a.half[1].x_head == a.dim && a.half[1].out_head == a.dim && (!BACK || a.half[1].g_head == a.dim)));
+    const T* own_x = static_cast<const T*>(own.x);
+    const T* own_g = static_cast<const T*>(own.g);
+    T* own_out = static_cast<T*>(own.out);
+    const int64_t x_batch = own.x_batch, x_token = own.x_token, g_batch = own.g_batch, g_token = own.g_token, out_batch = own.out_batch,
+                  out_token = own.out_token;
+    const auto rows_of = [](const auto& unit, auto* p, int64_t batch, int64_t tokens, int64_t head) {
+        return p + unit.batch * batch + unit.token * tokens + head;
     };
-    // Asks for a unit's rows: run by run where its heads lie side by side, else a lane a head.
-    const auto ask = [&](const typename Rot<T, V, NB, NV>::Token& token, int s) {
-        const uint32_t to = tc::smem_addr(mine + s * stage), bar = bars + 8 * s;
+    const auto ask = [&](const typename Rot<T, V, NB, NV>::Unit& unit) {
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // each lane's own: the stage's last rows have left
         __syncwarp();
-        if (me.lane == 0) {
-            int n = 0;
-            for (int k = 0; k < 2; ++k) n += rot_run(a, me.rows, token.chunk, k).n;
-            tc::bar_expect(bar, n * bytes * (BACK && a.norm ? 2 : 1));
-        }
+        if (lane == 0) tc::bar_expect(bar, (unit.run[0].n + unit.run[1].n) * bytes * (BACK && a.norm ? 2 : 1));
         __syncwarp();
-        const auto copy = [&](const T* from, int64_t heads, const RotRun& run, uint32_t at) {
-            if (heads == a.dim) {
-                if (me.lane == 0) tc::bulk_load(at, from, run.n * bytes, bar);
-            } else {
-                for (int i = me.lane; i < run.n; i += 32) tc::bulk_load(at + i * bytes, from + i * heads, bytes, bar);
+        if (joined) {
+            const RotRun run = lane ? unit.run[1] : unit.run[0];
+            if (lane < 2 && run.n) {
+                if (BACK) tc::bulk_load(mine_at + run.at * bytes, rows_of(unit, own_g, g_batch, g_token, run.head * a.dim), run.n * bytes, bar);
+                if (!BACK || a.norm)
+                    tc::bulk_load(mine_at + (BACK ? a.stage : 0) + run.at * bytes, rows_of(unit, own_x, x_batch, x_token, run.head * a.dim), run.n * bytes, bar);
             }
-        };
-#pragma unroll
+            return;
+        }
         for (int k = 0; k < 2; ++k) {
             const RotHalf& h = a.half[k];
-            const RotRun run = rot_run(a, me.rows, token.chunk, k);
-            if (run.n == 0) continue;
-            if (BACK) copy(rows_of(token, h.g, h.g_batch, h.g_token, h.g_head, run.head), h.g_head, run, to + run.at * bytes);
-            if (!BACK || a.norm)
-                copy(rows_of(token, h.x, h.x_batch, h.x_token, h.x_head, run.head), h.x_head, run, to + (BACK ? a.stage : 0) + run.at * bytes);
+            const RotRun run = unit.run[k];
+            for (int i = lane; i < run.n; i += 32) {
+                const int64_t head = run.head + i;
+                if (BACK) tc::bulk_load(mine_at + (run.at + i) * bytes, rows_of(unit, static_cast<const T*>(h.g), h.g_batch, h.g_token, head * h.g_head), bytes, bar);
+                if (!BACK || a.norm)
+                    tc::bulk_load(mine_at + (BACK ? a.stage : 0) + (run.at + i) * bytes,
+                                  rows_of(unit, static_cast<const T*>(h.x), h.x_batch, h.x_token, head * h.x_head), bytes, bar);
+            }
         }
     };
-    const int64_t step = static_cast<int64_t>(gridDim.x) * kRotWarps;
+    const auto send = [&](const typename Rot<T, V, NB, NV>::Unit& unit) {
+        tc::fence_smem_to_async();
+        __syncwarp();
+        if (joined) {
+            const RotRun run = lane ? unit.run[1] : unit.run[0];
+            if (lane < 2 && run.n) bulk_store(rows_of(unit, own_out, out_batch, out_token, run.head * a.dim), mine_at + run.at * bytes, run.n * bytes);
+        } else {
+            for (int k = 0; k < 2; ++k) {
+                const RotHalf& h = a.half[k];
+                const RotRun run = unit.run[k];
+                for (int i = lane; i < run.n; i += 32)
+                    bulk_store(rows_of(unit, static_cast<T*>(h.out), h.out_batch, h.out_token, (run.head + i) * h.out_head), mine_at + (run.at + i) * bytes, bytes);
+            }
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    };
+    const int step = static_cast<int>(gridDim.x) * kRotWarps;
     int64_t unit = static_cast<int64_t>(blockIdx.x) * kRotWarps + warp;
     bool ok = true;
-    typename Rot<T, V, NB, NV>::Token token{}, next{};
+    auto here = me.first_unit(unit), next = here;
     double position = 0.;
-    int asked = 0;
     if (unit < a.units) {
-        token = me.token_of(unit);
-        ask(token, 0);
-        asked = 1;
-        position = me.position(token);
+        ask(here);
+        position = me.position(here);
     }
-    for (int count = 0; unit < a.units; ++count) {
-        const int s = count & 1;
-        const bool more = unit + step < a.units;
+    uint32_t parity = 0;
+    for (; unit < a.units; unit += step, parity ^= 1) {
         me.angles(position);
-        if (more) {
-            next = me.token_of(unit + step);
-            ask(next, s ^ 1);  // its last rows have left while the angles were made
-            ++asked;
+        if (unit + step < a.units) {
+            me.next_unit(next, step);
             position = me.position(next);
         }
-        ok = tc::bar_wait(bars + 8 * s, count >> 1 & 1, failed);
+        ok = tc::bar_wait(bar, parity, failed);
         if (!ok) break;
-        T* rows = reinterpret_cast<T*>(mine + s * stage);
+        T* rows = reinterpret_cast<T*>(mine);
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-            const RotRun run = rot_run(a, me.rows, token.chunk, k);
+            const RotRun run = here.run[k];
             T* row = rows + (run.at + me.group) * a.dim;
             for (int i = 0; i < run.n; i += me.rows, row += me.rows * a.dim) {
                 const bool there = i + me.group < run.n;
@@ -553,27 +604,13 @@ __global__ void __launch_bounds__(kRotThreads, V > 2 ? (BACK ? 4 : 7) : (BACK ? 
                 else me.forward(row, row, k, there);
             }
         }
-        tc::fence_smem_to_async();
-        __syncwarp();
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const RotHalf& h = a.half[k];
-            const RotRun run = rot_run(a, me.rows, token.chunk, k);
-            T* to = const_cast<T*>(rows_of(token, h.out, h.out_batch, h.out_token, h.out_head, run.head));
-            const uint32_t from = tc::smem_addr(rows) + run.at * bytes;
-            if (h.out_head == a.dim) {
-                if (me.lane == 0 && run.n) bulk_store(to, from, run.n * bytes);
-            } else {
-                for (int i = me.lane; i < run.n; i += 32) bulk_store(to + i * h.out_head, from + i * bytes, bytes);
-            }
-        }
-        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        token = next;
-        unit += step;
+        send(here);
+        here = next;
+        if (unit + step < a.units) ask(here);
     }
     if (!ok) {  // nothing may land in this CTA's memory after it has gone
-        for (int i = max(0, asked - 2); i < asked; ++i) tc::bar_drain(bars + 8 * (i & 1), i >> 1 & 1);
-        if (me.lane == 0) atomicOr(&g_rotary_status, 1u);
+        tc::bar_drain(bar, parity);
+        if (lane == 0) atomicOr(&g_rotary_status, 1u);
     }
     asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     if constexpr (BACK) me.leave(sum);
@@ -605,7 +642,6 @@ __global__ void __launch_bounds__(1024) rotary_sums_kernel(const float* q_part, 
 }
 
 // ---- host ----
-constexpr int kRotMostPerSm = 8;
 bool view_fits(const SxAttentionView& x, int64_t size, int64_t bytes) {
     const auto fits = [&](int64_t n) { return n * size % bytes == 0; };
     return reinterpret_cast<uintptr_t>(x.data) % bytes == 0 && fits(x.batch_stride) && fits(x.token_stride) && fits(x.head_stride);
@@ -667,7 +703,7 @@ RotArgs rot_args(const SxRotaryInputs& in, int v) {
 // stage holds them; where there are fewer tokens than half the warps that fit, one turn of a warp's groups.
 constexpr int kRotStage = 8192;
 template <typename K>
-int rot_launch(RotArgs& a, int64_t tokens, K kernel, int row_bytes, int kinds, cudaStream_t s, float* part, bool q_part, bool k_part) {
+int rot_launch(RotArgs& a, int64_t tokens, K kernel, int per_sm, int row_bytes, int kinds, cudaStream_t s, float* part, bool q_part, bool k_part) {
     const int rows = 32 / a.lanes;
     for (RotHalf& h : a.half) h.turns = (h.heads + rows - 1) / rows;
     const int turns = a.half[0].turns + a.half[1].turns;
@@ -678,13 +714,13 @@ int rot_launch(RotArgs& a, int64_t tokens, K kernel, int row_bytes, int kinds, c
         a.chunks = (turns + chunk - 1) / chunk;
         a.units = tokens * a.chunks;
         a.stage = (chunk * rows * row_bytes + 127) / 128 * 128;
-        smem = static_cast<int64_t>(kRotWarps) * 2 * kinds * a.stage;
+        smem = static_cast<int64_t>(kRotWarps) * kinds * a.stage;
     };
     divide((turns + (turns + fits - 1) / fits - 1) / ((turns + fits - 1) / fits));
-    if (smem > 16384) smem_limit_once(reinterpret_cast<const void*>(kernel), 4 * kRotWarps * kRotStage, "qk_norm_rotary");
-    int per_sm = 0;
-    cuda_check(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kRotThreads, smem), "qk_norm_rotary");
-    const int64_t most = static_cast<int64_t>(sm_count()) * std::min(std::max(per_sm, 1), kRotMostPerSm);
+    if (smem > 16384) smem_limit_once(reinterpret_cast<const void*>(kernel), 2 * kRotWarps * kRotStage, "qk_norm_rotary");
+    // what registers and shared memory leave room for
+    const int held = static_cast<int>(std::min<int64_t>(per_sm, (227 << 10) / (smem + sizeof(RotShared) + 1024)));
+    const int64_t most = static_cast<int64_t>(sm_count()) * held;
     if (a.units * 2 < most * kRotWarps) divide(1);
     const int blocks = static_cast<int>(std::min(most, (a.units + kRotWarps - 1) / kRotWarps));
     if (q_part) a.half[0].part = part;
@@ -726,8 +762,8 @@ void launch_qk_norm_rotary_fwd(const SxRotaryInputs& in, const SxAttentionView& 
     if (in.k_heads) set(a.half[1], k_out);
     by_layout(in, v, [&](auto t, auto n, auto nb, auto slots) {
         using T = decltype(t);
-        if (bulk) rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, false>, row, 1, s, nullptr, false, false);
-        else if constexpr (decltype(n)::value == 1) rot_launch(a, tokens, rotary_plain_kernel<T, false>, row, 0, s, nullptr, false, false);
+        if (bulk) rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, false>, kRotPerSm<decltype(n)::value, false>, row, 1, s, nullptr, false, false);
+        else if constexpr (decltype(n)::value == 1) rot_launch(a, tokens, rotary_plain_kernel<T, false>, kRotPerSm<1, false>, row, 0, s, nullptr, false, false);
     });
 }
 
@@ -762,10 +798,10 @@ void launch_qk_norm_rotary_bwd(const SxRotaryInputs& in, const SxRotaryGrads& g,
         float* part = static_cast<float*>(ws);
         int blocks = 0;
         if (bulk)
-            blocks = rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, true>, row, 2, s, part,
+            blocks = rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, true>, kRotPerSm<decltype(n)::value, true>, row, 2, s, part,
                                 g.v_q_weight, g.v_k_weight);
         else if constexpr (decltype(n)::value == 1)
-            blocks = rot_launch(a, tokens, rotary_plain_kernel<T, true>, row, 0, s, part, g.v_q_weight, g.v_k_weight);
+            blocks = rot_launch(a, tokens, rotary_plain_kernel<T, true>, kRotPerSm<1, true>, row, 0, s, part, g.v_q_weight, g.v_k_weight);
         if (g.v_q_weight || g.v_k_weight)
             SX_LAUNCH(rotary_sums_kernel, dim3(blocks_for(in.head_dim, 32), 2), 1024, 0, s, a.half[0].part, a.half[1].part, blocks,
                       in.head_dim, g.v_q_weight, g.v_k_weight, in.param_dtype);

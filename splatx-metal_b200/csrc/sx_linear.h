@@ -2,6 +2,8 @@
 // divided among workers, and what follows the sums.
 #pragma once
 
+#include <type_traits>
+
 #include "sx_internal.h"
 #include "sx_network.h"
 #include "sx_two.cuh"
@@ -158,10 +160,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 constexpr float kLog2Of = 1.4426950408889634f;  // of e
-struct Normal {
-    float below, density;  // Phi(z), and exp(-z^2 / 2)
-};
-__device__ __forceinline__ Normal normal_fast(float z) {
+__device__ __forceinline__ float normal_fast(float z) {  // Phi(z)
     const float a = fabsf(z), t = rcp_fast(fmaf(0.3f, a, 1.f)), e = exp2_fast(-0.5f * kLog2Of * a * a);
     float p = fmaf(-0x1.3bca6ap-4f, t, 0x1.ba7182p-3f);
     p = fmaf(p, t, -0x1.15ac44p-6f);
@@ -169,35 +168,16 @@ __device__ __forceinline__ Normal normal_fast(float z) {
     p = fmaf(p, t, 0x1.d1e316p-4f);
     p = fmaf(p, t, 0x1.ebd2f4p-4f);
     const float tail = p * t * e;
-    return {z < 0.f ? tail : 1.f - tail, e};
+    return z < 0.f ? tail : 1.f - tail;
 }
 __device__ __forceinline__ float gate_fast(float z) { return rcp_fast(1.f + exp2_fast(-kLog2Of * z)); }
 template <int ACT>
 __device__ __forceinline__ float act_fast(float z) {
     if constexpr (ACT == SXCUDA_ACT_RELU) return z < 0.f ? 0.f : z;
     if constexpr (ACT == SXCUDA_ACT_SILU) return z * gate_fast(z);
-    if constexpr (ACT == SXCUDA_ACT_GELU) return z * normal_fast(z).below;
+    if constexpr (ACT == SXCUDA_ACT_GELU) return z * normal_fast(z);
     if constexpr (ACT == SXCUDA_ACT_GELU_TANH) return z * gate_fast(tanh_gate_at(z));
     return z;
-}
-__device__ __forceinline__ float slope_fast(int32_t act, float z) {
-    z = fabsf(z) > 1e4f ? copysignf(1e4f, z) : z;
-    switch (act) {
-        case SXCUDA_ACT_RELU: return z > 0.f ? 1.f : z != z ? z : 0.f;
-        case SXCUDA_ACT_SILU: {
-            const float g = gate_fast(z);
-            return fmaf(z * g, 1.f - g, g);
-        }
-        case SXCUDA_ACT_GELU: {
-            const Normal n = normal_fast(z);
-            return fmaf(z * 0.3989422804014327f, n.density, n.below);
-        }
-        case SXCUDA_ACT_GELU_TANH: {
-            const float g = gate_fast(tanh_gate_at(z));
-            return fmaf(z * g * (1.f - g), kGeluTanh * fmaf(3.f * kGeluCube * z, z, 1.f), g);
-        }
-        default: return 1.f;
-    }
 }
 // act_fast of two values, by instructions that work on two where there are such.
 template <int ACT>
@@ -243,10 +223,70 @@ __device__ __forceinline__ float act_of(int32_t act, float z) {
         default: return z;
     }
 }
-template <typename T>
-__device__ __forceinline__ float slope_of(int32_t act, float z) {
-    if constexpr (sizeof(T) == 4) return linear_slope(act, z);
-    else return slope_fast(act, z);
+// The slopes at two values. Beyond 1e4 they have their limits long since, and infinity times zero would be NaN.
+template <int ACT>
+__device__ __forceinline__ void slope_pair(float& x, float& y) {
+    using namespace tc;
+    const Two one = two(1.f, 1.f);
+    if constexpr (ACT == SXCUDA_ACT_RELU) {
+        x = x > 0.f ? 1.f : x != x ? x : 0.f, y = y > 0.f ? 1.f : y != y ? y : 0.f;
+    } else {
+        x = fabsf(x) > 1e4f ? copysignf(1e4f, x) : x, y = fabsf(y) > 1e4f ? copysignf(1e4f, y) : y;
+        const Two z = two(x, y);
+        float u, v;
+        if constexpr (ACT == SXCUDA_ACT_GELU) {
+            split(fma2(two(fabsf(x), fabsf(y)), two(0.3f, 0.3f), one), u, v);
+            const Two t = two(rcp_fast(u), rcp_fast(v));
+            split(mul2(mul2(z, two(-0.5f * kLog2Of, -0.5f * kLog2Of)), z), u, v);
+            const Two e = two(exp2_fast(u), exp2_fast(v));
+            Two p = fma2(two(-0x1.3bca6ap-4f, -0x1.3bca6ap-4f), t, two(0x1.ba7182p-3f, 0x1.ba7182p-3f));
+            p = fma2(p, t, two(-0x1.15ac44p-6f, -0x1.15ac44p-6f));
+            p = fma2(p, t, two(0x1.27505cp-3f, 0x1.27505cp-3f));
+            p = fma2(p, t, two(0x1.d1e316p-4f, 0x1.d1e316p-4f));
+            p = fma2(p, t, two(0x1.ebd2f4p-4f, 0x1.ebd2f4p-4f));
+            const Two tail = mul2(mul2(p, t), e);
+            float a, b;
+            split(tail, a, b);
+            split(fma2(tail, two(-1.f, -1.f), one), u, v);
+            split(fma2(mul2(z, two(0.3989422804014327f, 0.3989422804014327f)), e, two(x < 0.f ? a : u, y < 0.f ? b : v)), x, y);
+        } else {
+            const Two w = mul2(z, z);
+            Two at = z, steep = one;
+            if constexpr (ACT == SXCUDA_ACT_GELU_TANH) {
+                at = mul2(z, fma2(w, two(kGeluTanh * kGeluCube, kGeluTanh * kGeluCube), two(kGeluTanh, kGeluTanh)));
+                steep = fma2(w, two(3.f * kGeluTanh * kGeluCube, 3.f * kGeluTanh * kGeluCube), two(kGeluTanh, kGeluTanh));
+            }
+            split(mul2(at, two(-kLog2Of, -kLog2Of)), u, v);
+            split(add2(two(exp2_fast(u), exp2_fast(v)), one), u, v);
+            const Two g = two(rcp_fast(u), rcp_fast(v)), off = fma2(g, two(-1.f, -1.f), one);
+            split(fma2(mul2(mul2(z, g), off), steep, g), x, y);
+        }
+    }
+}
+// Times the slopes at z, for N values.
+template <typename T, int N>
+__device__ __forceinline__ void times_slopes(int32_t act, const float (&z)[N], float (&x)[N]) {
+    float s[N + 1];
+#pragma unroll
+    for (int i = 0; i < N + 1; ++i) s[i] = i < N ? z[i] : 0.f;
+    const auto pairs = [&](auto a) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) slope_pair<decltype(a)::value>(s[i], s[i + 1]);
+    };
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = linear_slope(act, s[i]);
+    } else if (act == SXCUDA_ACT_RELU) {
+        pairs(std::integral_constant<int, SXCUDA_ACT_RELU>{});
+    } else if (act == SXCUDA_ACT_SILU) {
+        pairs(std::integral_constant<int, SXCUDA_ACT_SILU>{});
+    } else if (act == SXCUDA_ACT_GELU) {
+        pairs(std::integral_constant<int, SXCUDA_ACT_GELU>{});
+    } else {
+        pairs(std::integral_constant<int, SXCUDA_ACT_GELU_TANH>{});
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] *= s[i];
 }
 
 // ---- products on the tensor cores (linear_tc.cu), of operands that tensor maps take ----

@@ -8,6 +8,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/splatx_cuda.h"
 #include "sx_common.cuh"
 
@@ -34,9 +36,12 @@ struct alignas(N * sizeof(T)) Pack {
 };
 
 inline int sm_count() {
+    static std::atomic<int> known[64];  // of each device, once asked for
     int dev = 0, n = 0;
     cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
     cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "SM count");
+    if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 

@@ -22,6 +22,7 @@ not synchronise. Contract violations raise ``ValueError``, device failures ``Run
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -427,15 +428,21 @@ _PAIRS = {"axis": 0, "whole": 1, "neighbours": 2}
 _POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
 
-def _ladder(what, axes, base, freqs):
-    """The pairs' frequencies as a C array: given ones, or base^(-2 j / dim) for pair j of an axis."""
-    if freqs is None:
-        if not (isinstance(base, (int, float)) and base > 0 and math.isfinite(base)):
-            raise ValueError(f"{what}: base must be a number above zero")
-        freqs = [float(base) ** (-2.0 * j / d) for d in axes for j in range(d // 2)]
-    elif len(freqs) != sum(axes) // 2:
-        raise ValueError(f"{what}: {sum(axes) // 2} freqs needed, got {len(freqs)}")
-    return (C.c_double * max(len(freqs), 1))(*[float(f) for f in freqs])
+@functools.lru_cache(maxsize=64)
+def _ladder(axes, base):
+    """The pairs' frequencies base^(-2 j / dim), pair j of each axis, as a C array that is only read."""
+    freqs = [base ** (-2.0 * j / d) for d in axes for j in range(d // 2)]
+    return (C.c_double * max(len(freqs), 1))(*freqs)
+
+
+def _freqs(what, axes, base, freqs):
+    if freqs is not None:
+        if len(freqs) != sum(axes) // 2:
+            raise ValueError(f"{what}: {sum(axes) // 2} freqs needed, got {len(freqs)}")
+        return (C.c_double * max(len(freqs), 1))(*[float(f) for f in freqs])
+    if not (isinstance(base, (int, float)) and base > 0 and math.isfinite(base)):
+        raise ValueError(f"{what}: base must be a number above zero")
+    return _ladder(axes, float(base))
 
 
 def _head_rows(t, what):
@@ -475,7 +482,7 @@ def _rotary_inputs(what, q, k, positions, axes, base, freqs, pairs, norm, q_weig
                              f"[{d}] with one dtype")
     _on(device, what, k, positions, q_weight, k_weight)
     at = positions.stride()
-    table = _ladder(what, axes, base, freqs)
+    table = _freqs(what, axes, base, freqs)
     ins = _nat.SxRotaryInputs(
         _view(q), _view(q) if k is None else _view(k), positions.data_ptr(), at[0] if len(at) == 3 else 0,
         at[-2], at[-1], C.addressof(table), None if q_weight is None else q_weight.data_ptr(),
