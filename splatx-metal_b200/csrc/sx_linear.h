@@ -223,7 +223,9 @@ __device__ __forceinline__ float act_of(int32_t act, float z) {
         default: return z;
     }
 }
-// The slopes at two values. Beyond 1e4 they have their limits long since, and infinity times zero would be NaN.
+// The slopes at two values, within some 2^-21: their products with v_y are also summed to the bias' gradient, which
+// may be held in 32 bits. So P has its 8th power (2.8e-8, with t = 1 / (1 + 0.26 a)). Beyond 1e4 the slopes have
+// their limits long since, and infinity times zero would be NaN.
 template <int ACT>
 __device__ __forceinline__ void slope_pair(float& x, float& y) {
     using namespace tc;
@@ -235,15 +237,19 @@ __device__ __forceinline__ void slope_pair(float& x, float& y) {
         const Two z = two(x, y);
         float u, v;
         if constexpr (ACT == SXCUDA_ACT_GELU) {
-            split(fma2(two(fabsf(x), fabsf(y)), two(0.3f, 0.3f), one), u, v);
+            split(fma2(two(fabsf(x), fabsf(y)), two(0.26f, 0.26f), one), u, v);
             const Two t = two(rcp_fast(u), rcp_fast(v));
             split(mul2(mul2(z, two(-0.5f * kLog2Of, -0.5f * kLog2Of)), z), u, v);
             const Two e = two(exp2_fast(u), exp2_fast(v));
-            Two p = fma2(two(-0x1.3bca6ap-4f, -0x1.3bca6ap-4f), t, two(0x1.ba7182p-3f, 0x1.ba7182p-3f));
-            p = fma2(p, t, two(-0x1.15ac44p-6f, -0x1.15ac44p-6f));
-            p = fma2(p, t, two(0x1.27505cp-3f, 0x1.27505cp-3f));
-            p = fma2(p, t, two(0x1.d1e316p-4f, 0x1.d1e316p-4f));
-            p = fma2(p, t, two(0x1.ebd2f4p-4f, 0x1.ebd2f4p-4f));
+            Two p = two(0x1.ef4a64p-6f, 0x1.ef4a64p-6f);
+            p = fma2(p, t, two(-0x1.364252p-3f, -0x1.364252p-3f));
+            p = fma2(p, t, two(0x1.fd6710p-3f, 0x1.fd6710p-3f));
+            p = fma2(p, t, two(-0x1.2eab5ap-3f, -0x1.2eab5ap-3f));
+            p = fma2(p, t, two(0x1.4522c6p-3f, 0x1.4522c6p-3f));
+            p = fma2(p, t, two(0x1.a9b2fep-5f, 0x1.a9b2fep-5f));
+            p = fma2(p, t, two(0x1.a505a4p-4f, 0x1.a505a4p-4f));
+            p = fma2(p, t, two(0x1.a618cap-4f, 0x1.a618cap-4f));
+            p = fma2(p, t, two(0x1.a8fd20p-4f, 0x1.a8fd20p-4f));
             const Two tail = mul2(mul2(p, t), e);
             float a, b;
             split(tail, a, b);
@@ -256,9 +262,11 @@ __device__ __forceinline__ void slope_pair(float& x, float& y) {
                 at = mul2(z, fma2(w, two(kGeluTanh * kGeluCube, kGeluTanh * kGeluCube), two(kGeluTanh, kGeluTanh)));
                 steep = fma2(w, two(3.f * kGeluTanh * kGeluCube, 3.f * kGeluTanh * kGeluCube), two(kGeluTanh, kGeluTanh));
             }
+            // g = 1 / (1 + e), and 1 - g = e g, which loses no digits; e stays finite, and a NaN comes back by z
             split(mul2(at, two(-kLog2Of, -kLog2Of)), u, v);
-            split(add2(two(exp2_fast(u), exp2_fast(v)), one), u, v);
-            const Two g = two(rcp_fast(u), rcp_fast(v)), off = fma2(g, two(-1.f, -1.f), one);
+            const Two e = two(fminf(exp2_fast(u), 1e30f), fminf(exp2_fast(v), 1e30f));
+            split(add2(e, one), u, v);
+            const Two g = two(rcp_fast(u), rcp_fast(v)), off = mul2(e, g);
             split(fma2(mul2(mul2(z, g), off), steep, g), x, y);
         }
     }
