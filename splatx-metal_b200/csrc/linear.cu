@@ -340,6 +340,12 @@ struct Matrix {
     LinearOperand across_k() const { return {data, stride, true}; }  // its columns are
 };
 
+__device__ __forceinline__ void linear_param_to(void* w, int32_t dtype, int64_t i, float x) {
+    if (dtype == SXCUDA_F32) static_cast<float*>(w)[i] = x;
+    else if (dtype == SXCUDA_F16) static_cast<__half*>(w)[i] = __float2half_rn(x);
+    else static_cast<__nv_bfloat16*>(w)[i] = __float2bfloat16_rn(x);
+}
+
 // ---- v_z = v_y act'(pre), and the sum of its rows ----
 // A CTA has 32 V columns (a warp's lanes V each) and a slice of the rows, which its warps take in turn; the grid
 // is what the SMs hold. Bound by memory: gelu over bf16 32768 x 4096 163 us (4.9 TB/s); several rows asked for
@@ -350,8 +356,9 @@ struct SlopeArgs {
     const void* pre;
     void* v_z;    // NULL: v_y itself
     float* sums;  // [slices, cols] or NULL
+    void* v_bias;  // written by the only slice there is, else NULL
     int64_t v_y_stride, pre_stride, v_z_stride, rows, cols, slice;
-    int32_t act;
+    int32_t act, bias_dtype;
 };
 template <typename T, int V>
 __global__ void __launch_bounds__(kSlopeWarps * 32, kSlopePerSm) linear_slope_kernel(const SlopeArgs a) {
@@ -373,7 +380,7 @@ __global__ void __launch_bounds__(kSlopeWarps * 32, kSlopePerSm) linear_slope_ke
             for (int i = 0; i < V; ++i) sum[i] += x[i], to.v[i] = from_f32<T>(x[i]);
             if (a.v_z) *reinterpret_cast<Pack<T, V>*>(static_cast<T*>(a.v_z) + r * a.v_z_stride + c) = to;
         }
-    if (!a.sums) return;
+    if (!a.sums && !a.v_bias) return;
 #pragma unroll
     for (int i = 0; i < V; ++i) part[warp][lane * V + i] = sum[i];
     __syncthreads();
@@ -381,7 +388,9 @@ __global__ void __launch_bounds__(kSlopeWarps * 32, kSlopePerSm) linear_slope_ke
         const int64_t col = static_cast<int64_t>(blockIdx.x) * 32 * V + i;
         float x = 0.f;
         for (int w = 0; w < kSlopeWarps; ++w) x += part[w][i];
-        if (col < a.cols) a.sums[blockIdx.y * a.cols + col] = x;
+        if (col >= a.cols) continue;
+        if (a.v_bias) linear_param_to(a.v_bias, a.bias_dtype, col, x);
+        else a.sums[blockIdx.y * a.cols + col] = x;
     }
 }
 // Adds the slices' sums of 32 columns: warp w takes every 32nd slice, eight in flight, then the warps are
@@ -405,9 +414,7 @@ __global__ void __launch_bounds__(1024) linear_bias_kernel(const float* part, in
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
     const int64_t at = static_cast<int64_t>(blockIdx.x) * 32 + warp;
     if (lane || at >= cols) return;
-    if (dtype == SXCUDA_F32) static_cast<float*>(v_bias)[at] = s;
-    else if (dtype == SXCUDA_F16) static_cast<__half*>(v_bias)[at] = __float2half_rn(s);
-    else static_cast<__nv_bfloat16*>(v_bias)[at] = __float2bfloat16_rn(s);
+    linear_param_to(v_bias, dtype, at, s);
 }
 
 struct SlopePlan {
@@ -423,7 +430,7 @@ SlopePlan slope_plan(const SxLinearInputs& in, const SxLinearGradsIn& g) {
     p.v = in.out_features % most == 0 && wide(g.v_y, g.v_y_stride) && wide(g.pre, g.pre_stride) ? static_cast<int>(most) : 1;
     p.strips = (in.out_features + 32 * p.v - 1) / (32 * p.v);
     const int64_t want = std::max<int64_t>(static_cast<int64_t>(sm_count()) * kSlopePerSm / p.strips, 1);
-    p.slice = std::max<int64_t>((in.rows + want - 1) / want, 4 * kSlopeWarps);
+    p.slice = std::max<int64_t>((in.rows + want - 1) / want, 16 * kSlopeWarps);  // a few rows: no second kernel
     p.slices = (in.rows + p.slice - 1) / p.slice;
     return p;
 }
@@ -503,15 +510,16 @@ void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const
     Matrix v_z = space.v_y;
     if (space.v_z || out.v_bias) {
         const SlopePlan plan = slope_plan(in, g);
-        SlopeArgs a{g.v_y, g.pre, nullptr, nullptr, g.v_y_stride, g.pre_stride, pitch_of(in.out_features), in.rows, in.out_features, plan.slice, in.activation};
+        SlopeArgs a{g.v_y, g.pre, nullptr, nullptr, nullptr, g.v_y_stride, g.pre_stride, pitch_of(in.out_features), in.rows, in.out_features, plan.slice, in.activation, in.bias_dtype};
         if (space.v_z) v_z = {a.v_z = at + space.v_z_at, a.v_z_stride, in.rows, in.out_features};
-        if (out.v_bias) a.sums = reinterpret_cast<float*>(at + space.sums_at);
+        if (out.v_bias && plan.slices > 1) a.sums = reinterpret_cast<float*>(at + space.sums_at);
+        else a.v_bias = out.v_bias;
         by_dtype(in.dtype, [&](auto t) {
             using T = decltype(t);
             const auto kernel = plan.v == 1 ? linear_slope_kernel<T, 1> : linear_slope_kernel<T, 16 / sizeof(T)>;
             SX_LAUNCH(kernel, dim3(static_cast<unsigned>(plan.strips), static_cast<unsigned>(plan.slices)), kSlopeWarps * 32, 0, s, a);
         });
-        if (out.v_bias)
+        if (a.sums)
             SX_LAUNCH(linear_bias_kernel, blocks_for(in.out_features, 32), 1024, 0, s, a.sums, plan.slices, in.out_features, out.v_bias, in.bias_dtype);
     }
     LinearProduct p{};

@@ -7,7 +7,9 @@ with its three degree-0 SH coefficients. A step writes them into the executor's 
 renders one view with the executor's forward and backward (``step_accumulate``), takes the loss
 gradient of the coefficients from the resident gradient buffers as the gradient of the network's
 output, and updates the network's weights with ``AdamW``. Attention, layer norm and AdamW are
-``splatx_cuda.network``'s; the matrix products of the layers are torch's.
+``splatx_cuda.network``'s; the matrix products of the layers are torch's. With ``--spatial`` the
+products, with their gelu and residuals, are ``splatx_cuda.network``'s too, and queries and keys are
+normalised and rotated by the Gaussians' places.
 """
 from __future__ import annotations
 
@@ -32,9 +34,10 @@ SH0 = 4  # the parameter group of the degree-0 coefficients
 
 
 class ColorNetwork(torch.nn.Module):
-    """[splats, features] -> [splats, 3]; 32-bit weights, bfloat16 activations."""
+    """[splats, features] -> [splats, 3]; 32-bit weights, bfloat16 activations. spatial: attention knows where
+    the splats are, and ``forward`` takes their places, [splats, 3], from about -128 to 128."""
 
-    def __init__(self, features: int, width: int = 128, heads: int = 2, layers: int = 2):
+    def __init__(self, features: int, width: int = 128, heads: int = 2, layers: int = 2, spatial: bool = False):
         super().__init__()
         self.heads, self.layers = heads, layers
         sizes = {"embed": (width, features), "head": (3, width)}
@@ -45,6 +48,9 @@ class ColorNetwork(torch.nn.Module):
             {k: torch.randn(s) * s[1] ** -0.5 for k, s in sizes.items()})
         norms = [f"{n}{i}" for i in range(layers) for n in ("attn", "mlp")] + ["last"]
         self.scale = torch.nn.ParameterDict({k: torch.ones(width) for k in norms})
+        d = width // heads
+        self.axes = (d - 2 * (d // 3 // 2 * 2), d // 3 // 2 * 2, d // 3 // 2 * 2) if spatial else None
+        self.qk = torch.nn.ParameterDict({f"{n}{i}": torch.ones(d) for i in range(layers if spatial else 0) for n in "qk"})
         self.shift = torch.nn.ParameterDict({k: torch.zeros(width) for k in norms})
 
     def _linear(self, x, name):
@@ -53,7 +59,9 @@ class ColorNetwork(torch.nn.Module):
     def _norm(self, x, name):
         return network.layer_norm(x, self.scale[name], self.shift[name])
 
-    def forward(self, features):
+    def forward(self, features, places=None):
+        if self.axes is not None:
+            return self._spatial(features.to(torch.bfloat16)[None], places[None])
         x = self._linear(features.to(torch.bfloat16)[None], "embed")
         for i in range(self.layers):
             qkv = self._linear(self._norm(x, f"attn{i}"), f"qkv{i}")
@@ -61,6 +69,20 @@ class ColorNetwork(torch.nn.Module):
             x = x + self._linear(network.attention(q, k, v).flatten(2), f"proj{i}")
             x = x + self._linear(F.gelu(self._linear(self._norm(x, f"mlp{i}"), f"up{i}")), f"down{i}")
         return self._linear(self._norm(x, "last"), "head")[0].float()
+
+    def _spatial(self, x, places):
+        def linear(x, name, **how):
+            return network.linear(x, self.w[name].to(x.dtype), **how)
+
+        x = linear(x, "embed")
+        for i in range(self.layers):
+            qkv = linear(self._norm(x, f"attn{i}"), f"qkv{i}")
+            q, k, v = qkv.unflatten(-1, (3, self.heads, -1)).unbind(2)
+            q, k = network.qk_norm_rotary(q, k, places, axes=self.axes, base=100.0, q_weight=self.qk[f"q{i}"],
+                                          k_weight=self.qk[f"k{i}"])
+            x = linear(network.attention(q, k, v).flatten(2), f"proj{i}", residual=x)
+            x = linear(linear(self._norm(x, f"mlp{i}"), f"up{i}", activation="gelu"), f"down{i}", residual=x)
+        return linear(self._norm(x, "last"), "head")[0].float()
 
 
 class ResidentGroup:
@@ -82,7 +104,7 @@ class ResidentGroup:
 
 
 def train(splats: int = 2048, steps: int = 80, width: int = 128, state_bits: int = 32, seed: int = 0,
-          lr: float = 2e-3, device: int = 0) -> list[float]:
+          lr: float = 2e-3, device: int = 0, spatial: bool = False) -> list[float]:
     """The loss of every step."""
     torch.manual_seed(seed)
     scene, cam = small_scene(seed=seed, n=splats)
@@ -99,7 +121,8 @@ def train(splats: int = 2048, steps: int = 80, width: int = 128, state_bits: int
         features = np.concatenate([scene.means, scene.scales, scene.quats, scene.opacities[:, None]], 1)
         features = torch.from_numpy(features).to(target.device)
         features = (features - features.mean(0)) / features.std(0)
-        net = ColorNetwork(features.shape[1], width).to(target.device)
+        net = ColorNetwork(features.shape[1], width, spatial=spatial).to(target.device)
+        places = features[:, :3] * 32.0 if spatial else None
         opt = network.AdamW(net.parameters(), lr=lr, weight_decay=0.01, state_bits=state_bits)
         sh0 = ResidentGroup(ex, SH0, splats, device)
         torch.cuda.synchronize(device)
@@ -107,7 +130,7 @@ def train(splats: int = 2048, steps: int = 80, width: int = 128, state_bits: int
         # everything on the executor's stream: its steps and torch's kernels follow one another
         with torch.cuda.stream(torch.cuda.ExternalStream(ex.stream_handle(), device=device)):
             for _ in range(steps):
-                out = net(features)
+                out = net(features, places)
                 sh0.write(out.detach())
                 ex.clear_grads()
                 ex.step_accumulate(cam.viewmat, cam.K, cam.width, cam.height, target.data_ptr(), splats)
@@ -126,8 +149,9 @@ def main():
     p.add_argument("--width", type=int, default=128)
     p.add_argument("--state-bits", type=int, default=32, choices=(8, 32))
     p.add_argument("--lr", type=float, default=2e-3)
+    p.add_argument("--spatial", action="store_true")
     a = p.parse_args()
-    losses = train(a.splats, a.steps, a.width, a.state_bits, lr=a.lr)
+    losses = train(a.splats, a.steps, a.width, a.state_bits, lr=a.lr, spatial=a.spatial)
     for i in range(0, len(losses), max(1, len(losses) // 10)):
         print(f"step {i:4d}  loss {losses[i]:.5f}")
     print(f"step {len(losses) - 1:4d}  loss {losses[-1]:.5f}")
