@@ -51,7 +51,7 @@ struct Smem {
     static constexpr int kPatchesAt = kStages * kStage;
     static constexpr int kBias = kPatchesAt + kPatches * kPatch;  // [2][TN] floats
     static constexpr int kBars = kBias + 2 * TN * 4;
-    static constexpr int kBytes = kBars + (2 * kStages + 5 + kPatches) * 8 + 16;
+    static constexpr int kBytes = kBars + (2 * kStages + 9 + kPatches) * 8 + 16;
     static_assert(kBytes <= 232448, "shared memory");
 };
 
@@ -63,7 +63,8 @@ struct Bars {
     __device__ uint32_t acc_full(int i) const { return base + (2 * STAGES + i) * 8; }  // each CTA's
     __device__ uint32_t acc_empty(int i) const { return base + (2 * STAGES + 2 + i) * 8; }  // the leader's
     __device__ uint32_t drained() const { return base + (2 * STAGES + 4) * 8; }
-    __device__ uint32_t residual(int warp) const { return base + (2 * STAGES + 5 + warp) * 8; }
+    __device__ uint32_t bias(int part) const { return base + (2 * STAGES + 5 + part) * 8; }
+    __device__ uint32_t residual(int warp) const { return base + (2 * STAGES + 9 + warp) * 8; }
 };
 
 // ---- what a pair of CTAs needs ----
@@ -322,6 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<B_ACROSS>, 
         for (int s = 0; s < kStages; ++s) tc::bar_init(bars.full(s), 1), tc::bar_init(bars.empty(s), 1);
         for (int i = 0; i < 2; ++i) tc::bar_init(bars.acc_full(i), 1), tc::bar_init(bars.acc_empty(i), 2 * kWarps);
         tc::bar_init(bars.drained(), 1);
+        for (int i = 0; i < 4; ++i) tc::bar_init(bars.bias(i), 4);
         for (int i = 0; i < kWarps; ++i) tc::bar_init(bars.residual(i), 1);
         tc::bar_init_fence();
         *failed = 0;
@@ -433,7 +435,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<B_ACROSS>, 
             float* bias = reinterpret_cast<float*>(smem + S::kBias) + (count & 1) * TN;
             if (lane < kCols / 4) bias[bias_at] = here.bias;
             bias += part * kCols;
-            asm volatile("bar.sync %0, 128;" ::"r"(part + 1) : "memory");
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(bars.bias(part));
+            ok = tc::bar_wait(bars.bias(part), count & 1, failed);  // a warp may have given up: no barrier without a limit
+            if (!ok) break;
             more = walk.next(p.plan, piece);
             if (more) next = place();
             if (COPIES && finishes && p.residual && n0 < p.n) ask(row, n0);
@@ -607,11 +612,20 @@ bool linear_tc_takes(const void* data, int64_t stride, int64_t rows) {
     return reinterpret_cast<uintptr_t>(data) % 16 == 0 && (rows <= 1 || (stride % 8 == 0 && stride < (1ll << 38)));
 }
 
+// Tiles of 256 or of 128 columns, cut or not: by what they take. Measured on a pair of CTAs: 64 values of K 0.27 and
+// 0.155 us (the tensor cores' rate, and 0.87 of it), an epilogue that nothing hides 3.1 and 1.6 us, a cut (the parts'
+// way through memory and the second kernel) some 6 us. 5001 x 333 x 777 with a residual, 128 and 256: 25 and 37 us.
 LinearPlan linear_tc_plan(int64_t m, int64_t n, int64_t k) {
     const int64_t pairs = sm_count() / 2;
-    const int64_t tiles = (m + kTileM - 1) / kTileM * ((n + 255) / 256);
-    const bool narrow = n <= 128 || (tiles < pairs && tiles * ((k + kDepth - 1) / kDepth) < 16 * pairs);
-    return linear_plan(m, n, k, kTileM, narrow ? 128 : 256, kDepth, pairs, 4, 24);
+    const auto time = [&](const LinearPlan& p, double block, double least) {
+        const double tile = std::max(static_cast<double>(p.kblocks) * block, least);
+        const int64_t turns = (p.whole + pairs - 1) / pairs;
+        return static_cast<double>(turns) * tile + (p.cut() ? static_cast<double>(p.share) * block + 6. : 0.);
+    };
+    const LinearPlan narrow = linear_plan(m, n, k, kTileM, 128, kDepth, pairs, 4, 39);
+    if (n <= 128) return narrow;
+    const LinearPlan wide = linear_plan(m, n, k, kTileM, 256, kDepth, pairs, 4, 23);
+    return time(narrow, 0.155, 1.6) < time(wide, 0.27, 3.1) ? narrow : wide;
 }
 
 void launch_linear_tc(const LinearProduct& p, cudaStream_t s) {

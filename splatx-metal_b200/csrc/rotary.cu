@@ -207,7 +207,11 @@ struct Rot {
         } else {
             u.token += step;
         }
-        while (u.token >= a.tokens) u.token -= a.tokens, ++u.batch;
+        if (u.token >= a.tokens) {
+            const uint32_t t = static_cast<uint32_t>(u.token), n = static_cast<uint32_t>(a.tokens), b = t / n;  // both below 2^31
+            u.token = t - b * n;
+            u.batch += b;
+        }
     }
     // Lane i's position along axis i.
     __device__ double position(const Unit& t) const {
