@@ -64,6 +64,9 @@ struct Bars {
     __device__ uint32_t acc_empty(int i) const { return base + (2 * STAGES + 2 + i) * 8; }  // the leader's
     __device__ uint32_t drained() const { return base + (2 * STAGES + 4) * 8; }
     __device__ uint32_t bias(int part) const { return base + (2 * STAGES + 5 + part) * 8; }
+    static constexpr int kCount = 2 * STAGES + 9 + kPatches;
+    static __device__ bool is_acc_empty(int i) { return i / 2 == STAGES + 1; }
+    static __device__ bool is_bias(int i) { return i >= 2 * STAGES + 5 && i < 2 * STAGES + 9; }
     __device__ uint32_t residual(int warp) const { return base + (2 * STAGES + 9 + warp) * 8; }
 };
 
@@ -73,8 +76,9 @@ __device__ __forceinline__ uint32_t in_cta(uint32_t addr, uint32_t rank) {  // t
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Without a release of its own, which would wait for the CTA's memory: what has to be seen is fenced where it is written.
 __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ void arrive_in(uint32_t cluster_bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
@@ -97,7 +101,6 @@ __device__ __forceinline__ void store_box(const CUtensorMap* map, int x, int y, 
 __device__ __forceinline__ void stores_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int N>  // all but the last N groups of the thread's stores have left shared memory
 __device__ __forceinline__ void stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void pair_alloc(uint32_t to_smem, uint32_t columns) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(to_smem), "r"(columns) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
@@ -317,16 +320,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<B_ACROSS>, 
     LinearPiece piece;
     int asked = 0;  // stages that this warp has asked for
 
-    if (warp == kLoader && lane == 0) {
-        tc::prefetch_map(&maps.a);
-        tc::prefetch_map(&maps.b);
-        for (int s = 0; s < kStages; ++s) tc::bar_init(bars.full(s), 1), tc::bar_init(bars.empty(s), 1);
-        for (int i = 0; i < 2; ++i) tc::bar_init(bars.acc_full(i), 1), tc::bar_init(bars.acc_empty(i), 2 * kWarps);
-        tc::bar_init(bars.drained(), 1);
-        for (int i = 0; i < 4; ++i) tc::bar_init(bars.bias(i), 4);
-        for (int i = 0; i < kWarps; ++i) tc::bar_init(bars.residual(i), 1);
+    if (warp == kLoader) {
+        if (lane == 0) {
+            tc::prefetch_map(&maps.a);
+            tc::prefetch_map(&maps.b);
+            *failed = 0;
+        }
+        for (int i = lane; i < Bars<kStages>::kCount; i += 32)
+            tc::bar_init(bars.base + i * 8, Bars<kStages>::is_acc_empty(i) ? 2 * kWarps : Bars<kStages>::is_bias(i) ? 4 : 1);
         tc::bar_init_fence();
-        *failed = 0;
     }
     __syncwarp();
     if (warp == kIssuer) pair_alloc(tc::smem_addr(tmem_at), 2 * TN);
@@ -383,6 +385,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<B_ACROSS>, 
                 }
                 if (ok) pair_commit(one, bars.acc_full(count & 1));
             }
+            // the other CTA's last arrivals, without which this CTA's memory must not go
+            for (int i = max(0, count - 2); ok && i < count; ++i) ok = tc::bar_wait(bars.acc_empty(i & 1), (i >> 1) & 1, failed);
         }
     } else {
         constexpr int kCols = TN / (kWarps / 4), kOwn = kPatches / kWarps;  // columns and patches of a warp
@@ -506,13 +510,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<B_ACROSS>, 
             }
         }
         if (due) tc::bar_drain(bars.residual(warp), turn);
-        if (lane == 0) stores_done();
+        if (lane == 0) stores_read<0>();
     }
 
     tc::fence_before();
     __syncthreads();
     if (threadIdx.x == 0 && *failed) {
         asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(in_cta(tc::smem_addr(const_cast<uint32_t*>(failed)), rank ^ 1)), "r"(1) : "memory");
+        asm volatile("fence.acq_rel.cluster;" ::: "memory");
     }
     cluster_sync();
     if (*failed) {  // nothing may land in the pair's memory after it has gone
