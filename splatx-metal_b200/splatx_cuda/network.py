@@ -52,6 +52,11 @@ def _on(device: torch.device, what: str, *others) -> None:
             raise ValueError(f"{what}: a tensor is on {t.device}, not on {device}")
 
 
+# the current stream's handle without a torch.cuda.Stream made for it, which takes a short call 3 of its 20 us
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 class _at:
     """The device made current for one call (left alone where it is already) and its stream."""
 
@@ -63,7 +68,7 @@ class _at:
     def __enter__(self):
         if self.was != self.index:
             torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         if self.was != self.index:
@@ -428,11 +433,31 @@ _PAIRS = {"axis": 0, "whole": 1, "neighbours": 2}
 _POSITIONS = {torch.float32: 0, torch.int32: 1, torch.int64: 2}
 
 
+_Four = C.c_int32 * 4
+
+
 @functools.lru_cache(maxsize=64)
 def _ladder(axes, base):
     """The pairs' frequencies base^(-2 j / dim), pair j of each axis, as a C array that is only read."""
     freqs = [base ** (-2.0 * j / d) for d in axes for j in range(d // 2)]
     return (C.c_double * max(len(freqs), 1))(*freqs)
+
+
+@functools.lru_cache(maxsize=64)
+def _axes_for(axes, d):
+    """The axes as C has them; None where they do not fit heads of d values."""
+    if not 1 <= len(axes) <= 4 or any(a < 0 or a % 2 for a in axes) or sum(axes) > d:
+        return None
+    return _Four(*axes)
+
+
+@functools.lru_cache(maxsize=256)
+def _rotary_space(index, d, norm):
+    """Bytes of the backward's workspace, which the device, the head's size and norm decide."""
+    ins = _nat.SxRotaryInputs(batch=0, tokens=0, q_heads=1, head_dim=d, axes=1, norm=norm)
+    nbytes = C.c_size_t(0)
+    check(_nat.lib().sxcuda_qk_norm_rotary_bwd(C.byref(ins), None, None, C.byref(nbytes), None))
+    return nbytes.value
 
 
 def _freqs(what, axes, base, freqs):
@@ -464,8 +489,9 @@ def _rotary_inputs(what, q, k, positions, axes, base, freqs, pairs, norm, q_weig
         raise ValueError(f"{what}: k_weight needs k")
     if pairs not in _PAIRS:
         raise ValueError(f"{what}: pairs must be one of {list(_PAIRS)}")
-    axes = tuple(int(a) for a in axes)
-    if not 1 <= len(axes) <= 4 or any(a < 0 or a % 2 for a in axes) or sum(axes) > d:
+    axes = tuple(map(int, axes))
+    c_axes = _axes_for(axes, d)
+    if c_axes is None:
         raise ValueError(f"{what}: axes must be 1 to 4 even numbers of values, at most {d} together, got {axes}")
     code_at = _POSITIONS.get(positions.dtype)
     if code_at is None:
@@ -487,7 +513,7 @@ def _rotary_inputs(what, q, k, positions, axes, base, freqs, pairs, norm, q_weig
         _view(q), _view(q) if k is None else _view(k), positions.data_ptr(), at[0] if len(at) == 3 else 0,
         at[-2], at[-1], C.addressof(table), None if q_weight is None else q_weight.data_ptr(),
         None if k_weight is None else k_weight.data_ptr(), b, n, h, 0 if k is None else k.shape[2], d,
-        len(axes), (C.c_int32 * 4)(*axes), _PAIRS[pairs], code, 0 if first is None else _dtype(first, what),
+        len(axes), c_axes, _PAIRS[pairs], code, 0 if first is None else _dtype(first, what),
         code_at, bool(norm), eps)
     return q, k, ins, device, table
 
@@ -534,14 +560,16 @@ def qk_norm_rotary_bwd(v_q_out, v_k_out, q, k, positions, *, axes, base=10000.0,
         grads.append(None if t is None else _head_rows(g, what))
     _on(device, what, *grads)
     outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k)]
+    d = q.shape[3]
     v_w = [None if w is None else torch.empty_like(w) for w in (q_weight, k_weight)]
     none = (None, 0, 0, 0)
     g = _nat.SxRotaryGrads(*(none if t is None else _view(t) for t in (*grads, *outs)),
                            *(None if w is None else w.data_ptr() for w in v_w))
-    entry = _nat.lib().sxcuda_qk_norm_rotary_bwd
     with _at(device) as stream:
-        ws, at, nbytes = _space(device, entry, C.byref(ins), C.byref(g))
-        check(entry(C.byref(ins), C.byref(g), at, C.byref(nbytes), stream))
+        nbytes = C.c_size_t(_rotary_space(device.index, d, bool(norm)))
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=device) if nbytes.value else None
+        check(_nat.lib().sxcuda_qk_norm_rotary_bwd(C.byref(ins), C.byref(g), 16 if ws is None else ws.data_ptr(),
+                                                   C.byref(nbytes), stream))
     return (*outs, *v_w)
 
 
