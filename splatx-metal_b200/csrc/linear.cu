@@ -430,7 +430,9 @@ SlopePlan slope_plan(const SxLinearInputs& in, const SxLinearGradsIn& g) {
     p.v = in.out_features % most == 0 && wide(g.v_y, g.v_y_stride) && wide(g.pre, g.pre_stride) ? static_cast<int>(most) : 1;
     p.strips = (in.out_features + 32 * p.v - 1) / (32 * p.v);
     const int64_t want = std::max<int64_t>(static_cast<int64_t>(sm_count()) * kSlopePerSm / p.strips, 1);
-    p.slice = std::max<int64_t>((in.rows + want - 1) / want, 16 * kSlopeWarps);  // a few rows: no second kernel
+    p.slice = std::max<int64_t>((in.rows + want - 1) / want, 4 * kSlopeWarps);
+    // few: no second kernel (us in one slice and in several: 128 x 2560 gelu 13.2 and 8, without an activation 4.9 and 6)
+    if (in.rows <= (g.pre ? 8 : 16) * kSlopeWarps) p.slice = in.rows;
     p.slices = (in.rows + p.slice - 1) / p.slice;
     return p;
 }

@@ -261,14 +261,15 @@ struct Rot {
             return which ? (second < 0 ? -1 : second + e) : first + e;
         }
     }
-    // A row's values, first ones and partners. A slot that is not the thread's own is zeros.
+    // A row's values, first ones and partners. A slot that is not the thread's own has others' values, which its sums
+    // leave out.
     __device__ __forceinline__ void load(const T* row, Values<V> (&p)[NV], Values<V> (&q)[NV]) const {
 #pragma unroll
         for (int n = 0; n < NV; ++n) {
             const auto x = *reinterpret_cast<const Pack<T, V>*>(row + first[n]), y = *reinterpret_cast<const Pack<T, V>*>(row + second[n]);
             if constexpr (V == 1) {
-                p[n].v[0] = tc::two(mine[n] ? to_f32(x.v[0]) : 0.f, 0.f);
-                q[n].v[0] = tc::two(mine[n] && pair[n] ? to_f32(y.v[0]) : 0.f, 0.f);
+                p[n].v[0] = tc::two(to_f32(x.v[0]), 0.f);
+                q[n].v[0] = tc::two(pair[n] ? to_f32(y.v[0]) : 0.f, 0.f);
             } else {
 #pragma unroll
                 for (int e = 0; e < V; e += 2) {
@@ -280,7 +281,6 @@ struct Rot {
                         p[n].v[e / 2] = tc::two(one.x, one.y), q[n].v[e / 2] = tc::two(other.x, other.y);
                     }
                 }
-                if (!mine[n]) p[n] = q[n] = Values<V>{};
             }
         }
     }
@@ -324,22 +324,27 @@ struct Rot {
         else if constexpr (std::is_same_v<T, __nv_bfloat16>) reinterpret_cast<__nv_bfloat162*>(x.v)[i / 2] = __floats2bfloat162_rn(lo, hi);
         else x.v[i] = lo, x.v[i + 1] = hi;
     }
-    __device__ float group_sum(tc::Two x) const {
+    static __device__ float both(tc::Two x) {
         float lo, hi;
         tc::split(x, lo, hi);
-        lo += hi;
+        return lo + hi;
+    }
+    __device__ float group_sum(float x) const {
 #pragma unroll
         for (int o = 16; o; o >>= 1)
-            if (a.lanes > o) lo += __shfl_xor_sync(kFullMask, lo, o);
-        return lo;
+            if (a.lanes > o) x += __shfl_xor_sync(kFullMask, x, o);
+        return x;
     }
     __device__ float rstd(const Values<V> (&p)[NV], const Values<V> (&q)[NV]) const {
-        tc::Two ss = tc::two(0.f, 0.f);
+        float sum = 0.f;
 #pragma unroll
-        for (int n = 0; n < NV; ++n)
+        for (int n = 0; n < NV; ++n) {
+            tc::Two ss = tc::two(0.f, 0.f);
 #pragma unroll
             for (int e = 0; e < N; ++e) ss = tc::fma2(p[n].v[e], p[n].v[e], tc::fma2(q[n].v[e], q[n].v[e], ss));
-        return rsqrtf(fmaf(group_sum(ss), a.inv_dim, a.eps));  // within 2 units of the last place
+            sum += mine[n] ? both(ss) : 0.f;
+        }
+        return rsqrtf(fmaf(group_sum(sum), a.inv_dim, a.eps));  // within 2 units of the last place
     }
 
     // A row of the group's, forward: from `x` to `out` where there is one.
@@ -392,9 +397,10 @@ struct Rot {
             load(x, x0, x1);
             const float r = rstd(x0, x1);
             const tc::Two rr = tc::two(r, r);
-            tc::Two dot = tc::two(0.f, 0.f);
+            float dots = 0.f;
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
+                tc::Two dot = tc::two(0.f, 0.f);
                 const Values<V> w0 = entries(sh.weights[k], n, 0), w1 = entries(sh.weights[k], n, V);
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
@@ -406,8 +412,9 @@ struct Rot {
                     p[n].v[e] = tc::mul2(p[n].v[e], w0.v[e]), q[n].v[e] = tc::mul2(q[n].v[e], w1.v[e]);
                     dot = tc::fma2(p[n].v[e], x0[n].v[e], tc::fma2(q[n].v[e], x1[n].v[e], dot));
                 }
+                dots += mine[n] ? both(dot) : 0.f;
             }
-            const float m = -group_sum(dot) * a.inv_dim;
+            const float m = -group_sum(dots) * a.inv_dim;
             const tc::Two mm = tc::two(m, m);
 #pragma unroll
             for (int n = 0; n < NV; ++n)
