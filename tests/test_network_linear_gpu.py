@@ -206,6 +206,13 @@ def test_linear_strides_and_shapes(dtype):
         got = _check(wide[:, start:start + 96], w, b, r, g, "silu")
         assert all(torch.equal(a, c) for a, c in zip(got, want))
         wide[:] = math.nan
+    for pitch, start in ((144, 8), (144, 32), (104, 0)):  # rows that copies reach, between what must not be read
+        wide = torch.full((120, pitch), math.nan, dtype=x.dtype, device="cuda")
+        wide[:, start:start + 96] = x
+        heavy = torch.full((136, pitch), math.nan, dtype=x.dtype, device="cuda")
+        heavy[:, start:start + 96] = w
+        got = _check(wide[:, start:start + 96], heavy[:, start:start + 96], b, r, g, "silu")
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
     got = _check(x.view(2, 5, 12, 96), w, b, r.view(2, 5, 12, 136), g.view(2, 5, 12, 136), "silu")
     assert got[0].shape == (2, 5, 12, 136) and got[2].shape == (2, 5, 12, 96)
     _check(x.t().contiguous().t(), w.t().contiguous().t(), b, r[:1].expand(120, -1), g[:, :1].expand(-1, 136), "silu")
@@ -390,3 +397,32 @@ def test_linear_refusals():
               lambda: network.linear_bwd(g.cpu(), x, w)):
         with pytest.raises(ValueError):
             f()
+
+
+def test_linear_beyond_32_bits():
+    """x of more than 2^31 values: its last rows, and all of them in the weight's gradient."""
+    import torch
+    from splatx_cuda import network
+    rows, k, n = 1_100_003, 2048, 24
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    w = (torch.randn(n, k, generator=gen, device="cuda") * k ** -0.5).bfloat16()
+    b = torch.randn(n, generator=gen, device="cuda")
+    y, _ = network.linear_fwd(x, w, b)
+    for part in (slice(0, 300), slice(rows // 2, rows // 2 + 300), slice(rows - 300, rows)):
+        X = x[part].double()
+        want = X @ w.double().T + b.double()
+        bound = _sums(k) * (X.abs() @ w.double().abs().T + b.double().abs()) + ROUND["bfloat16"] * want.abs()
+        _near("y", y[part], want, bound * (1 + 2.0 ** -7))
+    g = torch.zeros(rows, n, dtype=torch.bfloat16, device="cuda")
+    at = torch.tensor([0, 5, rows // 2, rows - 2, rows - 1], device="cuda")
+    g[at] = torch.randn(5, n, generator=gen, device="cuda").bfloat16()
+    v_x, v_w, v_b = network.linear_bwd(g, x, w, b)
+    G = g[at].double()
+    want = G.T @ x[at].double()
+    _near("v_weight", v_w, want, 2.0 ** -21 * (G.abs().T @ x[at].double().abs()) + ROUND["bfloat16"] * want.abs())
+    _near("v_bias", v_b, G.sum(0), 2.0 ** -21 * G.abs().sum(0))
+    want = G @ w.double()
+    _near("v_x", v_x[at], want, _sums(n) * (G.abs() @ w.double().abs()) + ROUND["bfloat16"] * want.abs())
+    v_x[at] = 0
+    assert not v_x.any()

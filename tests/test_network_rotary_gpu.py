@@ -339,6 +339,36 @@ def test_streams_graphs_and_repeats():
             assert all(torch.equal(a, b) for a, b in zip(o, v))
 
 
+def test_many_batches_of_one_token():
+    """More warps than a batch entry has tokens, by far; and a token's many heads cut into units."""
+    q, k, pos, w, g = _inputs(12, 9000, 1, 4, 2, 64, 2, "bfloat16")
+    _check(q, k, pos, w, g, (32, 32))
+    q, k, pos, w, g = _inputs(13, 5000, 2, 1, 1, 16, 1, "float32")
+    _check(q, k, pos, w, g, (16,))
+    q, k, pos, w, g = _inputs(14, 2, 3000, 70, 50, 32, 2, "bfloat16")
+    _check(q, k, pos, w, g, (16, 16))
+    q, k, pos, w, g = _inputs(15, 3, 1000, 40, 33, 128, 3, "float32")
+    _check(q, k, pos, w, g, (32, 48, 48), pairs="neighbours")
+
+
+def test_beyond_32_bits():
+    """Queries of more than 2^31 values: the last tokens are what they are by themselves."""
+    import torch
+    from splatx_cuda import network
+    n, h, d = 140_001, 128, 128
+    q = torch.empty(1, n, h, d, dtype=torch.bfloat16, device="cuda").normal_()
+    pos = torch.rand(1, n, 3, device="cuda") * 256
+    w = torch.rand(d, device="cuda") + 0.5
+    how = {"axes": (32, 48, 48), "q_weight": w}
+    out, _ = network.qk_norm_rotary_fwd(q, None, pos, **how)
+    for part in (slice(0, 50), slice(n - 50, n)):
+        assert torch.equal(out[:, part], network.qk_norm_rotary_fwd(q[:, part], None, pos[:, part], **how)[0])
+    v = network.qk_norm_rotary_bwd(out, None, q, None, pos, **how)
+    part = slice(n - 50, n)
+    assert torch.equal(v[0][:, part], network.qk_norm_rotary_bwd(out[:, part], None, q[:, part], None, pos[:, part], **how)[0])
+    assert bool(torch.isfinite(v[2]).all())
+
+
 def test_refusals():
     import torch
     from splatx_cuda import network
