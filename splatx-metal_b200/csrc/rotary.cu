@@ -11,8 +11,7 @@
 // needs no other lane, and 16-byte accesses where the pairs' layout allows them (V = 8 values of 16 bits).
 // A warp takes one token at a time, its queries and then its keys: its lanes make the token's sines and
 // cosines once for all heads, in shared memory, in the order in which lanes read them; the weights lie there
-// in the same way. Groups of a warp read the same entries at the same time, so that a read is one pass of
-// shared memory. The token's rows come to shared memory by bulk copies, while other warps work on theirs,
+// in the same way. The token's rows come to shared memory by bulk copies, while other warps work on theirs,
 // and leave from their place there by bulk copies: the loops then have no addresses of memory and no
 // registers for rows on their way. Rows that such copies do not reach (16 bytes) are read and written value by
 // value.

@@ -2,7 +2,8 @@
 
 ``CudaBackend`` mirrors ``KernelBackend`` (per-kernel verification surface), ``TrainStepExecutor``
 mirrors the resident step executor; both call libsplatx_cuda.so through include/splatx_cuda.h.
-``network`` has the operators of a network beside the splats (attention, layer norm, AdamW).
+``network`` has the operators of a network beside the splats (attention, linear layers, norm and rotation
+of queries and keys, layer norm, AdamW).
 """
 from .build import build, lib_path  # noqa: F401
 
