@@ -104,7 +104,7 @@ __device__ __forceinline__ void linear_biases(const LinearProduct& p, int64_t co
 }
 
 template <int TILE>
-__global__ void __launch_bounds__(kThreads<TILE>, TILE == 128 ? 2 : 8) linear_kernel(const __grid_constant__ LinearProduct p, bool a_wide, bool b_wide) {
+__global__ void __launch_bounds__(kThreads<TILE>, TILE == 128 ? 2 : 6) linear_kernel(const __grid_constant__ LinearProduct p, bool a_wide, bool b_wide) {
     constexpr int kSide = TILE / 8, kHalf = TILE / 2, kPitch = TILE + 4;
     __shared__ __align__(16) float smem[2][2][kDepth][kPitch];  // of A, of B; twice
     const int tx = threadIdx.x % kSide, ty = threadIdx.x / kSide;
@@ -241,7 +241,7 @@ namespace {
 LinearPlan product_plan(int32_t dtype, int64_t m, int64_t n, int64_t k) {
     if (dtype != SXCUDA_F32) return linear_tc_plan(m, n, k);
     const int64_t sms = sm_count(), large = (m + 127) / 128 * ((n + 127) / 128);
-    return large >= sms ? linear_plan(m, n, k, 128, 128, kDepth, sms * 2, 8, 32) : linear_plan(m, n, k, 64, 64, kDepth, sms * 8, 4, 12);
+    return large >= sms ? linear_plan(m, n, k, 128, 128, kDepth, sms * 2, 8, 32) : linear_plan(m, n, k, 64, 64, kDepth, sms * 6, 4, 12);
 }
 
 void launch_product(const LinearProduct& p, cudaStream_t s) {
