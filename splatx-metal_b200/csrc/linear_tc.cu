@@ -617,8 +617,8 @@ bool linear_tc_takes(const void* data, int64_t stride, int64_t rows) {
     return reinterpret_cast<uintptr_t>(data) % 16 == 0 && (rows <= 1 || (stride % 8 == 0 && stride < (1ll << 38)));
 }
 
-// Tiles of 256 or of 128 columns, cut or not: by what they take. Measured on a pair of CTAs: 64 values of K 0.27 and
-// 0.155 us (the tensor cores' rate, and 0.87 of it), an epilogue that nothing hides 3.1 and 1.6 us, a cut (the parts'
+// Tiles of 256 or of 128 columns, cut or not: by what they take. Measured with all pairs at work: 64 values of K 0.38 and
+// 0.23 us, an epilogue that nothing hides 3.1 and 1.6 us, a cut (the parts'
 // way through memory and the second kernel) some 6 us. 5001 x 333 x 777 with a residual, 128 and 256: 25 and 37 us.
 LinearPlan linear_tc_plan(int64_t m, int64_t n, int64_t k) {
     const int64_t pairs = sm_count() / 2;
@@ -627,10 +627,10 @@ LinearPlan linear_tc_plan(int64_t m, int64_t n, int64_t k) {
         const int64_t turns = (p.whole + pairs - 1) / pairs;
         return static_cast<double>(turns) * tile + (p.cut() ? static_cast<double>(p.share) * block + 6. : 0.);
     };
-    const LinearPlan narrow = linear_plan(m, n, k, kTileM, 128, kDepth, pairs, 4, 39);
+    const LinearPlan narrow = linear_plan(m, n, k, kTileM, 128, kDepth, pairs, 4, 26);
     if (n <= 128) return narrow;
-    const LinearPlan wide = linear_plan(m, n, k, kTileM, 256, kDepth, pairs, 4, 23);
-    return time(narrow, 0.155, 1.6) < time(wide, 0.27, 3.1) ? narrow : wide;
+    const LinearPlan wide = linear_plan(m, n, k, kTileM, 256, kDepth, pairs, 4, 16);
+    return time(narrow, 0.23, 1.6) < time(wide, 0.38, 3.1) ? narrow : wide;
 }
 
 void launch_linear_tc(const LinearProduct& p, cudaStream_t s) {
