@@ -103,12 +103,26 @@ __device__ __forceinline__ void linear_biases(const LinearProduct& p, int64_t co
     for (int i = 0; i < N; ++i) bias[i] = i < n ? linear_param(p.bias, p.bias_dtype, col + i) : 0.f;
 }
 
-template <int TILE>
-__global__ void __launch_bounds__(kThreads<TILE>, TILE == 128 ? 2 : 6) linear_kernel(const __grid_constant__ LinearProduct p, bool a_wide, bool b_wide) {
+// A launch's one product, or the backward's two, which have nothing to wait for in one another: small ones fill the
+// SMs better together. Backward calls with two launches and with one, us: 604 x 77 x 913 35 and 26, 300 x 256 x 256 with
+// relu 26 and 17, 2048 x 128 x 512 with gelu 42 and 35. A kernel that finds its product at run time is slower
+// (forward 2048 x 128 x 512: 19 and 25), so one product has a kernel of its own.
+template <int N>
+struct LinearProducts {
+    LinearProduct p[N];
+    bool a_wide[N], b_wide[N];  // rows are read 16 bytes at a time
+};
+
+template <int TILE, int N>
+__global__ void __launch_bounds__(kThreads<TILE>, TILE == 128 ? 2 : 6) linear_kernel(const __grid_constant__ LinearProducts<N> of) {
+    const int32_t first = N == 2 ? of.p[0].plan.workers : 0, block = static_cast<int32_t>(blockIdx.x);
+    const int which = N == 2 && block >= first;
+    const LinearProduct& p = of.p[which];
+    const bool a_wide = of.a_wide[which], b_wide = of.b_wide[which];
     constexpr int kSide = TILE / 8, kHalf = TILE / 2, kPitch = TILE + 4;
     __shared__ __align__(16) float smem[2][2][kDepth][kPitch];  // of A, of B; twice
     const int tx = threadIdx.x % kSide, ty = threadIdx.x / kSide;
-    LinearWalk walk(p.plan, blockIdx.x);
+    LinearWalk walk(p.plan, which ? block - first : block);
     LinearPiece piece;
     while (walk.next(p.plan, piece)) {
         const LinearTile tile = linear_tile(p.plan, piece.tile);
@@ -177,11 +191,14 @@ __global__ void __launch_bounds__(kThreads<TILE>, TILE == 128 ? 2 : 6) linear_ke
 }
 
 // Adds the parts of the tiles that are cut, in the order of K, and finishes them. A thread has 8 columns of
-// a row; blockIdx.y is the tile's number among them.
-template <typename T>
-__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinearProduct p) {
+// a row; blockIdx.y is the tile's number among them, blockIdx.z the product.
+template <typename T, int N>
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinearProducts<N> of) {
+    const LinearProduct& p = of.p[N == 2 ? blockIdx.z : 0];
     const LinearPlan& plan = p.plan;
-    const int32_t t = static_cast<int32_t>(blockIdx.y), parts = plan.parts(t);
+    const int32_t t = static_cast<int32_t>(blockIdx.y);
+    if (N == 2 && t >= plan.rest) return;
+    const int32_t parts = plan.parts(t);
     const LinearTile tile = linear_tile(plan, plan.whole + t);
     const int64_t m0 = static_cast<int64_t>(tile.m) * plan.tile_m, n0 = static_cast<int64_t>(tile.n) * plan.tile_n;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.tile_m), p.m - m0)), groups = plan.tile_n / 8;
@@ -244,19 +261,42 @@ LinearPlan product_plan(int32_t dtype, int64_t m, int64_t n, int64_t k) {
     return large >= sms ? linear_plan(m, n, k, 128, 128, kDepth, sms * 2, 8, 32) : linear_plan(m, n, k, 64, 64, kDepth, sms * 6, 4, 12);
 }
 
+template <int N>
+LinearProducts<N> products_of(const LinearProduct (&p)[N]) {
+    LinearProducts<N> of;
+    for (int i = 0; i < N; ++i) of.p[i] = p[i], of.a_wide[i] = linear_wide(p[i].a, 4), of.b_wide[i] = linear_wide(p[i].b, 4);
+    return of;
+}
+template <typename T, int N>
+void launch_join(const LinearProducts<N>& of, cudaStream_t s) {
+    int64_t units = 0, rest = 0;
+    for (const LinearProduct& p : of.p) {
+        if (!p.plan.cut()) continue;
+        units = std::max(units, (std::min<int64_t>(p.m, p.plan.tile_m) + 7) / 8 * (p.plan.tile_n / 32));
+        rest = std::max<int64_t>(rest, p.plan.rest);
+    }
+    const auto join = linear_join_kernel<T, N>;
+    if (rest) SX_LAUNCH(join, dim3(blocks_for(units, 8), static_cast<unsigned>(rest), N), 256, 0, s, of);
+}
+
 void launch_product(const LinearProduct& p, cudaStream_t s) {
-    const auto run = [&](auto kernel, int threads) {
-        SX_LAUNCH(kernel, static_cast<unsigned>(p.plan.workers), threads, 0, s, p, linear_wide(p.a, 4), linear_wide(p.b, 4));
-    };
+    const LinearProducts<1> of = products_of({p});
+    const auto run = [&](auto kernel, int threads) { SX_LAUNCH(kernel, static_cast<unsigned>(p.plan.workers), threads, 0, s, of); };
     if (p.dtype != SXCUDA_F32) launch_linear_tc(p, s);
-    else if (p.plan.tile_m == 128) run(linear_kernel<128>, kThreads<128>);
-    else run(linear_kernel<64>, kThreads<64>);
-    if (!p.plan.cut()) return;
-    by_dtype(p.dtype, [&](auto t) {
-        const auto join = linear_join_kernel<decltype(t)>;
-        const int64_t rows = std::min<int64_t>(p.m, p.plan.tile_m);
-        SX_LAUNCH(join, dim3(blocks_for((rows + 7) / 8 * (p.plan.tile_n / 32), 8), static_cast<unsigned>(p.plan.rest)), 256, 0, s, p);
-    });
+    else if (p.plan.tile_m == 128) run(linear_kernel<128, 1>, kThreads<128>);
+    else run(linear_kernel<64, 1>, kThreads<64>);
+    by_dtype(p.dtype, [&](auto t) { launch_join<decltype(t)>(of, s); });
+}
+
+// Two products of which neither reads what the other writes, each with memory of its own for its parts.
+bool go_together(const LinearProduct& a, const LinearProduct& b) {
+    return a.dtype == SXCUDA_F32 && a.plan.tile_m == 64 && b.plan.tile_m == 64;
+}
+void launch_together(const LinearProduct (&p)[2], cudaStream_t s) {
+    const LinearProducts<2> of = products_of(p);
+    const auto kernel = linear_kernel<64, 2>;
+    SX_LAUNCH(kernel, static_cast<unsigned>(p[0].plan.workers + p[1].plan.workers), kThreads<64>, 0, s, of);
+    launch_join<float>(of, s);
 }
 
 // ---- a few rows ----
@@ -441,7 +481,7 @@ SlopePlan slope_plan(const SxLinearInputs& in, const SxLinearGradsIn& g) {
 struct BwdSpace {
     Matrix x, weight, v_y;
     bool v_z = false;  // made
-    size_t x_at = 0, weight_at = 0, v_z_at = 0, sums_at = 0, parts_at = 0, bytes = 0;
+    size_t x_at = 0, weight_at = 0, v_z_at = 0, sums_at = 0, parts_at[2] = {}, bytes = 0;
     BwdSpace(const SxLinearInputs& in, const SxLinearGradsIn& g, const SxLinearGrads& out)
         : x{in.x, in.x_stride, in.rows, in.in_features}, weight{in.weight, in.weight_stride, in.out_features, in.in_features},
           v_y{g.v_y, g.v_y_stride, in.rows, in.out_features} {
@@ -455,10 +495,8 @@ struct BwdSpace {
         if (out.v_weight) take(x_at, x.bytes(in.dtype));
         if (out.v_x) take(weight_at, weight.bytes(in.dtype));
         if (out.v_bias) take(sums_at, static_cast<size_t>(slope_plan(in, g).slices) * in.out_features * 4);
-        size_t parts = 0;
-        if (out.v_x) parts = product_plan(in.dtype, in.rows, in.in_features, in.out_features).workspace();
-        if (out.v_weight) parts = std::max(parts, product_plan(in.dtype, in.out_features, in.in_features, in.rows).workspace());
-        take(parts_at, parts);
+        if (out.v_x) take(parts_at[0], product_plan(in.dtype, in.rows, in.in_features, in.out_features).workspace());
+        if (out.v_weight) take(parts_at[1], product_plan(in.dtype, in.out_features, in.in_features, in.rows).workspace());
     }
 };
 
@@ -524,25 +562,32 @@ void launch_linear_bwd(const SxLinearInputs& in, const SxLinearGradsIn& g, const
         if (a.sums)
             SX_LAUNCH(linear_bias_kernel, blocks_for(in.out_features, 32), 1024, 0, s, a.sums, plan.slices, in.out_features, out.v_bias, in.bias_dtype);
     }
-    LinearProduct p{};
-    p.dtype = in.dtype;
-    p.parts = reinterpret_cast<float*>(at + space.parts_at);
+    LinearProduct products[2]{};
+    auto& [p, w] = products;
     if (out.v_x) {
         p.a = v_z.along_k();
         p.b = space.weight.ready(in.dtype, at + space.weight_at, s).across_k();
         p.m = in.rows, p.n = in.in_features, p.k = in.out_features;
         p.y = out.v_x, p.y_stride = out.v_x_stride;
-        p.plan = product_plan(in.dtype, p.m, p.n, p.k);
-        launch_product(p, s);
     }
     if (out.v_weight) {
-        p.a = v_z.across_k();
-        p.b = space.x.ready(in.dtype, at + space.x_at, s).across_k();
-        p.m = in.out_features, p.n = in.in_features, p.k = in.rows;
-        p.y = out.v_weight, p.y_stride = out.v_weight_stride;
-        p.plan = product_plan(in.dtype, p.m, p.n, p.k);
-        launch_product(p, s);
+        w.a = v_z.across_k();
+        w.b = space.x.ready(in.dtype, at + space.x_at, s).across_k();
+        w.m = in.out_features, w.n = in.in_features, w.k = in.rows;
+        w.y = out.v_weight, w.y_stride = out.v_weight_stride;
     }
+    for (LinearProduct& each : products) {
+        if (!each.y) continue;
+        each.dtype = in.dtype;
+        each.parts = reinterpret_cast<float*>(at + space.parts_at[&each - products]);
+        each.plan = product_plan(in.dtype, each.m, each.n, each.k);
+    }
+    if (p.y && w.y && go_together(p, w)) {
+        launch_together(products, s);
+        return;
+    }
+    for (const LinearProduct& each : products)
+        if (each.y) launch_product(each, s);
 }
 
 }  // namespace sx
