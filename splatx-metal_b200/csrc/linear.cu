@@ -105,7 +105,7 @@ __device__ __forceinline__ void linear_biases(const LinearProduct& p, int64_t co
 
 // A launch's one product, or the backward's two, which have nothing to wait for in one another: small ones fill the
 // SMs better together. Backward calls with two launches and with one, us: 604 x 77 x 913 35 and 26, 300 x 256 x 256 with
-// relu 26 and 17, 2048 x 128 x 512 with gelu 42 and 35. A kernel that finds its product at run time is slower
+// relu 26 and 17, 2048 x 128 x 512 with gelu 42 and 35 (with one launch for the joins). A kernel that finds its product at run time is slower
 // (forward 2048 x 128 x 512: 19 and 25), so one product has a kernel of its own.
 template <int N>
 struct LinearProducts {
@@ -190,10 +190,15 @@ __global__ void __launch_bounds__(kThreads<TILE>, TILE == 128 ? 2 : 6) linear_ke
     }
 }
 
-// Adds the parts of the tiles that are cut, in the order of K, and finishes them. A thread has 8 columns of
-// a row; blockIdx.y is the tile's number among them, blockIdx.z the product.
-template <typename T, int N>
-__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ LinearProducts<N> of) {
+// Adds the parts of the tiles that are cut, in an order of K that the sizes alone decide, and finishes them. A unit
+// is 8 rows by 32 columns, 256 bytes of a part side by side and 64 of a row of y, a lane's 8 columns of a row.
+// blockIdx.y is the tile's number among those that are cut, blockIdx.z the product. With few parts of many tiles
+// each warp adds a unit; where a tile has many, W = 8 or 32 warps share one, every W-th part each (backward calls with
+// one warp a unit and with this, us: float32 20000 x 64 x 64, 313 parts, 57 and 31, 40000 x 3 x 64 105 and 47; bf16
+// 40000 x 256 x 256 with gelu 65 and 55).
+constexpr int join_warps(int w) { return w == 1 ? 8 : w; }
+template <typename T, int N, int W>
+__global__ void __launch_bounds__(32 * join_warps(W)) linear_join_kernel(const __grid_constant__ LinearProducts<N> of) {
     const LinearProduct& p = of.p[N == 2 ? blockIdx.z : 0];
     const LinearPlan& plan = p.plan;
     const int32_t t = static_cast<int32_t>(blockIdx.y);
@@ -202,19 +207,35 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
     const LinearTile tile = linear_tile(plan, plan.whole + t);
     const int64_t m0 = static_cast<int64_t>(tile.m) * plan.tile_m, n0 = static_cast<int64_t>(tile.n) * plan.tile_n;
     const int rows = static_cast<int>(min(static_cast<int64_t>(plan.tile_m), p.m - m0)), groups = plan.tile_n / 8;
-    // a warp has 8 rows and 4 times 8 columns: 256 bytes of a part side by side, 64 of a row of y
-    const int at = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int warp = static_cast<int>(threadIdx.x) >> 5, lane = static_cast<int>(threadIdx.x) & 31;
+    const int at = W == 1 ? static_cast<int>(blockIdx.x) * 8 + warp : static_cast<int>(blockIdx.x);
     const int row = at / (groups / 4) * 8 + lane % 8, col = (at % (groups / 4) * 4 + lane / 8) * 8;
     const int64_t n = min(p.n - n0 - col, static_cast<int64_t>(8));
-    if (row >= rows || n <= 0) return;
+    const bool here = row < rows && n > 0;
     float z[8] = {};
+    if (here) {
 #pragma unroll 4
-    for (int i = 0; i < parts; ++i) {
-        const float4* part = reinterpret_cast<const float4*>(linear_part(p, t * plan.slots + i, row, col));
-        const float4 x = part[0], y = part[1];
-        z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w;
-        z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
+        for (int i = W == 1 ? 0 : warp; i < parts; i += W) {
+            const float4* part = reinterpret_cast<const float4*>(linear_part(p, t * plan.slots + i, row, col));
+            const float4 x = part[0], y = part[1];
+            z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w;
+            z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
+        }
     }
+    if constexpr (W > 1) {
+        __shared__ float4 sums[W][2][32];
+        sums[warp][0][lane] = make_float4(z[0], z[1], z[2], z[3]);
+        sums[warp][1][lane] = make_float4(z[4], z[5], z[6], z[7]);
+        __syncthreads();
+        if (warp) return;
+#pragma unroll 4
+        for (int w = 1; w < W; ++w) {
+            const float4 x = sums[w][0][lane], y = sums[w][1][lane];
+            z[0] += x.x, z[1] += x.y, z[2] += x.z, z[3] += x.w;
+            z[4] += y.x, z[5] += y.y, z[6] += y.z, z[7] += y.w;
+        }
+    }
+    if (!here) return;
     float bias[8];
     linear_biases(p, n0 + col, static_cast<int>(n), bias);
     linear_finish<T, 8>(p, m0 + row, n0 + col, z, bias, static_cast<int>(n));
@@ -267,22 +288,41 @@ LinearPlan product_plan(int32_t dtype, int64_t m, int64_t n, int64_t k) {
     return large ? linear_plan(m, n, k, 128, 128, kDepth, sms * 2, 8, 32) : linear_plan(m, n, k, 64, 64, kDepth, sms * 6, 4, 12);
 }
 
+int64_t join_units(const LinearProduct& p) { return (std::min<int64_t>(p.m, p.plan.tile_m) + 7) / 8 * (p.plan.tile_n / 32); }
+int join_share(const LinearProduct& p) {
+    if (p.plan.slots < 16) return 1;
+    return p.plan.slots >= 64 && join_units(p) * p.plan.rest <= 128 ? 32 : 8;
+}
+
 template <int N>
 LinearProducts<N> products_of(const LinearProduct (&p)[N]) {
     LinearProducts<N> of;
     for (int i = 0; i < N; ++i) of.p[i] = p[i], of.a_wide[i] = linear_wide(p[i].a, 4), of.b_wide[i] = linear_wide(p[i].b, 4);
     return of;
 }
+// Two products are joined by one launch where they are joined alike. Otherwise they have one each: for the sums not to
+// depend on whether the other product is asked for, and as warps without a part cost more (3000 x 256 x 256 backward, one
+// launch of warps with and without parts 52 us, two 41).
 template <typename T, int N>
 void launch_join(const LinearProducts<N>& of, cudaStream_t s) {
-    int64_t units = 0, rest = 0;
-    for (const LinearProduct& p : of.p) {
-        if (!p.plan.cut()) continue;
-        units = std::max(units, (std::min<int64_t>(p.m, p.plan.tile_m) + 7) / 8 * (p.plan.tile_n / 32));
-        rest = std::max<int64_t>(rest, p.plan.rest);
+    if constexpr (N == 2) {
+        if (!of.p[0].plan.cut() || !of.p[1].plan.cut() || join_share(of.p[0]) != join_share(of.p[1])) {
+            for (const LinearProduct& p : of.p) launch_join<T>(products_of({p}), s);
+            return;
+        }
     }
-    const auto join = linear_join_kernel<T, N>;
-    if (rest) SX_LAUNCH(join, dim3(blocks_for(units, 8), static_cast<unsigned>(rest), N), 256, 0, s, of);
+    int64_t units = 0, rest = 0;
+    for (const LinearProduct& p : of.p) units = std::max(units, join_units(p)), rest = std::max<int64_t>(rest, p.plan.rest);
+    if (!rest) return;
+    const auto run = [&](auto warps) {
+        constexpr int W = decltype(warps)::value;
+        const auto join = linear_join_kernel<T, N, W>;
+        SX_LAUNCH(join, dim3(blocks_for(units, W == 1 ? 8 : 1), static_cast<unsigned>(rest), N), 32 * join_warps(W), 0, s, of);
+    };
+    const int share = join_share(of.p[0]);
+    if (share == 32) run(std::integral_constant<int, 32>{});
+    else if (share == 8) run(std::integral_constant<int, 8>{});
+    else run(std::integral_constant<int, 1>{});
 }
 
 void launch_product(const LinearProduct& p, cudaStream_t s) {
@@ -309,8 +349,8 @@ void launch_together(const LinearProduct (&p)[2], cudaStream_t s) {
 // A warp has an output feature: its lanes go along the weight's row, V values at a time, and each of up to ROWS
 // rows of x has a sum. The weight is read once, by as many warps as there are features; a product on the tensor
 // cores needs its parts of K joined to read it as widely. 1024 -> 4096 features, this and the tiles, in us: bf16
-// 1 row 3.6 and 12, 4 rows 5.6 and 10, 8 rows 9.3 and 10 (4096 -> 4096: 24 and 19); float32 1 row 4.5 and 27, 8
-// rows 12 and 27.
+// 1 row 3.4 and 12, 4 rows 5.2 and 12, 8 rows 9.3 and 9.5 (4096 -> 4096: 24 and 18); float32 1 row 3.7 and 23, 8
+// rows 11 and 24.
 constexpr int few_rows_of(int32_t dtype) { return dtype == SXCUDA_F32 ? 8 : 4; }
 template <typename T, int V, int ROWS>
 __global__ void __launch_bounds__(128) linear_few_kernel(const __grid_constant__ LinearProduct p) {

@@ -426,3 +426,23 @@ def test_linear_beyond_32_bits():
     _near("v_x", v_x[at], want, _sums(n) * (G.abs() @ w.double().abs()) + ROUND["bfloat16"] * want.abs())
     v_x[at] = 0
     assert not v_x.any()
+
+
+# float32 in tiles of 128 that are cut along K, forward and in the gradient of x beside one of 64; weight gradients
+# of few features and many rows, whose tiles have tens to hundreds of parts.
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("size", [(9700, 700, 1020), (9701, 1019, 701), (30001, 64, 3), (30001, 3, 64), (60000, 48, 64),
+                                  (3000, 256, 256), (604, 77, 913)], ids=name)
+def test_linear_many_parts(size, dtype):
+    x, w, b, r, g = _inputs(31, *size, dtype, residual=True)
+    first = _check(x, w, b, r, g, "gelu")
+    again = _check(x, w, b, r, g, "gelu")
+    for a, c in zip(first, again):
+        assert (a == c).all()
+    from splatx_cuda import network
+    v_x, v_w, v_b = first[2:]
+    for needs_x, needs_weight in ((True, False), (False, True)):  # either product without the other
+        one = network.linear_bwd(g, x, w, b, first[1], activation="gelu", needs_x=needs_x, needs_weight=needs_weight)
+        assert (one[0] is None) != needs_x and (one[1] is None) != needs_weight
+        assert (one[2] == v_b).all()
+        assert all((a == c).all() for a, c in zip(one[:2], (v_x, v_w)) if a is not None)
