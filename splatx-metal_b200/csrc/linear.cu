@@ -105,8 +105,8 @@ __device__ __forceinline__ void linear_biases(const LinearProduct& p, int64_t co
 
 // A launch's one product, or the backward's two, which have nothing to wait for in one another: small ones fill the
 // SMs better together. Backward calls with two launches and with one, us: 604 x 77 x 913 35 and 26, 300 x 256 x 256 with
-// relu 26 and 17, 2048 x 128 x 512 with gelu 42 and 35 (with one launch for the joins). A kernel that finds its product at run time is slower
-// (forward 2048 x 128 x 512: 19 and 25), so one product has a kernel of its own.
+// relu 26 and 17, 2048 x 128 x 512 with gelu 42 and 35 (with one launch for the joins). A kernel that finds its product
+// at run time is slower (forward 2048 x 128 x 512: 19 and 25), so one product has a kernel of its own.
 template <int N>
 struct LinearProducts {
     LinearProduct p[N];

@@ -618,8 +618,8 @@ bool linear_tc_takes(const void* data, int64_t stride, int64_t rows) {
 }
 
 // Tiles of 256 or of 128 columns, cut or not: by what they take. Measured with all pairs at work: 64 values of K 0.38 and
-// 0.23 us, an epilogue that nothing hides 3.1 and 1.6 us, a cut (the parts'
-// way through memory and the second kernel) some 6 us. 5001 x 333 x 777 with a residual, 128 and 256: 25 and 37 us.
+// 0.23 us, an epilogue that nothing hides 3.1 and 1.6 us, a cut (the parts' way through memory and the second
+// kernel) some 6 us. 5001 x 333 x 777 with a residual, 128 and 256: 25 and 37 us.
 LinearPlan linear_tc_plan(int64_t m, int64_t n, int64_t k) {
     const int64_t pairs = sm_count() / 2;
     const auto time = [&](const LinearPlan& p, double block, double least) {
