@@ -928,7 +928,8 @@ typedef struct SxLinearInputs {
 /* residual: [rows, out_features] of dtype, or NULL. y and pre (x weight^T + bias before the activation,
  * which the backward of an activation reads; NULL where that is not wanted): [rows, out_features] of
  * dtype. residual may be y itself. Workspace query protocol (the size may be 0; a non-NULL workspace
- * pointer is then not read); x's and weight's addresses and strides count for the size. */
+ * pointer is then not read); x's and weight's addresses and strides count for the size. The workspace starts
+ * on 32 bytes for 16-bit types and on 16 for float32. */
 typedef struct SxLinearOutputs {
     const void* residual;
     int64_t residual_stride;
@@ -957,7 +958,7 @@ typedef struct SxLinearGrads {
 
 /* v_z = v_y act'(pre), held in dtype; v_x = v_z weight, v_weight = v_z^T x, v_bias = the sum of v_z over
  * the rows before v_z is rounded. Sums in a fixed order: the result is the same in every call. Workspace query
- * protocol; the query reads gin and out, too. */
+ * protocol, aligned as the forward's; the query reads gin and out, too. */
 int32_t sxcuda_linear_bwd(const SxLinearInputs* in, const SxLinearGradsIn* gin, const SxLinearGrads* out,
                           void* workspace, size_t* workspace_bytes, sxcuda_stream_t stream);
 

@@ -270,6 +270,13 @@ void validate_linear(const SxLinearInputs* in, const char* w) {
     if (in->bias) validate_pointer(in->bias, in->bias_dtype, w, "bias");
 }
 
+// Before anything is launched on it: the parts of 16-bit tiles that are cut along K are stored 32 bytes at a time.
+void validate_linear_workspace(const void* ws, const size_t* bytes, int32_t dtype, const char* w) {
+    const int align = dtype == SXCUDA_F32 ? 16 : 32;
+    if (ws && bytes && *bytes && reinterpret_cast<uintptr_t>(ws) % align != 0)
+        throw_invalid(w, "workspace must be " + std::to_string(align) + "-byte aligned");
+}
+
 void validate_head_view(const SxAttentionView& v, const SxRotaryInputs& in, int32_t heads, bool written, const char* w, const char* what) {
     if (in.batch == 0 || in.tokens == 0 || heads == 0) return;
     validate_pointer(v.data, in.dtype, w, what);
@@ -1201,12 +1208,12 @@ int32_t sxcuda_linear_fwd(const SxLinearInputs* in, const SxLinearOutputs* out, 
     return guarded([&] {
         const char* w = "linear_fwd";
         validate_linear(in, w);
+        validate_linear_workspace(ws, ws_bytes, in->dtype, w);
         if (workspace_query(ws, ws_bytes, linear_fwd_workspace(*in), w)) return;
         if (!out) throw_invalid(w, "null outputs");
         validate_matrix(out->y, out->y_stride, in->rows, in->out_features, in->dtype, w, "y");
         if (out->pre) validate_matrix(out->pre, out->pre_stride, in->rows, in->out_features, in->dtype, w, "pre");
         if (out->residual) validate_matrix(out->residual, out->residual_stride, in->rows, in->out_features, in->dtype, w, "residual");
-        if (*ws_bytes && reinterpret_cast<uintptr_t>(ws) % 16 != 0) throw_invalid(w, "workspace must be 16-byte aligned");
         launch_linear_fwd(*in, *out, ws, as_stream(stream));
     });
 }
@@ -1224,8 +1231,8 @@ int32_t sxcuda_linear_bwd(const SxLinearInputs* in, const SxLinearGradsIn* g, co
         if (out->v_x) validate_matrix(out->v_x, out->v_x_stride, in->rows, in->in_features, in->dtype, w, "v_x");
         if (out->v_weight) validate_matrix(out->v_weight, out->v_weight_stride, in->out_features, in->in_features, in->dtype, w, "v_weight");
         if (out->v_bias) validate_pointer(out->v_bias, in->bias_dtype, w, "v_bias");
+        validate_linear_workspace(ws, ws_bytes, in->dtype, w);
         if (workspace_query(ws, ws_bytes, linear_bwd_workspace(*in, *g, *out), w)) return;
-        if (*ws_bytes && reinterpret_cast<uintptr_t>(ws) % 16 != 0) throw_invalid(w, "workspace must be 16-byte aligned");
         launch_linear_bwd(*in, *g, *out, ws, as_stream(stream));
     });
 }
