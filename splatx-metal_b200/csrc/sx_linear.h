@@ -199,7 +199,7 @@ template <int ACT>
 __device__ __forceinline__ float act_fast(float z) {
     if constexpr (ACT == SXCUDA_ACT_RELU) return z < 0.f ? 0.f : z;
     if constexpr (ACT == SXCUDA_ACT_SILU) return z * gate_fast(z);
-    if constexpr (ACT == SXCUDA_ACT_GELU) return z * normal_fast(z);
+    if constexpr (ACT == SXCUDA_ACT_GELU) return fmaxf(z, -64.f) * normal_fast(z);  // -inf gives its limit, as in act_pair
     if constexpr (ACT == SXCUDA_ACT_GELU_TANH) return z * gate_fast(tanh_gate_at(z));
     return z;
 }

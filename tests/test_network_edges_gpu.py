@@ -1,0 +1,35 @@
+"""Linear layers and the rotation where a call's plan, a value that is not finite or a caller's own list must not
+decide the answer."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+# one row and few rows; tiles that are cut along K; whole tiles; results that copies do not reach, cut and whole
+PLANS = [(1, 64, 32), (4, 4096, 40), (5, 4096, 32), (300, 4096, 256), (300, 64, 256), (40, 64, 101), (40, 4096, 101),
+         (5, 64, 32)]
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("act", [None, "relu", "silu", "gelu", "gelu_tanh"])
+def test_infinite_pre_activations_in_every_plan(act, dtype):
+    """z of -inf gives the limit of relu and gelu and NaN of what is inf / inf, +inf and NaN stay, whichever kernel
+    ends the call; the other columns are what they are without them."""
+    import torch
+    from splatx_cuda import network
+    T = getattr(torch, dtype)
+    below = {None: -math.inf, "relu": 0.0, "gelu": 0.0}.get(act, math.nan)
+    for m, k, n in PLANS:
+        gen = torch.Generator().manual_seed(m + k)
+        x, w = torch.randn(m, k, generator=gen).to(T).cuda(), (torch.randn(n, k, generator=gen) * k ** -0.5).to(T).cuda()
+        b = torch.zeros(n, device="cuda")
+        want = network.linear_fwd(x, w, b, activation=act)[0]
+        b[3], b[8], b[n - 1] = -math.inf, math.inf, math.nan
+        y, pre = network.linear_fwd(x, w, b, activation=act, keep=True)
+        assert bool((pre[:, 3] == -math.inf).all()) and bool((pre[:, 8] == math.inf).all()) and bool(pre[:, n - 1].isnan().all())
+        assert bool(y[:, 3].isnan().all() if math.isnan(below) else (y[:, 3] == below).all()), (m, k, n)
+        assert bool((y[:, 8] == math.inf).all()) and bool(y[:, n - 1].isnan().all()), (m, k, n)
+        others = [i for i in range(n) if i not in (3, 8, n - 1)]
+        assert torch.equal(y[:, others], want[:, others]), (m, k, n)
