@@ -139,7 +139,7 @@ struct Rot {
     float* table;
     int lane, group, in_group, rows;  // rows: groups of a warp
     int first[NV], second[NV];        // where the slots are in a head; 0 where the slot is not the thread's own
-    bool mine[NV], pair[NV];
+    bool mine[NV], pair[NV], turned[NV];
 
     __device__ Rot(const RotArgs& a, RotShared& sh) : a(a), sh(sh), table(sh.angles[threadIdx.x >> 5]), lane(threadIdx.x & 31) {
         for (int i = threadIdx.x; i < a.pairs; i += kRotThreads) sh.turns[i] = a.turns[i], sh.axis[i] = a.axis[i];
@@ -157,6 +157,7 @@ struct Rot {
         for (int n = 0; n < NV; ++n) {
             const int slot = in_group + n * a.lanes;
             mine[n] = slot < a.slots;
+            turned[n] = slot * V < a.pairs;
             const Slot s = mine[n] ? slot_at<V>(a, slot) : Slot{0, 0};
             pair[n] = V > 1 || s.second >= 0;
             first[n] = s.first, second[n] = pair[n] ? s.second : 0;
@@ -364,7 +365,11 @@ struct Rot {
             }
         }
     }
-    // A row of the group's, forward: from `x` to `out` where there is one.
+    // A row of the group's, forward: from `x` to `out` where there is one. REST: the head has values that are not rotated,
+    // which are left out of the turn: times a sine of zero an infinite one would be NaN in a value that has no part in
+    // it. That costs 1 to 4% (4 x 8192 tokens, 16 (4) heads x 128, 96 of them rotated 64 -> 66 us, backward 105 -> 106), which
+    // heads that are rotated as a whole do not pay: a kernel each.
+    template <bool REST>
     __device__ __forceinline__ void forward(const T* x, T* out, const Turn& t, bool there) const {
         Values<V> p[NV], q[NV];
         load(x, p, q);
@@ -381,12 +386,15 @@ struct Rot {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const tc::Two x1 = p[n].v[e], x2 = q[n].v[e];
-                p[n].v[e] = tc::fma2(x1, t.a[n].v[e], tc::mul2(x2, t.b[n].v[e]));
-                q[n].v[e] = tc::fma2(x1, t.c[n].v[e], tc::mul2(x2, t.d[n].v[e]));
+                const tc::Two other = tc::mul2(x2, t.b[n].v[e]);
+                if (REST) p[n].v[e] = tc::mul2(x1, t.a[n].v[e]);
+                q[n].v[e] = tc::mul2(x2, t.d[n].v[e]);
+                if (!REST || turned[n]) p[n].v[e] = tc::fma2(x1, t.a[n].v[e], other), q[n].v[e] = tc::fma2(x1, t.c[n].v[e], q[n].v[e]);
             }
         if (there) store(out, p, q);
     }
     // The same backward, from the gradient `g` (and x, with norm) to `out`; adds to the weight's sums.
+    template <bool REST>
     __device__ __forceinline__ void backward(const T* x, const T* g, T* out, int k, bool there, Values<V> (&sum)[2][NV]) const {
         const tc::Two minus = tc::two(-1.f, -1.f);
         Values<V> p[NV], q[NV];
@@ -397,8 +405,8 @@ struct Rot {
 #pragma unroll
             for (int e = 0; e < N; ++e) {
                 const tc::Two g1 = p[n].v[e], g2 = q[n].v[e];
-                p[n].v[e] = tc::fma2(g1, c.v[e], tc::mul2(g2, s.v[e]));
-                q[n].v[e] = tc::fma2(g2, c.v[e], tc::mul2(tc::mul2(g1, minus), s.v[e]));
+                const tc::Two u1 = tc::fma2(g1, c.v[e], tc::mul2(g2, s.v[e])), u2 = tc::fma2(g2, c.v[e], tc::mul2(tc::mul2(g1, minus), s.v[e]));
+                if (!REST || turned[n]) p[n].v[e] = u1, q[n].v[e] = u2;
             }
         }
         if (a.norm) {
@@ -509,8 +517,8 @@ __global__ void __launch_bounds__(kRotThreads, kRotPerSm<1, BACK>) rotary_plain_
                 };
                 const T* x = row(h.x, h.x_batch, h.x_token, h.x_head);
                 T* out = const_cast<T*>(row(h.out, h.out_batch, h.out_token, h.out_head));
-                if constexpr (BACK) me.backward(x, row(h.g, h.g_batch, h.g_token, h.g_head), out, k, there, sum[k]);
-                else me.forward(x, out, turn, there);
+                if constexpr (BACK) me.template backward<true>(x, row(h.g, h.g_batch, h.g_token, h.g_head), out, k, there, sum[k]);
+                else me.template forward<true>(x, out, turn, there);
             }
         }
     }
@@ -526,7 +534,7 @@ __device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t byt
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
 }
 
-template <typename T, int V, bool NB, int NV, bool BACK>
+template <typename T, int V, bool NB, int NV, bool REST, bool BACK>
 __global__ void __launch_bounds__(kRotThreads, kRotPerSm<V, BACK>) rotary_kernel(const __grid_constant__ RotArgs a) {
     __shared__ RotShared sh;
     extern __shared__ __align__(128) uint8_t stages[];
@@ -626,8 +634,8 @@ __global__ void __launch_bounds__(kRotThreads, kRotPerSm<V, BACK>) rotary_kernel
             if (!BACK && run.n) me.turn_of(k, turn);
             for (int i = 0; i < run.n; i += me.rows, row += me.rows * a.dim) {
                 const bool there = i + me.group < run.n;
-                if constexpr (BACK) me.backward(row + a.stage / static_cast<int>(sizeof(T)), row, row, k, there, sum[k]);
-                else me.forward(row, row, turn, there);
+                if constexpr (BACK) me.template backward<REST>(row + a.stage / static_cast<int>(sizeof(T)), row, row, k, there, sum[k]);
+                else me.template forward<REST>(row, row, turn, there);
             }
         }
         send(here);
@@ -678,12 +686,16 @@ bool bulk_fits(const SxRotaryInputs& in, const SxAttentionView& x) {
     return in.head_dim * dtype_bytes(in.dtype) % 16 == 0 && view_fits(x, dtype_bytes(in.dtype), 16);
 }
 
+int rotated_values(const SxRotaryInputs& in) {
+    int n = 0;
+    for (int i = 0; i < in.axes; ++i) n += in.axis_dims[i];
+    return n;
+}
+
 // The most pairs a thread can take at once: runs of pairs, of their partners and of what is not rotated are
 // multiples of it.
 int most_pairs(const SxRotaryInputs& in) {
-    int pairs = 0;
-    for (int i = 0; i < in.axes; ++i) pairs += in.axis_dims[i] / 2;
-    const int rest = in.head_dim - 2 * pairs;
+    const int pairs = rotated_values(in) / 2, rest = in.head_dim - 2 * pairs;
     const auto holds = [&](int n) {
         if (rest % 2 || rest / 2 % n || pairs % n) return false;
         if (in.pairs == SXCUDA_PAIRS_AXIS)
@@ -755,21 +767,25 @@ int rot_launch(RotArgs& a, int64_t tokens, K kernel, int per_sm, int row_bytes, 
     return blocks;
 }
 
-// Calls f(element, pairs a thread, neighbours, slots a thread).
+// Calls f(element, pairs a thread, neighbours, slots a thread, values that are not rotated).
 template <typename F>
 void by_layout(const SxRotaryInputs& in, int v, F&& f) {
     by_dtype(in.dtype, [&](auto t) {
         using T = decltype(t);
+        const auto rest = [&](auto n, auto nb, auto slots) {
+            if (rotated_values(in) < in.head_dim) f(t, n, nb, slots, std::true_type{});
+            else f(t, n, nb, slots, std::false_type{});
+        };
         const auto order = [&](auto n, auto slots) {
-            if (in.pairs == SXCUDA_PAIRS_NEIGHBOURS) f(t, n, std::true_type{}, slots);
-            else f(t, n, std::false_type{}, slots);
+            if (in.pairs == SXCUDA_PAIRS_NEIGHBOURS) rest(n, std::true_type{}, slots);
+            else rest(n, std::false_type{}, slots);
         };
         // up to 256 values are 16, 32, 64 and 128 slots for 32 lanes
         if constexpr (sizeof(T) == 2)
             if (v == 8) return order(std::integral_constant<int, 8>{}, std::integral_constant<int, 1>{});
         if (v == 4) return order(std::integral_constant<int, 4>{}, std::integral_constant<int, 1>{});
         if (v == 2) return order(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
-        f(t, std::integral_constant<int, 1>{}, std::false_type{}, std::integral_constant<int, 4>{});  // no order within one
+        rest(std::integral_constant<int, 1>{}, std::false_type{}, std::integral_constant<int, 4>{});  // no order within one
     });
 }
 
@@ -786,9 +802,9 @@ void launch_qk_norm_rotary_fwd(const SxRotaryInputs& in, const SxAttentionView& 
     };
     set(a.half[0], q_out);
     if (in.k_heads) set(a.half[1], k_out);
-    by_layout(in, v, [&](auto t, auto n, auto nb, auto slots) {
+    by_layout(in, v, [&](auto t, auto n, auto nb, auto slots, auto rest) {
         using T = decltype(t);
-        if (bulk) rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, false>, kRotPerSm<decltype(n)::value, false>, row, 1, s, nullptr, false, false);
+        if (bulk) rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, decltype(rest)::value, false>, kRotPerSm<decltype(n)::value, false>, row, 1, s, nullptr, false, false);
         else if constexpr (decltype(n)::value == 1) rot_launch(a, tokens, rotary_plain_kernel<T, false>, kRotPerSm<1, false>, row, 0, s, nullptr, false, false);
     });
 }
@@ -819,12 +835,12 @@ void launch_qk_norm_rotary_bwd(const SxRotaryInputs& in, const SxRotaryGrads& g,
     };
     set(a.half[0], g.v_q_out, g.v_q);
     if (in.k_heads) set(a.half[1], g.v_k_out, g.v_k);
-    by_layout(in, v, [&](auto t, auto n, auto nb, auto slots) {
+    by_layout(in, v, [&](auto t, auto n, auto nb, auto slots, auto rest) {
         using T = decltype(t);
         float* part = static_cast<float*>(ws);
         int blocks = 0;
         if (bulk)
-            blocks = rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, true>, kRotPerSm<decltype(n)::value, true>, row, 2, s, part,
+            blocks = rot_launch(a, tokens, rotary_kernel<T, decltype(n)::value, decltype(nb)::value, decltype(slots)::value, decltype(rest)::value, true>, kRotPerSm<decltype(n)::value, true>, row, 2, s, part,
                                 g.v_q_weight, g.v_k_weight);
         else if constexpr (decltype(n)::value == 1)
             blocks = rot_launch(a, tokens, rotary_plain_kernel<T, true>, kRotPerSm<1, true>, row, 0, s, part, g.v_q_weight, g.v_k_weight);

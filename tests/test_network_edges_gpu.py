@@ -33,3 +33,34 @@ def test_infinite_pre_activations_in_every_plan(act, dtype):
         assert bool((y[:, 8] == math.inf).all()) and bool(y[:, n - 1].isnan().all()), (m, k, n)
         others = [i for i in range(n) if i not in (3, 8, n - 1)]
         assert torch.equal(y[:, others], want[:, others]), (m, k, n)
+
+
+# the last values of a head are not rotated: 16-byte accesses of 8, 4 and 2 pairs, and value by value
+@pytest.mark.parametrize("pairs", ["axis", "whole", "neighbours"])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("dim, axes", [(64, (16, 16)), (64, (24, 16)), (48, (20, 20)), (40, (2, 4)), (37, (8, 6))])
+def test_values_that_are_not_rotated_pass(dim, axes, dtype, pairs):
+    """Without norm a NaN or an infinity among them is nobody else's, forward and backward; with norm an infinity makes
+    the others 0 and itself NaN."""
+    import torch
+    from splatx_cuda import network
+    T, rotated = getattr(torch, dtype), sum(axes)
+    gen = torch.Generator().manual_seed(dim)
+    x = torch.randn(2, 9, 3, dim, generator=gen).to(T).cuda()
+    pos = (torch.rand(2, 9, 2, generator=gen) * 100).cuda()
+    how = {"axes": axes, "pairs": pairs}
+    turn = lambda t, **kw: network.qk_norm_rotary_fwd(t, None, pos, **how, **kw)[0]  # noqa: E731
+    back = lambda t: network.qk_norm_rotary_bwd(t, None, x, None, pos, **how, norm=False)[0]  # noqa: E731
+    for value in (math.nan, math.inf, -math.inf):
+        for at in range(rotated, dim):
+            bad = x.clone()
+            bad[1, 4, 2, at] = value
+            for f in (lambda t: turn(t, norm=False), back):
+                got, want = f(bad), f(x)
+                assert torch.equal(want[..., rotated:], x[..., rotated:])
+                want[1, 4, 2, at] = value
+                assert torch.equal(got.nan_to_num(7.0, 8.0, 9.0), want.nan_to_num(7.0, 8.0, 9.0)), (value, at)
+            if value == math.inf:
+                got, want = turn(bad), turn(x)
+                want[1, 4, 2], want[1, 4, 2, at] = 0.0, math.nan
+                assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)), at
