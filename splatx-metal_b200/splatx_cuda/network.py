@@ -423,7 +423,10 @@ class _Linear(torch.autograd.Function):
 
 
 def linear(x, weight, bias=None, *, activation=None, residual=None):
-    """linear_fwd's y, differentiable in x, weight, bias and residual."""
+    """linear_fwd's y, differentiable in x, weight, bias and residual. Without gradients to come (no_grad, inference
+    mode, inputs that need none) nothing is kept for them."""
+    if not torch.is_grad_enabled():  # needs_input_grad does not say: it goes by the inputs alone
+        return linear_fwd(x, weight, bias, activation=activation, residual=residual)[0]
     return _Linear.apply(x, weight, bias, residual, activation)
 
 
