@@ -64,3 +64,24 @@ def test_values_that_are_not_rotated_pass(dim, axes, dtype, pairs):
                 got, want = turn(bad), turn(x)
                 want[1, 4, 2], want[1, 4, 2, at] = 0.0, math.nan
                 assert torch.equal(got.nan_to_num(7.0), want.nan_to_num(7.0)), at
+
+
+def test_gelu_in_float32_over_its_tail():
+    """z Phi(z) relative to its value as far as that is a normal number. In units of 2^-24: the reciprocal and its
+    argument 2, with the polynomial after them 2 more, CUDA's exponential 4 (2 ulp), the lost part of z^2, the three
+    products and the fit 4.2, with z 1: 14 of 16. And Phi's own slope beside the largest and infinite z."""
+    import torch
+    from splatx_cuda import network
+    z = torch.cat([torch.linspace(-12.9, 12.9, 200_001, dtype=torch.float64), -torch.logspace(-30, 1.1, 5000, dtype=torch.float64)])
+    z = z.float().cuda()[:, None]
+    one = torch.ones(1, 1, device="cuda")
+    y, pre = network.linear_fwd(z, one, activation="gelu", keep=True)
+    assert torch.equal(pre, z)
+    want = z.double() * 0.5 * torch.special.erfc(-z.double() / math.sqrt(2))
+    off = (y.double() - want).abs() / want.abs().clamp(min=2.0 ** -126)
+    assert float(off.max()) <= 2.0 ** -20, (float(off.max()), float(z[off.argmax()]))
+    far = torch.tensor([[14.0], [1e10], [3e38], [math.inf], [-20.0], [-1e10], [-3e38]], device="cuda").repeat(3, 1)  # more than a few rows
+    y = network.linear_fwd(far, one, activation="gelu")[0]
+    assert torch.equal(y, far.clamp(min=0.0))
+    v_b = network.linear_bwd(torch.ones(1, 1, device="cuda"), far[:1], one, one[0], far[3:4], activation="gelu")[2]
+    assert float(v_b) == 1.0
