@@ -973,7 +973,8 @@ int32_t sxcuda_linear_status(uint32_t* status);
  * are a pair: SXCUDA_PAIRS_AXIS: value j of the axis' own run and value j + axis_dims[a] / 2 of it;
  * SXCUDA_PAIRS_WHOLE: values i and i + (sum of axis_dims) / 2, i the pair's number over all axes;
  * SXCUDA_PAIRS_NEIGHBOURS: values 2 i and 2 i + 1. Values behind the sum of axis_dims are not rotated.
- * Angles are taken in 64 bits, whole turns off; norms, sines and products in 32 bits, rounded once. */
+ * Positions are taken as 64-bit floating point, angles to 2^-28 of a turn up to 2^76 turns (from 2^80 on as 0);
+ * norms, sines and products in 32 bits, rounded once. */
 #define SXCUDA_PAIRS_AXIS 0
 #define SXCUDA_PAIRS_WHOLE 1
 #define SXCUDA_PAIRS_NEIGHBOURS 2

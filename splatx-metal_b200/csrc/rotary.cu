@@ -15,8 +15,9 @@
 // and leave from their place there by bulk copies: the loops then have no addresses of memory and no
 // registers for rows on their way. Rows that such copies do not reach (16 bytes) are read and written value by
 // value.
-// Angles: position x frequency in turns in 64 bits, the nearest quarter turn taken off there; what is left
-// is at most an eighth, and its 32 bits are exact to 2^-28 of a turn however far the position.
+// Angles: position x frequency in turns, the frequency / 2 pi and the product as two 64-bit numbers each, whole turns
+// taken off both and then the nearest quarter; what is left is at most an eighth, which 32 bits have to 2^-28 of a
+// turn. N turns are off by N 2^-104 of one; from 2^80 on the angle is 0.
 #include <algorithm>
 #include <cmath>
 
@@ -64,7 +65,7 @@ struct RotArgs {
     int32_t mode, norm;
     int32_t axis_dims[4];
     float eps, inv_dim;
-    double turns[kRotMostPairs];  // frequency / 2 pi
+    double turns[2][kRotMostPairs];  // frequency / 2 pi, and what that lacks
     uint8_t axis[kRotMostPairs];
 };
 
@@ -122,7 +123,7 @@ constexpr int kTable = 2 * kRotMostPairs;  // floats of a table: V first entries
 struct RotShared {
     alignas(16) float weights[2][kTable];       // of queries and keys
     alignas(16) float angles[kRotWarps][kTable];  // cosines and sines of each warp's token
-    double turns[kRotMostPairs];
+    double turns[2][kRotMostPairs];
     uint64_t full[kRotWarps];  // barriers of the stages
     uint8_t axis[kRotMostPairs];
     uint32_t failed;
@@ -142,7 +143,7 @@ struct Rot {
     bool mine[NV], pair[NV], turned[NV];
 
     __device__ Rot(const RotArgs& a, RotShared& sh) : a(a), sh(sh), table(sh.angles[threadIdx.x >> 5]), lane(threadIdx.x & 31) {
-        for (int i = threadIdx.x; i < a.pairs; i += kRotThreads) sh.turns[i] = a.turns[i], sh.axis[i] = a.axis[i];
+        for (int i = threadIdx.x; i < a.pairs; i += kRotThreads) sh.turns[0][i] = a.turns[0][i], sh.turns[1][i] = a.turns[1][i], sh.axis[i] = a.axis[i];
         for (int i = threadIdx.x; i < 2 * a.slots * V; i += kRotThreads) {
             const int k = i >= a.slots * V, at = i - k * a.slots * V;
             const Slot s = slot_at<V>(a, at / V);
@@ -225,7 +226,10 @@ struct Rot {
         __syncwarp();
         for (int i = lane; i - lane < a.pairs; i += 32) {
             const int j = i < a.pairs ? i : 0;
-            const double t = __shfl_sync(kFullMask, mine_position, sh.axis[j]) * sh.turns[j];
+            const double at = __shfl_sync(kFullMask, mine_position, sh.axis[j]), turn = sh.turns[0][j];
+            const double all = at * turn, rest = fma(at, sh.turns[1][j], fma(at, turn, -all));
+            // of a position that is not finite NaN is left
+            const double t = fabs(all) < 0x1p80 ? (all - rint(all)) + (rest - rint(rest)) : at - at;
             // t in quarters, rounded to a whole number by the sum: its low bits say which quarter
             const double magic = 6755399441055744., up = fma(4., t, magic);
             const int q = __double2loint(up);
@@ -239,9 +243,7 @@ struct Rot {
         __syncwarp();
     }
     // Cosine and sine of r turns, |r| <= 1/8, by their series to the 10th and 9th power (1.1e-10 and 2e-9 are left).
-    // Further off a position was too far for a turn to be left of it: it stands at 0 (of an infinity NaN is left).
     static __device__ __forceinline__ float2 eighth(float r) {
-        r = fabsf(r) > 0.25f ? 0.f : r;
         const float x = 6.2831853071795865f * r, z = x * x;
         float c = fmaf(z, -2.7557319e-7f, 2.4801587e-5f);
         c = fmaf(z, c, -1.3888889e-3f);
@@ -710,7 +712,7 @@ int most_pairs(const SxRotaryInputs& in) {
 
 RotArgs rot_args(const SxRotaryInputs& in, int v) {
     RotArgs a{};
-    const double tau = 6.283185307179586476925286766559;
+    const double tau = 6.283185307179586476925286766559, tau_rest = 2.4492935982947064e-16;  // 2 pi is their sum
     a.positions = in.positions;
     a.pos_batch = in.pos_batch_stride, a.pos_token = in.pos_token_stride, a.pos_axis = in.pos_axis_stride;
     a.tokens = in.tokens;
@@ -721,7 +723,8 @@ RotArgs rot_args(const SxRotaryInputs& in, int v) {
     for (int i = 0; i < in.axes; ++i) {
         a.axis_dims[i] = in.axis_dims[i];
         for (int j = 0; j < in.axis_dims[i] / 2; ++j, ++a.pairs) {
-            a.turns[a.pairs] = in.freqs[a.pairs] / tau;
+            const double f = in.freqs[a.pairs], turn = f / tau;
+            a.turns[0][a.pairs] = turn, a.turns[1][a.pairs] = (std::fma(-turn, tau, f) - turn * tau_rest) / tau;
             a.axis[a.pairs] = static_cast<uint8_t>(i);
         }
     }

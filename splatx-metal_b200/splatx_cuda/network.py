@@ -534,7 +534,8 @@ def qk_norm_rotary_fwd(q, k, positions, *, axes, base=10000.0, freqs=None, pairs
     Pair j of an axis with d values turns by position * base^(-2 j / d), or by position * freqs[i], i
     counting the pairs of all axes. pairs: which values are one: "axis": j and j + d / 2 of the axis' own
     run of values; "whole": i and i + sum(axes) / 2; "neighbours": 2 i and 2 i + 1. norm=False only
-    rotates. q_weight, k_weight: [head_dim], None for ones."""
+    rotates. q_weight, k_weight: [head_dim], None for ones. Positions are taken as float64, angles to 2^-28
+    of a turn up to 2^76 turns (from 2^80 on as 0)."""
     what = "qk_norm_rotary_fwd"
     q, k, ins, device, table = _rotary_inputs(what, q, k, positions, axes, base, freqs, pairs, norm,
                                               q_weight, k_weight, eps)

@@ -85,3 +85,35 @@ def test_gelu_in_float32_over_its_tail():
     assert torch.equal(y, far.clamp(min=0.0))
     v_b = network.linear_bwd(torch.ones(1, 1, device="cuda"), far[:1], one, one[0], far[3:4], activation="gelu")[2]
     assert float(v_b) == 1.0
+
+
+def test_far_positions():
+    """An angle is off by 2^-28 of a turn and by the series and their roundings (2^-22), however far the position: up to
+    2^76 turns. From 2^80 on it is 0, and what is not finite stays NaN."""
+    import torch
+    from decimal import Decimal, getcontext
+    from splatx_cuda import network
+    getcontext().prec = 100
+    tau = 2 * Decimal("3.14159265358979323846264338327950288419716939937510582097494459230781640628620899")
+    whole = [0, 1, -1, 7, 1 << 20, (1 << 30) - 1, -(1 << 33) + 5, (1 << 40) + 3, (1 << 46) + 1, -(1 << 48) + 1, (1 << 51) - 1,
+             *[(1 << 52) + i for i in range(7)], 1 << 53, -(1 << 53) - 2, 1 << 60, -(1 << 62) - 4096]
+    real = torch.tensor([0.3, 1e5 / 3, -2.0 ** 52 * 1.5, 2.0 ** 53 * 1.25, -2.0 ** 54, 1e20, -3e22]).tolist()  # as float32 has them
+    freqs = [1.0, 0.1, 10000.0 ** -0.25, 3.7]
+    for positions, dtype in ((whole, torch.int64), (real, torch.float32)):
+        n = len(positions)
+        x = torch.tensor([1.0, 0.0]).repeat(n, 4)[None, :, None].cuda()
+        y = network.qk_norm_rotary_fwd(x, None, torch.tensor(positions, dtype=dtype)[:, None].cuda(), axes=(8,), freqs=freqs,
+                                       pairs="neighbours", norm=False)[0]
+        for p, row in zip(positions, y[0, :, 0].view(n, 4, 2).tolist()):
+            for f, (c, s) in zip(freqs, row):
+                turns = Decimal(p) * Decimal(f) / tau
+                rest = 2 * math.pi * float(turns - turns.to_integral_value())
+                bound = 2 * math.pi * 2.0 ** -28 + 2.0 ** -22
+                assert abs(c - math.cos(rest)) <= bound and abs(s - math.sin(rest)) <= bound, (p, f, c, s)
+    x = torch.randn(1, 4, 3, 8, generator=torch.Generator().manual_seed(1)).cuda()
+    y = network.qk_norm_rotary_fwd(x, None, torch.tensor([[1e26], [-1e30], [3e38], [-2e38]], device="cuda"), axes=(8,),
+                                   freqs=[1.0, 2.0, 1e100, 1e300], norm=False)[0]
+    assert torch.equal(y, x)
+    for p in (math.inf, -math.inf, math.nan):
+        y = network.qk_norm_rotary_fwd(x, None, torch.full((4, 1), p, device="cuda"), axes=(4,), norm=False)[0]
+        assert bool(y[..., :4].isnan().all()) and torch.equal(y[..., 4:], x[..., 4:])
