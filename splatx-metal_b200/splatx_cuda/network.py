@@ -596,7 +596,9 @@ class _QkNormRotary(torch.autograd.Function):
 def qk_norm_rotary(q, k, positions, *, axes, base=10000.0, freqs=None, pairs="axis", norm=True,
                    q_weight=None, k_weight=None, eps=1e-6):
     """qk_norm_rotary_fwd's (q, k), differentiable in q, k and the weights."""
-    how = {"axes": axes, "base": base, "freqs": freqs, "pairs": pairs, "norm": norm, "eps": eps}
+    # as they are now: the backward must not see what a caller makes of its lists meanwhile
+    freqs = None if freqs is None else tuple(map(float, freqs))
+    how = {"axes": tuple(axes), "base": base, "freqs": freqs, "pairs": pairs, "norm": norm, "eps": eps}
     return _QkNormRotary.apply(q, k, positions, q_weight, k_weight, how)
 
 
