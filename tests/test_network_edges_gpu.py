@@ -117,3 +117,65 @@ def test_far_positions():
     for p in (math.inf, -math.inf, math.nan):
         y = network.qk_norm_rotary_fwd(x, None, torch.full((4, 1), p, device="cuda"), axes=(4,), norm=False)[0]
         assert bool(y[..., :4].isnan().all()) and torch.equal(y[..., 4:], x[..., 4:])
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("size", [(300, 72, 101), (300, 4096, 101), (5, 72, 333), (131, 64, 3)], ids=lambda s: "x".join(map(str, s)))
+def test_copies_end_with_the_row(size, dtype):
+    """At the C entry: rows of an odd length on a start and a pitch that copies reach. They must end inside 16 bytes and
+    leave what is behind the row, and read a residual as far as its row."""
+    import ctypes as C
+    import torch
+    from splatx_cuda import _native as n, network
+    m, k, o = size
+    gen = torch.Generator().manual_seed(o)
+    T, code = getattr(torch, dtype), {"float16": 1, "bfloat16": 2}[dtype]
+    x, w, r = (torch.randn(s, generator=gen).to(T).cuda() for s in ((m, k), (o, k), (m, o)))
+    b = torch.randn(o, generator=gen).cuda()
+    pitch, first = (o + 15) // 8 * 8, 8
+    for residual in (False, True):
+        want, want_pre = network.linear_fwd(x, w, b, activation="gelu", residual=r if residual else None, keep=True)
+        y, pre, add = (torch.full((m + 2, pitch), 7.0, dtype=T, device="cuda") for _ in range(3))
+        inner = lambda t: torch.as_strided(t, (m, o), (pitch, 1), pitch + first)  # noqa: E731
+        add.fill_(math.nan)
+        inner(add).copy_(r)
+        at = [t.data_ptr() + (pitch + first) * 2 for t in (y, pre, add)]
+        assert not any(p % 16 for p in at)
+        ins = n.SxLinearInputs(x.data_ptr(), w.data_ptr(), b.data_ptr(), m, k, o, k, k, code, 0, 3)
+        outs = n.SxLinearOutputs(at[2] if residual else None, pitch, at[0], pitch, at[1], pitch)
+        nbytes, entry = C.c_size_t(0), n.lib().sxcuda_linear_fwd
+        n.check(entry(C.byref(ins), C.byref(outs), None, C.byref(nbytes), None))
+        ws = torch.empty(max(nbytes.value, 32), dtype=torch.uint8, device="cuda")
+        n.check(entry(C.byref(ins), C.byref(outs), ws.data_ptr(), C.byref(nbytes), torch.cuda.current_stream().cuda_stream))
+        for t, v in ((y, want), (pre, want_pre)):
+            assert torch.equal(inner(t), v)
+            inner(t).fill_(7.0)
+            assert bool((t == 7.0).all())
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("size", [(1, 101, 72), (300, 101, 1), (300, 101, 72), (4000, 333, 40)], ids=lambda s: "x".join(map(str, s)))
+def test_gradient_copies_end_with_the_row(size, dtype):
+    """The same of v_x and v_weight, one row of them among the cases, which any pitch is good for."""
+    import ctypes as C
+    import torch
+    from splatx_cuda import _native as n, network
+    m, k, o = size
+    gen = torch.Generator().manual_seed(m + o)
+    T, code = getattr(torch, dtype), {"float16": 1, "bfloat16": 2}[dtype]
+    x, w, g = (torch.randn(s, generator=gen).to(T).cuda() for s in ((m, k), (o, k), (m, o)))
+    want = network.linear_bwd(g, x, w)[:2]
+    pitch = (k + 15) // 8 * 8
+    got = [torch.full((rows + 2, pitch), 7.0, dtype=T, device="cuda") for rows in (m, o)]
+    at = [t.data_ptr() + (pitch + 8) * 2 for t in got]
+    ins = n.SxLinearInputs(x.data_ptr(), w.data_ptr(), None, m, k, o, k, k, code, 0, 0)
+    gin, out = n.SxLinearGradsIn(g.data_ptr(), o, None, 0), n.SxLinearGrads(at[0], pitch, at[1], pitch, None)
+    nbytes, entry = C.c_size_t(0), n.lib().sxcuda_linear_bwd
+    n.check(entry(C.byref(ins), C.byref(gin), C.byref(out), None, C.byref(nbytes), None))
+    ws = torch.empty(max(nbytes.value, 32), dtype=torch.uint8, device="cuda")
+    n.check(entry(C.byref(ins), C.byref(gin), C.byref(out), ws.data_ptr(), C.byref(nbytes), torch.cuda.current_stream().cuda_stream))
+    for t, v in zip(got, want):
+        rows = torch.as_strided(t, v.shape, (pitch, 1), pitch + 8)
+        assert torch.equal(rows, v)
+        rows.fill_(7.0)
+        assert bool((t == 7.0).all())
