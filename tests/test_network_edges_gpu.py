@@ -119,6 +119,34 @@ def test_far_positions():
         assert bool(y[..., :4].isnan().all()) and torch.equal(y[..., 4:], x[..., 4:])
 
 
+@pytest.mark.parametrize("rows", [0, 1, 7, 300])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_one_row_may_have_any_stride(dtype, rows):
+    """At the C entry: a weight and its gradient of one row, and x, v_y and their like of one, are not asked for a stride."""
+    import ctypes as C
+    import torch
+    from splatx_cuda import _native as n, network
+    k, o, code = 72, 1, {"bfloat16": 2, "float32": 0}[dtype]
+    gen = torch.Generator().manual_seed(rows)
+    x, w, g = (torch.randn(s, generator=gen).to(getattr(torch, dtype)).cuda() for s in ((rows, k), (o, k), (rows, o)))
+    b = torch.ones(o, device="cuda")
+    y, pre = network.linear_fwd(x, w, b, activation="silu", keep=True)
+    want = (y, pre, *network.linear_bwd(g, x, w, b, pre, activation="silu"))
+    got = [torch.full_like(t, 7.0) for t in want]
+    y, pre, v_x, v_w, v_b = got
+    x_stride, y_stride = (0, 0) if rows <= 1 else (k, o)
+    ins = n.SxLinearInputs(x.data_ptr(), w.data_ptr(), b.data_ptr(), rows, k, o, x_stride, 0, code, 0, 2)
+    stream = torch.cuda.current_stream().cuda_stream
+    for entry, args in ((n.lib().sxcuda_linear_fwd, (n.SxLinearOutputs(None, 0, y.data_ptr(), y_stride, pre.data_ptr(), y_stride),)),
+                        (n.lib().sxcuda_linear_bwd, (n.SxLinearGradsIn(g.data_ptr(), y_stride, want[1].data_ptr(), y_stride),
+                                                     n.SxLinearGrads(v_x.data_ptr(), x_stride, v_w.data_ptr(), 0, v_b.data_ptr())))):
+        nbytes, args = C.c_size_t(0), [C.byref(a) for a in (ins, *args)]
+        n.check(entry(*args, None, C.byref(nbytes), None))
+        ws = torch.empty(max(nbytes.value, 32), dtype=torch.uint8, device="cuda")
+        n.check(entry(*args, ws.data_ptr(), C.byref(nbytes), stream))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("size", [(300, 72, 101), (300, 4096, 101), (5, 72, 333), (131, 64, 3)], ids=lambda s: "x".join(map(str, s)))
 def test_copies_end_with_the_row(size, dtype):
