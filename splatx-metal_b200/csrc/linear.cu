@@ -104,9 +104,9 @@ __device__ __forceinline__ void linear_biases(const LinearProduct& p, int64_t co
 }
 
 // A launch's one product, or the backward's two, which have nothing to wait for in one another: small ones fill the
-// SMs better together. Backward calls with two launches and with one, us: 604 x 77 x 913 35 and 26, 300 x 256 x 256 with
-// relu 26 and 17, 2048 x 128 x 512 with gelu 42 and 35 (with one launch for the joins). A kernel that finds its product
-// at run time is slower (forward 2048 x 128 x 512: 19 and 25), so one product has a kernel of its own.
+// SMs better together. Backward calls with two launches and with one, us: 604 x 77 x 913 33 and 28, 300 x 256 x 256 with
+// relu 26 and 17, 2048 x 128 x 512 with gelu 37 and 35, 20000 x 64 x 64 36 and 29 (with one launch for the joins). A kernel
+// that finds its product at run time is slower (forward 2048 x 128 x 512: 19 and 25), so one product has a kernel of its own.
 template <int N>
 struct LinearProducts {
     LinearProduct p[N];
@@ -433,6 +433,9 @@ __device__ __forceinline__ void linear_param_to(void* w, int32_t dtype, int64_t 
 }
 
 // ---- v_z = v_y act'(pre), and the sum of its rows ----
+// v_z is rounded to the element type, as the tensor cores take it: the gradients of x and of the weight behind an activation
+// are then off by 0.0023 of their size in bfloat16 where a v_z of 32 bits leaves 0.0017 (float16 an eighth of both). Two
+// 16-bit parts of it would double both products. The bias' sum takes it before the rounding.
 // A CTA has 32 V columns (a warp's lanes V each) and a slice of the rows, which its warps take in turn; the grid
 // is what the SMs hold. Bound by memory: gelu over bf16 32768 x 4096 163 us (4.9 TB/s); several rows asked for
 // at once by a warp, with fewer warps, were slower (2 rows 185 us, 4 rows 222 us).

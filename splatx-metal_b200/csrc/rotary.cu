@@ -531,7 +531,8 @@ __global__ void __launch_bounds__(kRotThreads, kRotPerSm<1, BACK>) rotary_plain_
 // fills, other warps work: more warps with a stage each were faster than fewer with two (68 and 72 us for
 // 4 x 8192 tokens, 16 (4) heads x 128; backward of 8 x 4096, 16 heads x 64: 93 and 97 us). The forward has a
 // token's weights times sines in registers (66 us; the same read for every row from shared memory 68 us).
-// bf16: forward 66 us (5.1 TB/s), backward 92 us (4.4 TB/s, instructions).
+// bf16: forward 67 us (5.1 TB/s), backward 95 us (4.3 TB/s; latency: 128 registers leave 16 warps an SM, which issue in 55%
+// of the cycles with no pipe full).
 __device__ __forceinline__ void bulk_store(void* to, uint32_t from, uint32_t bytes) {
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(from), "r"(bytes) : "memory");
 }

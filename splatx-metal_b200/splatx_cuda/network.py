@@ -371,7 +371,8 @@ def _space(device, entry, *args):
 def linear_bwd(v_y, x, weight, bias=None, pre=None, *, activation=None, needs_x=True, needs_weight=True):
     """Gradients (v_x, v_weight, v_bias) of linear_fwd for the gradient v_y of its y (which is also the
     residual's). pre is the forward's, needed with an activation and only then. v_bias is like bias, None
-    without one; v_x and v_weight are None where they are not needed. Deterministic."""
+    without one; v_x and v_weight are None where they are not needed. v_y act'(pre) is rounded to x's dtype
+    before the products with x and weight, not before its sum. Deterministic."""
     what = "linear_bwd"
     flat, w, ins, device = _linear_inputs(what, x, weight, bias, activation)
     n = weight.shape[0]
