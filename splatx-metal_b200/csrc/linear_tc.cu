@@ -595,7 +595,7 @@ void launch_tile(const LinearProduct& p, cudaStream_t s) {
         SX_LAUNCH(kernel, static_cast<unsigned>(2 * p.plan.workers), kThreads<B_ACROSS>, Smem<TN>::kBytes, s, p, maps);
     };
     const auto reached = [&](const void* x, int64_t stride) { return !x || linear_tc_takes(x, stride, p.m); };
-    // a copy to memory ends on 16 bytes: with an odd length of row (measured) it also writes behind the row
+    // a copy to memory ends on 16 bytes (measured): with any other length of row it also writes behind the row
     if (p.n % 8 == 0 && reached(p.y, p.y_stride) && reached(p.pre, p.pre_stride) && reached(p.residual, p.residual_stride)) {
         maps.y = patch_map(p, p.y, p.y_stride);
         maps.pre = patch_map(p, p.pre, p.pre_stride);
